@@ -83,6 +83,28 @@ class GateArgs(ctypes.Structure):
                 ("a_stride_row", I64), ("b_stride_row", I64)]
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", U32), ("flags", U32)]
+                + [(n, P) for n in ("q", "k", "v", "g", "o", "initial_state", "final_state", "cu_seqlens", "state_indices", "status", "workspace")]
+                + [("workspace_bytes", U64)]
+                + [(n, I32) for n in ("B", "T", "Hk", "Hv", "dk", "dv", "n_seqs", "num_slots")]
+                + [(f"{t}_stride_{d}", I64) for t in ("q", "k", "v", "o") for d in ("b", "t", "h")]
+                + [("g_stride_b", I64), ("g_stride_t", I64), ("scale", F32), ("reserved0", F32)])
+
+
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", U32), ("flags", U32)] + [(n, P) for n in ("x", "weight", "bias", "y", "mean", "rstd")]
+                + [(n, I64) for n in ("rows", "n", "x_stride", "y_stride")]
+                + [("x_dtype", I32), ("w_dtype", I32), ("eps", F32), ("reserved0", F32)])
+
+
+class LayerNormBwdArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", U32), ("flags", U32)]
+                + [(n, P) for n in ("d_y", "x", "mean", "rstd", "weight", "d_x", "d_weight", "d_bias", "workspace")]
+                + [("workspace_bytes", U64)] + [(n, I64) for n in ("rows", "n", "dy_stride", "x_stride", "dx_stride")]
+                + [("x_dtype", I32), ("w_dtype", I32)])
+
+
 # every symbol include/ave_gdn.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "ave_gdn_chunk_prefill": (ctypes.c_int, [ctypes.POINTER(GdnArgs), P]),
@@ -102,6 +124,12 @@ SYMBOLS = {
     "ave_gdn_decode_layer_step": (ctypes.c_int, [ctypes.POINTER(DecodeLayerArgs), P]),
     "ave_gdn_recurrent_backward": (ctypes.c_int, [ctypes.POINTER(BwdArgs), P]),
     "ave_gdn_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(BwdArgs)]),
+    "ave_linear_chunk_prefill": (ctypes.c_int, [ctypes.POINTER(LinearArgs), P]),
+    "ave_linear_prefill_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LinearArgs)]),
+    "ave_linear_decode_step": (ctypes.c_int, [ctypes.POINTER(LinearArgs), P]),
+    "ave_layer_norm": (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), P]),
+    "ave_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(LayerNormBwdArgs), P]),
+    "ave_layer_norm_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LayerNormBwdArgs)]),
     "ave_gdn_abi_version": (ctypes.c_int, []),
     "ave_gdn_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ave_gdn_last_cuda_error": (ctypes.c_int, []),

@@ -91,6 +91,12 @@ struct Api {
   decltype(&ave_gdn_decode_layer_step) decode_layer_step = nullptr;
   decltype(&ave_gdn_recurrent_backward) recurrent_backward = nullptr;
   decltype(&ave_gdn_backward_workspace_bytes) backward_workspace_bytes = nullptr;
+  decltype(&ave_linear_chunk_prefill) linear_prefill = nullptr;
+  decltype(&ave_linear_prefill_workspace_bytes) linear_prefill_workspace_bytes = nullptr;
+  decltype(&ave_linear_decode_step) linear_decode = nullptr;
+  decltype(&ave_layer_norm) layer_norm = nullptr;
+  decltype(&ave_layer_norm_backward) layer_norm_backward = nullptr;
+  decltype(&ave_layer_norm_backward_workspace_bytes) layer_norm_backward_workspace_bytes = nullptr;
   decltype(&ave_gdn_status_string) status_string = nullptr;
   decltype(&ave_gdn_last_cuda_error) last_cuda_error = nullptr;
 } api;
@@ -652,10 +658,87 @@ void op_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   check(launch([&] { return api.recurrent_backward(&a, launch.stream); }), "gated_delta_rule_backward");
 }
 
+// g: [B, T, Hv], or [Hv] for every token alike
+AveLinearArgs fill_linear(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor* g, const Tensor& o, double scale, const Tensor* s0,
+                          const Tensor* final, const Tensor* cu, const Tensor* idx) {
+  AveLinearArgs a{};
+  a.struct_size = sizeof(a);
+  a.q = ptr(&q); a.k = ptr(&k); a.v = ptr(&v); a.g = ptr_as<float>(g); a.o = const_cast<void*>(ptr(&o));
+  a.initial_state = ptr_as<float>(s0); a.final_state = ptr_as<float>(final);
+  a.cu_seqlens = ptr_as<int32_t>(cu); a.state_indices = ptr_as<int32_t>(idx);
+  a.status = reinterpret_cast<uint32_t*>(status_word(q.device()).data_ptr());
+  a.B = (int32_t)q.size(0); a.T = (int32_t)q.size(1); a.Hk = (int32_t)q.size(2); a.Hv = (int32_t)v.size(2);
+  a.dk = (int32_t)q.size(3); a.dv = (int32_t)v.size(3);
+  const int64_t n = n_sequences(q, cu);
+  a.n_seqs = (int32_t)n; a.num_slots = (int32_t)n_slots(s0, final, n);
+  STRIDES4(a, q, q); STRIDES4(a, k, k); STRIDES4(a, v, v); STRIDES4(a, o, o);
+  if (g != nullptr && g->dim() == 3) { a.g_stride_b = g->stride(0); a.g_stride_t = g->stride(1); }
+  a.scale = (float)scale;
+  return a;
+}
+
+void op_linear_prefill(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g, const Tensor& out, double scale, const OptTensor& initial_state,
+                       const OptTensor& final_state, const OptTensor& cu_seqlens, const OptTensor& state_indices) {
+  loaded();
+  AveLinearArgs a = fill_linear(q, k, v, some(g), out, scale, some(initial_state), some(final_state), some(cu_seqlens), some(state_indices));
+  Launch launch(q);
+  const Scratch ws(q, launch.stream, api.linear_prefill_workspace_bytes(&a));
+  a.workspace = ws.data(); a.workspace_bytes = ws.size();
+  check(launch([&] { return api.linear_prefill(&a, launch.stream); }), "chunk_linear_attention");
+}
+
+void op_linear_decode(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g, const Tensor& out, double scale, const OptTensor& initial_state,
+                      const OptTensor& final_state, const OptTensor& cu_seqlens, const OptTensor& state_indices) {
+  loaded();
+  AveLinearArgs a = fill_linear(q, k, v, some(g), out, scale, some(initial_state), some(final_state), some(cu_seqlens), some(state_indices));
+  Launch launch(q);
+  check(launch([&] { return api.linear_decode(&a, launch.stream); }), "fused_recurrent_linear_attention");
+}
+
+int32_t dtype_code(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return AVE_DTYPE_BF16;
+    case at::kHalf: return AVE_DTYPE_FP16;
+    case at::kFloat: return AVE_DTYPE_FP32;
+    default: BAD_ARGUMENT(name, " must have dtype torch.bfloat16, torch.float16 or torch.float32, got ", dtype_name(t), ".");
+  }
+}
+
+// x, out: [rows, n] views with contiguous rows
+void op_layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, const Tensor& out, const OptTensor& mean, const OptTensor& rstd) {
+  loaded();
+  AveLayerNormArgs a{};
+  a.struct_size = sizeof(a);
+  a.x = ptr(&x); a.y = const_cast<void*>(ptr(&out)); a.weight = ptr(some(weight)); a.bias = ptr(some(bias));
+  a.mean = ptr_as<float>(some(mean)); a.rstd = ptr_as<float>(some(rstd));
+  a.rows = x.size(0); a.n = x.size(1); a.x_stride = x.stride(0); a.y_stride = out.stride(0);
+  a.x_dtype = dtype_code(x, "x"); a.w_dtype = some(weight) != nullptr ? dtype_code(*some(weight), "weight") : a.x_dtype;
+  a.eps = (float)eps;
+  Launch launch(x);
+  check(launch([&] { return api.layer_norm(&a, launch.stream); }), "layer_norm");
+}
+
+void op_layer_norm_backward(const Tensor& d_y, const Tensor& x, const Tensor& mean, const Tensor& rstd, const OptTensor& weight, const Tensor& d_x,
+                            const OptTensor& d_weight, const OptTensor& d_bias) {
+  loaded();
+  AveLayerNormBwdArgs a{};
+  a.struct_size = sizeof(a);
+  a.d_y = ptr(&d_y); a.x = ptr(&x); a.mean = ptr_as<float>(&mean); a.rstd = ptr_as<float>(&rstd); a.weight = ptr(some(weight));
+  a.d_x = const_cast<void*>(ptr(&d_x)); a.d_weight = const_cast<void*>(ptr(some(d_weight))); a.d_bias = const_cast<void*>(ptr(some(d_bias)));
+  a.rows = x.size(0); a.n = x.size(1); a.dy_stride = d_y.stride(0); a.x_stride = x.stride(0); a.dx_stride = d_x.stride(0);
+  a.x_dtype = dtype_code(x, "x"); a.w_dtype = some(weight) != nullptr ? dtype_code(*some(weight), "weight") : a.x_dtype;
+  Launch launch(x);
+  const Scratch ws(x, launch.stream, api.layer_norm_backward_workspace_bytes(&a));
+  a.workspace = ws.data(); a.workspace_bytes = ws.size();
+  check(launch([&] { return api.layer_norm_backward(&a, launch.stream); }), "layer_norm_backward");
+}
+
 #define OPERATORS(X)                                                                                                        \
   X("chunk_prefill", op_prefill) X("decode_step", op_decode) X("mixed_step", op_mixed) X("decode_layer_step", op_decode_layer) \
   X("gated_rmsnorm", op_rmsnorm) X("conv1d_silu", op_conv) X("conv1d_update", op_conv_update) X("gate_beta", op_gate)          \
-  X("gemm_bf16_nt", op_gemm) X("recurrent_backward", op_backward)
+  X("gemm_bf16_nt", op_gemm) X("recurrent_backward", op_backward)                                                           \
+  X("linear_prefill", op_linear_prefill) X("linear_decode", op_linear_decode)                                               \
+  X("layer_norm", op_layer_norm) X("layer_norm_backward", op_layer_norm_backward)
 TORCH_LIBRARY_IMPL(avelang_gdn, CUDA, m) {
 #define CUDA_KERNEL(name, f) m.impl(name, f);
   OPERATORS(CUDA_KERNEL)
@@ -906,6 +989,146 @@ PyObject* backward(PyObject* const* p) {
   return r;
 }
 
+PyObject* wrap_all(std::initializer_list<const Tensor*> out) {  // undefined: None
+  PyObject* r = PyTuple_New((Py_ssize_t)out.size());
+  if (r == nullptr) throw python_error();
+  Py_ssize_t i = 0;
+  for (const Tensor* t : out) {
+    if (!t->defined()) Py_INCREF(Py_None);
+    PyTuple_SET_ITEM(r, i++, t->defined() ? wrap(*t) : Py_None);
+  }
+  return r;
+}
+
+// A tensor map takes no stride of zero, which a gradient of a sum or an expanded input has.
+Tensor spread(const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) return t.contiguous();
+  return t;
+}
+
+Shape check_linear(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor* g, const Tensor* cu) {
+  const std::pair<const char*, const Tensor*> qkv[] = {{"q", &q}, {"k", &k}, {"v", &v}};
+  for (const auto& [name, t] : qkv) {
+    REQ(t->dim() == 4, name, " must be a 4-D tensor [B, T, H, d]");
+    REQ(t->scalar_type() == at::kBFloat16, name, " must have dtype torch.bfloat16, got ", dtype_name(*t), ".");
+    REQ(t->is_cuda(), name, " must be a CUDA tensor");
+    REQ(t->stride(3) == 1, name, " must be contiguous in its last dimension");
+    REQ(t->device() == q.device(), name, " must be on device ", q.device(), ", got ", t->device(), ".");
+  }
+  Shape s;
+  s.B = q.size(0); s.T = q.size(1); s.Hk = q.size(2); s.dk = q.size(3);
+  REQ(k.sizes() == q.sizes(), "k must have shape ", shape_of(q.sizes()), ", got ", shape_of(k.sizes()), ".");
+  REQ(v.size(0) == s.B && v.size(1) == s.T, "v must have leading shape ", shape_of(q.sizes().slice(0, 2)), ", got ",
+      shape_of(v.sizes().slice(0, 2)), ".");
+  s.Hv = v.size(2); s.dv = v.size(3);
+  REQ(s.Hk > 0 && s.Hv > 0 && s.Hv % s.Hk == 0, "value heads (", s.Hv, ") must be a multiple of key heads (", s.Hk, ").");
+  REQ((s.dk == 128 || s.dk == 64) && (s.dv == 128 || s.dv == 64), "head dims dk and dv must be 128 or 64, got (", s.dk, ", ", s.dv, ").");
+  if (g != nullptr) {
+    REQ(g->scalar_type() == at::kFloat, "g must have dtype torch.float32, got ", dtype_name(*g), ".");
+    REQ((g->dim() == 1 && g->size(0) == s.Hv) || (g->dim() == 3 && g->size(0) == s.B && g->size(1) == s.T && g->size(2) == s.Hv), "g must have shape ",
+        shape_of({s.B, s.T, s.Hv}), " or ", shape_of({s.Hv}), ", got ", shape_of(g->sizes()), ".");
+    REQ(g->device() == q.device(), "g must be on device ", q.device(), ", got ", g->device(), ".");
+    REQ(g->stride(-1) == 1 || s.Hv == 1, "g must be contiguous in its last dimension");
+  }
+  s.n = s.B;
+  if (cu != nullptr) {
+    REQ(s.B == 1, "cu_seqlens requires B == 1 (packed layout)");
+    REQ(cu->scalar_type() == at::kInt && cu->dim() == 1 && cu->numel() >= 1, "cu_seqlens must be a 1-D int32 tensor [N+1]");
+    REQ(cu->device() == q.device() && cu->is_contiguous(), "cu_seqlens must be contiguous on ", q.device());
+    s.n = cu->numel() - 1;
+  }
+  REQ(s.B < (1ll << 31) && s.T < (1ll << 31), "B and T must be below 2^31");
+  return s;
+}
+
+// linear_prefill / linear_decode(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, state_indices, inplace_state, out, chunk_size)
+//   -> (o, final or None)
+template <bool kPrefill>
+PyObject* linear_forward(PyObject* const* p) {
+  const Tensor &q = tensor(p[0], "q"), &k = tensor(p[1], "k"), &v = tensor(p[2], "v");
+  const Tensor *g = opt_tensor(p[3], "g"), *s0 = opt_tensor(p[5], "initial_state"), *cu = opt_tensor(p[7], "cu_seqlens"),
+               *idx = opt_tensor(p[8], "state_indices"), *out = opt_tensor(p[10], "out");
+  const Shape s = check_linear(q, k, v, g, cu);
+  const int64_t chunk = integer(p[11]);
+  REQ(chunk == 64, "chunk_size must be 64, got ", chunk, ".");
+  const Tensor o = prep_out(out, v);
+  const Tensor final = prep_states(s0, idx, s, q, truth(p[6]), truth(p[9]));
+  if constexpr (kPrefill)
+    call<op_linear_prefill>("avelang_gdn::linear_prefill", spread(q), spread(k), spread(v), opt(g), o, scale_or(p[4], s.dk), opt(s0), opt(final), opt(cu), opt(idx));
+  else
+    call<op_linear_decode>("avelang_gdn::linear_decode", q, k, v, opt(g), o, scale_or(p[4], s.dk), opt(s0), opt(final), opt(cu), opt(idx));
+  return wrap_pair(o, final);
+}
+
+// The rows of x as [rows, n]
+Tensor as_rows(const Tensor& x) { return x.dim() == 2 ? x : x.reshape({x.numel() / x.size(-1), x.size(-1)}); }
+void check_norm_input(const Tensor& x, const Tensor* w, const Tensor* b) {
+  dtype_code(x, "x");
+  REQ(x.is_cuda(), "x must be a CUDA tensor");
+  REQ(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 32768, "the last dimension of x must lie in [1, 32768], got ", x.dim() > 0 ? x.size(-1) : 0, ".");
+  const int64_t n = x.size(-1);
+  REQ(b == nullptr || w != nullptr, "bias needs weight");
+  const std::pair<const char*, const Tensor*> wb[] = {{"weight", w}, {"bias", b}};
+  for (const auto& [name, t] : wb)
+    if (t != nullptr) {
+      REQ(t->dim() == 1 && t->size(0) == n, name, " must have shape ", shape_of({n}), ", got ", shape_of(t->sizes()), ".");
+      REQ(t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat, name, " must have the dtype of x or torch.float32, got ", dtype_name(*t), ".");
+      REQ(t->device() == x.device(), name, " must be on device ", x.device(), ", got ", t->device(), ".");
+    }
+  REQ(b == nullptr || b->scalar_type() == w->scalar_type(), "weight and bias must share a dtype");
+}
+
+// layer_norm(x, weight, bias, eps, return_stats, out) -> out or (out, mean, rstd)
+PyObject* layer_norm(PyObject* const* p) {
+  const Tensor& x = tensor(p[0], "x");
+  const Tensor *w = opt_tensor(p[1], "weight"), *b = opt_tensor(p[2], "bias"), *out = opt_tensor(p[5], "out");
+  check_norm_input(x, w, b);
+  const Tensor y = out != nullptr ? *out : empty(x.sizes(), x.scalar_type(), x);
+  REQ(y.sizes() == x.sizes() && y.scalar_type() == x.scalar_type() && y.device() == x.device(), "out must be a ", dtype_name(x), " tensor of shape ",
+      shape_of(x.sizes()), " on ", x.device());
+  Tensor x2 = as_rows(x);
+  const Tensor y2 = as_rows(y);
+  if (x2.stride(1) != 1) x2 = x2.contiguous();
+  REQ(y2.is_alias_of(y) && (y2.stride(1) == 1 || y2.size(1) == 1), "out must be viewable as [rows, n] with contiguous rows");
+  const Tensor wc = w != nullptr ? w->contiguous() : Tensor(), bc = b != nullptr ? b->contiguous() : Tensor();
+  const bool stats = truth(p[4]);
+  Tensor mean, rstd;
+  if (stats) {
+    mean = empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+    rstd = empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+  }
+  call<op_layer_norm>("avelang_gdn::layer_norm", x2, opt(wc), opt(bc), number(p[3]), y2, opt(mean), opt(rstd));
+  return stats ? wrap_all({&y, &mean, &rstd}) : wrap(y);
+}
+
+// layer_norm_backward(d_y, x, mean, rstd, weight) -> (dx, dweight or None, dbias or None)
+PyObject* layer_norm_backward(PyObject* const* p) {
+  const Tensor &d_y = tensor(p[0], "d_y"), &x = tensor(p[1], "x"), &mean = tensor(p[2], "mean"), &rstd = tensor(p[3], "rstd");
+  const Tensor* w = opt_tensor(p[4], "weight");
+  check_norm_input(x, w, nullptr);
+  REQ(d_y.sizes() == x.sizes() && d_y.scalar_type() == x.scalar_type() && d_y.device() == x.device(), "d_y must be a ", dtype_name(x), " tensor of shape ",
+      shape_of(x.sizes()), " on ", x.device());
+  const int64_t n = x.size(-1), rows = x.numel() / n;
+  const std::pair<const char*, const Tensor*> stats[] = {{"mean", &mean}, {"rstd", &rstd}};
+  for (const auto& [name, t] : stats)
+    REQ(t->scalar_type() == at::kFloat && t->numel() == rows && t->is_contiguous() && t->device() == x.device(), name, " must be a contiguous fp32 tensor of ",
+        rows, " elements on ", x.device());
+  Tensor x2 = as_rows(x), dy2 = as_rows(d_y);
+  if (x2.stride(1) != 1) x2 = x2.contiguous();
+  if (dy2.stride(1) != 1) dy2 = dy2.contiguous();
+  const Tensor dx = empty(x.sizes(), x.scalar_type(), x);
+  Tensor wc, dw, db;
+  if (w != nullptr) {
+    wc = w->contiguous();
+    dw = empty({n}, w->scalar_type(), x);
+    db = empty({n}, w->scalar_type(), x);
+    if (rows == 0) { dw.zero_(); db.zero_(); }  // no kernel runs
+  }
+  call<op_layer_norm_backward>("avelang_gdn::layer_norm_backward", dy2, x2, mean, rstd, opt(wc), as_rows(dx), opt(dw), opt(db));
+  return wrap_all({&dx, &dw, &db});
+}
+
 PyObject* none() { Py_RETURN_NONE; }
 // status_word(device_index) -> the device status word; workspace-independent
 PyObject* py_status_word(PyObject* const* p) { return wrap(status_word(at::Device(at::kCUDA, (c10::DeviceIndex)integer(p[0])))); }
@@ -931,6 +1154,12 @@ PyObject* bind(PyObject* const* p) {
   RESOLVE(decode_layer_step, ave_gdn_decode_layer_step);
   RESOLVE(recurrent_backward, ave_gdn_recurrent_backward);
   RESOLVE(backward_workspace_bytes, ave_gdn_backward_workspace_bytes);
+  RESOLVE(linear_prefill, ave_linear_chunk_prefill);
+  RESOLVE(linear_prefill_workspace_bytes, ave_linear_prefill_workspace_bytes);
+  RESOLVE(linear_decode, ave_linear_decode_step);
+  RESOLVE(layer_norm, ave_layer_norm);
+  RESOLVE(layer_norm_backward, ave_layer_norm_backward);
+  RESOLVE(layer_norm_backward_workspace_bytes, ave_layer_norm_backward_workspace_bytes);
   RESOLVE(status_string, ave_gdn_status_string);
   RESOLVE(last_cuda_error, ave_gdn_last_cuda_error);
 #undef RESOLVE
@@ -963,6 +1192,10 @@ PyMethodDef methods[] = {
     ENTRY("gate", gate, 4),
     ENTRY("gemm", gemm, 3),
     ENTRY("backward", backward, 10),
+    ENTRY("linear_prefill", linear_forward<true>, 12),
+    ENTRY("linear_decode", linear_forward<false>, 12),
+    ENTRY("layer_norm", layer_norm, 6),
+    ENTRY("layer_norm_backward", layer_norm_backward, 5),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

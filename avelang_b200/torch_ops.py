@@ -35,6 +35,13 @@ SCHEMAS = {
     "decode_layer_step": "(Tensor proj, Tensor conv_w, Tensor? conv_bias, Tensor(a!) conv_state, Tensor A_log, Tensor dt_bias, "
                          "Tensor? norm_weight, Tensor(b!) state_pool, Tensor? state_indices, Tensor(c!) out, int Hk, int Hv, "
                          "float scale, float norm_eps, bool gate_first) -> ()",
+    "linear_prefill": "(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor(a!) out, float scale, Tensor? initial_state, "
+                      "Tensor(b!)? final_state, Tensor? cu_seqlens, Tensor? state_indices) -> ()",
+    "linear_decode": "(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor(a!) out, float scale, Tensor? initial_state, "
+                     "Tensor(b!)? final_state, Tensor? cu_seqlens, Tensor? state_indices) -> ()",
+    "layer_norm": "(Tensor x, Tensor? weight, Tensor? bias, float eps, Tensor(a!) out, Tensor(b!)? mean, Tensor(c!)? rstd) -> ()",
+    "layer_norm_backward": "(Tensor d_y, Tensor x, Tensor mean, Tensor rstd, Tensor? weight, Tensor(a!) d_x, Tensor(b!)? d_weight, "
+                           "Tensor(c!)? d_bias) -> ()",
 }
 for _name, _schema in SCHEMAS.items():
     _library.define(_name + _schema)

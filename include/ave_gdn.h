@@ -329,6 +329,84 @@ typedef struct AveGateArgs {
 } AveGateArgs;
 int ave_gdn_gate_beta(const AveGateArgs* args, void* stream);
 
+/* Linear attention with a decay for each head, without the delta rule's correction:
+ *   M <- exp(g_t) M + k_t v_t^T,   o_t = scale * M^T q_t,
+ * in the layouts of the recurrences above, for dk and dv of 64 or 128 each.  g (the decay's logarithm) is fp32 [B,T,Hv], or one
+ * number a head with both strides zero, or null (no decay).  g is meant to be <= 0: minus infinity empties the state (values below
+ * -1e6 are taken as -1e6, whose exponential is zero too); positive values let it grow. */
+typedef struct AveLinearArgs {
+  uint32_t struct_size;
+  uint32_t flags;             /* 0 */
+  const void* q;              /* bf16 */
+  const void* k;              /* bf16 */
+  const void* v;              /* bf16 */
+  const float* g;             /* optional */
+  void* o;                    /* bf16 */
+  const float* initial_state; /* optional (zero state when null) */
+  float* final_state;         /* optional (not written when null); may be initial_state */
+  const int32_t* cu_seqlens;    /* optional int32 [n_seqs+1]; requires B == 1 */
+  const int32_t* state_indices; /* optional int32 [n_seqs], as in AveGdnArgs */
+  uint32_t* status;           /* optional device status word */
+  void* workspace;            /* prefill only: ave_linear_prefill_workspace_bytes(), 16-byte aligned */
+  uint64_t workspace_bytes;
+  int32_t B, T, Hk, Hv, dk, dv;
+  int32_t n_seqs;             /* B when cu_seqlens is null */
+  int32_t num_slots;          /* tiles in the state arrays; n_seqs when state_indices is null */
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  int64_t k_stride_b, k_stride_t, k_stride_h;
+  int64_t v_stride_b, v_stride_t, v_stride_h;
+  int64_t o_stride_b, o_stride_t, o_stride_h;
+  int64_t g_stride_b, g_stride_t; /* head stride 1 */
+  float scale;
+  float reserved0;
+} AveLinearArgs;
+/* Whole sequences, dense [B,T] or packed via cu_seqlens.  A packed batch whose offsets are not monotone inside [0, T] is skipped as a
+ * whole (AVE_GDN_DEV_BAD_SEQLEN); rows behind the last offset are left as they were. */
+int ave_linear_chunk_prefill(const AveLinearArgs* args, void* stream);
+size_t ave_linear_prefill_workspace_bytes(const AveLinearArgs* args);
+/* Token by token; T == 1 with state_indices is the continuous-batching decode step.  A sequence with bad offsets is skipped. */
+int ave_linear_decode_step(const AveLinearArgs* args, void* stream);
+
+/* y = (x - mean) * rstd * weight + bias over rows of n elements, 1 <= n <= 32768, rstd = 1 / sqrt(var + eps). */
+#define AVE_DTYPE_BF16 0
+#define AVE_DTYPE_FP16 1
+#define AVE_DTYPE_FP32 2
+typedef struct AveLayerNormArgs {
+  uint32_t struct_size;
+  uint32_t flags;       /* 0 */
+  const void* x;        /* [rows, n], row stride x_stride elements */
+  const void* weight;   /* [n] of w_dtype, optional */
+  const void* bias;     /* [n] of w_dtype, optional, only with weight */
+  void* y;              /* [rows, n] of x_dtype, row stride y_stride */
+  float* mean;          /* fp32 [rows], optional */
+  float* rstd;          /* fp32 [rows], optional */
+  int64_t rows, n, x_stride, y_stride;
+  int32_t x_dtype, w_dtype; /* w_dtype: x_dtype or AVE_DTYPE_FP32 */
+  float eps;
+  float reserved0;
+} AveLayerNormArgs;
+int ave_layer_norm(const AveLayerNormArgs* args, void* stream);
+
+/* Its gradients.  d_weight and d_bias are sums over the rows, formed in fp32 in a fixed order and rounded once. */
+typedef struct AveLayerNormBwdArgs {
+  uint32_t struct_size;
+  uint32_t flags;         /* 0 */
+  const void* d_y;        /* [rows, n] of x_dtype, row stride dy_stride */
+  const void* x;          /* [rows, n], row stride x_stride */
+  const float* mean;      /* fp32 [rows] */
+  const float* rstd;      /* fp32 [rows] */
+  const void* weight;     /* [n] of w_dtype, optional */
+  void* d_x;              /* [rows, n] of x_dtype, row stride dx_stride */
+  void* d_weight;         /* [n] of w_dtype, optional */
+  void* d_bias;           /* [n] of w_dtype, optional */
+  void* workspace;        /* ave_layer_norm_backward_workspace_bytes(), 16-byte aligned; needed with d_weight or d_bias */
+  uint64_t workspace_bytes;
+  int64_t rows, n, dy_stride, x_stride, dx_stride;
+  int32_t x_dtype, w_dtype;
+} AveLayerNormBwdArgs;
+int ave_layer_norm_backward(const AveLayerNormBwdArgs* args, void* stream);
+size_t ave_layer_norm_backward_workspace_bytes(const AveLayerNormBwdArgs* args);
+
 int ave_gdn_abi_version(void);
 const char* ave_gdn_status_string(int status);
 /* cudaError_t of the most recent failing CUDA call made by this thread through the library (0 if none). */
