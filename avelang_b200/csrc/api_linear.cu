@@ -4,6 +4,8 @@
 
 namespace ave {
 int launch_linear_decode(const AveLinearArgs& a, cudaStream_t stream);
+int launch_linear_prefill(const AveLinearArgs& a, cudaStream_t stream);
+size_t linear_prefill_workspace_bytes(const AveLinearArgs& a);
 int64_t layer_norm_max_n();
 int launch_layer_norm(const AveLayerNormArgs& a, cudaStream_t stream);
 size_t layer_norm_backward_workspace_bytes(const AveLayerNormBwdArgs& a);
@@ -50,15 +52,18 @@ using namespace ave;
 extern "C" {
 
 size_t ave_linear_prefill_workspace_bytes(const AveLinearArgs* a) {
-  if (validate_linear(a) != AVE_GDN_OK) return 0;
-  return 0;
+  if (validate_linear(a) != AVE_GDN_OK || nothing_to_do(*a)) return 0;
+  return linear_prefill_workspace_bytes(*a);
 }
 
 int ave_linear_chunk_prefill(const AveLinearArgs* a, void* stream) {
   const int rc = validate_linear(a);
   if (rc != AVE_GDN_OK) return rc;
   if (nothing_to_do(*a)) return AVE_GDN_OK;
-  return launch_linear_decode(*a, reinterpret_cast<cudaStream_t>(stream));
+  const size_t need = linear_prefill_workspace_bytes(*a);
+  if (need > 0 && (a->workspace == nullptr || !aligned16(a->workspace))) return AVE_GDN_INVALID_ARGUMENT;
+  if (a->workspace_bytes < need) return AVE_GDN_WORKSPACE_TOO_SMALL;
+  return launch_linear_prefill(*a, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int ave_linear_decode_step(const AveLinearArgs* a, void* stream) {

@@ -1,0 +1,106 @@
+// Host side of the scans of linear attention: how a batch is cut into segments, tensor maps, launches.
+#pragma once
+#include <atomic>
+
+#include "linear_scan.cuh"
+
+namespace ave {
+namespace {
+namespace lin {
+
+constexpr int MAX_DEVICES = 64;
+
+// One CTA walks a segment of one (sequence, value head), a chunk in about the time `1`.  Whole sequences need one pass; segments need their own
+// increments first (a pass that reads Y and W alone), so they pay where there are too few sequences and heads for the SMs, or where one sequence is so
+// long that the others wait for it.  The lengths of packed sequences are not known here: the longest is taken to be four times the mean.
+inline Plan plan_of(int B, int64_t T, int n_seqs, bool packed, int heads) {
+  constexpr double SMS = 148, STATES = 0.6, FIXED = 8.0;  // a chunk of the first pass, and its launches, in chunks of the scan
+  const double chunks = (double)((T * B + C - 1) / C);
+  const double longest = packed ? (n_seqs > 1 ? fmin((double)T, 4.0 * T / n_seqs) : (double)T) / C : (double)((T + C - 1) / C);
+  auto pass = [&](double units, double each) {  // units of about `each` chunks
+    const double waves = units / SMS;
+    return packed ? waves * each + 0.5 * each : (double)(int64_t)(waves + 0.999999) * each;
+  };
+  const double seqs = packed ? (double)n_seqs : (double)B;
+  double best = packed ? fmax(chunks * heads / SMS, longest) + 0.25 * longest : pass(seqs * heads, longest);
+  int64_t len = 0;
+  for (int parts = 2; parts <= 256; ++parts) {
+    const int64_t each = (int64_t)((longest + parts - 1) / parts);
+    if (each < 4 || each * (parts - 1) >= longest + each) continue;
+    const double units = packed ? chunks / (double)each * heads : seqs * heads * (double)(((int64_t)longest + each - 1) / each);
+    const double t = pass(units, (double)each) + STATES * pass(units * (parts - 1) / parts, (double)each) + FIXED + 0.15 * parts;
+    if (t < 0.95 * best) { best = t; len = each * C; }
+  }
+  Plan p;
+  p.cut = len > 0;
+  p.len = p.cut ? (int)len : 1 << 30;
+  p.slots = p.cut ? T * B / len + n_seqs + 1 : n_seqs;
+  return p;
+}
+
+inline size_t state_bytes(const Plan& p, int heads, int dk, int dv) {  // increments and entering states, and the segments' decays
+  return p.cut ? (size_t)p.slots * heads * ((size_t)dk * dv * 4) + (((size_t)p.slots * heads * 4 + 255) & ~(size_t)255) : 0;
+}
+inline void place_states(Args& a, void* ws, int dk, int dv) {
+  a.seg_state = reinterpret_cast<float*>(ws);
+  a.seg_decay = a.seg_state + (size_t)a.plan.slots * a.Hv * dk * dv;
+}
+
+// 64 features of 64 tokens of a [B, T, heads, d] tensor
+inline int operand_map(CUtensorMap* m, const void* p, int d, int heads, int B, int T, int64_t sb, int64_t st, int64_t sh) {
+  const uint32_t box[4] = {64, 1, 64, 1};
+  const uint64_t dims[4] = {(uint64_t)d, (uint64_t)heads, (uint64_t)T, (uint64_t)B};
+  const uint64_t str[4] = {2, (uint64_t)(heads > 1 ? sh : d) * 2, (uint64_t)(T > 1 ? st : d) * 2, (uint64_t)(B > 1 ? sb : d) * 2};
+  return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// 32 features of 64 tokens of the result; where its layout has no map, rows leave by 16-byte stores
+inline bool result_map(CUtensorMap* m, void* p, int d, int heads, int B, int T, int64_t sb, int64_t st, int64_t sh) {
+  const uint32_t box[4] = {32, 1, 64, 1};
+  const uint64_t dims[4] = {(uint64_t)d, (uint64_t)heads, (uint64_t)T, (uint64_t)B};
+  const uint64_t str[4] = {2, (uint64_t)(heads > 1 ? sh : d) * 2, (uint64_t)(T > 1 ? st : d) * 2, (uint64_t)(B > 1 ? sb : d) * 2};
+  const int last_error = g_last_cuda_error;
+  const bool ok = make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_64B) == AVE_GDN_OK;
+  if (!ok) g_last_cuda_error = last_error;
+  return ok;
+}
+
+// The register split of the roles counts on the registers that the kernel is launched with.
+template <int DK, int DV, bool kRev, bool kState, bool kGrad>
+int launch_scan(const Args& a, const Maps& maps, cudaStream_t stream) {
+  auto* kernel = scan_kernel<DK, DV, kRev, kState, kGrad>;
+  constexpr int smem = Cfg<kState, kGrad>::SMEM;
+  static std::atomic<bool> ready[MAX_DEVICES];
+  int dev = 0;
+  AVE_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= MAX_DEVICES) return AVE_GDN_UNSUPPORTED;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    cudaFuncAttributes at;
+    AVE_CUDA_TRY(cudaFuncGetAttributes(&at, kernel));
+    if (at.numRegs != REGS_LAUNCH) return cuda_fail(cudaErrorInvalidKernelImage);
+    AVE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ready[dev].store(true, std::memory_order_release);
+  }
+  const int64_t grid = a.plan.slots * a.Hv;
+  if (grid > 0x7fffffff) return AVE_GDN_UNSUPPORTED;
+  AVE_CUDA_TRY(launch_after(kernel, (unsigned)grid, THREADS, smem, stream, a, maps));
+  return AVE_GDN_OK;
+}
+template <int DK, int DV, bool kRev>
+int launch_chain(const Args& a, cudaStream_t stream) {
+  const int64_t grid = (int64_t)a.n_seqs * a.Hv * (DK * DV / 1024);
+  if (grid > 0x7fffffff) return AVE_GDN_UNSUPPORTED;
+  AVE_CUDA_TRY(launch_after(chain_kernel<DK, DV, kRev>, (unsigned)grid, 256, 0, stream, a));
+  return AVE_GDN_OK;
+}
+
+template <class F>
+int by_dims(int dk, int dv, F f) {
+  if (dk == 128) return dv == 128 ? f(std::integral_constant<int, 128>(), std::integral_constant<int, 128>())
+                                  : f(std::integral_constant<int, 128>(), std::integral_constant<int, 64>());
+  return dv == 128 ? f(std::integral_constant<int, 64>(), std::integral_constant<int, 128>())
+                   : f(std::integral_constant<int, 64>(), std::integral_constant<int, 64>());
+}
+
+}  // namespace lin
+}  // namespace
+}  // namespace ave
