@@ -92,6 +92,16 @@ class LinearArgs(ctypes.Structure):
                 + [("g_stride_b", I64), ("g_stride_t", I64), ("scale", F32), ("reserved0", F32)])
 
 
+class LinearBwdArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", U32), ("flags", U32)]
+                + [(n, P) for n in ("q", "k", "v", "g", "d_o", "initial_state", "d_final_state", "cu_seqlens", "d_q", "d_k", "d_v", "d_g",
+                                    "d_initial_state", "status", "workspace")]
+                + [("workspace_bytes", U64)]
+                + [(n, I32) for n in ("B", "T", "Hk", "Hv", "dk", "dv", "n_seqs", "reserved0")]
+                + [(f"{t}_stride_{d}", I64) for t in ("q", "k", "v", "do") for d in ("b", "t", "h")]
+                + [("g_stride_b", I64), ("g_stride_t", I64), ("scale", F32), ("reserved1", F32)])
+
+
 class LayerNormArgs(ctypes.Structure):
     _fields_ = ([("struct_size", U32), ("flags", U32)] + [(n, P) for n in ("x", "weight", "bias", "y", "mean", "rstd")]
                 + [(n, I64) for n in ("rows", "n", "x_stride", "y_stride")]
@@ -127,6 +137,8 @@ SYMBOLS = {
     "ave_linear_chunk_prefill": (ctypes.c_int, [ctypes.POINTER(LinearArgs), P]),
     "ave_linear_prefill_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LinearArgs)]),
     "ave_linear_decode_step": (ctypes.c_int, [ctypes.POINTER(LinearArgs), P]),
+    "ave_linear_backward": (ctypes.c_int, [ctypes.POINTER(LinearBwdArgs), P]),
+    "ave_linear_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LinearBwdArgs)]),
     "ave_layer_norm": (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), P]),
     "ave_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(LayerNormBwdArgs), P]),
     "ave_layer_norm_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LayerNormBwdArgs)]),

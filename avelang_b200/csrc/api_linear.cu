@@ -6,6 +6,8 @@ namespace ave {
 int launch_linear_decode(const AveLinearArgs& a, cudaStream_t stream);
 int launch_linear_prefill(const AveLinearArgs& a, cudaStream_t stream);
 size_t linear_prefill_workspace_bytes(const AveLinearArgs& a);
+int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream);
+size_t linear_backward_workspace_bytes(const AveLinearBwdArgs& a);
 int64_t layer_norm_max_n();
 int launch_layer_norm(const AveLayerNormArgs& a, cudaStream_t stream);
 size_t layer_norm_backward_workspace_bytes(const AveLayerNormBwdArgs& a);
@@ -41,6 +43,21 @@ int validate_linear(const AveLinearArgs* a) {
   return AVE_GDN_OK;
 }
 
+int validate_linear_bwd(const AveLinearBwdArgs* a) {
+  const int rc = validate_shape(a);
+  if (rc != AVE_GDN_OK) return rc;
+  if (nothing_to_do(*a)) return AVE_GDN_OK;
+  if (!a->q || !a->k || !a->v || !a->d_o || !a->d_q || !a->d_k || !a->d_v || (a->g && !a->d_g) || (a->initial_state && !a->d_initial_state)) return AVE_GDN_INVALID_ARGUMENT;
+  if ((a->flags & AVE_LINEAR_FLAG_HEAD_GATE) && (a->g_stride_b != 0 || a->g_stride_t != 0)) return AVE_GDN_INVALID_ARGUMENT;
+  if (!rows_on16(a->q, a->q_stride_b, a->q_stride_t, a->q_stride_h) || !rows_on16(a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h) ||
+      !rows_on16(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h) || !rows_on16(a->d_o, a->do_stride_b, a->do_stride_t, a->do_stride_h))
+    return AVE_GDN_MISALIGNED;
+  if (!aligned16(a->d_q) || !aligned16(a->d_k) || !aligned16(a->d_v) || !aligned16(a->initial_state) || !aligned16(a->d_final_state) || !aligned16(a->d_initial_state) ||
+      ((reinterpret_cast<uintptr_t>(a->g) | reinterpret_cast<uintptr_t>(a->d_g)) & 3u))
+    return AVE_GDN_MISALIGNED;
+  return AVE_GDN_OK;
+}
+
 bool dtype_ok(int x, int w) { return x >= AVE_DTYPE_BF16 && x <= AVE_DTYPE_FP32 && (w == x || w == AVE_DTYPE_FP32); }
 bool on_elem(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == AVE_DTYPE_FP32 ? 3u : 1u)) == 0; }
 
@@ -71,6 +88,21 @@ int ave_linear_decode_step(const AveLinearArgs* a, void* stream) {
   if (rc != AVE_GDN_OK) return rc;
   if (nothing_to_do(*a)) return AVE_GDN_OK;
   return launch_linear_decode(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t ave_linear_backward_workspace_bytes(const AveLinearBwdArgs* a) {
+  if (validate_linear_bwd(a) != AVE_GDN_OK || nothing_to_do(*a)) return 0;
+  return linear_backward_workspace_bytes(*a);
+}
+
+int ave_linear_backward(const AveLinearBwdArgs* a, void* stream) {
+  const int rc = validate_linear_bwd(a);
+  if (rc != AVE_GDN_OK) return rc;
+  if (nothing_to_do(*a)) return AVE_GDN_OK;
+  const size_t need = linear_backward_workspace_bytes(*a);
+  if (need > 0 && (a->workspace == nullptr || !aligned16(a->workspace))) return AVE_GDN_INVALID_ARGUMENT;
+  if (a->workspace_bytes < need) return AVE_GDN_WORKSPACE_TOO_SMALL;
+  return launch_linear_backward(*a, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int ave_layer_norm(const AveLayerNormArgs* a, void* stream) {

@@ -94,6 +94,8 @@ struct Api {
   decltype(&ave_linear_chunk_prefill) linear_prefill = nullptr;
   decltype(&ave_linear_prefill_workspace_bytes) linear_prefill_workspace_bytes = nullptr;
   decltype(&ave_linear_decode_step) linear_decode = nullptr;
+  decltype(&ave_linear_backward) linear_backward = nullptr;
+  decltype(&ave_linear_backward_workspace_bytes) linear_backward_workspace_bytes = nullptr;
   decltype(&ave_layer_norm) layer_norm = nullptr;
   decltype(&ave_layer_norm_backward) layer_norm_backward = nullptr;
   decltype(&ave_layer_norm_backward_workspace_bytes) layer_norm_backward_workspace_bytes = nullptr;
@@ -695,6 +697,32 @@ void op_linear_decode(const Tensor& q, const Tensor& k, const Tensor& v, const O
   check(launch([&] { return api.linear_decode(&a, launch.stream); }), "fused_recurrent_linear_attention");
 }
 
+// dq, dk, dv, dg, d_initial_state: contiguous
+void op_linear_backward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g_in, const Tensor& d_o, double scale, const OptTensor& initial_state,
+                        const OptTensor& d_final_state, const OptTensor& cu_seqlens, const Tensor& dq, const Tensor& dk, const Tensor& dv, const OptTensor& dg,
+                        const OptTensor& d_initial_state) {
+  loaded();
+  const Tensor *g = some(g_in), *cu = some(cu_seqlens);
+  AveLinearBwdArgs a{};
+  a.struct_size = sizeof(a);
+  a.flags = g != nullptr && g->dim() == 1 ? AVE_LINEAR_FLAG_HEAD_GATE : 0;
+  a.q = ptr(&q); a.k = ptr(&k); a.v = ptr(&v); a.g = ptr_as<float>(g); a.d_o = ptr(&d_o);
+  a.initial_state = ptr_as<float>(some(initial_state)); a.d_final_state = ptr_as<float>(some(d_final_state)); a.cu_seqlens = ptr_as<int32_t>(cu);
+  a.d_q = ptr_as<void>(&dq); a.d_k = ptr_as<void>(&dk); a.d_v = ptr_as<void>(&dv);
+  a.d_g = ptr_as<float>(some(dg)); a.d_initial_state = ptr_as<float>(some(d_initial_state));
+  a.status = reinterpret_cast<uint32_t*>(status_word(q.device()).data_ptr());
+  a.B = (int32_t)q.size(0); a.T = (int32_t)q.size(1); a.Hk = (int32_t)q.size(2); a.Hv = (int32_t)v.size(2);
+  a.dk = (int32_t)q.size(3); a.dv = (int32_t)v.size(3);
+  a.n_seqs = (int32_t)n_sequences(q, cu);
+  STRIDES4(a, q, q); STRIDES4(a, k, k); STRIDES4(a, v, v); STRIDES4(a, do, d_o);
+  if (g != nullptr && g->dim() == 3) { a.g_stride_b = g->stride(0); a.g_stride_t = g->stride(1); }
+  a.scale = (float)scale;
+  Launch launch(q);
+  const Scratch ws(q, launch.stream, api.linear_backward_workspace_bytes(&a));
+  a.workspace = ws.data(); a.workspace_bytes = ws.size();
+  check(launch([&] { return api.linear_backward(&a, launch.stream); }), "linear_attention_backward");
+}
+
 int32_t dtype_code(const Tensor& t, const char* name) {
   switch (t.scalar_type()) {
     case at::kBFloat16: return AVE_DTYPE_BF16;
@@ -738,6 +766,7 @@ void op_layer_norm_backward(const Tensor& d_y, const Tensor& x, const Tensor& me
   X("gated_rmsnorm", op_rmsnorm) X("conv1d_silu", op_conv) X("conv1d_update", op_conv_update) X("gate_beta", op_gate)          \
   X("gemm_bf16_nt", op_gemm) X("recurrent_backward", op_backward)                                                           \
   X("linear_prefill", op_linear_prefill) X("linear_decode", op_linear_decode)                                               \
+  X("linear_backward", op_linear_backward)                                                                                  \
   X("layer_norm", op_layer_norm) X("layer_norm_backward", op_layer_norm_backward)
 TORCH_LIBRARY_IMPL(avelang_gdn, CUDA, m) {
 #define CUDA_KERNEL(name, f) m.impl(name, f);
@@ -1061,6 +1090,33 @@ PyObject* linear_forward(PyObject* const* p) {
   return wrap_pair(o, final);
 }
 
+// linear_backward(q, k, v, g, d_o, scale, initial_state, d_final_state, cu_seqlens) -> (dq, dk, dv, dg or None, ds0 or None)
+PyObject* linear_backward(PyObject* const* p) {
+  const Tensor &q = tensor(p[0], "q"), &k = tensor(p[1], "k"), &v = tensor(p[2], "v"), &d_o = tensor(p[4], "d_o");
+  const Tensor *g = opt_tensor(p[3], "g"), *s0 = opt_tensor(p[6], "initial_state"), *ds = opt_tensor(p[7], "d_final_state"), *cu = opt_tensor(p[8], "cu_seqlens");
+  const Shape s = check_linear(q, k, v, g, cu);
+  REQ(d_o.scalar_type() == at::kBFloat16 && d_o.sizes() == v.sizes() && d_o.device() == q.device() && d_o.stride(3) == 1,
+      "d_o must be a bf16 tensor of shape ", shape_of(v.sizes()), " on ", q.device());
+  const std::pair<const char*, const Tensor*> states[] = {{"initial_state", s0}, {"d_final_state", ds}};
+  for (const auto& [name, t] : states)
+    if (t != nullptr)
+      REQ(t->scalar_type() == at::kFloat && t->dim() == 4 && t->size(0) == s.n && t->size(1) == s.Hv && t->size(2) == s.dk &&
+              t->size(3) == s.dv && t->is_contiguous() && t->device() == q.device(),
+          name, " must be a contiguous fp32 tensor (", s.n, ", ", s.Hv, ", ", s.dk, ", ", s.dv, ") on ", q.device());
+  const Tensor dq = empty(q.sizes(), at::kBFloat16, q), dk = empty(q.sizes(), at::kBFloat16, q), dv = empty(v.sizes(), at::kBFloat16, v);
+  Tensor dg, ds0;
+  if (g != nullptr) dg = empty(g->sizes(), at::kFloat, q);
+  if (s0 != nullptr) ds0 = empty({s.n, s.Hv, s.dk, s.dv}, at::kFloat, q);
+  if (s.B * s.T == 0 || s.n == 0) {  // no kernel runs: the gradient of the states passes through, everything else is zero
+    const Tensor* grads[] = {&dq, &dk, &dv, &dg};
+    for (const Tensor* t : grads) if (t->defined()) t->zero_();
+    if (ds0.defined()) { if (ds != nullptr) ds0.copy_(*ds); else ds0.zero_(); }
+  }
+  call<op_linear_backward>("avelang_gdn::linear_backward", spread(q), spread(k), spread(v), opt(g), spread(d_o), scale_or(p[5], s.dk), opt(s0), opt(ds), opt(cu), dq, dk, dv,
+                           opt(dg), opt(ds0));
+  return wrap_all({&dq, &dk, &dv, &dg, &ds0});
+}
+
 // The rows of x as [rows, n]
 Tensor as_rows(const Tensor& x) { return x.dim() == 2 ? x : x.reshape({x.numel() / x.size(-1), x.size(-1)}); }
 void check_norm_input(const Tensor& x, const Tensor* w, const Tensor* b) {
@@ -1157,6 +1213,8 @@ PyObject* bind(PyObject* const* p) {
   RESOLVE(linear_prefill, ave_linear_chunk_prefill);
   RESOLVE(linear_prefill_workspace_bytes, ave_linear_prefill_workspace_bytes);
   RESOLVE(linear_decode, ave_linear_decode_step);
+  RESOLVE(linear_backward, ave_linear_backward);
+  RESOLVE(linear_backward_workspace_bytes, ave_linear_backward_workspace_bytes);
   RESOLVE(layer_norm, ave_layer_norm);
   RESOLVE(layer_norm_backward, ave_layer_norm_backward);
   RESOLVE(layer_norm_backward_workspace_bytes, ave_layer_norm_backward_workspace_bytes);
@@ -1194,6 +1252,7 @@ PyMethodDef methods[] = {
     ENTRY("backward", backward, 10),
     ENTRY("linear_prefill", linear_forward<true>, 12),
     ENTRY("linear_decode", linear_forward<false>, 12),
+    ENTRY("linear_backward", linear_backward, 9),
     ENTRY("layer_norm", layer_norm, 6),
     ENTRY("layer_norm_backward", layer_norm_backward, 5),
     {nullptr, nullptr, 0, nullptr}};

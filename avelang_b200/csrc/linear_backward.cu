@@ -1,0 +1,291 @@
+// Gradients of linear attention with a decay for each head.  With R_t the gradient of the state after token t,
+//     R_t = scale q_t do_t^T + e^{g_{t+1}} R_{t+1},
+//     dq_t = scale S_t do_t,   dk_t = R_t v_t,   dv_t = R_t^T k_t
+// are scans of the forward pass's form: (do, v, k) forwards in time, (v, do, q) and (k, q, do) backwards.  The gradient of g_t is the sum over all pairs
+// s < t <= u of m_us = e^{G_u - G_s} scale (q_u.k_s)(do_u.v_s) (the initial state counts as a token in front of all others, the final state's gradient as one
+// behind them), so that with the strictly causal parts A_t = sum over s < t of m_ts and B_t = sum over u > t of m_ut
+//     dg_{t+1} = dg_t - A_t + B_t,
+// and dg at the first token of a segment is the product <S, R> of the state and the gradient that meet there.  A and B come with the scans for dq
+// and dk: inside a chunk from P' and a second product q k^T in 32 bits, across chunks as q_t . (e_t S do_t) and k_t . (e_t R v_t) in front of the
+// diagonal's term; the shorter formula with q.dq - k.dk would take that term, which is far larger where decays are strong, from both sides.
+#include "linear_scan_host.cuh"
+
+namespace ave {
+namespace {
+namespace lin {
+
+// The value heads of a key head, summed: out[row][hk][d] = sum over r of part[row][hk rep + r][d]; eight features a thread
+__global__ void __launch_bounds__(256) sum_heads_kernel(const float* part, __nv_bfloat16* out, int64_t pieces, int d8, int hk, int rep) {
+  pdl_wait();
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
+    const int64_t head = i / d8;  // row * hk + key head
+    const float* src = part + (head * rep * d8 + i % d8) * 8;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+    for (int r = 0; r < rep; ++r) {
+      const float4 p = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)r * d8 * 8)), q = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)r * d8 * 8 + 4));
+      x.x += p.x; x.y += p.y; x.z += p.z; x.w += p.w;
+      y.x += q.x; y.y += q.y; y.z += q.z; y.w += q.w;
+    }
+    *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w), pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+  }
+}
+
+struct GateGrad {
+  const float *inter_a, *intra_a, *inter_b, *intra_b;  // of the scans for dq and dk
+  int parts;                 // of inter: dk / 32
+  const float *seg_s, *seg_r;  // states that enter the segments, from the front and from behind
+  const float *s0, *ds0;     // null: no initial state
+  float* dg;                 // [B, T, Hv], or null
+  float* sums;               // [slot][Hv]: sums over the segment's tokens, or null
+  int dk, dv;
+};
+
+__device__ __forceinline__ double block_sum(double x, double* sm) {  // 256 threads, all get it
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = x;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += sm[w];
+  return s;
+}
+
+// One CTA a segment and head: the running sum of B - A from the segment's first token, in 64 bits.
+__global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const GateGrad q) {
+  __shared__ double sm[8], wsum[8];
+  pdl_wait();
+  if (!offsets_fit(a, false)) return;
+  const int h = blockIdx.x % a.Hv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t slot = blockIdx.x / a.Hv;
+  const Seg seg = seg_of_slot(a, slot);
+  if (!seg.ok || seg.len == 0) {
+    if (q.sums != nullptr && tid == 0) q.sums[slot * a.Hv + h] = 0.f;
+    return;
+  }
+  const int64_t size = (int64_t)q.dk * q.dv;
+  const float *x = nullptr, *y = nullptr;
+  if (seg.j > 0) {
+    x = q.seg_s + (slot * a.Hv + h) * size;
+    y = q.seg_r + ((slot - 1) * a.Hv + h) * size;
+  } else if (q.s0 != nullptr) {
+    x = q.s0 + ((int64_t)seg.n * a.Hv + h) * size;
+    y = q.ds0 + ((int64_t)seg.n * a.Hv + h) * size;
+  }
+  double dot = 0.0;
+  if (x != nullptr)
+    for (int i = tid * 4; i < size; i += 1024) {
+      const float4 u = *reinterpret_cast<const float4*>(x + i), v = *reinterpret_cast<const float4*>(y + i);
+      dot += ((double)u.x * v.x + (double)u.y * v.y) + ((double)u.z * v.z + (double)u.w * v.w);
+    }
+  double run = block_sum(dot, sm), total = 0.0;  // dg of the next token
+  const int64_t base = ((int64_t)h * a.B + seg.b) * a.T + seg.t0, plane = (int64_t)a.Hv * a.B * a.T;
+  for (int t0 = 0; t0 < seg.len; t0 += 256) {
+    const int t = t0 + tid;
+    double d = 0.0;
+    if (t < seg.len) {
+      float ia = 0.f, ib = 0.f;
+      for (int p = 0; p < q.parts; ++p) { ia += q.inter_a[p * plane + base + t]; ib += q.inter_b[p * plane + base + t]; }
+      d = ((double)ib - (double)ia) + ((double)q.intra_b[base + t] - (double)q.intra_a[base + t]);
+    }
+    double inc = d;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    __syncthreads();
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    double before = 0.0, whole = 0.0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) before += wsum[w];
+      whole += wsum[w];
+    }
+    const double mine = run + before + inc - d;
+    if (t < seg.len) {
+      if (q.dg != nullptr) q.dg[((int64_t)seg.b * a.T + seg.t0 + t) * a.Hv + h] = (float)mine;
+      total += mine;
+    }
+    run += whole;
+  }
+  if (q.sums != nullptr) {
+    total = block_sum(total, sm);
+    if (tid == 0) q.sums[slot * a.Hv + h] = (float)total;
+  }
+}
+// One decay a head: its gradient is the sum over all segments, in order
+__global__ void __launch_bounds__(256) head_gate_grad_kernel(const Args a, const float* sums, float* dg) {
+  __shared__ double sm[8];
+  pdl_wait();
+  if (!offsets_fit(a, false)) return;
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < a.plan.slots; i += 256) s += (double)sums[i * a.Hv + blockIdx.x];
+  s = block_sum(s, sm);
+  if (threadIdx.x == 0) dg[blockIdx.x] = (float)s;
+}
+
+// Rows of a packed batch in front of its first offset and behind its last belong to no sequence: their gradients are zero.
+__global__ void __launch_bounds__(128) clear_outside_kernel(const Args a, __nv_bfloat16* dq, __nv_bfloat16* dk, __nv_bfloat16* dv, float* dg, int wk, int wv) {
+  pdl_wait();
+  if (!offsets_fit(a, false)) return;
+  const int lo = a.n_seqs > 0 ? a.cu_seqlens[0] : 0, hi = a.n_seqs > 0 ? a.cu_seqlens[a.n_seqs] : 0;
+  const int outside = lo + (a.T - hi);
+  for (int r = blockIdx.x; r < outside; r += gridDim.x) {
+    const int64_t row = r < lo ? r : hi + (r - lo);
+    for (int i = threadIdx.x; i < wk / 8; i += 128) {
+      *reinterpret_cast<uint4*>(dq + row * wk + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(dk + row * wk + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    for (int i = threadIdx.x; i < wv / 8; i += 128) *reinterpret_cast<uint4*>(dv + row * wv + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
+    if (dg != nullptr)
+      for (int i = threadIdx.x; i < a.Hv; i += 128) dg[row * a.Hv + i] = 0.f;
+  }
+}
+
+struct Layout {
+  Plan plan;
+  size_t s, s_decay, r, r_decay, part, inter_a, inter_b, intra_a, intra_b, sums, bytes;
+};
+Layout layout_of(const AveLinearBwdArgs& a) {
+  Layout l{};
+  l.plan = plan_of(a.B, a.T, a.n_seqs, a.cu_seqlens != nullptr, a.Hv);
+  const size_t rows = (size_t)a.B * a.T * a.Hv;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return p;
+  };
+  if (l.plan.cut) {
+    const size_t tiles = (size_t)l.plan.slots * a.Hv;
+    l.s = take(tiles * a.dk * a.dv * 4); l.s_decay = take(tiles * 4);
+    l.r = take(tiles * a.dk * a.dv * 4); l.r_decay = take(tiles * 4);
+  }
+  if (a.Hv > a.Hk) l.part = take(rows * a.dk * 4);
+  if (a.g != nullptr) {
+    l.inter_a = take(rows * (a.dk / 32) * 4); l.inter_b = take(rows * (a.dk / 32) * 4);
+    l.intra_a = take(rows * 4); l.intra_b = take(rows * 4);
+    l.sums = take((size_t)l.plan.slots * a.Hv * 4);
+  }
+  l.bytes = at;
+  return l;
+}
+
+}  // namespace lin
+}  // namespace
+
+size_t linear_backward_workspace_bytes(const AveLinearBwdArgs& a) { return lin::layout_of(a).bytes; }
+
+int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
+  const lin::Layout l = lin::layout_of(a);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(a.workspace);
+  auto f32 = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
+  const int rep = a.Hv / a.Hk;
+  const bool grad = a.g != nullptr;
+  int rc;
+  CUtensorMap mq, mk, mv, mo;
+  if ((rc = lin::operand_map(&mq, a.q, a.dk, a.Hk, a.B, a.T, a.q_stride_b, a.q_stride_t, a.q_stride_h))) return rc;
+  if ((rc = lin::operand_map(&mk, a.k, a.dk, a.Hk, a.B, a.T, a.k_stride_b, a.k_stride_t, a.k_stride_h))) return rc;
+  if ((rc = lin::operand_map(&mv, a.v, a.dv, a.Hv, a.B, a.T, a.v_stride_b, a.v_stride_t, a.v_stride_h))) return rc;
+  if ((rc = lin::operand_map(&mo, a.d_o, a.dv, a.Hv, a.B, a.T, a.do_stride_b, a.do_stride_t, a.do_stride_h))) return rc;
+  lin::Args base{};
+  base.cu_seqlens = a.cu_seqlens; base.status = a.status;
+  base.B = a.B; base.T = a.T; base.Hv = a.Hv; base.n_seqs = a.n_seqs; base.num_slots = a.n_seqs;
+  base.g = a.g; base.g_stride_b = a.g_stride_b; base.g_stride_t = a.g_stride_t;
+  base.plan = l.plan;
+  lin::Args fwd = base, rev = base;  // states from the front, and their gradients from behind, as [dk][dv]
+  fwd.y_div = rep; fwd.w_div = 1; fwd.scale_w = 1.f;
+  fwd.state_in = a.initial_state; fwd.st_y = a.dv; fwd.st_w = 1;
+  rev.y_div = rep; rev.w_div = 1; rev.scale_w = a.scale;
+  rev.state_in = a.d_final_state; rev.st_y = a.dv; rev.st_w = 1;
+  if (l.plan.cut) {
+    fwd.seg_state = f32(l.s); fwd.seg_decay = f32(l.s_decay);
+    rev.seg_state = f32(l.r); rev.seg_decay = f32(l.r_decay);
+  }
+  // gradient of q or k: dk features of Hk heads, summed over the value heads
+  auto rows_of = [&](lin::Args& s, lin::Maps& m, void* out) {
+    s.o = out; s.o_stride_h = a.dk; s.o_stride_t = (int64_t)a.Hk * a.dk; s.o_stride_b = s.o_stride_t * a.T;
+    if (rep == 1) {
+      m.o_ok = lin::result_map(&m.o, out, a.dk, a.Hk, a.B, a.T, s.o_stride_b, s.o_stride_t, s.o_stride_h);
+      return (int)AVE_GDN_OK;
+    }
+    s.o_part = f32(l.part);
+    const uint64_t row = (uint64_t)a.Hv * a.dk * 4;
+    const uint64_t dims[4] = {(uint64_t)a.dk, (uint64_t)a.Hv, (uint64_t)a.T, (uint64_t)a.B}, str[4] = {4, (uint64_t)a.dk * 4, row, row * a.T};
+    const uint32_t box[4] = {32, 1, 64, 1};
+    return make_tmap(&m.o32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, s.o_part, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  auto sum_heads = [&](void* out) {
+    if (rep == 1) return (int)AVE_GDN_OK;
+    const int64_t pieces = (int64_t)a.B * a.T * a.Hk * (a.dk / 8), ctas = (pieces + 255) / 256;
+    AVE_CUDA_TRY(launch_after(lin::sum_heads_kernel, (unsigned)(ctas < 148 * 16 ? ctas : 148 * 16), 256, 0, stream, (const float*)f32(l.part),
+                              reinterpret_cast<__nv_bfloat16*>(out), pieces, a.dk / 8, a.Hk, rep));
+    return (int)AVE_GDN_OK;
+  };
+  rc = lin::by_dims(a.dk, a.dv, [&](auto dk, auto dv) {
+    constexpr int DK = decltype(dk)::value, DV = decltype(dv)::value;
+    int r;
+    if (l.plan.cut) {
+      lin::Maps m{};
+      m.y = mk; m.w = mv;
+      if ((r = lin::launch_scan<DK, DV, false, true, false>(fwd, m, stream))) return r;
+      m.y = mq; m.w = mo;
+      if ((r = lin::launch_scan<DK, DV, true, true, false>(rev, m, stream))) return r;
+      if ((r = lin::launch_chain<DK, DV, false>(fwd, stream))) return r;
+      if ((r = lin::launch_chain<DK, DV, true>(rev, stream))) return r;
+    }
+    {  // dv, and the gradient of the initial state
+      lin::Args s = rev;
+      lin::Maps m{};
+      s.x_div = rep; s.scale_p = a.scale; s.scale_e = 1.f;
+      s.state_out = a.d_initial_state;
+      m.x = mk; m.y = mq; m.w = mo;
+      s.o = a.d_v; s.o_stride_h = a.dv; s.o_stride_t = (int64_t)a.Hv * a.dv; s.o_stride_b = s.o_stride_t * a.T;
+      m.o_ok = lin::result_map(&m.o, a.d_v, a.dv, a.Hv, a.B, a.T, s.o_stride_b, s.o_stride_t, s.o_stride_h);
+      if ((r = lin::launch_scan<DK, DV, true, false, false>(s, m, stream))) return r;
+    }
+    {  // dq
+      lin::Args s = fwd;
+      lin::Maps m{};
+      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; s.scale_p = s.scale_e = a.scale; s.st_y = 1; s.st_w = a.dv;
+      m.x = mo; m.y = mv; m.w = mk; m.e = mq;
+      if ((r = rows_of(s, m, a.d_q))) return r;
+      if (grad) { s.inter = f32(l.inter_a); s.intra = f32(l.intra_a); }
+      r = grad ? lin::launch_scan<DV, DK, false, false, true>(s, m, stream) : lin::launch_scan<DV, DK, false, false, false>(s, m, stream);
+      if (r || (r = sum_heads(a.d_q))) return r;
+    }
+    {  // dk
+      lin::Args s = rev;
+      lin::Maps m{};
+      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; s.scale_p = a.scale; s.scale_e = 1.f; s.st_y = 1; s.st_w = a.dv;
+      m.x = mv; m.y = mo; m.w = mq; m.e = mk;
+      if ((r = rows_of(s, m, a.d_k))) return r;
+      if (grad) { s.inter = f32(l.inter_b); s.intra = f32(l.intra_b); }
+      r = grad ? lin::launch_scan<DV, DK, true, false, true>(s, m, stream) : lin::launch_scan<DV, DK, true, false, false>(s, m, stream);
+      if (r || (r = sum_heads(a.d_k))) return r;
+    }
+    return (int)AVE_GDN_OK;
+  });
+  if (rc != AVE_GDN_OK) return rc;
+  const bool by_token = grad && (a.flags & AVE_LINEAR_FLAG_HEAD_GATE) == 0;
+  if (grad) {
+    lin::GateGrad q{};
+    q.inter_a = f32(l.inter_a); q.inter_b = f32(l.inter_b); q.intra_a = f32(l.intra_a); q.intra_b = f32(l.intra_b);
+    q.parts = a.dk / 32; q.dk = a.dk; q.dv = a.dv;
+    if (l.plan.cut) { q.seg_s = f32(l.s); q.seg_r = f32(l.r); }
+    if (a.initial_state != nullptr) { q.s0 = a.initial_state; q.ds0 = a.d_initial_state; }
+    if (by_token) q.dg = a.d_g; else q.sums = f32(l.sums);
+    const int64_t grid = l.plan.slots * a.Hv;
+    AVE_CUDA_TRY(launch_after(lin::gate_grad_kernel, (unsigned)grid, 256, 0, stream, base, q));
+    if (!by_token) AVE_CUDA_TRY(launch_after(lin::head_gate_grad_kernel, (unsigned)a.Hv, 256, 0, stream, base, (const float*)q.sums, a.d_g));
+  }
+  if (a.cu_seqlens != nullptr)
+    AVE_CUDA_TRY(launch_after(lin::clear_outside_kernel, 148, 128, 0, stream, base, reinterpret_cast<__nv_bfloat16*>(a.d_q), reinterpret_cast<__nv_bfloat16*>(a.d_k),
+                              reinterpret_cast<__nv_bfloat16*>(a.d_v), by_token ? a.d_g : (float*)nullptr, a.Hk * a.dk, a.Hv * a.dv));
+  return AVE_GDN_OK;
+}
+
+}  // namespace ave

@@ -46,8 +46,8 @@ struct Args {
   int st_y, st_w;
   float* seg_state;                // [segment slot, Hv, ..] likewise
   float* seg_decay;                // [segment slot, Hv]
-  float* inter;                    // [B, T, Hv]: e_t E_t . (H^T X_t)          (gradients of g)
-  float* intra;                    // [B, T, Hv]: sum over s < t of P'_ts (E_t . W_s)
+  float* inter;                    // [dv / 32][Hv][B T]: e_t E_t . (H^T X_t), 32 features each      (for the gradient of g)
+  float* intra;                    // [Hv][B T]: sum over s < t of P'_ts (E_t . W_s)
   Plan plan;
 };
 struct Maps { CUtensorMap x, y, w, e, o, o32; bool o_ok; };
@@ -137,9 +137,8 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   uint64_t* h_read = bars + 15;    // H^T X^T accumulated
   uint64_t* o_full = bars + 16;    // both outputs accumulated, P' read
   uint64_t* o_empty = bars + 17;   // outputs drained
-  uint64_t* x_sum = bars + 18;     // partial sums of E . (H^T X) written by the four output warps
-  uint64_t* mma_end = bars + 19;   // the MMAs are complete, when a wait has expired
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* mma_end = bars + 18;   // the MMAs are complete, when a wait has expired
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -151,7 +150,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
     for (uint64_t* b : {p_full, ds_full, h_read, o_full, mma_end}) tc::mbar_init(b, 1);
     tc::mbar_init(pp_ready, 2); tc::mbar_init(yw_ready, kState ? 4 : 2);
     tc::mbar_init(ds_empty, 8); tc::mbar_init(h_ready, 8);
-    tc::mbar_init(o_empty, 4); tc::mbar_init(x_sum, 4);
+    tc::mbar_init(o_empty, 4);
     *abort_flag = 0;
     tc::fence_barrier_init();
   }
@@ -443,8 +442,6 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       const int wq = warp & 3, gr = lane >> 2, t2 = 2 * (lane & 3), r8 = lane & 7, m4 = lane >> 3;
       const uint32_t lane_addr = tm + ((uint32_t)(wq * 32) << 16);
       const bool mine = 32 * wq < DV, f32 = a.o_part != nullptr;
-      const float* red = reinterpret_cast<const float*>(smem + K::PP);
-      (void)red;
       int s = 0;
       for (int c = 0; c < n_chunks; ++c) {
         const uint32_t cp = (uint32_t)c & 1u;
@@ -455,6 +452,10 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         const uint32_t stage_s = tc::smem_u32(stage);
         const int at_tok = chunk_at(c) * C, len = min(C, seg.len - at_tok);
         const int64_t tok0 = seg.t0 + at_tok;
+        [[maybe_unused]] float xs[16];
+        if constexpr (kGrad)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) xs[i] = 0.f;
         if (mine) {
 #pragma unroll 1
           for (int hf = 0; hf < 2; ++hf) {  // 16 features
@@ -462,6 +463,22 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
             tc::tmem_ld_frags(lane_addr + ((uint32_t)hf << 20) + K::OI, oi);
             tc::tmem_ld_frags(lane_addr + ((uint32_t)hf << 20) + K::OA, oa);
             tc::tmem_ld_wait();
+            if constexpr (kGrad) {  // E's pieces in the layout of the fragments
+              const uint32_t e_s = tc::smem_u32(smem + s * K::STAGE + K::E) + (uint32_t)((wq >> 1) * HALF + (8 * (m4 >> 1) + r8) * 128 +
+                                                                                      (((4 * (wq & 1) + 2 * hf + (m4 & 1)) ^ r8) << 4));
+#pragma unroll
+              for (int g = 0; g < 8; g += 2) {
+                uint32_t e[4];
+                ldsm4t(e, e_s + 1024 * g);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                  const float2 f = bf16x2_to_float2(e[m]);
+                  const int gg = g + (m >> 1);
+                  xs[2 * gg] = fmaf(f.x, __uint_as_float(oi[4 * gg + 2 * (m & 1)]), xs[2 * gg]);
+                  xs[2 * gg + 1] = fmaf(f.y, __uint_as_float(oi[4 * gg + 2 * (m & 1) + 1]), xs[2 * gg + 1]);
+                }
+              }
+            }
 #pragma unroll
             for (int g = 0; g < 8; ++g) {
               const float2 e = *reinterpret_cast<const float2*>(gv + GV_E + 8 * g + t2);
@@ -500,6 +517,23 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(o_empty);
+        if constexpr (kGrad) {
+          // sums over the eight lanes of a token's features; lane (gr, t2 / 2) ends with the tokens 8 gr + t2, 8 gr + t2 + 1
+#pragma unroll
+          for (int w = 8; w >= 2; w >>= 1) {
+            const int mask = 2 * w;  // 16, 8, 4: bit of gr
+            const bool upper = (lane & mask) != 0;
+#pragma unroll
+            for (int i = 0; i < w; ++i) {
+              const float send = upper ? xs[i] : xs[i + w];
+              xs[i] = (upper ? xs[i + w] : xs[i]) + __shfl_xor_sync(0xffffffffu, send, mask);
+            }
+          }
+          const int t = 8 * gr + t2;
+          float* dst = a.inter + (((int64_t)wq * a.Hv + h) * a.B + seg.b) * a.T + tok0;
+          if (mine && t < len) dst[t] = gv[GV_E + t] * xs[0];
+          if (mine && t + 1 < len) dst[t + 1] = gv[GV_E + t + 1] * xs[1];
+        }
         if (mine) {
           if (len == C && (f32 || maps.o_ok)) {
             if (lane == 0) tc::tma_store_4d(f32 ? &maps.o32 : &maps.o, stage, 32 * wq, h, (int)tok0, seg.b);
@@ -576,7 +610,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(pp_ready);
         if constexpr (kGrad)
-          if (t < len) a.intra[((int64_t)seg.b * a.T + seg.t0 + at_tok + t) * a.Hv + h] = sum;
+          if (t < len) a.intra[((int64_t)h * a.B + seg.b) * a.T + seg.t0 + at_tok + t] = sum;
         if (++s == K::STAGES) { s = 0; ph ^= 1u; }
       }
     } else {

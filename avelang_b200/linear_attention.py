@@ -14,9 +14,11 @@ decay).  It is meant to be <= 0; minus infinity empties the state.
 """
 from __future__ import annotations
 
+import torch
+
 from . import _lib, torch_ops  # noqa: F401  (torch_ops declares the operators the native functions call)
 
-__all__ = ["chunk_linear_attention", "fused_recurrent_linear_attention"]
+__all__ = ["chunk_linear_attention", "fused_recurrent_linear_attention", "linear_attention_backward", "LinearAttentionFunction"]
 
 _native = _lib.host
 _lib.register_operators()
@@ -40,3 +42,31 @@ def fused_recurrent_linear_attention(q, k, v, g=None, scale=None, initial_state=
     read once from its slot of the ``initial_state`` pool and written once, in place unless ``inplace_state=False``.  A negative
     slot skips the sequence.  Returns ``(o, state)``."""
     return _native.linear_decode(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, state_indices, inplace_state, out, 64)
+
+
+def linear_attention_backward(q, k, v, g, d_o, scale=None, initial_state=None, d_final_state=None, cu_seqlens=None):
+    """Gradients of ``chunk_linear_attention`` / ``fused_recurrent_linear_attention``.  ``d_o``: bf16, shaped like ``v``; ``d_final_state``:
+    optional fp32 gradient of the final states.  Returns ``(dq, dk, dv, dg, d_initial_state)``: dq, dk bf16 in the shape of q, k (the
+    value heads sharing a key head are summed in fp32), dv bf16, dg fp32 in the shape of g (None without one), ``d_initial_state``
+    fp32 (None when no initial state was given).  Rows of a packed batch that belong to no sequence get zeros."""
+    return _native.linear_backward(q, k, v, g, d_o, scale, initial_state, d_final_state, cu_seqlens)
+
+
+class LinearAttentionFunction(torch.autograd.Function):
+    """``o, final_state = LinearAttentionFunction.apply(q, k, v, g, scale, initial_state, cu_seqlens)``: the chunked forward pass with
+    the chunked backward pass attached (g, scale, initial_state and cu_seqlens may be None)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, scale, initial_state, cu_seqlens):
+        o, final = chunk_linear_attention(q, k, v, g, scale, initial_state, True, cu_seqlens)
+        ctx.save_for_backward(q, k, v, g, initial_state, cu_seqlens)
+        ctx.scale = scale
+        return o, final
+
+    @staticmethod
+    def backward(ctx, d_o, d_final):
+        q, k, v, g, s0, cu = ctx.saved_tensors
+        d_o = d_o.to(torch.bfloat16).contiguous()
+        d_final = None if d_final is None else d_final.float().contiguous()
+        dq, dk, dv, dg, ds0 = linear_attention_backward(q, k, v, g, d_o, ctx.scale, s0, d_final, cu)
+        return dq, dk, dv, dg, None, ds0, None

@@ -39,6 +39,8 @@ SCHEMAS = {
                       "Tensor(b!)? final_state, Tensor? cu_seqlens, Tensor? state_indices) -> ()",
     "linear_decode": "(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor(a!) out, float scale, Tensor? initial_state, "
                      "Tensor(b!)? final_state, Tensor? cu_seqlens, Tensor? state_indices) -> ()",
+    "linear_backward": "(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor d_o, float scale, Tensor? initial_state, Tensor? d_final_state, "
+                       "Tensor? cu_seqlens, Tensor(a!) dq, Tensor(b!) dk, Tensor(c!) dv, Tensor(d!)? dg, Tensor(e!)? d_initial_state) -> ()",
     "layer_norm": "(Tensor x, Tensor? weight, Tensor? bias, float eps, Tensor(a!) out, Tensor(b!)? mean, Tensor(c!)? rstd) -> ()",
     "layer_norm_backward": "(Tensor d_y, Tensor x, Tensor mean, Tensor rstd, Tensor? weight, Tensor(a!) d_x, Tensor(b!)? d_weight, "
                            "Tensor(c!)? d_bias) -> ()",

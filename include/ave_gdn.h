@@ -367,6 +367,42 @@ size_t ave_linear_prefill_workspace_bytes(const AveLinearArgs* args);
 /* Token by token; T == 1 with state_indices is the continuous-batching decode step.  A sequence with bad offsets is skipped. */
 int ave_linear_decode_step(const AveLinearArgs* args, void* stream);
 
+/* Gradients of the whole-sequence form.  Inputs as there plus d_o and the optional gradient of the final states; outputs are contiguous:
+ * bf16 d_q, d_k [B,T,Hk,dk] (summed over the value heads of a key head in fp32) and d_v [B,T,Hv,dv]; d_g fp32, [B,T,Hv], or [Hv] with
+ * AVE_LINEAR_FLAG_HEAD_GATE (g one number a head: its strides are zero); d_initial_state fp32, needed when initial_state is given.
+ * A packed batch with bad offsets is skipped as a whole (its outputs are undefined); rows of no sequence have zero gradients. */
+#define AVE_LINEAR_FLAG_HEAD_GATE 1u
+typedef struct AveLinearBwdArgs {
+  uint32_t struct_size;
+  uint32_t flags;               /* AVE_LINEAR_FLAG_HEAD_GATE */
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* g;               /* optional; without it d_g is not written */
+  const void* d_o;              /* bf16 [B,T,Hv,dv] */
+  const float* initial_state;   /* optional fp32 [n_seqs,Hv,dk,dv] */
+  const float* d_final_state;   /* optional fp32 [n_seqs,Hv,dk,dv] */
+  const int32_t* cu_seqlens;    /* optional int32 [n_seqs+1]; requires B == 1 */
+  void* d_q;
+  void* d_k;
+  void* d_v;
+  float* d_g;
+  float* d_initial_state;       /* fp32 [n_seqs,Hv,dk,dv]; required with initial_state */
+  uint32_t* status;
+  void* workspace;              /* ave_linear_backward_workspace_bytes(), 16-byte aligned */
+  uint64_t workspace_bytes;
+  int32_t B, T, Hk, Hv, dk, dv, n_seqs, reserved0;
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  int64_t k_stride_b, k_stride_t, k_stride_h;
+  int64_t v_stride_b, v_stride_t, v_stride_h;
+  int64_t do_stride_b, do_stride_t, do_stride_h;
+  int64_t g_stride_b, g_stride_t;
+  float scale;
+  float reserved1;
+} AveLinearBwdArgs;
+int ave_linear_backward(const AveLinearBwdArgs* args, void* stream);
+size_t ave_linear_backward_workspace_bytes(const AveLinearBwdArgs* args);
+
 /* y = (x - mean) * rstd * weight + bias over rows of n elements, 1 <= n <= 32768, rstd = 1 / sqrt(var + eps). */
 #define AVE_DTYPE_BF16 0
 #define AVE_DTYPE_FP16 1

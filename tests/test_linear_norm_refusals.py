@@ -25,6 +25,7 @@ CALLS = {
     "linear_prefill": lambda L, N: L.chunk_linear_attention(bf(1, 9, 2, 128), bf(1, 9, 2, 128), bf(1, 9, 4, 64), f32(4), output_final_state=True),
     "linear_decode": lambda L, N: L.fused_recurrent_linear_attention(bf(3, 1, 2, 64), bf(3, 1, 2, 64), bf(3, 1, 4, 128), f32(3, 1, 4), initial_state=f32(5, 4, 64, 128),
                                                                      state_indices=i32(3)),
+    "linear_backward": lambda L, N: L.linear_attention_backward(bf(1, 9, 2, 128), bf(1, 9, 2, 128), bf(1, 9, 4, 64), f32(1, 9, 4), bf(1, 9, 4, 64)),
     "layer_norm": lambda L, N: N.layer_norm(bf(2, 3, 100), f32(100), f32(100), return_stats=True),
     "layer_norm_backward": lambda L, N: N.layer_norm_backward(bf(6, 100), bf(6, 100), f32(6), f32(6), bf(100)),
 }
@@ -79,6 +80,39 @@ def test_linear_refusals(built_lib, entry):
     if entry == "chunk_linear_attention":
         with FakeTensorMode(), pytest.raises(ValueError, match="chunk_size must be 64"):
             f(q(), q(), v(), chunk_size=32)
+
+
+def test_backward_refusals(built_lib):
+    from avelang_b200 import linear_attention as L
+    q, v = lambda: bf(1, 9, 2, 128), lambda: bf(1, 9, 4, 64)
+    f = L.linear_attention_backward
+    with FakeTensorMode():
+        for match, call in [
+            ("d_o must be a bf16", lambda: f(q(), q(), v(), None, f32(1, 9, 4, 64))),
+            ("d_o must be a bf16", lambda: f(q(), q(), v(), None, bf(1, 9, 4, 128))),
+            ("initial_state must be a contiguous", lambda: f(q(), q(), v(), None, v(), None, f32(1, 4, 64, 128))),
+            ("d_final_state must be a contiguous", lambda: f(q(), q(), v(), None, v(), None, None, f32(2, 4, 128, 64))),
+            ("g must have shape", lambda: f(q(), q(), v(), f32(3), v())),
+            ("cu_seqlens requires B == 1", lambda: f(bf(2, 9, 2, 128), bf(2, 9, 2, 128), bf(2, 9, 4, 64), None, bf(2, 9, 4, 64), None, None, None, i32(2))),
+        ]:
+            with pytest.raises(ValueError, match=match):
+                call()
+    lib = _lib.load()
+    a = _lib.LinearBwdArgs()
+    assert lib.ave_linear_backward(None, None) == lib.ave_linear_backward(ctypes.byref(a), None) == _lib.INVALID_ARGUMENT
+    a.struct_size = ctypes.sizeof(a)
+    a.B, a.T, a.Hk, a.Hv, a.dk, a.dv, a.n_seqs = 1, 100, 2, 4, 128, 64, 1
+    for n in ("q", "k", "v", "d_o", "d_q", "d_k", "d_v", "g", "d_g"):
+        setattr(a, n, 0x1000)
+    a.initial_state = 0x1000
+    assert lib.ave_linear_backward(ctypes.byref(a), None) == _lib.INVALID_ARGUMENT  # its gradient has no place
+    a.initial_state = None
+    assert lib.ave_linear_backward(ctypes.byref(a), None) == _lib.INVALID_ARGUMENT  # no scratch
+    a.workspace, a.workspace_bytes = 0x1000, 16
+    assert lib.ave_linear_backward(ctypes.byref(a), None) == _lib.WORKSPACE_TOO_SMALL
+    assert lib.ave_linear_backward_workspace_bytes(ctypes.byref(a)) > 0
+    a.d_q = 0x1004
+    assert lib.ave_linear_backward(ctypes.byref(a), None) == _lib.MISALIGNED
 
 
 def test_norm_refusals(built_lib):
@@ -146,7 +180,7 @@ def test_struct_mirrors(tmp_path):
     import os
     import subprocess
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    names = [("AveLinearArgs", _lib.LinearArgs, "scale"), ("AveLayerNormArgs", _lib.LayerNormArgs, "eps"), ("AveLayerNormBwdArgs", _lib.LayerNormBwdArgs, "w_dtype")]
+    names = [("AveLinearArgs", _lib.LinearArgs, "scale"), ("AveLinearBwdArgs", _lib.LinearBwdArgs, "scale"), ("AveLayerNormArgs", _lib.LayerNormArgs, "eps"), ("AveLayerNormBwdArgs", _lib.LayerNormBwdArgs, "w_dtype")]
     src = tmp_path / "sz.c"
     src.write_text('#include "ave_gdn.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(void){' + "".join(
         f'printf("%zu %zu\\n", sizeof({c}), offsetof({c}, {f}));' for c, _, f in names) + "return 0;}\n")
