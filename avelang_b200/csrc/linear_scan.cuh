@@ -91,8 +91,9 @@ __device__ __forceinline__ bool offsets_fit(const Args& a, bool flag) {
 }
 
 // Shared memory: a ring of stages {X, Y, W, (E), gate vectors}, then the three terms of Yw and the two of P'
-constexpr int GATES = 1088;  // floats e[64] | w[64] | G hi[64] | G lo[64] | decay (and padding to 64 bytes)
-constexpr int GV_E = 0, GV_W = 64, GV_H = 128, GV_L = 192, GV_TOT = 256;
+// Gate vectors of a chunk, floats: e[64] | w[64] | G hi[64] | G lo[64] | e^{-|G_i - G_31|}[64] (signs for g <= 0) | decay (and padding to 64 bytes)
+constexpr int GATES = 1344;
+constexpr int GV_E = 0, GV_W = 64, GV_H = 128, GV_L = 192, GV_F = 256, GV_TOT = 320;
 template <bool kState, bool kGrad>
 struct Cfg {
   static constexpr int TILES = kState ? 2 : kGrad ? 4 : 3;
@@ -102,13 +103,14 @@ struct Cfg {
   static constexpr int YW = STAGES * STAGE, PP = YW + 3 * TILE, GV = PP + (kState ? 0 : TILE), BARS = GV + STAGES * GATES;
   static constexpr int SMEM = BARS + 256 + 1024;
   static_assert(SMEM <= 232448, "shared memory of an SM");
-  // TMEM columns; with the gradient of g the state has three terms and W^T P'^T takes the columns of P
-  static constexpr uint32_t P = 0, PE = 64, OI = kGrad ? 128 : 64, OA = kGrad ? 0 : 128, DS = kState ? 0 : 192, H = 320, COLS = kState ? 128 : 512;
+  // TMEM columns; with the gradient of g the state has three terms, W^T P'^T takes the columns of P and H^T X^T has one accumulator
+  static constexpr uint32_t P = 0, PE = 64, OI = kGrad ? 128 : 64, OA = kGrad ? 0 : 192, DS = kState ? 0 : kGrad ? 192 : 256, H = kGrad ? 320 : 384, COLS = kState ? 128 : 512;
   static constexpr int HT = kGrad ? 3 : 2;
+  static constexpr uint32_t OI2 = kGrad ? 0 : 64;  // H^T X^T has a second accumulator
 };
 
-constexpr int THREADS = 640;  // warpgroups: loader, issuer and gates; two for the state; outputs; P' and Yw
-constexpr int REGS_LAUNCH = 96, REGS_CTRL = 56, REGS_STATE = 120, REGS_OUT = 112, REGS_PREP = 72;
+constexpr int THREADS = 640;  // warpgroups: P' (two warps, whose lanes are the chunk's rows), loader and gates, issuer; two for the state; outputs; Yw
+constexpr int REGS_LAUNCH = 96, REGS_CTRL = 80, REGS_STATE = 112, REGS_OUT = 104, REGS_PREP = 72;
 static_assert(REGS_CTRL + 2 * REGS_STATE + REGS_OUT + REGS_PREP <= 5 * REGS_LAUNCH, "register redistribution exceeds the launch allocation");
 static_assert(THREADS * REGS_LAUNCH <= 65536, "launch allocation exceeds the register file");
 
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       tc::mbar_init(&empty[i], kState ? 9 : 12);  // the state's warps have read the decay, and: the issuer's commit, or the output warps
     }
     for (uint64_t* b : {p_full, ds_full, h_read, o_full, mma_end}) tc::mbar_init(b, 1);
-    tc::mbar_init(pp_ready, 2); tc::mbar_init(yw_ready, kState ? 4 : 2);
+    tc::mbar_init(pp_ready, 2); tc::mbar_init(yw_ready, 4);
     tc::mbar_init(ds_empty, 8); tc::mbar_init(h_ready, 8);
     tc::mbar_init(o_empty, 4);
     *abort_flag = 0;
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   }
   const int n_chunks = (seg.len + C - 1) / C;
   auto chunk_at = [&](int c) { return kRev ? n_chunks - 1 - c : c; };  // place of the c-th chunk of the walk
-  if (warp == 1) tc::tmem_alloc(tmem_slot, K::COLS);
+  if (warp == 3) tc::tmem_alloc(tmem_slot, K::COLS);
   tc::tc_fence_before_sync();
   __syncthreads();
   tc::tc_fence_after_sync();
@@ -195,33 +197,153 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
 
   if (warp < 4) {
     tc::reg_set<REGS_CTRL, REGS_LAUNCH>();
-    if (warp == 0 && lane == 0) {
-      // ---------------------------------------------------------------- loader
-      if (!kState) tc::prefetch_tmap(&maps.x);
-      tc::prefetch_tmap(&maps.y); tc::prefetch_tmap(&maps.w);
+    if (warp < 2) {
+      if constexpr (!kState) {
+        // -------------------------------------------------------------- P': row t a lane
+        const int t = 32 * warp + lane, r8 = lane & 7;
+        const uint32_t lane_addr = tm + ((uint32_t)(32 * warp) << 16);
+        int s = 0;
+        uint32_t ph = 0;
+        for (int c = 0; c < n_chunks; ++c) {
+          const uint32_t cp = (uint32_t)c & 1u;
+          const int at_tok = chunk_at(c) * C, len = min(C, seg.len - at_tok);
+          if (!all(tc::mbar_wait3(p_full, cp, &gates[s], ph, o_full, cp ^ 1u, abort_flag))) break;
+          tc::tc_fence_after_sync();
+          const float* gv = reinterpret_cast<const float*>(smem + K::GV + s * GATES);
+          uint8_t* row = smem + K::PP + t * 128;
+          [[maybe_unused]] float sum = 0.f;
+          // 16 columns from 16 k on, with factors f(column)
+          auto step = [&](int k, auto factors, bool diagonal) {
+            uint32_t x[16], hi[8], lo[8];
+            [[maybe_unused]] uint32_t pe[16];
+            tc::tmem_ld16(lane_addr + K::P + 16 * k, x);
+            if constexpr (kGrad) tc::tmem_ld16(lane_addr + K::PE + 16 * k, pe);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              float p[4];
+              factors(16 * k + i, p);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                p[j] *= __uint_as_float(x[i + j]);
+                const int col = 16 * k + i + j;
+                // what is masked may be anything; backwards also what lies behind the sequence
+                if (diagonal && (kRev ? col < t : col > t)) p[j] = 0.f;
+                if (kRev && col >= len) p[j] = 0.f;
+                if constexpr (kGrad) {
+                  const bool counts = !(diagonal && (kRev ? col <= t : col >= t)) && !(kRev && col >= len);
+                  sum += counts ? p[j] * __uint_as_float(pe[i + j]) : 0.f;
+                }
+              }
+              split_pair(make_float2(p[0], p[1]), hi[i / 2], lo[i / 2]);
+              split_pair(make_float2(p[2], p[3]), hi[i / 2 + 1], lo[i / 2 + 1]);
+            }
+            *reinterpret_cast<uint4*>(row + (((2 * k) ^ r8) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(row + (((2 * k + 1) ^ r8) << 4)) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+            *reinterpret_cast<uint4*>(row + HALF + (((2 * k) ^ r8) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            *reinterpret_cast<uint4*>(row + HALF + (((2 * k + 1) ^ r8) << 4)) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+          };
+          if (warp == (kRev ? 0 : 1)) {  // the 32 x 32 block off the diagonal: a factor a row and one a column, meeting at token 31
+            const float r = a.scale_p * gv[GV_F + t];
+#pragma unroll 1
+            for (int k = kRev ? 2 : 0; k < (kRev ? 4 : 2); ++k)
+              step(k, [&](int col, float (&p)[4]) {
+                const float4 f = *reinterpret_cast<const float4*>(gv + GV_F + col);
+                p[0] = r * f.x; p[1] = r * f.y; p[2] = r * f.z; p[3] = r * f.w;
+              }, false);
+          }
+          const float gh = gv[GV_H + t], gl = gv[GV_L + t];
+#pragma unroll 1
+          for (int k = 2 * warp; k < 2 * warp + 2; ++k)
+            step(k, [&](int col, float (&p)[4]) {
+              const float4 h4 = *reinterpret_cast<const float4*>(gv + GV_H + col), l4 = *reinterpret_cast<const float4*>(gv + GV_L + col);
+              p[0] = a.scale_p * ex2((gh - h4.x) + (gl - l4.x)); p[1] = a.scale_p * ex2((gh - h4.y) + (gl - l4.y));
+              p[2] = a.scale_p * ex2((gh - h4.z) + (gl - l4.z)); p[3] = a.scale_p * ex2((gh - h4.w) + (gl - l4.w));
+            }, true);
+          tc::tc_fence_before_sync();
+          tc::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(pp_ready);
+          if constexpr (kGrad)
+            if (t < len) a.intra[((int64_t)h * a.B + seg.b) * a.T + seg.t0 + at_tok + t] = sum;
+          if (++s == K::STAGES) { s = 0; ph ^= 1u; }
+        }
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- loader (one lane), and gate vectors, two tokens a lane; sums of logarithms in 64 bits
+      if (lane == 0) {
+        if (!kState) tc::prefetch_tmap(&maps.x);
+        tc::prefetch_tmap(&maps.y); tc::prefetch_tmap(&maps.w);
+      }
+      constexpr double LOG2E = 1.4426950408889634;
+      double seg_total = 0.0;
+      const float* g = a.g != nullptr ? a.g + seg.b * a.g_stride_b + h : nullptr;
+      auto fetch = [&](int c, int e) {
+        const int t = chunk_at(c) * C + 2 * lane + e;
+        if (g == nullptr || t >= seg.len) return 0.f;
+        const float x = g[(int64_t)(seg.t0 + t) * a.g_stride_t];
+        return x < -1e6f ? -1e6f : x;  // (a NaN stays one)
+      };
+      float n0 = fetch(0, 0), n1 = fetch(0, 1);
       int s = 0, issued = 0;
       uint32_t ph = 1;
       for (int c = 0; c < n_chunks; ++c) {
-        if (c >= K::STAGES && !tc::mbar_wait(&empty[s], ph, abort_flag)) break;
-        uint8_t* st = smem + s * K::STAGE;
-        const int tok = seg.t0 + chunk_at(c) * C;
-        constexpr uint32_t bytes = (kState ? 1 : 2) * (DK / 64) * HALF + (kGrad ? 2 : 1) * (DV / 64) * HALF;
-        tc::mbar_expect_tx(&full[s], bytes);
-        auto load = [&](const CUtensorMap* m, int at, int halves, int head) {
+        if (c >= K::STAGES && !all(tc::mbar_wait(&empty[s], ph, abort_flag))) break;
+        if (lane == 0) {
+          uint8_t* st = smem + s * K::STAGE;
+          const int tok = seg.t0 + chunk_at(c) * C;
+          constexpr uint32_t bytes = (kState ? 1 : 2) * (DK / 64) * HALF + (kGrad ? 2 : 1) * (DV / 64) * HALF;
+          tc::mbar_expect_tx(&full[s], bytes);
+          auto load = [&](const CUtensorMap* m, int at, int halves, int head) {
 #pragma unroll
-          for (int i = 0; i < halves; ++i) tc::tma_load_4d(st + at + i * HALF, m, &full[s], 64 * i, head, tok, seg.b);
-        };
-        load(&maps.y, K::Y, DK / 64, h / a.y_div);
-        load(&maps.w, K::W, DV / 64, h / a.w_div);
-        if constexpr (!kState) load(&maps.x, K::X, DK / 64, h / a.x_div);
-        if constexpr (kGrad) load(&maps.e, K::E, DV / 64, h / a.e_div);
+            for (int i = 0; i < halves; ++i) tc::tma_load_4d(st + at + i * HALF, m, &full[s], 64 * i, head, tok, seg.b);
+          };
+          load(&maps.y, K::Y, DK / 64, h / a.y_div);
+          load(&maps.w, K::W, DV / 64, h / a.w_div);
+          if constexpr (!kState) load(&maps.x, K::X, DK / 64, h / a.x_div);
+          if constexpr (kGrad) load(&maps.e, K::E, DV / 64, h / a.e_div);
+        }
+        __syncwarp();
         ++issued;
+        const double x0 = (double)n0 * LOG2E, x1 = (double)n1 * LOG2E;
+        if (c + 1 < n_chunks) { n0 = fetch(c + 1, 0); n1 = fetch(c + 1, 1); }
+        double sum = x0 + x1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += y;
+        }
+        const double total = __shfl_sync(0xffffffffu, sum, 31), mid = __shfl_sync(0xffffffffu, sum, 15);
+        const double G0 = sum - x1, G1 = sum;
+        seg_total += total;
+        const int left = seg.len - chunk_at(c) * C - 2 * lane;  // tokens from this lane's first on
+        const double sg = kRev ? -1.0 : 1.0;
+        const float2 e = make_float2(a.scale_e * ex2((float)(kRev ? total - G0 : G0)), a.scale_e * ex2((float)(kRev ? total - G1 : G1)));
+        float2 w = make_float2(a.scale_w * ex2((float)(kRev ? G0 : total - G0)), a.scale_w * ex2((float)(kRev ? G1 : total - G1)));
+        if (left < 1) w.x = 0.f;
+        if (left < 2) w.y = 0.f;
+        const float2 hi = make_float2((float)(sg * G0), (float)(sg * G1)), lo = make_float2((float)(sg * G0 - hi.x), (float)(sg * G1 - hi.y));
+        const bool behind = lane >= 16;
+        const float2 f = make_float2(ex2((float)(behind ? G0 - mid : mid - G0)), ex2((float)(behind ? G1 - mid : mid - G1)));
+        const float tot = (float)exp2(total);  // exact to the last bit: a state is multiplied by it once a chunk
+        float* v = reinterpret_cast<float*>(smem + K::GV + s * GATES);
+        reinterpret_cast<float2*>(v + GV_E)[lane] = e;
+        reinterpret_cast<float2*>(v + GV_W)[lane] = w;
+        reinterpret_cast<float2*>(v + GV_H)[lane] = hi;
+        reinterpret_cast<float2*>(v + GV_L)[lane] = lo;
+        reinterpret_cast<float2*>(v + GV_F)[lane] = f;
+        if (lane == 0) v[GV_TOT] = tot;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&gates[s]);
         if (++s == K::STAGES) { s = 0; ph ^= 1u; }
       }
+      if (kState && lane == 0) a.seg_decay[seg_slot * a.Hv + h] = (float)exp2(seg_total);
       // nothing is on its way into the shared memory of a CTA that ends, whatever became of those who wait for it
+      if (lane == 0) {
 #pragma unroll 1
-      for (int c = max(0, issued - K::STAGES); c < issued; ++c) tc::drain(&full[c % K::STAGES], (uint32_t)(c / K::STAGES) & 1u);
-    } else if (warp == 1) {
+        for (int c = max(0, issued - K::STAGES); c < issued; ++c) tc::drain(&full[c % K::STAGES], (uint32_t)(c / K::STAGES) & 1u);
+      }
+    } else {
       // ---------------------------------------------------------------- MMA issuer
       const uint32_t smem0 = tc::smem_u32(smem) >> 4;
       constexpr uint32_t hi_sw = tc::desc_hi(1024, true);
@@ -268,7 +390,8 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         }
         __syncwarp();
         if constexpr (!kState) {
-          ok = all(tc::mbar_wait2(h_ready, cp, o_empty, cp ^ 1u, abort_flag));
+          // (the accumulator that this takes was drained with the outputs of two chunks ago; with one accumulator o_empty has been waited for)
+          ok = all(tc::mbar_wait(h_ready, cp, abort_flag));
           if (!ok) break;
           tc::tc_fence_after_sync();
           if (tc::elect_one()) {
@@ -276,12 +399,12 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
             for (int t = K::HT - 1; t >= 0; --t)
 #pragma unroll
               for (int k = 0; k < DK / 16; ++k)
-                tc::mma_ts(tm + K::OI, tm + K::H + t * 64 + 8 * k, tc::smem_desc(at + tc::desc_lo(K::X + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw),
+                tc::mma_ts(tm + K::OI + cp * K::OI2, tm + K::H + t * 64 + 8 * k, tc::smem_desc(at + tc::desc_lo(K::X + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw),
                            tc::idesc_f16(128, 64, 1, 1, false, false), !(t == K::HT - 1 && k == 0));
             tc::mma_commit(h_read);
           }
           __syncwarp();
-          ok = all(tc::mbar_wait(pp_ready, cp, abort_flag));
+          ok = all(tc::mbar_wait2(pp_ready, cp, o_empty, cp ^ 1u, abort_flag));
           if (!ok) break;
           tc::tc_fence_after_sync();
           if (tc::elect_one()) {
@@ -309,52 +432,6 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         }
         s = s_next; ph = ph_next;
       }
-    } else if (warp == 2) {
-      // ---------------------------------------------------------------- gate vectors, two tokens a lane; sums of logarithms in 64 bits
-      constexpr double LOG2E = 1.4426950408889634;
-      double seg_total = 0.0;
-      const float* g = a.g != nullptr ? a.g + seg.b * a.g_stride_b + h : nullptr;
-      auto fetch = [&](int c, int e) {
-        const int t = chunk_at(c) * C + 2 * lane + e;
-        if (g == nullptr || t >= seg.len) return 0.f;
-        const float x = g[(int64_t)(seg.t0 + t) * a.g_stride_t];
-        return x < -1e6f ? -1e6f : x;  // (a NaN stays one)
-      };
-      float n0 = fetch(0, 0), n1 = fetch(0, 1);
-      int s = 0;
-      uint32_t ph = 1;
-      for (int c = 0; c < n_chunks; ++c) {
-        const double x0 = (double)n0 * LOG2E, x1 = (double)n1 * LOG2E;
-        if (c + 1 < n_chunks) { n0 = fetch(c + 1, 0); n1 = fetch(c + 1, 1); }
-        double sum = x0 + x1;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += y;
-        }
-        const double total = __shfl_sync(0xffffffffu, sum, 31);
-        const double G0 = sum - x1, G1 = sum;
-        seg_total += total;
-        const int left = seg.len - chunk_at(c) * C - 2 * lane;  // tokens from this lane's first on
-        const double sg = kRev ? -1.0 : 1.0;
-        const float2 e = make_float2(a.scale_e * ex2((float)(kRev ? total - G0 : G0)), a.scale_e * ex2((float)(kRev ? total - G1 : G1)));
-        float2 w = make_float2(a.scale_w * ex2((float)(kRev ? G0 : total - G0)), a.scale_w * ex2((float)(kRev ? G1 : total - G1)));
-        if (left < 1) w.x = 0.f;
-        if (left < 2) w.y = 0.f;
-        const float2 hi = make_float2((float)(sg * G0), (float)(sg * G1)), lo = make_float2((float)(sg * G0 - hi.x), (float)(sg * G1 - hi.y));
-        const float tot = (float)exp2(total);  // exact to the last bit: a state is multiplied by it once a chunk
-        if (c >= K::STAGES && !all(tc::mbar_wait(&empty[s], ph, abort_flag))) break;
-        float* v = reinterpret_cast<float*>(smem + K::GV + s * GATES);
-        reinterpret_cast<float2*>(v + GV_E)[lane] = e;
-        reinterpret_cast<float2*>(v + GV_W)[lane] = w;
-        reinterpret_cast<float2*>(v + GV_H)[lane] = hi;
-        reinterpret_cast<float2*>(v + GV_L)[lane] = lo;
-        if (lane == 0) v[GV_TOT] = tot;
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&gates[s]);
-        if (++s == K::STAGES) { s = 0; ph ^= 1u; }
-      }
-      if (kState && lane == 0) a.seg_decay[seg_slot * a.Hv + h] = (float)exp2(seg_total);
     }
   } else if (warp < 12) {
     tc::reg_set<REGS_STATE, REGS_LAUNCH>();
@@ -460,9 +537,14 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
 #pragma unroll 1
           for (int hf = 0; hf < 2; ++hf) {  // 16 features
             uint32_t oi[32], oa[32];
-            tc::tmem_ld_frags(lane_addr + ((uint32_t)hf << 20) + K::OI, oi);
+            tc::tmem_ld_frags(lane_addr + ((uint32_t)hf << 20) + K::OI + cp * K::OI2, oi);
             tc::tmem_ld_frags(lane_addr + ((uint32_t)hf << 20) + K::OA, oa);
             tc::tmem_ld_wait();
+            if (hf == 1) {
+              tc::tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) tc::mbar_arrive(o_empty);
+            }
             if constexpr (kGrad) {  // E's pieces in the layout of the fragments
               const uint32_t e_s = tc::smem_u32(smem + s * K::STAGE + K::E) + (uint32_t)((wq >> 1) * HALF + (8 * (m4 >> 1) + r8) * 128 +
                                                                                       (((4 * (wq & 1) + 2 * hf + (m4 & 1)) ^ r8) << 4));
@@ -513,10 +595,9 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
             }
           }
         }
-        tc::tc_fence_before_sync();
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(o_empty);
+        if (!mine && lane == 0) tc::mbar_arrive(o_empty);
         if constexpr (kGrad) {
           // sums over the eight lanes of a token's features; lane (gr, t2 / 2) ends with the tokens 8 gr + t2, 8 gr + t2 + 1
 #pragma unroll
@@ -561,62 +642,10 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
     }
   } else {
     tc::reg_set<REGS_PREP, REGS_LAUNCH>();
-    const int pw = warp - 16;
-    if (!kState && pw < 2) {
-      // ---------------------------------------------------------------- P': row t a lane
-      const int t = 32 * pw + lane, r8 = lane & 7;
-      const uint32_t lane_addr = tm + ((uint32_t)(32 * pw) << 16);
-      const int k_lo = kRev ? 2 * pw : 0, k_hi = kRev ? 4 : 2 * (pw + 1);  // steps of 16 columns in which this warp's rows have a part
-      int s = 0;
-      uint32_t ph = 0;
-      for (int c = 0; c < n_chunks; ++c) {
-        const uint32_t cp = (uint32_t)c & 1u;
-        const int at_tok = chunk_at(c) * C, len = min(C, seg.len - at_tok);
-        if (!all(tc::mbar_wait3(p_full, cp, &gates[s], ph, o_full, cp ^ 1u, abort_flag))) break;
-        tc::tc_fence_after_sync();
-        const float* gv = reinterpret_cast<const float*>(smem + K::GV + s * GATES);
-        const float gh = gv[GV_H + t], gl = gv[GV_L + t];
-        float sum = 0.f;
-#pragma unroll 1
-        for (int k = k_lo; k < k_hi; ++k) {
-          uint32_t x[16], pe[16];
-          tc::tmem_ld16(lane_addr + K::P + 16 * k, x);
-          if constexpr (kGrad) tc::tmem_ld16(lane_addr + K::PE + 16 * k, pe);
-          tc::tmem_ld_wait();
-          uint32_t hi[8], lo[8];
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float4 sh = *reinterpret_cast<const float4*>(gv + GV_H + 16 * k + i), sl = *reinterpret_cast<const float4*>(gv + GV_L + 16 * k + i);
-            const float dh[4] = {sh.x, sh.y, sh.z, sh.w}, dl[4] = {sl.x, sl.y, sl.z, sl.w};
-            float p[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int col = 16 * k + i + j;
-              const bool in = (kRev ? col >= t : col <= t) && col < len;
-              p[j] = in ? a.scale_p * ex2((gh - dh[j]) + (gl - dl[j])) * __uint_as_float(x[i + j]) : 0.f;
-              if constexpr (kGrad) sum += in && col != t ? p[j] * __uint_as_float(pe[i + j]) : 0.f;
-            }
-            split_pair(make_float2(p[0], p[1]), hi[i / 2], lo[i / 2]);
-            split_pair(make_float2(p[2], p[3]), hi[i / 2 + 1], lo[i / 2 + 1]);
-          }
-          uint8_t* row = smem + K::PP + t * 128;
-          *reinterpret_cast<uint4*>(row + (((2 * k) ^ r8) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(row + (((2 * k + 1) ^ r8) << 4)) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-          *reinterpret_cast<uint4*>(row + HALF + (((2 * k) ^ r8) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          *reinterpret_cast<uint4*>(row + HALF + (((2 * k + 1) ^ r8) << 4)) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-        }
-        tc::tc_fence_before_sync();
-        tc::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(pp_ready);
-        if constexpr (kGrad)
-          if (t < len) a.intra[((int64_t)h * a.B + seg.b) * a.T + seg.t0 + at_tok + t] = sum;
-        if (++s == K::STAGES) { s = 0; ph ^= 1u; }
-      }
-    } else {
+    {
       // ---------------------------------------------------------------- Yw: a piece (8 features of a token) at a time, in the places that Y's has
-      constexpr int WARPS = kState ? 4 : 2, N = 32 * WARPS;
-      const int tid = (kState ? pw : pw - 2) * 32 + lane;
+      constexpr int N = 128;
+      const int tid = (warp - 16) * 32 + lane;
       int s = 0;
       uint32_t ph = 0;
       for (int c = 0; c < n_chunks; ++c) {
@@ -629,13 +658,14 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         for (int i = tid; i < (DK / 64) * 512; i += N) {
           const int tok = (i >> 3) & 63;
           const float w = gv[GV_W + tok];
-          const uint4 y = *reinterpret_cast<const uint4*>(st + K::Y + 16 * i);
+          uint4 y = *reinterpret_cast<const uint4*>(st + K::Y + 16 * i);
+          if (tok >= len) y = make_uint4(0u, 0u, 0u, 0u);  // (may be anything, and w is zero)
           const uint32_t in[4] = {y.x, y.y, y.z, y.w};
           uint32_t h0[4], h1[4], h2[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 f = bf16x2_to_float2(in[j]);
-            split3(tok < len ? __fmul2_rn(f, make_float2(w, w)) : make_float2(0.f, 0.f), h0[j], h1[j], h2[j]);
+            split3(__fmul2_rn(f, make_float2(w, w)), h0[j], h1[j], h2[j]);
           }
           uint8_t* dst = smem + K::YW + 16 * i;
           *reinterpret_cast<uint4*>(dst) = make_uint4(h0[0], h0[1], h0[2], h0[3]);
@@ -661,11 +691,11 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   __syncthreads();
   if (*abort_flag != 0u) {  // (the roles have ended: it stays as it is)
     if (threadIdx.x == 0 && a.status != nullptr) atomicOr(a.status, AVE_GDN_DEV_WAIT_EXPIRED);
-    if (warp == 1) tc::drain_mmas(mma_end);
+    if (warp == 3) tc::drain_mmas(mma_end);
     tc::tc_fence_before_sync();
     __syncthreads();
   }
-  if (warp == 1) {
+  if (warp == 3) {
     tc::tc_fence_after_sync();
     tc::tmem_dealloc(tm, K::COLS);
   }

@@ -36,17 +36,20 @@ def check(got, q, k, v, g, scale, s0, cu, d_o, d_final):
         elif name == "ds0":
             tol = 2 * es * m
         else:
-            terms = (q.double().abs() * mag[0]).sum(-1).repeat_interleave(1, 2)
-            total = (terms.sum() + (k.double().abs() * mag[1]).sum()) if g.dim() == 1 else None
-            if g.dim() == 1:
-                tol = 2.0 ** -18 * (q.shape[1] * total + m)
-            else:
-                per_seq = torch.zeros_like(r)
-                for b, t0, n in O.spans(q, cu):
-                    per_seq[b, t0:t0 + n] = ((q[b, t0:t0 + n].double().abs() * mag[0][b, t0:t0 + n]).sum() + (k[b, t0:t0 + n].double().abs() * mag[1][b, t0:t0 + n]).sum())
-                tol = 2.0 ** -18 * (per_seq + m)
-            # and, as the errors of the many terms are independent, far nearer in the mean
-            assert (x - r).norm() <= 2.0 ** -17 * r.norm() + 1e-30, (name, float((x - r).norm() / r.norm()))
+            # |A| + |B| of each token (the sums over the value heads of a key head are larger still)
+            terms = ((q.double().abs() * mag[0]).sum(-1) + (k.double().abs() * mag[1]).sum(-1)).repeat_interleave(v.shape[2] // q.shape[2], 2)
+            tol, mean = torch.zeros_like(r), torch.zeros_like(r)
+            for b, t0, n in O.spans(q, cu):
+                part = terms[b, t0:t0 + n]
+                if g.dim() == 1:  # the sum over n tokens of such running sums: an error enters at most n of them
+                    tol += n * part.sum(0)
+                    mean += (n * part.norm(dim=0)) ** 2
+                else:
+                    tol[b, t0:t0 + n] = part.sum(0)
+                    mean[b, t0:t0 + n] = part.norm(dim=0) ** 2
+            tol = 2.0 ** -18 * (tol + m)
+            # the errors of different tokens' sums are independent, so that they add like their squares
+            assert ((x - r).abs() <= 2.0 ** -18 * (mean.sqrt() + m) + 1e-30).all(), name
         assert ((x - r).abs() <= tol + 1e-30).all(), (name, float(((x - r).abs() / (tol + 1e-30)).max()))
 
 
