@@ -87,7 +87,10 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const Gate
     if (t < seg.len) {
       float ia = 0.f, ib = 0.f;
       for (int p = 0; p < q.parts; ++p) { ia += q.inter_a[p * plane + base + t]; ib += q.inter_b[p * plane + base + t]; }
-      d = ((double)ib - (double)ia) + ((double)q.intra_b[base + t] - (double)q.intra_a[base + t]);
+      float ja = 0.f, jb = 0.f;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) { ja += q.intra_a[p * plane + base + t]; jb += q.intra_b[p * plane + base + t]; }
+      d = ((double)ib - (double)ia) + ((double)jb - (double)ja);
     }
     double inc = d;
 #pragma unroll
@@ -167,7 +170,7 @@ Layout layout_of(const AveLinearBwdArgs& a) {
   if (a.Hv > a.Hk) l.part = take(rows * a.dk * 4);
   if (a.g != nullptr) {
     l.inter_a = take(rows * (a.dk / 32) * 4); l.inter_b = take(rows * (a.dk / 32) * 4);
-    l.intra_a = take(rows * 4); l.intra_b = take(rows * 4);
+    l.intra_a = take(rows * 16); l.intra_b = take(rows * 16);
     l.sums = take((size_t)l.plan.slots * a.Hv * 4);
   }
   l.bytes = at;
@@ -195,6 +198,7 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
   base.cu_seqlens = a.cu_seqlens; base.status = a.status;
   base.B = a.B; base.T = a.T; base.Hv = a.Hv; base.n_seqs = a.n_seqs; base.num_slots = a.n_seqs;
   base.g = a.g; base.g_stride_b = a.g_stride_b; base.g_stride_t = a.g_stride_t;
+  base.x_div = base.y_div = base.w_div = base.e_div = 1;
   base.plan = l.plan;
   lin::Args fwd = base, rev = base;  // states from the front, and their gradients from behind, as [dk][dv]
   fwd.y_div = rep; fwd.w_div = 1; fwd.scale_w = 1.f;
@@ -216,7 +220,7 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
     const uint64_t row = (uint64_t)a.Hv * a.dk * 4;
     const uint64_t dims[4] = {(uint64_t)a.dk, (uint64_t)a.Hv, (uint64_t)a.T, (uint64_t)a.B}, str[4] = {4, (uint64_t)a.dk * 4, row, row * a.T};
     const uint32_t box[4] = {32, 1, 64, 1};
-    return make_tmap(&m.o32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, s.o_part, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    return make_tmap(&m.o, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, s.o_part, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   auto sum_heads = [&](void* out) {
     if (rep == 1) return (int)AVE_GDN_OK;
@@ -231,40 +235,41 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
     if (l.plan.cut) {
       lin::Maps m{};
       m.y = mk; m.w = mv;
-      if ((r = lin::launch_scan<DK, DV, false, true, false>(fwd, m, stream))) return r;
+      if ((r = lin::launch_scan<DK, DV, false, lin::STATE>(fwd, m, stream))) return r;
       m.y = mq; m.w = mo;
-      if ((r = lin::launch_scan<DK, DV, true, true, false>(rev, m, stream))) return r;
+      if ((r = lin::launch_scan<DK, DV, true, lin::STATE>(rev, m, stream))) return r;
       if ((r = lin::launch_chain<DK, DV, false>(fwd, stream))) return r;
       if ((r = lin::launch_chain<DK, DV, true>(rev, stream))) return r;
     }
     {  // dv, and the gradient of the initial state
       lin::Args s = rev;
       lin::Maps m{};
-      s.x_div = rep; s.scale_p = a.scale; s.scale_e = 1.f;
+      s.x_div = rep; lin::set_scale(s, a.scale); s.scale_e = 1.f;
       s.state_out = a.d_initial_state;
       m.x = mk; m.y = mq; m.w = mo;
       s.o = a.d_v; s.o_stride_h = a.dv; s.o_stride_t = (int64_t)a.Hv * a.dv; s.o_stride_b = s.o_stride_t * a.T;
       m.o_ok = lin::result_map(&m.o, a.d_v, a.dv, a.Hv, a.B, a.T, s.o_stride_b, s.o_stride_t, s.o_stride_h);
-      if ((r = lin::launch_scan<DK, DV, true, false, false>(s, m, stream))) return r;
+      r = s.state_out != nullptr ? lin::launch_scan<DK, DV, true, lin::OUT3>(s, m, stream) : lin::launch_scan<DK, DV, true, lin::OUT2>(s, m, stream);
+      if (r) return r;
     }
     {  // dq
       lin::Args s = fwd;
       lin::Maps m{};
-      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; s.scale_p = s.scale_e = a.scale; s.st_y = 1; s.st_w = a.dv;
+      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; lin::set_scale(s, a.scale); s.scale_e = a.scale; s.st_y = 1; s.st_w = a.dv;
       m.x = mo; m.y = mv; m.w = mk; m.e = mq;
       if ((r = rows_of(s, m, a.d_q))) return r;
       if (grad) { s.inter = f32(l.inter_a); s.intra = f32(l.intra_a); }
-      r = grad ? lin::launch_scan<DV, DK, false, false, true>(s, m, stream) : lin::launch_scan<DV, DK, false, false, false>(s, m, stream);
+      r = grad ? lin::launch_scan<DV, DK, false, lin::GRAD>(s, m, stream) : lin::launch_scan<DV, DK, false, lin::OUT2>(s, m, stream);
       if (r || (r = sum_heads(a.d_q))) return r;
     }
     {  // dk
       lin::Args s = rev;
       lin::Maps m{};
-      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; s.scale_p = a.scale; s.scale_e = 1.f; s.st_y = 1; s.st_w = a.dv;
+      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; lin::set_scale(s, a.scale); s.scale_e = 1.f; s.st_y = 1; s.st_w = a.dv;
       m.x = mv; m.y = mo; m.w = mq; m.e = mk;
       if ((r = rows_of(s, m, a.d_k))) return r;
       if (grad) { s.inter = f32(l.inter_b); s.intra = f32(l.intra_b); }
-      r = grad ? lin::launch_scan<DV, DK, true, false, true>(s, m, stream) : lin::launch_scan<DV, DK, true, false, false>(s, m, stream);
+      r = grad ? lin::launch_scan<DV, DK, true, lin::GRAD>(s, m, stream) : lin::launch_scan<DV, DK, true, lin::OUT2>(s, m, stream);
       if (r || (r = sum_heads(a.d_k))) return r;
     }
     return (int)AVE_GDN_OK;

@@ -14,7 +14,8 @@ int launch_linear_prefill(const AveLinearArgs& a, cudaStream_t stream) {
   s.B = a.B; s.T = a.T; s.Hv = a.Hv; s.n_seqs = a.n_seqs; s.num_slots = a.num_slots; s.state_indices = a.state_indices;
   s.x_div = s.y_div = a.Hv / a.Hk; s.w_div = s.e_div = 1;
   s.g = a.g; s.g_stride_b = a.g_stride_b; s.g_stride_t = a.g_stride_t;
-  s.scale_p = s.scale_e = a.scale; s.scale_w = 1.f;
+  lin::set_scale(s, a.scale);
+  s.scale_e = a.scale; s.scale_w = 1.f;
   s.o = a.o; s.o_stride_b = a.o_stride_b; s.o_stride_t = a.o_stride_t; s.o_stride_h = a.o_stride_h;
   s.state_in = a.initial_state; s.state_out = a.final_state; s.st_y = a.dv; s.st_w = 1;
   s.plan = prefill_plan(a);
@@ -27,11 +28,11 @@ int launch_linear_prefill(const AveLinearArgs& a, cudaStream_t stream) {
   m.o_ok = lin::result_map(&m.o, a.o, a.dv, a.Hv, a.B, a.T, a.o_stride_b, a.o_stride_t, a.o_stride_h);
   return lin::by_dims(a.dk, a.dv, [&](auto dk, auto dv) {
     if (s.plan.cut) {
-      int r = lin::launch_scan<dk, dv, false, true, false>(s, m, stream);
+      int r = lin::launch_scan<dk, dv, false, lin::STATE>(s, m, stream);
       if (r == AVE_GDN_OK) r = lin::launch_chain<dk, dv, false>(s, stream);
       if (r != AVE_GDN_OK) return r;
     }
-    return lin::launch_scan<dk, dv, false, false, false>(s, m, stream);
+    return s.state_out != nullptr ? lin::launch_scan<dk, dv, false, lin::OUT3>(s, m, stream) : lin::launch_scan<dk, dv, false, lin::OUT2>(s, m, stream);
   });
 }
 

@@ -1,8 +1,8 @@
 // The chunked scan of linear attention with a decay for each head, for one segment of one (sequence, value head):
 //     H^T  state [dv lanes][dk], fp32 in registers, with bf16 images in TMEM
-//     P    = X Y^T            masked and decayed: P'_ts = scale_p e^{G_t - G_s} P_ts for s <= t
+//     P    = X Y^T            masked and decayed: P'_ts = scale e^{G_t - G_s} P_ts for s <= t
 //     O^T  = e_t (H^T X^T) + W^T P'^T
-//     H^T <- decay H^T + W^T Yw,     Yw_s = w_s Y_s
+//     H^T <- decay H^T + (w W)^T Y,   w_s = e^{G_end - G_s}
 // over chunks of 64 tokens, X, Y, W = q, k, v in the forward pass.  The gradients are scans of the same form: (do, v, k) forwards gives dq;
 // (v, do, q) and (k, q, do) backwards in time give dk and dv, with the mask, the walk over the chunks and the decays' signs turned round.
 // G is the sum of the decays' logarithms inside the chunk, so every exponent of a product that counts is <= 0 for g <= 0.
@@ -37,7 +37,9 @@ struct Args {
   int x_div, y_div, w_div, e_div;
   const float* g;
   int64_t g_stride_b, g_stride_t;
-  float scale_p, scale_e, scale_w;
+  float log_scale;                 // P' carries scale as 2^log_scale, and the product W^T P'^T its sign
+  int negative;
+  float scale_e, scale_w;
   void* o;                         // bf16
   int64_t o_stride_b, o_stride_t, o_stride_h;
   float* o_part;                   // fp32 [B, T, Hv, dv] instead, for a sum over heads behind the scan
@@ -47,10 +49,14 @@ struct Args {
   float* seg_state;                // [segment slot, Hv, ..] likewise
   float* seg_decay;                // [segment slot, Hv]
   float* inter;                    // [dv / 32][Hv][B T]: e_t E_t . (H^T X_t), 32 features each      (for the gradient of g)
-  float* intra;                    // [Hv][B T]: sum over s < t of P'_ts (E_t . W_s)
+  float* intra;                    // [4][Hv][B T]: sum over s < t of P'_ts (E_t . W_s), 16 of a chunk's s each
   Plan plan;
 };
-struct Maps { CUtensorMap x, y, w, e, o, o32; bool o_ok; };
+struct Maps {
+  CUtensorMap x, y, w, e;  // 64 tokens of a head a copy
+  CUtensorMap o;           // 32 features of 64 tokens, of the result or of o_part
+  bool o_ok;               // the result's layout can be described by a map
+};
 
 __device__ __forceinline__ int64_t first_slot(const Args& a, int n) {
   return (a.cu_seqlens ? (int64_t)a.cu_seqlens[n] : (int64_t)n * a.T) / a.plan.len + n;
@@ -90,27 +96,36 @@ __device__ __forceinline__ bool offsets_fit(const Args& a, bool flag) {
   return bad == 0;
 }
 
-// Shared memory: a ring of stages {X, Y, W, (E), gate vectors}, then the three terms of Yw and the two of P'
-// Gate vectors of a chunk, floats: e[64] | w[64] | G hi[64] | G lo[64] | e^{-|G_i - G_31|}[64] (signs for g <= 0) | decay (and padding to 64 bytes)
-constexpr int GATES = 1344;
-constexpr int GV_E = 0, GV_W = 64, GV_H = 128, GV_L = 192, GV_F = 256, GV_TOT = 320;
-template <bool kState, bool kGrad>
+// Shared memory: a ring of stages {W, Y, (X), (E)} with their gate vectors, and the two terms of P'.
+// Gate vectors of a chunk, floats: e[64] | w[64] | G hi[64] | G lo[64] | decay (and padding to 64 bytes)
+constexpr int GATES = 1088;
+constexpr int GV_E = 0, GV_W = 64, GV_H = 128, GV_L = 192, GV_TOT = 256;
+// kMode: the state alone; outputs with a state in two terms (2) or three (3) bf16 terms an increment; and with what the gradient of g needs.
+// A product of a weight and a bf16 number, two terms of it, is off by 2^-18 in the mean: enough for outputs that are rounded to bf16, not for a state that
+// is itself a result, nor for the gradient of g.
+enum Mode { STATE, OUT2, OUT3, GRAD };
+template <Mode kMode>
 struct Cfg {
-  static constexpr int TILES = kState ? 2 : kGrad ? 4 : 3;
-  static constexpr int X = 0, Y = kState ? 0 : TILE, W = Y + TILE, E = W + TILE;
-  static constexpr int STAGE = TILES * TILE;
-  static constexpr int STAGES = kState ? 3 : kGrad ? 2 : 3;
-  static constexpr int YW = STAGES * STAGE, PP = YW + 3 * TILE, GV = PP + (kState ? 0 : TILE), BARS = GV + STAGES * GATES;
+  static constexpr bool kState = kMode == STATE, kGrad = kMode == GRAD;
+  static constexpr int TERMS = kMode == OUT2 ? 2 : 3;  // of an increment
+  static constexpr int HT = kGrad ? 3 : 2;             // of the state's image
+  static constexpr int W = 0, Y = TILE, X = 2 * TILE, E = 3 * TILE;
+  static constexpr int STAGE = (kState ? 2 : kGrad ? 4 : 3) * TILE;
+  static constexpr int STAGES = kGrad ? 3 : 4;
+  static constexpr int PP = STAGES * STAGE, GV = PP + (kState ? 0 : TILE), BARS = GV + STAGES * GATES;
   static constexpr int SMEM = BARS + 256 + 1024;
   static_assert(SMEM <= 232448, "shared memory of an SM");
-  // TMEM columns; with the gradient of g the state has three terms, W^T P'^T takes the columns of P and H^T X^T has one accumulator
-  static constexpr uint32_t P = 0, PE = 64, OI = kGrad ? 128 : 64, OA = kGrad ? 0 : 192, DS = kState ? 0 : kGrad ? 192 : 256, H = kGrad ? 320 : 384, COLS = kState ? 128 : 512;
-  static constexpr int HT = kGrad ? 3 : 2;
-  static constexpr uint32_t OI2 = kGrad ? 0 : 64;  // H^T X^T has a second accumulator
+  // TMEM columns.  With three terms W^T P'^T takes the columns of P, and with the gradient of g H^T X^T those of E W^T, and the increment's two halves (64 features
+  // of Y each) one another's.
+  static constexpr bool kAlias = TERMS == 3;
+  static constexpr uint32_t P = 0, OA = kAlias ? 0 : 64, OI = kAlias ? 64 : 128, PE = OI;
+  static constexpr uint32_t DS = kState ? 0 : kAlias ? 128 : 192, DS2 = kGrad ? 0 : 64, H = DS + (kGrad ? 64 : 128), IMG = kState ? 128 : H + 64 * HT;
+  static constexpr uint32_t COLS = kState ? 256 : 512;
+  static_assert(IMG + 32 * TERMS <= COLS, "tensor memory");
 };
 
-constexpr int THREADS = 640;  // warpgroups: P' (two warps, whose lanes are the chunk's rows), loader and gates, issuer; two for the state; outputs; Yw
-constexpr int REGS_LAUNCH = 96, REGS_CTRL = 80, REGS_STATE = 112, REGS_OUT = 104, REGS_PREP = 72;
+constexpr int THREADS = 640;  // warpgroups: loader, gate vectors and two issuers; two for the state and P'; outputs; images of W^T
+constexpr int REGS_LAUNCH = 96, REGS_CTRL = 56, REGS_STATE = 128, REGS_OUT = 96, REGS_PREP = 72;
 static_assert(REGS_CTRL + 2 * REGS_STATE + REGS_OUT + REGS_PREP <= 5 * REGS_LAUNCH, "register redistribution exceeds the launch allocation");
 static_assert(THREADS * REGS_LAUNCH <= 65536, "launch allocation exceeds the register file");
 
@@ -120,27 +135,58 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-template <int DK, int DV, bool kRev, bool kState, bool kGrad>
+// A number as the sum of two floats: 64-bit arithmetic is slow here (a chunk's gate vectors took 3.8 k cycles with it)
+struct Two { float h, l; };
+__device__ __forceinline__ Two add(Two a, Two b) {
+  const float s = a.h + b.h, t = s - a.h, e = (a.h - (s - t)) + (b.h - t), l = a.l + b.l + e, h = s + l;
+  return Two{h, l - (h - s)};
+}
+__device__ __forceinline__ float diff(Two a, Two b) { return (a.h - b.h) + (a.l - b.l); }
+__device__ __forceinline__ Two log2_of(float ln) {  // ln * log2(e)
+  constexpr float L = 1.44269504f, R = 1.925963033e-8f;
+  const float p = ln * L;
+  return Two{p, fmaf(ln, L, -p) + ln * R};
+}
+__device__ __forceinline__ Two shfl_up(Two x, int o) { return Two{__shfl_up_sync(0xffffffffu, x.h, o), __shfl_up_sync(0xffffffffu, x.l, o)}; }
+__device__ __forceinline__ Two shfl(Two x, int i) { return Two{__shfl_sync(0xffffffffu, x.h, i), __shfl_sync(0xffffffffu, x.l, i)}; }
+// 2^x to the last bit or two: a state is multiplied by the same number chunk after chunk, so that an error in it adds up.  Taylor's series of 2^r for |r| <= 1/2.
+__device__ __forceinline__ float pow2(Two x) {
+  const float n = rintf(x.h), r = ((x.h - n) + x.l) * 0.693147181f;
+  float p = 1.f / 5040.f;
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    constexpr float inv[6] = {1.f / 720.f, 1.f / 120.f, 1.f / 24.f, 1.f / 6.f, 0.5f, 1.f};
+    p = fmaf(p, r, inv[k]);
+  }
+  p = fmaf(p, r, 1.f);
+  if (n < -126.f) return 0.f;
+  return n > 127.f ? p * __int_as_float(0x7f800000) : p * __int_as_float(((int)n + 127) << 23);  // (a NaN stays one)
+}
+
+template <int DK, int DV, bool kRev, Mode kMode>
 __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __grid_constant__ Maps maps) {
-  using K = Cfg<kState, kGrad>;
-  static_assert(!(kState && kGrad), "states alone have no outputs");
+  using K = Cfg<kMode>;
+  constexpr bool kState = K::kState, kGrad = K::kGrad;
+  constexpr int FH = DK / 64;  // halves of the increment; group g of the state's warps takes half g, or half of the only one
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = tc::align1024(smem_raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + K::BARS);
-  uint64_t* full = bars;           // [3] tiles of the stage landed
-  uint64_t* gates = bars + 3;      // [3] its gate vectors written
-  uint64_t* empty = bars + 6;      // [3] the stage is read
-  uint64_t* p_full = bars + 9;     // P (and E W^T) accumulated
-  uint64_t* pp_ready = bars + 10;  // P' written, P drained
-  uint64_t* yw_ready = bars + 11;  // Yw written, W cleared behind the sequence
-  uint64_t* ds_full = bars + 12;   // increment accumulated, Yw read
-  uint64_t* ds_empty = bars + 13;  // increment drained
-  uint64_t* h_ready = bars + 14;   // images of the state written
-  uint64_t* h_read = bars + 15;    // H^T X^T accumulated
-  uint64_t* o_full = bars + 16;    // both outputs accumulated, P' read
-  uint64_t* o_empty = bars + 17;   // outputs drained
-  uint64_t* mma_end = bars + 18;   // the MMAs are complete, when a wait has expired
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  uint64_t* full = bars;            // [4] tiles of the stage landed
+  uint64_t* gates = bars + 4;       // [4] its gate vectors written
+  uint64_t* empty = bars + 8;       // [4] the stage is read
+  uint64_t* p_full = bars + 12;     // P (and E W^T) accumulated
+  uint64_t* pp_ready = bars + 13;   // P' written, P drained
+  uint64_t* img_ready = bars + 14;  // [2] images of 32 tokens of W^T written
+  uint64_t* img_read = bars + 16;   // [2] and read
+  uint64_t* ds_full = bars + 18;    // [2] half of the increment accumulated
+  uint64_t* ds_empty = bars + 20;   // [2] and drained
+  uint64_t* h_ready = bars + 22;    // images of the state written
+  uint64_t* h_read = bars + 23;     // H^T X^T accumulated
+  uint64_t* o_full = bars + 24;     // W^T P'^T accumulated, P' read
+  uint64_t* o_empty = bars + 25;    // outputs drained
+  uint64_t* cleared = bars + 26;    // what lies behind the sequence in the tiles of its last chunk cleared
+  uint64_t* mma_end = bars + 27;    // [2] the MMAs of warps 3 and 1 are complete, when a wait has expired
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -149,10 +195,13 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       tc::mbar_init(&full[i], 1); tc::mbar_init(&gates[i], 1);
       tc::mbar_init(&empty[i], kState ? 9 : 12);  // the state's warps have read the decay, and: the issuer's commit, or the output warps
     }
-    for (uint64_t* b : {p_full, ds_full, h_read, o_full, mma_end}) tc::mbar_init(b, 1);
-    tc::mbar_init(pp_ready, 2); tc::mbar_init(yw_ready, 4);
-    tc::mbar_init(ds_empty, 8); tc::mbar_init(h_ready, 8);
-    tc::mbar_init(o_empty, 4);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&img_ready[i], 4); tc::mbar_init(&img_read[i], 1);
+      tc::mbar_init(&ds_full[i], 1); tc::mbar_init(&ds_empty[i], 8 / FH);
+    }
+    for (uint64_t* b : {p_full, h_read, o_full, &mma_end[0], &mma_end[1]}) tc::mbar_init(b, 1);
+    tc::mbar_init(cleared, 4);
+    tc::mbar_init(pp_ready, 6); tc::mbar_init(h_ready, 8); tc::mbar_init(o_empty, 4);
     *abort_flag = 0;
     tc::fence_barrier_init();
   }
@@ -197,201 +246,121 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
 
   if (warp < 4) {
     tc::reg_set<REGS_CTRL, REGS_LAUNCH>();
-    if (warp < 2) {
-      if constexpr (!kState) {
-        // -------------------------------------------------------------- P': row t a lane
-        const int t = 32 * warp + lane, r8 = lane & 7;
-        const uint32_t lane_addr = tm + ((uint32_t)(32 * warp) << 16);
-        int s = 0;
-        uint32_t ph = 0;
-        for (int c = 0; c < n_chunks; ++c) {
-          const uint32_t cp = (uint32_t)c & 1u;
-          const int at_tok = chunk_at(c) * C, len = min(C, seg.len - at_tok);
-          if (!all(tc::mbar_wait3(p_full, cp, &gates[s], ph, o_full, cp ^ 1u, abort_flag))) break;
-          tc::tc_fence_after_sync();
-          const float* gv = reinterpret_cast<const float*>(smem + K::GV + s * GATES);
-          uint8_t* row = smem + K::PP + t * 128;
-          [[maybe_unused]] float sum = 0.f;
-          // 16 columns from 16 k on, with factors f(column)
-          auto step = [&](int k, auto factors, bool diagonal) {
-            uint32_t x[16], hi[8], lo[8];
-            [[maybe_unused]] uint32_t pe[16];
-            tc::tmem_ld16(lane_addr + K::P + 16 * k, x);
-            if constexpr (kGrad) tc::tmem_ld16(lane_addr + K::PE + 16 * k, pe);
-            tc::tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              float p[4];
-              factors(16 * k + i, p);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                p[j] *= __uint_as_float(x[i + j]);
-                const int col = 16 * k + i + j;
-                // what is masked may be anything; backwards also what lies behind the sequence
-                if (diagonal && (kRev ? col < t : col > t)) p[j] = 0.f;
-                if (kRev && col >= len) p[j] = 0.f;
-                if constexpr (kGrad) {
-                  const bool counts = !(diagonal && (kRev ? col <= t : col >= t)) && !(kRev && col >= len);
-                  sum += counts ? p[j] * __uint_as_float(pe[i + j]) : 0.f;
-                }
-              }
-              split_pair(make_float2(p[0], p[1]), hi[i / 2], lo[i / 2]);
-              split_pair(make_float2(p[2], p[3]), hi[i / 2 + 1], lo[i / 2 + 1]);
-            }
-            *reinterpret_cast<uint4*>(row + (((2 * k) ^ r8) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(row + (((2 * k + 1) ^ r8) << 4)) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-            *reinterpret_cast<uint4*>(row + HALF + (((2 * k) ^ r8) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            *reinterpret_cast<uint4*>(row + HALF + (((2 * k + 1) ^ r8) << 4)) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-          };
-          if (warp == (kRev ? 0 : 1)) {  // the 32 x 32 block off the diagonal: a factor a row and one a column, meeting at token 31
-            const float r = a.scale_p * gv[GV_F + t];
-#pragma unroll 1
-            for (int k = kRev ? 2 : 0; k < (kRev ? 4 : 2); ++k)
-              step(k, [&](int col, float (&p)[4]) {
-                const float4 f = *reinterpret_cast<const float4*>(gv + GV_F + col);
-                p[0] = r * f.x; p[1] = r * f.y; p[2] = r * f.z; p[3] = r * f.w;
-              }, false);
-          }
-          const float gh = gv[GV_H + t], gl = gv[GV_L + t];
-#pragma unroll 1
-          for (int k = 2 * warp; k < 2 * warp + 2; ++k)
-            step(k, [&](int col, float (&p)[4]) {
-              const float4 h4 = *reinterpret_cast<const float4*>(gv + GV_H + col), l4 = *reinterpret_cast<const float4*>(gv + GV_L + col);
-              p[0] = a.scale_p * ex2((gh - h4.x) + (gl - l4.x)); p[1] = a.scale_p * ex2((gh - h4.y) + (gl - l4.y));
-              p[2] = a.scale_p * ex2((gh - h4.z) + (gl - l4.z)); p[3] = a.scale_p * ex2((gh - h4.w) + (gl - l4.w));
-            }, true);
-          tc::tc_fence_before_sync();
-          tc::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(pp_ready);
-          if constexpr (kGrad)
-            if (t < len) a.intra[((int64_t)h * a.B + seg.b) * a.T + seg.t0 + at_tok + t] = sum;
-          if (++s == K::STAGES) { s = 0; ph ^= 1u; }
-        }
-      }
-    } else if (warp == 2) {
-      // ---------------------------------------------------------------- loader (one lane), and gate vectors, two tokens a lane; sums of logarithms in 64 bits
+    if (warp == 0) {
+      // ---------------------------------------------------------------- loader
       if (lane == 0) {
         if (!kState) tc::prefetch_tmap(&maps.x);
         tc::prefetch_tmap(&maps.y); tc::prefetch_tmap(&maps.w);
-      }
-      constexpr double LOG2E = 1.4426950408889634;
-      double seg_total = 0.0;
-      const float* g = a.g != nullptr ? a.g + seg.b * a.g_stride_b + h : nullptr;
-      auto fetch = [&](int c, int e) {
-        const int t = chunk_at(c) * C + 2 * lane + e;
-        if (g == nullptr || t >= seg.len) return 0.f;
-        const float x = g[(int64_t)(seg.t0 + t) * a.g_stride_t];
-        return x < -1e6f ? -1e6f : x;  // (a NaN stays one)
-      };
-      float n0 = fetch(0, 0), n1 = fetch(0, 1);
-      int s = 0, issued = 0;
-      uint32_t ph = 1;
-      for (int c = 0; c < n_chunks; ++c) {
-        if (c >= K::STAGES && !all(tc::mbar_wait(&empty[s], ph, abort_flag))) break;
-        if (lane == 0) {
+        const int hx = h / a.x_div, hy = h / a.y_div, hw = h / a.w_div, he = h / a.e_div;
+        int s = 0, issued = 0;
+        uint32_t ph = 1;
+#pragma unroll 1
+        for (int c = 0; c < n_chunks; ++c) {
+          if (c >= K::STAGES && !tc::mbar_wait(&empty[s], ph, abort_flag)) break;
           uint8_t* st = smem + s * K::STAGE;
           const int tok = seg.t0 + chunk_at(c) * C;
           constexpr uint32_t bytes = (kState ? 1 : 2) * (DK / 64) * HALF + (kGrad ? 2 : 1) * (DV / 64) * HALF;
           tc::mbar_expect_tx(&full[s], bytes);
-          auto load = [&](const CUtensorMap* m, int at, int halves, int head) {
-#pragma unroll
-            for (int i = 0; i < halves; ++i) tc::tma_load_4d(st + at + i * HALF, m, &full[s], 64 * i, head, tok, seg.b);
-          };
-          load(&maps.y, K::Y, DK / 64, h / a.y_div);
-          load(&maps.w, K::W, DV / 64, h / a.w_div);
-          if constexpr (!kState) load(&maps.x, K::X, DK / 64, h / a.x_div);
-          if constexpr (kGrad) load(&maps.e, K::E, DV / 64, h / a.e_div);
+          tc::tma_load_5d(st + K::Y, &maps.y, &full[s], 0, tok, 0, hy, seg.b);
+          tc::tma_load_5d(st + K::W, &maps.w, &full[s], 0, tok, 0, hw, seg.b);
+          if constexpr (!kState) tc::tma_load_5d(st + K::X, &maps.x, &full[s], 0, tok, 0, hx, seg.b);
+          if constexpr (kGrad) tc::tma_load_5d(st + K::E, &maps.e, &full[s], 0, tok, 0, he, seg.b);
+          ++issued;
+          if (++s == K::STAGES) { s = 0; ph ^= 1u; }
         }
-        __syncwarp();
-        ++issued;
-        const double x0 = (double)n0 * LOG2E, x1 = (double)n1 * LOG2E;
-        if (c + 1 < n_chunks) { n0 = fetch(c + 1, 0); n1 = fetch(c + 1, 1); }
-        double sum = x0 + x1;
-#pragma unroll
+        // nothing is on its way into the shared memory of a CTA that ends, whatever became of those who wait for it
+#pragma unroll 1
+        for (int c = max(0, issued - K::STAGES); c < issued; ++c) tc::drain(&full[c % K::STAGES], (uint32_t)(c / K::STAGES) & 1u);
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- gate vectors, two tokens a lane
+      Two seg_total{0.f, 0.f};
+      const float* g = a.g != nullptr ? a.g + seg.b * a.g_stride_b + h : nullptr;
+      auto fetch = [&](int c, int e) {
+        const int t = chunk_at(c) * C + 2 * lane + e;
+        if (g == nullptr || t >= seg.len) return 0.f;
+        return g[(int64_t)(seg.t0 + t) * a.g_stride_t];
+      };
+      float n0 = fetch(0, 0), n1 = fetch(0, 1);
+      int s = 0;
+      uint32_t ph = 1;
+      for (int c = 0; c < n_chunks; ++c) {
+        if (c >= K::STAGES && !all(tc::mbar_wait(&empty[s], ph, abort_flag))) break;
+        const Two x0 = log2_of(n0 < -1e6f ? -1e6f : n0), x1 = log2_of(n1 < -1e6f ? -1e6f : n1);  // (a NaN stays one)
+        if (c + 1 < n_chunks) { n0 = fetch(c + 1, 0); n1 = fetch(c + 1, 1); }  // (not looked at before the next round)
+        Two G1 = add(x0, x1);
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += y;
+          const Two y = add(G1, shfl_up(G1, o));
+          if (lane >= o) G1 = y;
         }
-        const double total = __shfl_sync(0xffffffffu, sum, 31), mid = __shfl_sync(0xffffffffu, sum, 15);
-        const double G0 = sum - x1, G1 = sum;
-        seg_total += total;
+        const Two total = shfl(G1, 31), before = shfl_up(G1, 1);
+        const Two G0 = lane > 0 ? add(before, x0) : x0;
+        if constexpr (kState) seg_total = add(seg_total, total);
         const int left = seg.len - chunk_at(c) * C - 2 * lane;  // tokens from this lane's first on
-        const double sg = kRev ? -1.0 : 1.0;
-        const float2 e = make_float2(a.scale_e * ex2((float)(kRev ? total - G0 : G0)), a.scale_e * ex2((float)(kRev ? total - G1 : G1)));
-        float2 w = make_float2(a.scale_w * ex2((float)(kRev ? G0 : total - G0)), a.scale_w * ex2((float)(kRev ? G1 : total - G1)));
+        const float2 from0 = make_float2(ex2(G0.h + G0.l), ex2(G1.h + G1.l)), to_end = make_float2(ex2(diff(total, G0)), ex2(diff(total, G1)));
+        const float2 e = __fmul2_rn(make_float2(a.scale_e, a.scale_e), kRev ? to_end : from0);
+        float2 w = __fmul2_rn(make_float2(a.scale_w, a.scale_w), kRev ? from0 : to_end);
         if (left < 1) w.x = 0.f;
         if (left < 2) w.y = 0.f;
-        const float2 hi = make_float2((float)(sg * G0), (float)(sg * G1)), lo = make_float2((float)(sg * G0 - hi.x), (float)(sg * G1 - hi.y));
-        const bool behind = lane >= 16;
-        const float2 f = make_float2(ex2((float)(behind ? G0 - mid : mid - G0)), ex2((float)(behind ? G1 - mid : mid - G1)));
-        const float tot = (float)exp2(total);  // exact to the last bit: a state is multiplied by it once a chunk
+        const float sg = kRev ? -1.f : 1.f;
+        const float2 hi = make_float2(sg * G0.h, sg * G1.h), lo = make_float2(sg * G0.l, sg * G1.l);
+        const float tot = pow2(total);
         float* v = reinterpret_cast<float*>(smem + K::GV + s * GATES);
         reinterpret_cast<float2*>(v + GV_E)[lane] = e;
         reinterpret_cast<float2*>(v + GV_W)[lane] = w;
         reinterpret_cast<float2*>(v + GV_H)[lane] = hi;
         reinterpret_cast<float2*>(v + GV_L)[lane] = lo;
-        reinterpret_cast<float2*>(v + GV_F)[lane] = f;
         if (lane == 0) v[GV_TOT] = tot;
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&gates[s]);
         if (++s == K::STAGES) { s = 0; ph ^= 1u; }
       }
-      if (kState && lane == 0) a.seg_decay[seg_slot * a.Hv + h] = (float)exp2(seg_total);
-      // nothing is on its way into the shared memory of a CTA that ends, whatever became of those who wait for it
-      if (lane == 0) {
-#pragma unroll 1
-        for (int c = max(0, issued - K::STAGES); c < issued; ++c) tc::drain(&full[c % K::STAGES], (uint32_t)(c / K::STAGES) & 1u);
-      }
-    } else {
-      // ---------------------------------------------------------------- MMA issuer
+      if (kState && lane == 0) a.seg_decay[seg_slot * a.Hv + h] = pow2(seg_total);
+    } else if (warp == 3) {
+      // ---------------------------------------------------------------- MMA issuer of the state: increments, H^T X^T
       const uint32_t smem0 = tc::smem_u32(smem) >> 4;
       constexpr uint32_t hi_sw = tc::desc_hi(1024, true);
-      auto scores = [&](uint32_t at) {  // lanes 0..63 are the chunk's rows; the others multiply what lies behind the tile, and nobody reads them
-        if (tc::elect_one()) {
+      // Half f of the increment, the tokens by halves as their images come, the smallest terms first
+      auto increment = [&](int f, uint32_t at, uint32_t cp) {
 #pragma unroll
-          for (int k = 0; k < DK / 16; ++k)
-            tc::mma_ss(tm + K::P, tc::smem_desc(at + tc::desc_lo(K::X + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw),
-                       tc::smem_desc(at + tc::desc_lo(K::Y + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw), tc::idesc_f16(128, 64, 1, 1, false, false), k != 0);
-          if constexpr (kGrad) {
-#pragma unroll
-            for (int k = 0; k < DV / 16; ++k)
-              tc::mma_ss(tm + K::PE, tc::smem_desc(at + tc::desc_lo(K::E + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw),
-                         tc::smem_desc(at + tc::desc_lo(K::W + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw), tc::idesc_f16(128, 64, 1, 1, false, false), k != 0);
+        for (int q = 0; q < 2; ++q) {
+          if (f == 0) {
+            if (!all(tc::mbar_wait(&img_ready[q], cp, abort_flag))) return false;
+            tc::tc_fence_after_sync();
           }
-          tc::mma_commit(p_full);
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int t = K::TERMS - 1; t >= 0; --t)
+#pragma unroll
+              for (int k = 2 * q; k < 2 * q + 2; ++k)  // 16 tokens a step
+                tc::mma_ts(tm + K::DS + f * K::DS2, tm + K::IMG + 32 * t + 8 * k, tc::smem_desc(at + tc::desc_lo(K::Y + f * HALF + 2048 * k, HALF), hi_sw),
+                           tc::idesc_f16(128, 64, 1, 1, false, true), !(q == 0 && t == K::TERMS - 1 && k == 0));
+            if (f == FH - 1) tc::mma_commit(&img_read[q]);
+            if (q == 1) tc::mma_commit(&ds_full[f]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        return true;
       };
       int s = 0;
-      uint32_t ph = 0;
-      bool ok = all(tc::mbar_wait(&full[0], 0u, abort_flag));
-      if constexpr (!kState) {
-        tc::tc_fence_after_sync();
-        if (ok) scores(smem0);
-      }
-      for (int c = 0; c < n_chunks && ok; ++c) {
+      bool ok = true;
+#pragma unroll 1
+      for (int c = 0; c < n_chunks; ++c) {
         const uint32_t cp = (uint32_t)c & 1u, at = smem0 + s * (K::STAGE >> 4);
-        const int s_next = s + 1 == K::STAGES ? 0 : s + 1;
-        const uint32_t ph_next = s_next == 0 ? ph ^ 1u : ph;
-        // increment: the smallest terms first
-        ok = all(tc::mbar_wait2(yw_ready, cp, ds_empty, cp ^ 1u, abort_flag));
+        // (with one place for both halves of the increment, the one before has to be gone)
+        ok = all(tc::mbar_wait(&ds_empty[kGrad ? FH - 1 : 0], cp ^ 1u, abort_flag)) && increment(0, at, cp);
         if (!ok) break;
-        tc::tc_fence_after_sync();
-        if (tc::elect_one()) {
-#pragma unroll
-          for (int t = 2; t >= 0; --t)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)  // 16 tokens a step
-              tc::mma_ss(tm + K::DS, tc::smem_desc(at + tc::desc_lo(K::W + 2048 * k, HALF), hi_sw),
-                         tc::smem_desc(smem0 + tc::desc_lo(K::YW + t * TILE + 2048 * k, HALF), hi_sw), tc::idesc_f16(128, DK, 1, 1, true, true), !(t == 2 && k == 0));
-          tc::mma_commit(ds_full);
-          if constexpr (kState) tc::mma_commit(&empty[s]);
+        if constexpr (FH == 2) {
+          ok = all(tc::mbar_wait(&ds_empty[kGrad ? 0 : 1], kGrad ? cp : cp ^ 1u, abort_flag)) && increment(1, at, cp);
+          if (!ok) break;
         }
-        __syncwarp();
-        if constexpr (!kState) {
-          // (the accumulator that this takes was drained with the outputs of two chunks ago; with one accumulator o_empty has been waited for)
-          ok = all(tc::mbar_wait(h_ready, cp, abort_flag));
+        if constexpr (kState) {
+          if (tc::elect_one()) tc::mma_commit(&empty[s]);
+          __syncwarp();
+        } else {
+          // (the gradient of g: E W^T, in whose place H^T X^T goes, is drained with P)
+          ok = kGrad ? all(tc::mbar_wait2(h_ready, cp, pp_ready, cp, abort_flag)) : all(tc::mbar_wait2(h_ready, cp, o_empty, cp ^ 1u, abort_flag));
           if (!ok) break;
           tc::tc_fence_after_sync();
           if (tc::elect_one()) {
@@ -399,45 +368,77 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
             for (int t = K::HT - 1; t >= 0; --t)
 #pragma unroll
               for (int k = 0; k < DK / 16; ++k)
-                tc::mma_ts(tm + K::OI + cp * K::OI2, tm + K::H + t * 64 + 8 * k, tc::smem_desc(at + tc::desc_lo(K::X + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw),
+                tc::mma_ts(tm + K::OI, tm + K::H + t * 64 + 8 * k, tc::smem_desc(at + tc::desc_lo(K::X + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw),
                            tc::idesc_f16(128, 64, 1, 1, false, false), !(t == K::HT - 1 && k == 0));
             tc::mma_commit(h_read);
           }
           __syncwarp();
-          ok = all(tc::mbar_wait2(pp_ready, cp, o_empty, cp ^ 1u, abort_flag));
-          if (!ok) break;
-          tc::tc_fence_after_sync();
-          if (tc::elect_one()) {
-            // only blocks of the triangle; the first step covers all tokens
-#pragma unroll
-            for (int t = 1; t >= 0; --t)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int k = kRev ? 3 - i : i, row = kRev ? 0 : 16 * k, n = kRev ? 16 * (k + 1) : 64 - 16 * k;
-                tc::mma_ss(tm + K::OA + row, tc::smem_desc(at + tc::desc_lo(K::W + 2048 * k, HALF), hi_sw),
-                           tc::smem_desc(smem0 + tc::desc_lo(K::PP + t * HALF + row * 128 + 32 * k, 16), hi_sw), tc::idesc_f16(128, n, 1, 1, true, false),
-                           !(t == 1 && i == 0));
-              }
-            tc::mma_commit(o_full);
-          }
-          __syncwarp();
         }
+        if (++s == K::STAGES) s = 0;
+      }
+    } else if (!kState && warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer of the scores and of what they weigh: with one warp for all products its waits and issues, 4.1 k
+      // cycles a chunk, were what a chunk took
+      const uint32_t smem0 = tc::smem_u32(smem) >> 4;
+      constexpr uint32_t hi_sw = tc::desc_hi(1024, true);
+      const uint32_t neg = a.negative ? 1u << 13 : 0u;
+      // Columns 0..31 of the scores have the chunk's rows in lanes 0..63, columns 32..63 in lanes 64..127 (the left operand begins 64 rows early): all lanes' warps take
+      // a part of them.  The other halves multiply what lies in front of the tile and behind it, and nobody reads them.
+      auto scores = [&](uint32_t at) {
+        if (tc::elect_one()) {
+          auto product = [&](uint32_t d, int left, int right, int steps) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+              for (int k = 0; k < steps; ++k)
+                tc::mma_ss(d + 32 * half, tc::smem_desc(at + tc::desc_lo(left - half * HALF + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw),
+                           tc::smem_desc(at + tc::desc_lo(right + half * 4096 + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw), tc::idesc_f16(128, 32, 1, 1, false, false), k != 0);
+          };
+          product(tm + K::P, K::X, K::Y, DK / 16);
+          if constexpr (kGrad) product(tm + K::PE, K::E, K::W, DV / 16);
+          tc::mma_commit(p_full);
+        }
+        __syncwarp();
+      };
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = all(tc::mbar_wait(&full[0], 0u, abort_flag));
+      tc::tc_fence_after_sync();
+      if (ok) scores(smem0);
+#pragma unroll 1
+      for (int c = 0; c < n_chunks && ok; ++c) {
+        const uint32_t cp = (uint32_t)c & 1u, at = smem0 + s * (K::STAGE >> 4);
+        if (++s == K::STAGES) { s = 0; ph ^= 1u; }
+        ok = K::kAlias ? all(tc::mbar_wait(pp_ready, cp, abort_flag)) : all(tc::mbar_wait2(pp_ready, cp, o_empty, cp ^ 1u, abort_flag));
+        if (ok && seg.len - chunk_at(c) * C < C) ok = all(tc::mbar_wait(cleared, 0u, abort_flag));
+        if (!ok) break;
+        tc::tc_fence_after_sync();
+        if (tc::elect_one()) {
+          // only blocks of the triangle; the first step covers all tokens
+#pragma unroll
+          for (int t = 1; t >= 0; --t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = kRev ? 3 - i : i, row = kRev ? 0 : 16 * k, n = kRev ? 16 * (k + 1) : 64 - 16 * k;
+              tc::mma_ss(tm + K::OA + row, tc::smem_desc(at + tc::desc_lo(K::W + 2048 * k, HALF), hi_sw),
+                         tc::smem_desc(smem0 + tc::desc_lo(K::PP + t * HALF + row * 128 + 32 * k, 16), hi_sw), tc::idesc_f16(128, n, 1, 1, true, false) | neg,
+                         !(t == 1 && i == 0));
+            }
+          tc::mma_commit(o_full);
+        }
+        __syncwarp();
         if (c + 1 < n_chunks) {
-          if (kGrad) ok = all(tc::mbar_wait2(&full[s_next], ph_next, o_empty, cp, abort_flag));
-          else ok = all(tc::mbar_wait(&full[s_next], ph_next, abort_flag));
-          if constexpr (!kState) {
-            tc::tc_fence_after_sync();
-            if (ok) scores(smem0 + s_next * (K::STAGE >> 4));
-          }
+          ok = K::kAlias ? all(tc::mbar_wait2(&full[s], ph, o_empty, cp, abort_flag)) : all(tc::mbar_wait(&full[s], ph, abort_flag));
+          tc::tc_fence_after_sync();
+          if (ok) scores(smem0 + s * (K::STAGE >> 4));
         }
-        s = s_next; ph = ph_next;
       }
     }
   } else if (warp < 12) {
     tc::reg_set<REGS_STATE, REGS_LAUNCH>();
-    // ------------------------------------------------------------------ state: group grp has half of the columns (features of Y)
+    // ------------------------------------------------------------------ state and P': group grp has half of the state's columns (features of Y)
     constexpr int HC = DK / 2;
-    const int grp = (warp - 4) >> 2, d = (warp & 3) * 32 + lane;
+    const int grp = (warp - 4) >> 2, half = FH == 2 ? grp : 0, d = (warp & 3) * 32 + lane;
     const uint32_t lane_addr = tm + ((uint32_t)((warp & 3) * 32) << 16);
     const bool mine = d < DV;
     float2 S[HC / 2];
@@ -472,19 +473,80 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(h_ready);
     };
-    if constexpr (!kState) publish();
-    int s = 0;
+    // P': 32 rows x 16 columns a warp, row t a lane.  Blocks in which no row has a part are neither written nor read: six warps are left.
+    const int t = 32 * (warp & 1) + lane, col0 = 32 * ((warp & 3) >> 1) + 16 * grp;
+    const bool has_part = kRev ? col0 + 15 >= 32 * (warp & 1) : col0 <= 32 * (warp & 1) + 31;
+    auto weigh = [&](int c, int s, uint32_t ph) {
+      const int at_tok = chunk_at(c) * C, len = min(C, seg.len - at_tok);
+      [[maybe_unused]] float sum = 0.f;
+      if (has_part) {
+        const uint32_t cp = (uint32_t)c & 1u;
+        if (!all(tc::mbar_wait3(p_full, cp, &gates[s], ph, o_full, cp ^ 1u, abort_flag))) return false;
+        tc::tc_fence_after_sync();
+        const float* gv = reinterpret_cast<const float*>(smem + K::GV + s * GATES);
+        uint8_t* row = smem + K::PP + t * 128;
+        const float2 gh = make_float2(gv[GV_H + t], gv[GV_H + t]);
+        const float gl1 = gv[GV_L + t] + a.log_scale;
+        const float2 gl = make_float2(gl1, gl1);
+        // eight columns at a time, in a loop that stays rolled: the code that a chunk runs has to fit the SM's instruction cache
+#pragma unroll 1
+        for (int k = col0; k < col0 + 16; k += 8) {
+          uint32_t x[8], hi[4], lo[4];
+          [[maybe_unused]] uint32_t pe[8];
+          tc::tmem_ld8(lane_addr + K::P + k, x);
+          if constexpr (kGrad) tc::tmem_ld8(lane_addr + K::PE + k, pe);
+          tc::tmem_ld_wait();
+          const int own = t - k, last = len - k;  // columns in front of own (forwards) or behind it have a part
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            const float4 h4 = *reinterpret_cast<const float4*>(gv + GV_H + k + i), l4 = *reinterpret_cast<const float4*>(gv + GV_L + k + i);
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+              const float2 d = __fadd2_rn(__fadd2_rn(gh, j ? make_float2(-h4.z, -h4.w) : make_float2(-h4.x, -h4.y)),
+                                          __fadd2_rn(gl, j ? make_float2(-l4.z, -l4.w) : make_float2(-l4.x, -l4.y)));
+              float2 p = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), make_float2(__uint_as_float(x[i + j]), __uint_as_float(x[i + j + 1])));
+              // what is masked may be anything; backwards also what lies behind the sequence
+              if (kRev ? i + j < own || i + j >= last : i + j > own) p.x = 0.f;
+              if (kRev ? i + j + 1 < own || i + j + 1 >= last : i + j + 1 > own) p.y = 0.f;
+              if constexpr (kGrad) {  // (masked columns have to be kept from a NaN in the other product too)
+                if (kRev ? i + j > own && i + j < last : i + j < own) sum = fmaf(p.x, __uint_as_float(pe[i + j]), sum);
+                if (kRev ? i + j + 1 > own && i + j + 1 < last : i + j + 1 < own) sum = fmaf(p.y, __uint_as_float(pe[i + j + 1]), sum);
+              }
+              split_pair(p, hi[(i + j) / 2], lo[(i + j) / 2]);
+            }
+          }
+          uint8_t* piece = row + (((k >> 3) ^ (lane & 7)) << 4);
+          *reinterpret_cast<uint4*>(piece) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(piece + HALF) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        tc::tc_fence_before_sync();
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(pp_ready);
+      }
+      if constexpr (kGrad)
+        if (t < len) a.intra[(((int64_t)(col0 >> 4) * a.Hv + h) * a.B + seg.b) * a.T + seg.t0 + at_tok + t] = a.negative ? -sum : sum;
+      return true;
+    };
     bool ok = true;
+    int s = 0;
+    uint32_t ph = 0;
+#pragma unroll 1
     for (int c = 0; c < n_chunks; ++c) {
       const uint32_t cp = (uint32_t)c & 1u;
-      ok = all(tc::mbar_wait(ds_full, cp, abort_flag));  // (the gate vectors were there before Yw was)
+      if constexpr (!kState) {
+        publish();
+        ok = weigh(c, s, ph);
+        if (!ok) break;
+      }
+      ok = all(tc::mbar_wait(&ds_full[half], cp, abort_flag));  // (the gate vectors were there before the images were)
       if (!ok) break;
       tc::tc_fence_after_sync();
       const float decay = reinterpret_cast<const float*>(smem + K::GV + s * GATES)[GV_TOT];
 #pragma unroll
       for (int q = 0; q < HC / 16; ++q) {
         uint32_t x[16];
-        tc::tmem_ld16(lane_addr + K::DS + HC * grp + 16 * q, x);
+        tc::tmem_ld16(lane_addr + K::DS + (FH == 2 ? half * K::DS2 : HC * grp) + 16 * q, x);
         tc::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -492,14 +554,13 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       }
       tc::tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) { tc::mbar_arrive(ds_empty); tc::mbar_arrive(&empty[s]); }
-      if (++s == K::STAGES) s = 0;
+      if (lane == 0) { tc::mbar_arrive(&ds_empty[half]); tc::mbar_arrive(&empty[s]); }
+      if (++s == K::STAGES) { s = 0; ph ^= 1u; }
       if constexpr (!kState) {
-        if (c + 1 < n_chunks) {
+        if (c + 1 < n_chunks) {  // the images may be written again
           ok = all(tc::mbar_wait(h_read, cp, abort_flag));
           if (!ok) break;
           tc::tc_fence_after_sync();
-          publish();
         }
       }
     }
@@ -514,18 +575,25 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   } else if (warp < 16) {
     tc::reg_set<REGS_OUT, REGS_LAUNCH>();
     // ------------------------------------------------------------------ outputs: 32 features a warp, as accumulator fragments of warp-level MMAs, which matrix stores
-    // transpose on their way into shared memory, in the place of the chunk's X (and Y, for 32-bit rows), whose readers are through
+    // transpose on their way into shared memory, in the place of the chunk's X (and Y, for 32-bit rows), whose readers are through; they leave by asynchronous copies
     if constexpr (!kState) {
       const int wq = warp & 3, gr = lane >> 2, t2 = 2 * (lane & 3), r8 = lane & 7, m4 = lane >> 3;
       const uint32_t lane_addr = tm + ((uint32_t)(wq * 32) << 16);
       const bool mine = 32 * wq < DV, f32 = a.o_part != nullptr;
+      int before = -1;  // stage of the chunk before, whose rows may still be on their way out: its next tiles come when they have been read
+      auto release = [&]() {
+        if (lane == 0 && before >= 0) {
+          tc::bulk_wait_read<0>();
+          tc::mbar_arrive(&empty[before]);
+        }
+      };
       int s = 0;
       for (int c = 0; c < n_chunks; ++c) {
         const uint32_t cp = (uint32_t)c & 1u;
-        if (!all(tc::mbar_wait(o_full, cp, abort_flag))) break;
+        if (!all(tc::mbar_wait2(o_full, cp, h_read, cp, abort_flag))) break;
         tc::tc_fence_after_sync();
         const float* gv = reinterpret_cast<const float*>(smem + K::GV + s * GATES);
-        uint8_t* stage = smem + s * K::STAGE + wq * (f32 ? 8192 : 4096);
+        uint8_t* stage = smem + s * K::STAGE + (f32 ? K::Y + 8192 * wq : K::X + 4096 * wq);
         const uint32_t stage_s = tc::smem_u32(stage);
         const int at_tok = chunk_at(c) * C, len = min(C, seg.len - at_tok);
         const int64_t tok0 = seg.t0 + at_tok;
@@ -537,13 +605,14 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
 #pragma unroll 1
           for (int hf = 0; hf < 2; ++hf) {  // 16 features
             uint32_t oi[32], oa[32];
-            tc::tmem_ld_frags(lane_addr + ((uint32_t)hf << 20) + K::OI + cp * K::OI2, oi);
+            tc::tmem_ld_frags(lane_addr + ((uint32_t)hf << 20) + K::OI, oi);
             tc::tmem_ld_frags(lane_addr + ((uint32_t)hf << 20) + K::OA, oa);
             tc::tmem_ld_wait();
             if (hf == 1) {
               tc::tc_fence_before_sync();
               __syncwarp();
               if (lane == 0) tc::mbar_arrive(o_empty);
+              release();
             }
             if constexpr (kGrad) {  // E's pieces in the layout of the fragments
               const uint32_t e_s = tc::smem_u32(smem + s * K::STAGE + K::E) + (uint32_t)((wq >> 1) * HALF + (8 * (m4 >> 1) + r8) * 128 +
@@ -597,7 +666,10 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (!mine && lane == 0) tc::mbar_arrive(o_empty);
+        if (!mine) {
+          if (lane == 0) tc::mbar_arrive(o_empty);
+          release();
+        }
         if constexpr (kGrad) {
           // sums over the eight lanes of a token's features; lane (gr, t2 / 2) ends with the tokens 8 gr + t2, 8 gr + t2 + 1
 #pragma unroll
@@ -617,7 +689,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         }
         if (mine) {
           if (len == C && (f32 || maps.o_ok)) {
-            if (lane == 0) tc::tma_store_4d(f32 ? &maps.o32 : &maps.o, stage, 32 * wq, h, (int)tok0, seg.b);
+            if (lane == 0) tc::tma_store_4d(&maps.o, stage, 32 * wq, h, (int)tok0, seg.b);
           } else if (f32) {
             float* dst = a.o_part + (((int64_t)seg.b * a.T + tok0) * a.Hv + h) * DV + 32 * wq + 4 * r8;
 #pragma unroll 1
@@ -629,61 +701,80 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
             for (int t = lane >> 2; t < len; t += 8) *reinterpret_cast<uint4*>(dst + (int64_t)t * a.o_stride_t) = *reinterpret_cast<const uint4*>(stage + t * 64 + (((lane & 3) ^ ((t >> 1) & 3)) << 4));
             tc::fence_proxy_async_smem();
           }
+          __syncwarp();
+          if (lane == 0) tc::bulk_commit();
         }
-        if (lane == 0) {  // the next tiles of this stage come when it has been read
-          tc::bulk_commit();
-          tc::bulk_wait_read<0>();
-        }
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&empty[s]);
+        before = s;
         if (++s == K::STAGES) s = 0;
       }
       if (lane == 0) tc::bulk_wait_all();
     }
   } else {
     tc::reg_set<REGS_PREP, REGS_LAUNCH>();
-    {
-      // ---------------------------------------------------------------- Yw: a piece (8 features of a token) at a time, in the places that Y's has
-      constexpr int N = 128;
-      const int tid = (warp - 16) * 32 + lane;
-      int s = 0;
-      uint32_t ph = 0;
-      for (int c = 0; c < n_chunks; ++c) {
-        const uint32_t cp = (uint32_t)c & 1u;
-        const int len = min(C, seg.len - chunk_at(c) * C);
-        if (!all(tc::mbar_wait3(&full[s], ph, &gates[s], ph, ds_full, cp ^ 1u, abort_flag))) break;
-        const float* gv = reinterpret_cast<const float*>(smem + K::GV + s * GATES);
-        uint8_t* st = smem + s * K::STAGE;
-#pragma unroll 2
-        for (int i = tid; i < (DK / 64) * 512; i += N) {
-          const int tok = (i >> 3) & 63;
-          const float w = gv[GV_W + tok];
-          uint4 y = *reinterpret_cast<const uint4*>(st + K::Y + 16 * i);
-          if (tok >= len) y = make_uint4(0u, 0u, 0u, 0u);  // (may be anything, and w is zero)
-          const uint32_t in[4] = {y.x, y.y, y.z, y.w};
-          uint32_t h0[4], h1[4], h2[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = bf16x2_to_float2(in[j]);
-            split3(__fmul2_rn(f, make_float2(w, w)), h0[j], h1[j], h2[j]);
-          }
-          uint8_t* dst = smem + K::YW + 16 * i;
-          *reinterpret_cast<uint4*>(dst) = make_uint4(h0[0], h0[1], h0[2], h0[3]);
-          *reinterpret_cast<uint4*>(dst + TILE) = make_uint4(h1[0], h1[1], h1[2], h1[3]);
-          *reinterpret_cast<uint4*>(dst + 2 * TILE) = make_uint4(h2[0], h2[1], h2[2], h2[3]);
-        }
-        // What lies behind the sequence in W's tile may be anything, and a product of zero with it need not be zero
-        if (len < C)
+    // ------------------------------------------------------------------ images of W^T, each token times its weight, in bf16 terms: 32 features a warp, which matrix loads transpose into
+    // pairs of tokens, the layout of a left operand.  (Y times the weights, in shared memory as right operand, was 64 KB more through shared memory a chunk, which
+    // bounded it, and a third more instructions.)
+    const int wq = warp & 3, r8 = lane & 7, m4 = lane >> 3, t2 = 2 * (lane & 3);
+    int s = 0;
+    uint32_t ph = 0;
 #pragma unroll 1
-          for (int i = 8 * len + tid; i < 512; i += N) {
-            *reinterpret_cast<uint4*>(st + K::W + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
-            if constexpr (DV == 128) *reinterpret_cast<uint4*>(st + K::W + HALF + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
-          }
+    for (int c = 0; c < n_chunks; ++c) {
+      const uint32_t cp = (uint32_t)c & 1u;
+      const int len = min(C, seg.len - chunk_at(c) * C);
+      bool ok = all(tc::mbar_wait2(&full[s], ph, &gates[s], ph, abort_flag));
+      const float* gv = reinterpret_cast<const float*>(smem + K::GV + s * GATES);
+      uint8_t* st = smem + s * K::STAGE;
+      if (ok && len < C) {  // What lies behind the sequence in the tiles may be anything, and a product of zero with it need not be zero
+        auto clear = [&](int at) { *reinterpret_cast<uint4*>(st + at) = make_uint4(0u, 0u, 0u, 0u); };
+#pragma unroll 1
+        for (int i = 8 * len + (threadIdx.x & 127); i < 512; i += 128) {
+          clear(K::Y + 16 * i);
+          if constexpr (DK == 128) clear(K::Y + HALF + 16 * i);
+          if constexpr (!kState) clear(K::W + 16 * i);
+          if constexpr (!kState && DV == 128) clear(K::W + HALF + 16 * i);
+        }
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(yw_ready);
-        if (++s == K::STAGES) { s = 0; ph ^= 1u; }
+        if (lane == 0) tc::mbar_arrive(cleared);
       }
+#pragma unroll 1
+      for (int q = 0; q < 2; ++q) {  // 32 tokens
+        ok = ok && all(tc::mbar_wait(&img_read[q], cp ^ 1u, abort_flag));
+        if (!ok) break;
+        tc::tc_fence_after_sync();
+        if (32 * wq < DV) {
+          float2 w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float2*>(gv + GV_W + 32 * q + 8 * i + t2);
+#pragma unroll 1
+          for (int hf = 0; hf < 2; ++hf) {  // 16 features
+            const uint32_t w_s = tc::smem_u32(st + K::W) + (uint32_t)((wq >> 1) * HALF + (32 * q + 8 * (m4 >> 1) + r8) * 128 + (((4 * (wq & 1) + 2 * hf + (m4 & 1)) ^ r8) << 4));
+            uint32_t x[8], terms[3][8];
+            ldsm4t(reinterpret_cast<uint32_t(&)[4]>(x[0]), w_s);
+            ldsm4t(reinterpret_cast<uint32_t(&)[4]>(x[4]), w_s + 2048);
+            if (len < C)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int t = 32 * q + 8 * (i >> 1) + t2;
+                if (t + 1 >= len) x[i] = t >= len ? 0u : x[i] & 0xffffu;
+              }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float2 f = __fmul2_rn(bf16x2_to_float2(x[i]), w[i >> 1]);
+              if constexpr (K::TERMS == 3) split3(f, terms[0][i], terms[1][i], terms[2][i]);
+              else split_pair(f, terms[0][i], terms[1][i]);
+            }
+#pragma unroll
+            for (int t = 0; t < K::TERMS; ++t) tc::tmem_st_pairs(tm + ((uint32_t)(32 * wq + 16 * hf) << 16) + K::IMG + 32 * t + 16 * q, terms[t]);
+          }
+          tc::tmem_st_wait();
+        }
+        tc::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&img_ready[q]);
+      }
+      if (!ok) break;
+      if (++s == K::STAGES) { s = 0; ph ^= 1u; }
     }
   }
 
@@ -691,7 +782,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   __syncthreads();
   if (*abort_flag != 0u) {  // (the roles have ended: it stays as it is)
     if (threadIdx.x == 0 && a.status != nullptr) atomicOr(a.status, AVE_GDN_DEV_WAIT_EXPIRED);
-    if (warp == 3) tc::drain_mmas(mma_end);
+    if (warp == 3 || (!kState && warp == 1)) tc::drain_mmas(&mma_end[warp == 1]);
     tc::tc_fence_before_sync();
     __syncthreads();
   }

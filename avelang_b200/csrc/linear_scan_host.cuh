@@ -1,6 +1,7 @@
 // Host side of the scans of linear attention: how a batch is cut into segments, tensor maps, launches.
 #pragma once
 #include <atomic>
+#include <cmath>
 
 #include "linear_scan.cuh"
 
@@ -38,6 +39,11 @@ inline Plan plan_of(int B, int64_t T, int n_seqs, bool packed, int heads) {
   return p;
 }
 
+inline void set_scale(Args& a, float scale) {  // of P'
+  a.log_scale = (float)log2(fabs((double)scale));
+  a.negative = scale < 0.f;
+}
+
 inline size_t state_bytes(const Plan& p, int heads, int dk, int dv) {  // increments and entering states, and the segments' decays
   return p.cut ? (size_t)p.slots * heads * ((size_t)dk * dv * 4) + (((size_t)p.slots * heads * 4 + 255) & ~(size_t)255) : 0;
 }
@@ -46,13 +52,14 @@ inline void place_states(Args& a, void* ws, int dk, int dv) {
   a.seg_decay = a.seg_state + (size_t)a.plan.slots * a.Hv * dk * dv;
 }
 
-// 64 features of 64 tokens of a [B, T, heads, d] tensor
+// A head's features of 64 tokens of a [B, T, heads, d] tensor: 64 features after 64 features, so that a tile is one copy
 inline int operand_map(CUtensorMap* m, const void* p, int d, int heads, int B, int T, int64_t sb, int64_t st, int64_t sh) {
-  const uint32_t box[4] = {64, 1, 64, 1};
-  const uint64_t dims[4] = {(uint64_t)d, (uint64_t)heads, (uint64_t)T, (uint64_t)B};
-  const uint64_t str[4] = {2, (uint64_t)(heads > 1 ? sh : d) * 2, (uint64_t)(T > 1 ? st : d) * 2, (uint64_t)(B > 1 ? sb : d) * 2};
-  return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint32_t box[5] = {64, 64, (uint32_t)d / 64, 1, 1};
+  const uint64_t dims[5] = {64, (uint64_t)T, (uint64_t)d / 64, (uint64_t)heads, (uint64_t)B};
+  const uint64_t str[5] = {2, (uint64_t)(T > 1 ? st : d) * 2, 128, (uint64_t)(heads > 1 ? sh : d) * 2, (uint64_t)(B > 1 ? sb : d) * 2};
+  return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), 5, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
+
 // 32 features of 64 tokens of the result; where its layout has no map, rows leave by 16-byte stores
 inline bool result_map(CUtensorMap* m, void* p, int d, int heads, int B, int T, int64_t sb, int64_t st, int64_t sh) {
   const uint32_t box[4] = {32, 1, 64, 1};
@@ -65,10 +72,10 @@ inline bool result_map(CUtensorMap* m, void* p, int d, int heads, int B, int T, 
 }
 
 // The register split of the roles counts on the registers that the kernel is launched with.
-template <int DK, int DV, bool kRev, bool kState, bool kGrad>
+template <int DK, int DV, bool kRev, Mode kMode>
 int launch_scan(const Args& a, const Maps& maps, cudaStream_t stream) {
-  auto* kernel = scan_kernel<DK, DV, kRev, kState, kGrad>;
-  constexpr int smem = Cfg<kState, kGrad>::SMEM;
+  auto* kernel = scan_kernel<DK, DV, kRev, kMode>;
+  constexpr int smem = Cfg<kMode>::SMEM;
   static std::atomic<bool> ready[MAX_DEVICES];
   int dev = 0;
   AVE_CUDA_TRY(cudaGetDevice(&dev));
