@@ -119,7 +119,7 @@ struct Cfg {
   // of Y each) one another's.
   static constexpr bool kAlias = TERMS == 3;
   static constexpr uint32_t P = 0, OA = kAlias ? 0 : 64, OI = kAlias ? 64 : 128, PE = OI;
-  static constexpr uint32_t DS = kState ? 0 : kAlias ? 128 : 192, DS2 = kGrad ? 0 : 64, H = DS + (kGrad ? 64 : 128), IMG = kState ? 128 : H + 64 * HT;
+  static constexpr uint32_t DS = kState ? 0 : kAlias ? 128 : 192, H = DS + (kGrad ? 64 : 128), IMG = kState ? 128 : H + 64 * HT;
   static constexpr uint32_t COLS = kState ? 256 : 512;
   static_assert(IMG + 32 * TERMS <= COLS, "tensor memory");
 };
@@ -167,7 +167,7 @@ template <int DK, int DV, bool kRev, Mode kMode>
 __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __grid_constant__ Maps maps) {
   using K = Cfg<kMode>;
   constexpr bool kState = K::kState, kGrad = K::kGrad;
-  constexpr int FH = DK / 64;  // halves of the increment; group g of the state's warps takes half g, or half of the only one
+  constexpr int FH = kGrad ? DK / 64 : 1;  // parts in which the increment comes: group g of the state's warps takes part g, or half of the only one
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = tc::align1024(smem_raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + K::BARS);
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   uint64_t* pp_ready = bars + 13;   // P' written, P drained
   uint64_t* img_ready = bars + 14;  // [2] images of 32 tokens of W^T written
   uint64_t* img_read = bars + 16;   // [2] and read
-  uint64_t* ds_full = bars + 18;    // [2] half of the increment accumulated
+  uint64_t* ds_full = bars + 18;    // [2] the increment accumulated; with the gradient of g one half after the other
   uint64_t* ds_empty = bars + 20;   // [2] and drained
   uint64_t* h_ready = bars + 22;    // images of the state written
   uint64_t* h_read = bars + 23;     // H^T X^T accumulated
@@ -187,6 +187,9 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   uint64_t* cleared = bars + 26;    // what lies behind the sequence in the tiles of its last chunk cleared
   uint64_t* mma_end = bars + 27;    // [2] the MMAs of warps 3 and 1 are complete, when a wait has expired
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+  // A wait sees only the parity of a barrier's phase, so no barrier may complete twice before each of its waiters has seen the first time.  All are ordered by the arrivals they
+  // need: the products of a chunk by what is written for them, that by the products of the chunk before, and o_full, for which the output warps wait too, by o_empty of the
+  // chunk before.
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -321,39 +324,46 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       // ---------------------------------------------------------------- MMA issuer of the state: increments, H^T X^T
       const uint32_t smem0 = tc::smem_u32(smem) >> 4;
       constexpr uint32_t hi_sw = tc::desc_hi(1024, true);
-      // Half f of the increment, the tokens by halves as their images come, the smallest terms first
-      auto increment = [&](int f, uint32_t at, uint32_t cp) {
+      // 32 tokens' part of the increment, or of half f of it, the smallest terms first
+      constexpr int N = kGrad ? 64 : DK;
+      auto part = [&](int f, int q, uint32_t at) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          if (f == 0) {
-            if (!all(tc::mbar_wait(&img_ready[q], cp, abort_flag))) return false;
-            tc::tc_fence_after_sync();
-          }
-          if (tc::elect_one()) {
+        for (int t = K::TERMS - 1; t >= 0; --t)
 #pragma unroll
-            for (int t = K::TERMS - 1; t >= 0; --t)
-#pragma unroll
-              for (int k = 2 * q; k < 2 * q + 2; ++k)  // 16 tokens a step
-                tc::mma_ts(tm + K::DS + f * K::DS2, tm + K::IMG + 32 * t + 8 * k, tc::smem_desc(at + tc::desc_lo(K::Y + f * HALF + 2048 * k, HALF), hi_sw),
-                           tc::idesc_f16(128, 64, 1, 1, false, true), !(q == 0 && t == K::TERMS - 1 && k == 0));
-            if (f == FH - 1) tc::mma_commit(&img_read[q]);
-            if (q == 1) tc::mma_commit(&ds_full[f]);
-          }
-          __syncwarp();
-        }
-        return true;
+          for (int k = 2 * q; k < 2 * q + 2; ++k)  // 16 tokens a step
+            tc::mma_ts(tm + K::DS, tm + K::IMG + 32 * t + 8 * k, tc::smem_desc(at + tc::desc_lo(K::Y + f * HALF + 2048 * k, HALF), hi_sw),
+                       tc::idesc_f16(128, N, 1, 1, false, true), !(q == 0 && t == K::TERMS - 1 && k == 0));
       };
       int s = 0;
       bool ok = true;
 #pragma unroll 1
       for (int c = 0; c < n_chunks; ++c) {
         const uint32_t cp = (uint32_t)c & 1u, at = smem0 + s * (K::STAGE >> 4);
-        // (with one place for both halves of the increment, the one before has to be gone)
-        ok = all(tc::mbar_wait(&ds_empty[kGrad ? FH - 1 : 0], cp ^ 1u, abort_flag)) && increment(0, at, cp);
-        if (!ok) break;
-        if constexpr (FH == 2) {
-          ok = all(tc::mbar_wait(&ds_empty[kGrad ? 0 : 1], kGrad ? cp : cp ^ 1u, abort_flag)) && increment(1, at, cp);
+        if constexpr (kGrad && FH == 2) {  // one place for both halves of the increment: they come one after the other
+          ok = all(tc::mbar_wait3(&ds_empty[1], cp ^ 1u, &img_ready[0], cp, &img_ready[1], cp, abort_flag));
           if (!ok) break;
+          tc::tc_fence_after_sync();
+          if (tc::elect_one()) { part(0, 0, at); part(0, 1, at); tc::mma_commit(&ds_full[0]); }
+          __syncwarp();
+          ok = all(tc::mbar_wait(&ds_empty[0], cp, abort_flag));
+          if (!ok) break;
+          tc::tc_fence_after_sync();
+          if (tc::elect_one()) {
+            part(1, 0, at); part(1, 1, at);
+            tc::mma_commit(&img_read[0]); tc::mma_commit(&img_read[1]); tc::mma_commit(&ds_full[1]);
+          }
+          __syncwarp();
+        } else {  // the tokens by halves, as their images come, so that those of the next chunk are written beside it
+          ok = all(tc::mbar_wait2(&ds_empty[0], cp ^ 1u, &img_ready[0], cp, abort_flag));
+          if (!ok) break;
+          tc::tc_fence_after_sync();
+          if (tc::elect_one()) { part(0, 0, at); tc::mma_commit(&img_read[0]); }
+          __syncwarp();
+          ok = all(tc::mbar_wait(&img_ready[1], cp, abort_flag));
+          if (!ok) break;
+          tc::tc_fence_after_sync();
+          if (tc::elect_one()) { part(0, 1, at); tc::mma_commit(&ds_full[0]); tc::mma_commit(&img_read[1]); }
+          __syncwarp();
         }
         if constexpr (kState) {
           if (tc::elect_one()) tc::mma_commit(&empty[s]);
@@ -546,7 +556,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
 #pragma unroll
       for (int q = 0; q < HC / 16; ++q) {
         uint32_t x[16];
-        tc::tmem_ld16(lane_addr + K::DS + (FH == 2 ? half * K::DS2 : HC * grp) + 16 * q, x);
+        tc::tmem_ld16(lane_addr + K::DS + (FH == 2 ? 0 : HC * grp) + 16 * q, x);
         tc::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 8; ++i)
