@@ -208,6 +208,7 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
   if (l.plan.cut) {
     fwd.seg_state = f32(l.s); fwd.seg_decay = f32(l.s_decay);
     rev.seg_state = f32(l.r); rev.seg_decay = f32(l.r_decay);
+    rev.state_out = a.d_initial_state; rev.final_by_chain = a.d_initial_state != nullptr;
   }
   // gradient of q or k: dk features of Hk heads, summed over the value heads
   auto rows_of = [&](lin::Args& s, lin::Maps& m, void* out) {
@@ -249,7 +250,7 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
       m.x = mk; m.y = mq; m.w = mo;
       s.o = a.d_v; s.o_stride_h = a.dv; s.o_stride_t = (int64_t)a.Hv * a.dv; s.o_stride_b = s.o_stride_t * a.T;
       m.o_ok = lin::result_map(&m.o, a.d_v, a.dv, a.Hv, a.B, a.T, s.o_stride_b, s.o_stride_t, s.o_stride_h);
-      r = s.state_out != nullptr ? lin::launch_scan<DK, DV, true, lin::OUT3>(s, m, stream) : lin::launch_scan<DK, DV, true, lin::OUT2>(s, m, stream);
+      r = s.state_out != nullptr && !s.final_by_chain ? lin::launch_scan<DK, DV, true, lin::OUT3>(s, m, stream) : lin::launch_scan<DK, DV, true, lin::OUT2>(s, m, stream);
       if (r) return r;
     }
     {  // dq
@@ -265,6 +266,7 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
     {  // dk
       lin::Args s = rev;
       lin::Maps m{};
+      s.state_out = nullptr;
       s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; lin::set_scale(s, a.scale); s.scale_e = 1.f; s.st_y = 1; s.st_w = a.dv;
       m.x = mv; m.y = mo; m.w = mq; m.e = mk;
       if ((r = rows_of(s, m, a.d_k))) return r;

@@ -19,7 +19,10 @@ int launch_linear_prefill(const AveLinearArgs& a, cudaStream_t stream) {
   s.o = a.o; s.o_stride_b = a.o_stride_b; s.o_stride_t = a.o_stride_t; s.o_stride_h = a.o_stride_h;
   s.state_in = a.initial_state; s.state_out = a.final_state; s.st_y = a.dv; s.st_w = 1;
   s.plan = prefill_plan(a);
-  if (s.plan.cut) lin::place_states(s, a.workspace, a.dk, a.dv);
+  if (s.plan.cut) {
+    lin::place_states(s, a.workspace, a.dk, a.dv);
+    s.final_by_chain = a.final_state != nullptr;
+  }
   lin::Maps m{};
   int rc;
   if ((rc = lin::operand_map(&m.x, a.q, a.dk, a.Hk, a.B, a.T, a.q_stride_b, a.q_stride_t, a.q_stride_h))) return rc;
@@ -32,7 +35,7 @@ int launch_linear_prefill(const AveLinearArgs& a, cudaStream_t stream) {
       if (r == AVE_GDN_OK) r = lin::launch_chain<dk, dv, false>(s, stream);
       if (r != AVE_GDN_OK) return r;
     }
-    return s.state_out != nullptr ? lin::launch_scan<dk, dv, false, lin::OUT3>(s, m, stream) : lin::launch_scan<dk, dv, false, lin::OUT2>(s, m, stream);
+    return s.state_out != nullptr && !s.final_by_chain ? lin::launch_scan<dk, dv, false, lin::OUT3>(s, m, stream) : lin::launch_scan<dk, dv, false, lin::OUT2>(s, m, stream);
   });
 }
 

@@ -45,6 +45,7 @@ struct Args {
   float* o_part;                   // fp32 [B, T, Hv, dv] instead, for a sum over heads behind the scan
   const float* state_in;           // [slot, Hv, ..]: element (y feature, w feature) at y * st_y + w * st_w
   float* state_out;
+  int final_by_chain;              // chain_kernel writes state_out, for all sequences with tokens
   int st_y, st_w;
   float* seg_state;                // [segment slot, Hv, ..] likewise
   float* seg_decay;                // [segment slot, Hv]
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   const Seg seg = seg_of_slot(a, seg_slot);
   if (!seg.ok) return;
   const bool last = kRev ? seg.j == 0 : seg.j == seg.count - 1;
-  if (kState && last) return;  // nobody takes its state from here: the scan itself ends with it
+  if (kState && last && !a.final_by_chain) return;  // nobody takes its state from here
   int slot = seg.n;
   if (a.state_indices != nullptr) {
     slot = a.state_indices[seg.n];
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       slot = -1;
     }
   }
-  if (kState && slot < 0) return;
+  if (kState && (slot < 0 || seg.len == 0)) return;
   const int64_t state_tile = ((int64_t)slot * a.Hv + h) * (DK * DV), seg_tile = (seg_slot * a.Hv + h) * (int64_t)(DK * DV);
   if constexpr (!kState) {
     __nv_bfloat16* og = reinterpret_cast<__nv_bfloat16*>(a.o) + seg.b * a.o_stride_b + (int64_t)h * a.o_stride_h;
@@ -574,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         }
       }
     }
-    float* dst = kState ? a.seg_state + seg_tile : last && a.state_out != nullptr ? a.state_out + state_tile : nullptr;
+    float* dst = kState ? a.seg_state + seg_tile : last && a.state_out != nullptr && !a.final_by_chain ? a.state_out + state_tile : nullptr;
     if (ok && mine && dst != nullptr) {
 #pragma unroll
       for (int i = 0; i < HC / 2; ++i) {
@@ -582,7 +583,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         p[0] = S[i].x; p[a.st_y] = S[i].y;
       }
     }
-  } else if (warp < 16) {
+  } else if (!kState && warp < 16) {
     tc::reg_set<REGS_OUT, REGS_LAUNCH>();
     // ------------------------------------------------------------------ outputs: 32 features a warp, as accumulator fragments of warp-level MMAs, which matrix stores
     // transpose on their way into shared memory, in the place of the chunk's X (and Y, for 32-bit rows), whose readers are through; they leave by asynchronous copies
@@ -745,10 +746,11 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(cleared);
+        if (!kState && lane == 0) tc::mbar_arrive(cleared);
       }
+      // 32 tokens; for the state alone the output's warps take half of them
 #pragma unroll 1
-      for (int q = 0; q < 2; ++q) {  // 32 tokens
+      for (int q = kState ? (warp >> 2) & 1 : 0; q < (kState ? ((warp >> 2) & 1) + 1 : 2); ++q) {
         ok = ok && all(tc::mbar_wait(&img_read[q], cp ^ 1u, abort_flag));
         if (!ok) break;
         tc::tc_fence_after_sync();
@@ -802,7 +804,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   }
 }
 
-// Between the two passes: seg_state goes from each segment's own increment to the state that enters it.
+// Between the two passes: seg_state goes from each segment's own increment to the state that enters it, and the last one's is the final state.
 template <int DK, int DV, bool kRev>
 __global__ void __launch_bounds__(256) chain_kernel(const Args a) {
   pdl_wait();
@@ -811,21 +813,23 @@ __global__ void __launch_bounds__(256) chain_kernel(const Args a) {
   const int part = blockIdx.x % PARTS, h = blockIdx.x / PARTS % a.Hv, n = blockIdx.x / PARTS / a.Hv;
   const SeqSpan sp = seq_span(a.cu_seqlens, n, a.T, nullptr);
   const int count = (sp.len + a.plan.len - 1) / a.plan.len;
-  if (!sp.ok || count < 2) return;
+  float* final = a.final_by_chain ? a.state_out : nullptr;
+  if (!sp.ok || count < (final != nullptr ? 1 : 2)) return;
   int slot = n;
   if (a.state_indices != nullptr) slot = a.state_indices[n];
   if (slot < 0 || (a.state_indices != nullptr && slot >= a.num_slots)) return;
-  const int64_t at = part * 1024 + threadIdx.x * 4, s0 = first_slot(a, n);
+  const int64_t at = part * 1024 + threadIdx.x * 4, s0 = first_slot(a, n), tile = ((int64_t)slot * a.Hv + h) * (DK * DV) + at;
   float4 cur = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (a.state_in != nullptr) cur = *reinterpret_cast<const float4*>(a.state_in + ((int64_t)slot * a.Hv + h) * (DK * DV) + at);
+  if (a.state_in != nullptr) cur = *reinterpret_cast<const float4*>(a.state_in + tile);
   float* base = a.seg_state + h * (int64_t)(DK * DV) + at;
   const int64_t step = (int64_t)a.Hv * (DK * DV);
+  const int own_until = final != nullptr ? count : count - 1;
   for (int i0 = 0; i0 < count; i0 += 4) {
     float4 own[4];
     float decay[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (i0 + u < count - 1) {
+      if (i0 + u < own_until) {
         const int64_t sl = s0 + (kRev ? count - 1 - i0 - u : i0 + u);
         own[u] = *reinterpret_cast<const float4*>(base + sl * step);
         decay[u] = a.seg_decay[sl * a.Hv + h];
@@ -834,13 +838,14 @@ __global__ void __launch_bounds__(256) chain_kernel(const Args a) {
     for (int u = 0; u < 4; ++u)
       if (i0 + u < count) {
         const int64_t sl = s0 + (kRev ? count - 1 - i0 - u : i0 + u);
-        *reinterpret_cast<float4*>(base + sl * step) = cur;
-        if (i0 + u < count - 1) {
+        if (count > 1) *reinterpret_cast<float4*>(base + sl * step) = cur;
+        if (i0 + u < own_until) {
           cur.x = fmaf(decay[u], cur.x, own[u].x); cur.y = fmaf(decay[u], cur.y, own[u].y);
           cur.z = fmaf(decay[u], cur.z, own[u].z); cur.w = fmaf(decay[u], cur.w, own[u].w);
         }
       }
   }
+  if (final != nullptr) *reinterpret_cast<float4*>(final + tile) = cur;
 }
 
 }  // namespace lin

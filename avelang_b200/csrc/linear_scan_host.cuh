@@ -11,25 +11,23 @@ namespace lin {
 
 constexpr int MAX_DEVICES = 64;
 
-// One CTA walks a segment of one (sequence, value head), a chunk in about the time `1`.  Whole sequences need one pass; segments need their own
-// increments first (a pass that reads Y and W alone), so they pay where there are too few sequences and heads for the SMs, or where one sequence is so
-// long that the others wait for it.  The lengths of packed sequences are not known here: the longest is taken to be four times the mean.
+// One CTA walks a segment of one (sequence, value head).  Whole sequences need one pass; segments need their own increments first (a pass that reads Y and W alone) and the chain
+// of them, so they pay where there are too few sequences and heads for the SMs, or where one sequence is so long that the others wait for it.  The lengths of packed sequences are
+// not known here: the longest is taken to be four times the mean.  Unit: a chunk of the scan, 2.2 us on every SM; a chunk of the first pass takes 0.45 of that, a CTA's
+// beginning and end 3 and 2.5, the chain and its launches 2.5 (2 x 4096 tokens x 32 heads, forward: whole 220 us, segments of 2048 tokens 127, of 256 221).
 inline Plan plan_of(int B, int64_t T, int n_seqs, bool packed, int heads) {
-  constexpr double SMS = 148, STATES = 0.6, FIXED = 8.0;  // a chunk of the first pass, and its launches, in chunks of the scan
+  constexpr double SMS = 148;
   const double chunks = (double)((T * B + C - 1) / C);
   const double longest = packed ? (n_seqs > 1 ? fmin((double)T, 4.0 * T / n_seqs) : (double)T) / C : (double)((T + C - 1) / C);
-  auto pass = [&](double units, double each) {  // units of about `each` chunks
-    const double waves = units / SMS;
-    return packed ? waves * each + 0.5 * each : (double)(int64_t)(waves + 0.999999) * each;
-  };
+  auto waves = [&](double units) { return packed ? units / SMS + 0.5 : (double)(int64_t)(units / SMS + 0.999999); };
   const double seqs = packed ? (double)n_seqs : (double)B;
-  double best = packed ? fmax(chunks * heads / SMS, longest) + 0.25 * longest : pass(seqs * heads, longest);
+  double best = packed ? fmax((chunks + 3.0 * seqs) * heads / SMS, longest + 3.0) + 0.25 * longest : waves(seqs * heads) * (longest + 3.0);
   int64_t len = 0;
   for (int parts = 2; parts <= 256; ++parts) {
     const int64_t each = (int64_t)((longest + parts - 1) / parts);
-    if (each < 4 || each * (parts - 1) >= longest + each) continue;
-    const double units = packed ? chunks / (double)each * heads : seqs * heads * (double)(((int64_t)longest + each - 1) / each);
-    const double t = pass(units, (double)each) + STATES * pass(units * (parts - 1) / parts, (double)each) + FIXED + 0.15 * parts;
+    if (each < 4) break;
+    const double units = packed ? (chunks / (double)each + 0.5 * seqs) * heads : seqs * heads * (double)(((int64_t)longest + each - 1) / each);
+    const double t = waves(units) * (1.45 * (double)each + 5.5) + 2.5 + 0.1 * parts;
     if (t < 0.95 * best) { best = t; len = each * C; }
   }
   Plan p;
