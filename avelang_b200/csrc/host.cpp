@@ -1122,7 +1122,7 @@ Tensor as_rows(const Tensor& x) { return x.dim() == 2 ? x : x.reshape({x.numel()
 void check_norm_input(const Tensor& x, const Tensor* w, const Tensor* b) {
   dtype_code(x, "x");
   REQ(x.is_cuda(), "x must be a CUDA tensor");
-  REQ(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 32768, "the last dimension of x must lie in [1, 32768], got ", x.dim() > 0 ? x.size(-1) : 0, ".");
+  REQ(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 28672, "the last dimension of x must lie in [1, 28672], got ", x.dim() > 0 ? x.size(-1) : 0, ".");
   const int64_t n = x.size(-1);
   REQ(b == nullptr || w != nullptr, "bias needs weight");
   const std::pair<const char*, const Tensor*> wb[] = {{"weight", w}, {"bias", b}};

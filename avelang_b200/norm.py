@@ -2,7 +2,7 @@
 
     y = (x - mean) * rstd * weight + bias,   rstd = 1 / sqrt(var + eps)
 
-over the last dimension (1 to 32768 elements).  ``x`` is bf16, fp16 or fp32; ``weight`` and ``bias`` have its dtype or fp32.  Sums and
+over the last dimension (1 to 28672 elements).  ``x`` is bf16, fp16 or fp32; ``weight`` and ``bias`` have its dtype or fp32.  Sums and
 statistics are fp32, results are rounded once.  Rows that are evenly spaced and contiguous are read as they are; others are copied first.
 Rows of a whole number of 16-byte pieces on 16-byte boundaries take wide loads, others go element by element.  Errors are ValueError, as
 in the reference's kernel library (python/avelang_kernels/amdgpu_gemm.py:463-486).

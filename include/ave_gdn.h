@@ -403,7 +403,7 @@ typedef struct AveLinearBwdArgs {
 int ave_linear_backward(const AveLinearBwdArgs* args, void* stream);
 size_t ave_linear_backward_workspace_bytes(const AveLinearBwdArgs* args);
 
-/* y = (x - mean) * rstd * weight + bias over rows of n elements, 1 <= n <= 32768, rstd = 1 / sqrt(var + eps). */
+/* y = (x - mean) * rstd * weight + bias over rows of n elements, 1 <= n <= 28672, rstd = 1 / sqrt(var + eps). */
 #define AVE_DTYPE_BF16 0
 #define AVE_DTYPE_FP16 1
 #define AVE_DTYPE_FP32 2

@@ -23,7 +23,7 @@ def reference(x, w, b, eps):
 
 
 def check_forward(got, x, w, b, eps):
-    """A sum of n numbers over a tree of partial sums loses at most (n / threads + log2 threads) half steps, 64 are enough up to 32768 columns; the mean's loss
+    """A sum of n numbers over a tree of partial sums loses at most (n / threads + log2 threads) half steps, 64 are enough up to 28672 columns; the mean's loss
     reaches y times rstd."""
     y, mean, rstd = got
     y_ref, m_ref, r_ref, xh = reference(x, w, b, eps)
@@ -40,7 +40,7 @@ def check_forward(got, x, w, b, eps):
 
 
 SHAPES = [(1, 1), (3, 2), (5, 7), (2, 64), (37, 65), (9, 255), (33, 256), (4, 257), (70, 512), (5, 1000), (3, 1409), (37, 2048), (2, 2047), (3, 4096), (2, 5000), (2, 8192),
-          (2, 16384), (1, 20001), (2, 32768)]
+          (2, 16384), (1, 20001), (2, 28672), (2, 25000), (1, 28671)]
 
 
 @pytest.mark.parametrize("rows,n", SHAPES)
@@ -70,6 +70,13 @@ def test_forward_and_gradients(built_lib, rows, n, dt, wdt):
     for d, ref, mag in ((dw, (dyd * xh).sum(0), (dyd * xh).abs().sum(0) + (dyd.abs() * xh_loss).sum(0) / u), (db, dyd.sum(0), dyd.abs().sum(0))):
         assert d.dtype == w.dtype
         assert ((d.cpu().double() - ref).abs() <= whalf * ref.abs() + (1 + whalf) * u * mag + tiny).all()
+
+
+@pytest.mark.parametrize("rows,n,dt", [(10700, 520, "bf16"), (10700, 1024, "fp16"), (4000, 1540, "fp32"), (11000, 1536, "bf16"), (5500, 4096, "bf16"), (2700, 8192, "bf16"), (1340, 8196, "fp32"),
+                                       (10700, 264, "bf16"), (1400, 16384, "fp16")])
+def test_rings_that_turn(built_lib, rows, n, dt):
+    """More rows a group than its ring has slots: each slot is filled several times."""
+    test_forward_and_gradients(built_lib, rows, n, dt, "fp32")
 
 
 @pytest.mark.parametrize("rows,n", [(3000, 64), (5001, 100), (2500, 2048), (1300, 1409), (700, 8192)])
