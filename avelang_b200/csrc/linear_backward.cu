@@ -5,9 +5,9 @@
 // s < t <= u of m_us = e^{G_u - G_s} scale (q_u.k_s)(do_u.v_s) (the initial state counts as a token in front of all others, the final state's gradient as one
 // behind them), so that with the strictly causal parts A_t = sum over s < t of m_ts and B_t = sum over u > t of m_ut
 //     dg_{t+1} = dg_t - A_t + B_t,
-// and dg at the first token of a segment is the product <S, R> of the state and the gradient that meet there.  A and B come with the scans for dq
-// and dk: inside a chunk from P' and a second product q k^T in 32 bits, across chunks as q_t . (e_t S do_t) and k_t . (e_t R v_t) in front of the
-// diagonal's term; the shorter formula with q.dq - k.dk would take that term, which is far larger where decays are strong, from both sides.
+// and dg at the first token of a segment is the product <S, R> of the state and the gradient that meet there.  The parts of A and B across chunks come with the
+// scans for dq and dk, as q_t . (e_t S do_t) and k_t . (e_t R v_t) in front of the chunk's own terms; those inside a chunk are sums over the rows and the columns of one product,
+// (q k^T) (do v^T) elementwise, in 32 bits.  The shorter formula with q.dq - k.dk would take the diagonal's terms, which are far larger where decays are strong, from both sides.
 #include "linear_scan_host.cuh"
 
 namespace ave {
@@ -28,6 +28,101 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* part, __nv_
     }
     *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w), pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
   }
+}
+
+// m_ts of a chunk's pairs s < t, summed over s into a[t] and over t into b[s]: one CTA a (chunk, value head), 16 rows t a warp, as warp-level MMAs; bound by the four tiles it reads.
+struct PairSums {
+  const __nv_bfloat16 *q, *k, *v, *d_o;
+  int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h, o_b, o_t, o_h;
+  int rep;
+  float scale;
+  float *a, *b;  // [Hv][B T]
+};
+template <int DK, int DV>
+__global__ void __launch_bounds__(128) pair_sums_kernel(const Args s, const PairSums p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = tc::align1024(smem_raw);
+  constexpr int KB = 2 * DK, VB = 2 * DV, Q0 = 0, K0 = 64 * KB, V0 = 2 * K0, O0 = V0 + 64 * VB;
+  float2* G = reinterpret_cast<float2*>(smem + O0 + 64 * VB);  // [64]
+  float* cols = reinterpret_cast<float*>(G + 64);              // [4][64]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  if (!offsets_fit(s, false)) return;
+  const int h = blockIdx.x % s.Hv, hk = h / p.rep;
+  const Seg c = seg_of_slot(s, blockIdx.x / s.Hv);
+  if (!c.ok || c.len == 0) return;
+  const uint32_t base = tc::smem_u32(smem);
+  load_tile<64, DK / 8, 128>(base + Q0, p.q + c.b * p.q_b + (int64_t)c.t0 * p.q_t + hk * p.q_h, p.q_t, c.len, threadIdx.x);
+  load_tile<64, DK / 8, 128>(base + K0, p.k + c.b * p.k_b + (int64_t)c.t0 * p.k_t + hk * p.k_h, p.k_t, c.len, threadIdx.x);
+  load_tile<64, DV / 8, 128>(base + V0, p.v + c.b * p.v_b + (int64_t)c.t0 * p.v_t + h * p.v_h, p.v_t, c.len, threadIdx.x);
+  load_tile<64, DV / 8, 128>(base + O0, p.d_o + c.b * p.o_b + (int64_t)c.t0 * p.o_t + h * p.o_h, p.o_t, c.len, threadIdx.x);
+  cp_commit();
+  if (warp == 0) {
+    auto fetch = [&](int t) { return t < c.len ? s.g[c.b * s.g_stride_b + (int64_t)(c.t0 + t) * s.g_stride_t + h] : 0.f; };
+    Two G0, G1;
+    gate_scan(fetch(2 * lane), fetch(2 * lane + 1), lane, G0, G1);
+    G[2 * lane] = make_float2(G0.h, G0.l);
+    G[2 * lane + 1] = make_float2(G1.h, G1.l);
+  }
+  cp_wait<0>();
+  __syncthreads();
+  const int r0 = 16 * warp, row = r0 + (lane >> 2);
+  float own[2] = {0.f, 0.f};
+  const float2 gt[2] = {G[row], G[row + 8]};
+#pragma unroll 1
+  for (int j = 0; j < 4; ++j) {  // 16 columns
+    float x[2][4], y[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) { zero(x[n]); zero(y[n]); }
+    if (j <= warp) {
+#pragma unroll
+      for (int k = 0; k < DK / 16; ++k) {
+        uint32_t l[4], r[4];
+        ldsm4(l, base + Q0 + at_a<KB>(r0, 2 * k, lane));
+        ldsm4(r, base + K0 + at_b<KB>(16 * j, 2 * k, lane));
+        mma_bf16(x[0], l, r[0], r[1]);
+        mma_bf16(x[1], l, r[2], r[3]);
+      }
+#pragma unroll
+      for (int k = 0; k < DV / 16; ++k) {
+        uint32_t l[4], r[4];
+        ldsm4(l, base + O0 + at_a<VB>(r0, 2 * k, lane));
+        ldsm4(r, base + V0 + at_b<VB>(16 * j, 2 * k, lane));
+        mma_bf16(y[0], l, r[0], r[1]);
+        mma_bf16(y[1], l, r[2], r[3]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = row + 8 * (i >> 1), col = 16 * j + 8 * n + 2 * (lane & 3) + (i & 1);
+        const float2 gs = G[col];
+        const float m = col < t ? p.scale * ex2((gt[i >> 1].x - gs.x) + (gt[i >> 1].y - gs.y)) * (x[n][i] * y[n][i]) : 0.f;
+        own[i >> 1] += m;
+        sum[i & 1] += m;
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
+        sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], o);
+      }
+      if (lane < 4) *reinterpret_cast<float2*>(cols + 64 * warp + 16 * j + 8 * n + 2 * lane) = make_float2(sum[0], sum[1]);
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    own[0] += __shfl_xor_sync(0xffffffffu, own[0], o);
+    own[1] += __shfl_xor_sync(0xffffffffu, own[1], o);
+  }
+  const int64_t at = ((int64_t)h * s.B + c.b) * s.T + c.t0;
+  if ((lane & 3) == 0) {
+    if (row < c.len) p.a[at + row] = own[0];
+    if (row + 8 < c.len) p.a[at + row + 8] = own[1];
+  }
+  __syncthreads();
+  if (threadIdx.x < c.len && threadIdx.x < 64) p.b[at + threadIdx.x] = (cols[threadIdx.x] + cols[64 + threadIdx.x]) + (cols[128 + threadIdx.x] + cols[192 + threadIdx.x]);
 }
 
 struct GateGrad {
@@ -87,10 +182,7 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const Gate
     if (t < seg.len) {
       float ia = 0.f, ib = 0.f;
       for (int p = 0; p < q.parts; ++p) { ia += q.inter_a[p * plane + base + t]; ib += q.inter_b[p * plane + base + t]; }
-      float ja = 0.f, jb = 0.f;
-#pragma unroll
-      for (int p = 0; p < 4; ++p) { ja += q.intra_a[p * plane + base + t]; jb += q.intra_b[p * plane + base + t]; }
-      d = ((double)ib - (double)ia) + ((double)jb - (double)ja);
+      d = ((double)ib - (double)ia) + ((double)q.intra_b[base + t] - (double)q.intra_a[base + t]);
     }
     double inc = d;
 #pragma unroll
@@ -170,7 +262,7 @@ Layout layout_of(const AveLinearBwdArgs& a) {
   if (a.Hv > a.Hk) l.part = take(rows * a.dk * 4);
   if (a.g != nullptr) {
     l.inter_a = take(rows * (a.dk / 32) * 4); l.inter_b = take(rows * (a.dk / 32) * 4);
-    l.intra_a = take(rows * 16); l.intra_b = take(rows * 16);
+    l.intra_a = take(rows * 4); l.intra_b = take(rows * 4);
     l.sums = take((size_t)l.plan.slots * a.Hv * 4);
   }
   l.bytes = at;
@@ -179,6 +271,8 @@ Layout layout_of(const AveLinearBwdArgs& a) {
 
 }  // namespace lin
 }  // namespace
+
+static const __nv_bfloat16* lin_bf(const void* p) { return reinterpret_cast<const __nv_bfloat16*>(p); }
 
 size_t linear_backward_workspace_bytes(const AveLinearBwdArgs& a) { return lin::layout_of(a).bytes; }
 
@@ -259,7 +353,7 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
       s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; lin::set_scale(s, a.scale); s.scale_e = a.scale; s.st_y = 1; s.st_w = a.dv;
       m.x = mo; m.y = mv; m.w = mk; m.e = mq;
       if ((r = rows_of(s, m, a.d_q))) return r;
-      if (grad) { s.inter = f32(l.inter_a); s.intra = f32(l.intra_a); }
+      if (grad) s.inter = f32(l.inter_a);
       r = grad ? lin::launch_scan<DV, DK, false, lin::GRAD>(s, m, stream) : lin::launch_scan<DV, DK, false, lin::OUT2>(s, m, stream);
       if (r || (r = sum_heads(a.d_q))) return r;
     }
@@ -270,9 +364,21 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
       s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; lin::set_scale(s, a.scale); s.scale_e = 1.f; s.st_y = 1; s.st_w = a.dv;
       m.x = mv; m.y = mo; m.w = mq; m.e = mk;
       if ((r = rows_of(s, m, a.d_k))) return r;
-      if (grad) { s.inter = f32(l.inter_b); s.intra = f32(l.intra_b); }
+      if (grad) s.inter = f32(l.inter_b);
       r = grad ? lin::launch_scan<DV, DK, true, lin::GRAD>(s, m, stream) : lin::launch_scan<DV, DK, true, lin::OUT2>(s, m, stream);
       if (r || (r = sum_heads(a.d_k))) return r;
+    }
+    if (grad) {
+      lin::Args s = base;
+      s.plan = lin::Plan{lin::C, 1, (int64_t)a.B * a.T / lin::C + a.n_seqs + 1};
+      const lin::PairSums p{lin_bf(a.q), lin_bf(a.k), lin_bf(a.v), lin_bf(a.d_o), a.q_stride_b, a.q_stride_t, a.q_stride_h, a.k_stride_b, a.k_stride_t, a.k_stride_h,
+                            a.v_stride_b, a.v_stride_t, a.v_stride_h, a.do_stride_b, a.do_stride_t, a.do_stride_h, rep, a.scale, f32(l.intra_a), f32(l.intra_b)};
+      auto* kernel = lin::pair_sums_kernel<DK, DV>;
+      constexpr int smem = 64 * 4 * (DK + DV) + 64 * 8 + 4 * 64 * 4 + 1024;
+      if ((r = lin::allow_smem<DK, DV>(kernel, smem))) return r;
+      const int64_t grid = s.plan.slots * a.Hv;
+      if (grid > 0x7fffffff) return (int)AVE_GDN_UNSUPPORTED;
+      AVE_CUDA_TRY(launch_after(kernel, (unsigned)grid, 128, smem, stream, s, p));
     }
     return (int)AVE_GDN_OK;
   });

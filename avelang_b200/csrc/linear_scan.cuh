@@ -50,7 +50,6 @@ struct Args {
   float* seg_state;                // [segment slot, Hv, ..] likewise
   float* seg_decay;                // [segment slot, Hv]
   float* inter;                    // [dv / 32][Hv][B T]: e_t E_t . (H^T X_t), 32 features each      (for the gradient of g)
-  float* intra;                    // [4][Hv][B T]: sum over s < t of P'_ts (E_t . W_s), 16 of a chunk's s each
   Plan plan;
 };
 struct Maps {
@@ -116,13 +115,13 @@ struct Cfg {
   static constexpr int PP = STAGES * STAGE, GV = PP + (kState ? 0 : TILE), BARS = GV + STAGES * GATES;
   static constexpr int SMEM = BARS + 256 + 1024;
   static_assert(SMEM <= 232448, "shared memory of an SM");
-  // TMEM columns.  With three terms W^T P'^T takes the columns of P, and with the gradient of g H^T X^T those of E W^T, and the increment's two halves (64 features
-  // of Y each) one another's.
+  // TMEM columns.  With three terms W^T P'^T takes the columns of P, and with the gradient of g the increment's two halves (64 features of Y each) one another's.
   static constexpr bool kAlias = TERMS == 3;
-  static constexpr uint32_t P = 0, OA = kAlias ? 0 : 64, OI = kAlias ? 64 : 128, PE = OI;
-  static constexpr uint32_t DS = kState ? 0 : kAlias ? 128 : 192, H = DS + (kGrad ? 64 : 128), IMG = kState ? 128 : H + 64 * HT;
-  static constexpr uint32_t COLS = kState ? 256 : 512;
-  static_assert(IMG + 32 * TERMS <= COLS, "tensor memory");
+  static constexpr uint32_t P = 0, OA = kAlias ? 0 : 64, OI = kAlias ? 64 : 128;
+  // (For the state alone the chunks take two places in turn for their increments and their images.)
+  static constexpr uint32_t DS = kState ? 0 : OI + 64, H = DS + (kGrad ? 64 : 128), IMG = kState ? 256 : H + 64 * HT;
+  static constexpr uint32_t TURN_DS = kState ? 128 : 0, TURN_IMG = kState ? 32 * TERMS : 0, COLS = 512;
+  static_assert(IMG + TURN_IMG + 32 * TERMS <= COLS, "tensor memory");
 };
 
 constexpr int THREADS = 640;  // warpgroups: loader, gate vectors and two issuers; two for the state and P'; outputs; images of W^T
@@ -136,20 +135,40 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A number as the sum of two floats: 64-bit arithmetic is slow here (a chunk's gate vectors took 3.8 k cycles with it)
-struct Two { float h, l; };
-__device__ __forceinline__ Two add(Two a, Two b) {
-  const float s = a.h + b.h, t = s - a.h, e = (a.h - (s - t)) + (b.h - t), l = a.l + b.l + e, h = s + l;
-  return Two{h, l - (h - s)};
-}
+// Sums of the decays' base-2 logarithms as 64-bit integers in units of 2^-36: exact, and a step of a running sum is two shuffles and an addition.  (In 64-bit floating point a chunk's
+// gate vectors took 3.8 k cycles, as sums of two floats 1.4 k.)  Logarithms are held inside +-1e6, so that 64 of them fit.
+constexpr float FIXED = 68719476736.f;  // 2^36
+struct Two { float h, l; };             // a number as the sum of two floats
 __device__ __forceinline__ float diff(Two a, Two b) { return (a.h - b.h) + (a.l - b.l); }
-__device__ __forceinline__ Two log2_of(float ln) {  // ln * log2(e)
+__device__ __forceinline__ long long fixed_log2(float ln) {  // ln * log2(e); a NaN is the caller's to see
   constexpr float L = 1.44269504f, R = 1.925963033e-8f;
+  ln = fminf(fmaxf(ln, -1e6f), 1e6f);
   const float p = ln * L;
-  return Two{p, fmaf(ln, L, -p) + ln * R};
+  return __float2ll_rn(p * FIXED) + __float2ll_rn((fmaf(ln, L, -p) + ln * R) * FIXED);
 }
-__device__ __forceinline__ Two shfl_up(Two x, int o) { return Two{__shfl_up_sync(0xffffffffu, x.h, o), __shfl_up_sync(0xffffffffu, x.l, o)}; }
-__device__ __forceinline__ Two shfl(Two x, int i) { return Two{__shfl_sync(0xffffffffu, x.h, i), __shfl_sync(0xffffffffu, x.l, i)}; }
+__device__ __forceinline__ Two two(long long x) {
+  const float h = __ll2float_rn(x);
+  return Two{h * (1.f / FIXED), __ll2float_rn(x - __float2ll_rn(h)) * (1.f / FIXED)};
+}
+// Running sums over 64 tokens, two a lane, from the logarithms; returns the whole sum.  From a NaN on they are NaN.
+__device__ __forceinline__ long long gate_scan(float n0, float n1, int lane, Two& G0, Two& G1) {
+  const long long x0 = fixed_log2(n0), x1 = fixed_log2(n1);
+  long long sum = x0 + x1;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += y;
+  }
+  G1 = two(sum);
+  G0 = two(sum - x1);
+  const unsigned bad = __ballot_sync(0xffffffffu, isnan(n0) || isnan(n1));
+  if (bad != 0u) {
+    const int first = __ffs(bad) - 1;
+    if (lane > first || (lane == first && isnan(n0))) G0.h = __int_as_float(0x7fffffff);
+    if (lane >= first) G1.h = __int_as_float(0x7fffffff);
+  }
+  return __shfl_sync(0xffffffffu, sum, 31);
+}
 // 2^x to the last bit or two: a state is multiplied by the same number chunk after chunk, so that an error in it adds up.  Taylor's series of 2^r for |r| <= 1/2.
 __device__ __forceinline__ float pow2(Two x) {
   const float n = rintf(x.h), r = ((x.h - n) + x.l) * 0.693147181f;
@@ -175,7 +194,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   uint64_t* full = bars;            // [4] tiles of the stage landed
   uint64_t* gates = bars + 4;       // [4] its gate vectors written
   uint64_t* empty = bars + 8;       // [4] the stage is read
-  uint64_t* p_full = bars + 12;     // P (and E W^T) accumulated
+  uint64_t* p_full = bars + 12;     // P accumulated
   uint64_t* pp_ready = bars + 13;   // P' written, P drained
   uint64_t* img_ready = bars + 14;  // [2] images of 32 tokens of W^T written
   uint64_t* img_read = bars + 16;   // [2] and read
@@ -278,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       }
     } else if (warp == 2) {
       // ---------------------------------------------------------------- gate vectors, two tokens a lane
-      Two seg_total{0.f, 0.f};
+      [[maybe_unused]] Two seg_total{0.f, 0.f};
       const float* g = a.g != nullptr ? a.g + seg.b * a.g_stride_b + h : nullptr;
       auto fetch = [&](int c, int e) {
         const int t = chunk_at(c) * C + 2 * lane + e;
@@ -290,17 +309,12 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       uint32_t ph = 1;
       for (int c = 0; c < n_chunks; ++c) {
         if (c >= K::STAGES && !all(tc::mbar_wait(&empty[s], ph, abort_flag))) break;
-        const Two x0 = log2_of(n0 < -1e6f ? -1e6f : n0), x1 = log2_of(n1 < -1e6f ? -1e6f : n1);  // (a NaN stays one)
+        Two G0, G1;
+        const long long whole = gate_scan(n0, n1, lane, G0, G1);
         if (c + 1 < n_chunks) { n0 = fetch(c + 1, 0); n1 = fetch(c + 1, 1); }  // (not looked at before the next round)
-        Two G1 = add(x0, x1);
-#pragma unroll 1
-        for (int o = 1; o < 32; o <<= 1) {
-          const Two y = add(G1, shfl_up(G1, o));
-          if (lane >= o) G1 = y;
-        }
-        const Two total = shfl(G1, 31), before = shfl_up(G1, 1);
-        const Two G0 = lane > 0 ? add(before, x0) : x0;
-        if constexpr (kState) seg_total = add(seg_total, total);
+        Two total = two(whole);
+        total.h += 0.f * __shfl_sync(0xffffffffu, G1.h, 31);  // (a NaN stays one)
+        if constexpr (kState) seg_total = Two{seg_total.h + total.h, seg_total.l + total.l + ((seg_total.h - (seg_total.h + total.h)) + total.h)};
         const int left = seg.len - chunk_at(c) * C - 2 * lane;  // tokens from this lane's first on
         const float2 from0 = make_float2(ex2(G0.h + G0.l), ex2(G1.h + G1.l)), to_end = make_float2(ex2(diff(total, G0)), ex2(diff(total, G1)));
         const float2 e = __fmul2_rn(make_float2(a.scale_e, a.scale_e), kRev ? to_end : from0);
@@ -327,13 +341,13 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       constexpr uint32_t hi_sw = tc::desc_hi(1024, true);
       // 32 tokens' part of the increment, or of half f of it, the smallest terms first
       constexpr int N = kGrad ? 64 : DK;
-      auto part = [&](int f, int q, uint32_t at) {
+      auto part = [&](int f, int q, uint32_t at, uint32_t turn) {
 #pragma unroll
         for (int t = K::TERMS - 1; t >= 0; --t)
 #pragma unroll
           for (int k = 2 * q; k < 2 * q + 2; ++k)  // 16 tokens a step
-            tc::mma_ts(tm + K::DS, tm + K::IMG + 32 * t + 8 * k, tc::smem_desc(at + tc::desc_lo(K::Y + f * HALF + 2048 * k, HALF), hi_sw),
-                       tc::idesc_f16(128, N, 1, 1, false, true), !(q == 0 && t == K::TERMS - 1 && k == 0));
+            tc::mma_ts(tm + K::DS + turn * K::TURN_DS, tm + K::IMG + turn * K::TURN_IMG + 32 * t + 8 * k,
+                       tc::smem_desc(at + tc::desc_lo(K::Y + f * HALF + 2048 * k, HALF), hi_sw), tc::idesc_f16(128, N, 1, 1, false, true), !(q == 0 && t == K::TERMS - 1 && k == 0));
       };
       int s = 0;
       bool ok = true;
@@ -344,34 +358,40 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
           ok = all(tc::mbar_wait3(&ds_empty[1], cp ^ 1u, &img_ready[0], cp, &img_ready[1], cp, abort_flag));
           if (!ok) break;
           tc::tc_fence_after_sync();
-          if (tc::elect_one()) { part(0, 0, at); part(0, 1, at); tc::mma_commit(&ds_full[0]); }
+          if (tc::elect_one()) { part(0, 0, at, 0u); part(0, 1, at, 0u); tc::mma_commit(&ds_full[0]); }
           __syncwarp();
           ok = all(tc::mbar_wait(&ds_empty[0], cp, abort_flag));
           if (!ok) break;
           tc::tc_fence_after_sync();
           if (tc::elect_one()) {
-            part(1, 0, at); part(1, 1, at);
+            part(1, 0, at, 0u); part(1, 1, at, 0u);
             tc::mma_commit(&img_read[0]); tc::mma_commit(&img_read[1]); tc::mma_commit(&ds_full[1]);
+          }
+          __syncwarp();
+        } else if constexpr (kState) {
+          const uint32_t turn = (uint32_t)(c >> 1) & 1u;
+          ok = all(tc::mbar_wait2(&ds_empty[cp], turn ^ 1u, &img_ready[cp], turn, abort_flag));
+          if (!ok) break;
+          tc::tc_fence_after_sync();
+          if (tc::elect_one()) {
+            part(0, 0, at, cp); part(0, 1, at, cp);
+            tc::mma_commit(&ds_full[cp]); tc::mma_commit(&img_read[cp]); tc::mma_commit(&empty[s]);
           }
           __syncwarp();
         } else {  // the tokens by halves, as their images come, so that those of the next chunk are written beside it
           ok = all(tc::mbar_wait2(&ds_empty[0], cp ^ 1u, &img_ready[0], cp, abort_flag));
           if (!ok) break;
           tc::tc_fence_after_sync();
-          if (tc::elect_one()) { part(0, 0, at); tc::mma_commit(&img_read[0]); }
+          if (tc::elect_one()) { part(0, 0, at, 0u); tc::mma_commit(&img_read[0]); }
           __syncwarp();
           ok = all(tc::mbar_wait(&img_ready[1], cp, abort_flag));
           if (!ok) break;
           tc::tc_fence_after_sync();
-          if (tc::elect_one()) { part(0, 1, at); tc::mma_commit(&ds_full[0]); tc::mma_commit(&img_read[1]); }
+          if (tc::elect_one()) { part(0, 1, at, 0u); tc::mma_commit(&ds_full[0]); tc::mma_commit(&img_read[1]); }
           __syncwarp();
         }
-        if constexpr (kState) {
-          if (tc::elect_one()) tc::mma_commit(&empty[s]);
-          __syncwarp();
-        } else {
-          // (the gradient of g: E W^T, in whose place H^T X^T goes, is drained with P)
-          ok = kGrad ? all(tc::mbar_wait2(h_ready, cp, pp_ready, cp, abort_flag)) : all(tc::mbar_wait2(h_ready, cp, o_empty, cp ^ 1u, abort_flag));
+        if constexpr (!kState) {
+          ok = all(tc::mbar_wait2(h_ready, cp, o_empty, cp ^ 1u, abort_flag));
           if (!ok) break;
           tc::tc_fence_after_sync();
           if (tc::elect_one()) {
@@ -397,16 +417,12 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       // a part of them.  The other halves multiply what lies in front of the tile and behind it, and nobody reads them.
       auto scores = [&](uint32_t at) {
         if (tc::elect_one()) {
-          auto product = [&](uint32_t d, int left, int right, int steps) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-              for (int k = 0; k < steps; ++k)
-                tc::mma_ss(d + 32 * half, tc::smem_desc(at + tc::desc_lo(left - half * HALF + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw),
-                           tc::smem_desc(at + tc::desc_lo(right + half * 4096 + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw), tc::idesc_f16(128, 32, 1, 1, false, false), k != 0);
-          };
-          product(tm + K::P, K::X, K::Y, DK / 16);
-          if constexpr (kGrad) product(tm + K::PE, K::E, K::W, DV / 16);
+            for (int k = 0; k < DK / 16; ++k)
+              tc::mma_ss(tm + K::P + 32 * half, tc::smem_desc(at + tc::desc_lo(K::X - half * HALF + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw),
+                         tc::smem_desc(at + tc::desc_lo(K::Y + half * 4096 + (k >> 2) * HALF + 32 * (k & 3), 16), hi_sw), tc::idesc_f16(128, 32, 1, 1, false, false), k != 0);
           tc::mma_commit(p_full);
         }
         __syncwarp();
@@ -489,7 +505,6 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
     const bool has_part = kRev ? col0 + 15 >= 32 * (warp & 1) : col0 <= 32 * (warp & 1) + 31;
     auto weigh = [&](int c, int s, uint32_t ph) {
       const int at_tok = chunk_at(c) * C, len = min(C, seg.len - at_tok);
-      [[maybe_unused]] float sum = 0.f;
       if (has_part) {
         const uint32_t cp = (uint32_t)c & 1u;
         if (!all(tc::mbar_wait3(p_full, cp, &gates[s], ph, o_full, cp ^ 1u, abort_flag))) return false;
@@ -503,9 +518,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
 #pragma unroll 1
         for (int k = col0; k < col0 + 16; k += 8) {
           uint32_t x[8], hi[4], lo[4];
-          [[maybe_unused]] uint32_t pe[8];
           tc::tmem_ld8(lane_addr + K::P + k, x);
-          if constexpr (kGrad) tc::tmem_ld8(lane_addr + K::PE + k, pe);
           tc::tmem_ld_wait();
           const int own = t - k, last = len - k;  // columns in front of own (forwards) or behind it have a part
 #pragma unroll
@@ -519,10 +532,6 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
               // what is masked may be anything; backwards also what lies behind the sequence
               if (kRev ? i + j < own || i + j >= last : i + j > own) p.x = 0.f;
               if (kRev ? i + j + 1 < own || i + j + 1 >= last : i + j + 1 > own) p.y = 0.f;
-              if constexpr (kGrad) {  // (masked columns have to be kept from a NaN in the other product too)
-                if (kRev ? i + j > own && i + j < last : i + j < own) sum = fmaf(p.x, __uint_as_float(pe[i + j]), sum);
-                if (kRev ? i + j + 1 > own && i + j + 1 < last : i + j + 1 < own) sum = fmaf(p.y, __uint_as_float(pe[i + j + 1]), sum);
-              }
               split_pair(p, hi[(i + j) / 2], lo[(i + j) / 2]);
             }
           }
@@ -535,8 +544,6 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(pp_ready);
       }
-      if constexpr (kGrad)
-        if (t < len) a.intra[(((int64_t)(col0 >> 4) * a.Hv + h) * a.B + seg.b) * a.T + seg.t0 + at_tok + t] = a.negative ? -sum : sum;
       return true;
     };
     bool ok = true;
@@ -545,19 +552,21 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
 #pragma unroll 1
     for (int c = 0; c < n_chunks; ++c) {
       const uint32_t cp = (uint32_t)c & 1u;
+      const int s_c = s;
+      const uint32_t ph_c = ph;
       if constexpr (!kState) {
         publish();
-        ok = weigh(c, s, ph);
+        if (!kGrad) ok = weigh(c, s_c, ph_c);  // (with the gradient of g the increment's second half waits for the first one to be taken)
         if (!ok) break;
       }
-      ok = all(tc::mbar_wait(&ds_full[half], cp, abort_flag));  // (the gate vectors were there before the images were)
+      ok = all(tc::mbar_wait(&ds_full[kState ? (int)cp : half], kState ? (uint32_t)(c >> 1) & 1u : cp, abort_flag));  // (the gate vectors were there before the images were)
       if (!ok) break;
       tc::tc_fence_after_sync();
       const float decay = reinterpret_cast<const float*>(smem + K::GV + s * GATES)[GV_TOT];
 #pragma unroll
       for (int q = 0; q < HC / 16; ++q) {
         uint32_t x[16];
-        tc::tmem_ld16(lane_addr + K::DS + (FH == 2 ? 0 : HC * grp) + 16 * q, x);
+        tc::tmem_ld16(lane_addr + K::DS + cp * K::TURN_DS + (FH == 2 ? 0 : HC * grp) + 16 * q, x);
         tc::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -565,9 +574,11 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
       }
       tc::tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) { tc::mbar_arrive(&ds_empty[half]); tc::mbar_arrive(&empty[s]); }
+      if (lane == 0) { tc::mbar_arrive(&ds_empty[kState ? (int)cp : half]); tc::mbar_arrive(&empty[s]); }
       if (++s == K::STAGES) { s = 0; ph ^= 1u; }
       if constexpr (!kState) {
+        if (kGrad) ok = weigh(c, s_c, ph_c);
+        if (!ok) break;
         if (c + 1 < n_chunks) {  // the images may be written again
           ok = all(tc::mbar_wait(h_read, cp, abort_flag));
           if (!ok) break;
@@ -726,10 +737,12 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
     // pairs of tokens, the layout of a left operand.  (Y times the weights, in shared memory as right operand, was 64 KB more through shared memory a chunk, which
     // bounded it, and a third more instructions.)
     const int wq = warp & 3, r8 = lane & 7, m4 = lane >> 3, t2 = 2 * (lane & 3);
-    int s = 0;
+    // For the state alone the output's warps take every other chunk.
+    constexpr int EACH = kState ? 2 : 1;
+    int s = kState ? (warp >> 2) & 1 : 0;
     uint32_t ph = 0;
 #pragma unroll 1
-    for (int c = 0; c < n_chunks; ++c) {
+    for (int c = s; c < n_chunks; c += EACH) {
       const uint32_t cp = (uint32_t)c & 1u;
       const int len = min(C, seg.len - chunk_at(c) * C);
       bool ok = all(tc::mbar_wait2(&full[s], ph, &gates[s], ph, abort_flag));
@@ -748,10 +761,9 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
         __syncwarp();
         if (!kState && lane == 0) tc::mbar_arrive(cleared);
       }
-      // 32 tokens; for the state alone the output's warps take half of them
 #pragma unroll 1
-      for (int q = kState ? (warp >> 2) & 1 : 0; q < (kState ? ((warp >> 2) & 1) + 1 : 2); ++q) {
-        ok = ok && all(tc::mbar_wait(&img_read[q], cp ^ 1u, abort_flag));
+      for (int q = 0; q < 2; ++q) {  // 32 tokens
+        if (kState ? q == 0 : true) ok = ok && all(kState ? tc::mbar_wait(&img_read[cp], ((uint32_t)(c >> 1) & 1u) ^ 1u, abort_flag) : tc::mbar_wait(&img_read[q], cp ^ 1u, abort_flag));
         if (!ok) break;
         tc::tc_fence_after_sync();
         if (32 * wq < DV) {
@@ -777,16 +789,16 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
               else split_pair(f, terms[0][i], terms[1][i]);
             }
 #pragma unroll
-            for (int t = 0; t < K::TERMS; ++t) tc::tmem_st_pairs(tm + ((uint32_t)(32 * wq + 16 * hf) << 16) + K::IMG + 32 * t + 16 * q, terms[t]);
+            for (int t = 0; t < K::TERMS; ++t) tc::tmem_st_pairs(tm + ((uint32_t)(32 * wq + 16 * hf) << 16) + K::IMG + cp * K::TURN_IMG + 32 * t + 16 * q, terms[t]);
           }
           tc::tmem_st_wait();
         }
         tc::tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&img_ready[q]);
+        if (lane == 0 && (!kState || q == 1)) tc::mbar_arrive(&img_ready[kState ? (int)cp : q]);
       }
       if (!ok) break;
-      if (++s == K::STAGES) { s = 0; ph ^= 1u; }
+      if ((s += EACH) >= K::STAGES) { s -= K::STAGES; ph ^= 1u; }
     }
   }
 

@@ -69,6 +69,20 @@ inline bool result_map(CUtensorMap* m, void* p, int d, int heads, int B, int T, 
   return ok;
 }
 
+// More shared memory than the default, asked for once a device
+template <int DK, int DV, class K>
+int allow_smem(K* kernel, int smem) {
+  static std::atomic<bool> ready[MAX_DEVICES];
+  int dev = 0;
+  AVE_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= MAX_DEVICES) return AVE_GDN_UNSUPPORTED;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    AVE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ready[dev].store(true, std::memory_order_release);
+  }
+  return AVE_GDN_OK;
+}
+
 // The register split of the roles counts on the registers that the kernel is launched with.
 template <int DK, int DV, bool kRev, Mode kMode>
 int launch_scan(const Args& a, const Maps& maps, cudaStream_t stream) {

@@ -67,12 +67,19 @@ class Scan:
             self.gates[s].arrive()
             s, ph = (0, ph ^ 1) if s + 1 == self.S else (s + 1, ph)
 
-    def images(self, w):
-        s, ph = 0, 0
-        for c in range(self.n):
+    def images(self, w, group=0):
+        s, ph = group, 0
+        for c in range(group, self.n, 2 if self.state else 1):
             cp = c & 1
             yield [(self.full[s], ph), (self.gates[s], ph)]
             self.need("loaded", c); self.need("gates", c)
+            if self.state:  # two groups, chunks and places in turn
+                yield [(self.img_read[cp], (c >> 1 & 1) ^ 1)]
+                self.need("increment", c - 2)
+                self.mark("image0", c); self.mark("image1", c)
+                self.img_ready[cp].arrive()
+                s, ph = (s + 2 - self.S, ph ^ 1) if s + 2 >= self.S else (s + 2, ph)
+                continue
             if c == self.ragged:
                 self.cleared.arrive()
             for q in range(2):
@@ -90,6 +97,14 @@ class Scan:
             def part(f, q):
                 self.need(f"image{q}", c, 4)
                 self.need("drained%d" % (f if not (self.grad and self.fh == 2) else 1 - f), c - 1 if f == 0 or not self.grad else c, 4 * GROUPS // self.fh)
+            if self.state:
+                yield [(self.ds_empty[cp], (c >> 1 & 1) ^ 1), (self.img_ready[cp], c >> 1 & 1)]
+                self.need("image1", c, 4); self.need("drained0", c - 2, 4 * GROUPS)
+                self.mark("increment", c)
+                for b in (self.ds_full[cp], self.img_read[cp], self.empty[s]):
+                    b.arrive()
+                s = 0 if s + 1 == self.S else s + 1
+                continue
             if self.grad and self.fh == 2:
                 yield [(self.ds_empty[1], cp ^ 1), (self.img_ready[0], cp), (self.img_ready[1], cp)]
                 part(0, 0); part(0, 1)
@@ -109,16 +124,11 @@ class Scan:
                 part(0, 1)
                 self.ds_full[0].arrive()
                 self.img_read[1].arrive()
-            if self.state:
-                self.empty[s].arrive()
-            else:
-                yield [(self.h_ready, cp), (self.pp_ready, cp) if self.grad else (self.o_empty, cp ^ 1)]
-                self.need("published", c, 4 * GROUPS)
-                self.need("taken", c - 1, 4)
-                if self.grad:
-                    self.need("weighed", c, 6)
-                self.mark("inter", c)
-                self.h_read.arrive()
+            yield [(self.h_ready, cp), (self.o_empty, cp ^ 1)]
+            self.need("published", c, 4 * GROUPS)
+            self.need("taken", c - 1, 4)
+            self.mark("inter", c)
+            self.h_read.arrive()
             s = 0 if s + 1 == self.S else s + 1
 
     def issue_scores(self):
@@ -155,21 +165,27 @@ class Scan:
         s, ph = 0, 0
         for c in range(self.n):
             cp = c & 1
-            if not self.state:
-                self.need("inter", c - 1)
-                self.mark("published", c)
-                self.h_ready.arrive()
+            def weigh():
                 if part:
                     yield [(self.p_full, cp), (self.gates[s], ph), (self.o_full, cp ^ 1)]
                     self.need("scores", c); self.need("intra", c - 1); self.need("gates", c)
                     self.mark("weighed", c)
                     self.pp_ready.arrive()
-            yield [(self.ds_full[half], cp)]
+            if not self.state:
+                self.need("inter", c - 1)
+                self.mark("published", c)
+                self.h_ready.arrive()
+                if not self.grad:
+                    yield from weigh()
+            at = cp if self.state else half
+            yield [(self.ds_full[at], c >> 1 & 1 if self.state else cp)]
             self.need("increment", c, half + 1)
             self.mark(f"drained{half}", c)
             self.mark("decayed", c)
-            self.ds_empty[half].arrive()
+            self.ds_empty[at].arrive()
             self.empty[s].arrive()
+            if self.grad:
+                yield from weigh()
             s, ph = (0, ph ^ 1) if s + 1 == self.S else (s + 1, ph)
             if not self.state and c + 1 < self.n:
                 yield [(self.h_read, cp)]
@@ -189,7 +205,9 @@ class Scan:
 
     def run(self, rng):
         roles = [self.loader(), self.gate(), self.issue_state()] + [self.images(w) for w in range(4)] + [self.states(w) for w in range(4 * GROUPS)]
-        if not self.state:
+        if self.state:
+            roles += [self.images(w, 1) for w in range(4)]
+        else:
             roles += [self.issue_scores()] + [self.outputs(w) for w in range(4)]
         speed = [rng.choice([1, 1, 4, 30]) for _ in roles]  # some roles are slow for a while
         waiting = [None] * len(roles)
