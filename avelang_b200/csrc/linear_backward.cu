@@ -30,7 +30,8 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* part, __nv_
   }
 }
 
-// m_ts of a chunk's pairs s < t, summed over s into a[t] and over t into b[s]: one CTA a (chunk, value head), 16 rows t a warp, as warp-level MMAs; bound by the four tiles it reads.
+// m_ts of a chunk's pairs s < t, summed over s into a[t] and over t into b[s]: one CTA a (chunk, value head), as warp-level MMAs, one of the ten 16 x 16 blocks on and below the diagonal
+// a warp, so that the CTA's time is a block's.  Bound by the four tiles it reads and the latencies in front of them.
 struct PairSums {
   const __nv_bfloat16 *q, *k, *v, *d_o;
   int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h, o_b, o_t, o_h;
@@ -38,13 +39,14 @@ struct PairSums {
   float scale;
   float *a, *b;  // [Hv][B T]
 };
+constexpr int PAIR_THREADS = 320;
 template <int DK, int DV>
-__global__ void __launch_bounds__(128) pair_sums_kernel(const Args s, const PairSums p) {
+__global__ void __launch_bounds__(PAIR_THREADS) pair_sums_kernel(const Args s, const PairSums p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = tc::align1024(smem_raw);
   constexpr int KB = 2 * DK, VB = 2 * DV, Q0 = 0, K0 = 64 * KB, V0 = 2 * K0, O0 = V0 + 64 * VB;
   float2* G = reinterpret_cast<float2*>(smem + O0 + 64 * VB);  // [64]
-  float* cols = reinterpret_cast<float*>(G + 64);              // [4][64]
+  float *cols = reinterpret_cast<float*>(G + 64), *rows = cols + 256;  // [4][64] each: of the block's row for the columns, of its column for the rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   if (!offsets_fit(s, false)) return;
@@ -52,82 +54,90 @@ __global__ void __launch_bounds__(128) pair_sums_kernel(const Args s, const Pair
   const Seg c = seg_of_slot(s, blockIdx.x / s.Hv);
   if (!c.ok || c.len == 0) return;
   const uint32_t base = tc::smem_u32(smem);
-  load_tile<64, DK / 8, 128>(base + Q0, p.q + c.b * p.q_b + (int64_t)c.t0 * p.q_t + hk * p.q_h, p.q_t, c.len, threadIdx.x);
-  load_tile<64, DK / 8, 128>(base + K0, p.k + c.b * p.k_b + (int64_t)c.t0 * p.k_t + hk * p.k_h, p.k_t, c.len, threadIdx.x);
-  load_tile<64, DV / 8, 128>(base + V0, p.v + c.b * p.v_b + (int64_t)c.t0 * p.v_t + h * p.v_h, p.v_t, c.len, threadIdx.x);
-  load_tile<64, DV / 8, 128>(base + O0, p.d_o + c.b * p.o_b + (int64_t)c.t0 * p.o_t + h * p.o_h, p.o_t, c.len, threadIdx.x);
-  cp_commit();
-  if (warp == 0) {
+  if (warp < 8) {
+    load_tile<64, DK / 8, 256>(base + Q0, p.q + c.b * p.q_b + (int64_t)c.t0 * p.q_t + hk * p.q_h, p.q_t, c.len, threadIdx.x);
+    load_tile<64, DK / 8, 256>(base + K0, p.k + c.b * p.k_b + (int64_t)c.t0 * p.k_t + hk * p.k_h, p.k_t, c.len, threadIdx.x);
+    cp_commit();
+    load_tile<64, DV / 8, 256>(base + V0, p.v + c.b * p.v_b + (int64_t)c.t0 * p.v_t + h * p.v_h, p.v_t, c.len, threadIdx.x);
+    load_tile<64, DV / 8, 256>(base + O0, p.d_o + c.b * p.o_b + (int64_t)c.t0 * p.o_t + h * p.o_h, p.o_t, c.len, threadIdx.x);
+    cp_commit();
+  } else if (warp == 8) {
     auto fetch = [&](int t) { return t < c.len ? s.g[c.b * s.g_stride_b + (int64_t)(c.t0 + t) * s.g_stride_t + h] : 0.f; };
     Two G0, G1;
     gate_scan(fetch(2 * lane), fetch(2 * lane + 1), lane, G0, G1);
     G[2 * lane] = make_float2(G0.h, G0.l);
     G[2 * lane + 1] = make_float2(G1.h, G1.l);
   }
-  cp_wait<0>();
+  cp_wait<1>();
   __syncthreads();
-  const int r0 = 16 * warp, row = r0 + (lane >> 2);
+  const int i = warp < 1 ? 0 : warp < 3 ? 1 : warp < 6 ? 2 : 3, j = warp - i * (i + 1) / 2, row = 16 * i + (lane >> 2);
+  float x[2][4], y[2][4];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) { zero(x[n]); zero(y[n]); }
+#pragma unroll
+  for (int k = 0; k < DK / 16; ++k) {
+    uint32_t l[4], r[4];
+    ldsm4(l, base + Q0 + at_a<KB>(16 * i, 2 * k, lane));
+    ldsm4(r, base + K0 + at_b<KB>(16 * j, 2 * k, lane));
+    mma_bf16(x[0], l, r[0], r[1]);
+    mma_bf16(x[1], l, r[2], r[3]);
+  }
   float own[2] = {0.f, 0.f};
   const float2 gt[2] = {G[row], G[row + 8]};
-#pragma unroll 1
-  for (int j = 0; j < 4; ++j) {  // 16 columns
-    float x[2][4], y[2][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) { zero(x[n]); zero(y[n]); }
-    if (j <= warp) {
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int k = 0; k < DK / 16; ++k) {
-        uint32_t l[4], r[4];
-        ldsm4(l, base + Q0 + at_a<KB>(r0, 2 * k, lane));
-        ldsm4(r, base + K0 + at_b<KB>(16 * j, 2 * k, lane));
-        mma_bf16(x[0], l, r[0], r[1]);
-        mma_bf16(x[1], l, r[2], r[3]);
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int t = row + 8 * (e >> 1), col = 16 * j + 8 * n + 2 * (lane & 3) + (e & 1);
+      const float2 gs = G[col];
+      x[n][e] = col < t ? p.scale * ex2((gt[e >> 1].x - gs.x) + (gt[e >> 1].y - gs.y)) * x[n][e] : 0.f;
+    }
+  cp_wait<0>();
+  __syncthreads();
 #pragma unroll
-      for (int k = 0; k < DV / 16; ++k) {
-        uint32_t l[4], r[4];
-        ldsm4(l, base + O0 + at_a<VB>(r0, 2 * k, lane));
-        ldsm4(r, base + V0 + at_b<VB>(16 * j, 2 * k, lane));
-        mma_bf16(y[0], l, r[0], r[1]);
-        mma_bf16(y[1], l, r[2], r[3]);
-      }
+  for (int k = 0; k < DV / 16; ++k) {
+    uint32_t l[4], r[4];
+    ldsm4(l, base + O0 + at_a<VB>(16 * i, 2 * k, lane));
+    ldsm4(r, base + V0 + at_b<VB>(16 * j, 2 * k, lane));
+    mma_bf16(y[0], l, r[0], r[1]);
+    mma_bf16(y[1], l, r[2], r[3]);
+  }
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = row + 8 * (e >> 1), col = 16 * j + 8 * n + 2 * (lane & 3) + (e & 1);
+      const float m = col < t ? x[n][e] * y[n][e] : 0.f;
+      own[e >> 1] += m;
+      sum[e & 1] += m;
     }
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      float sum[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = row + 8 * (i >> 1), col = 16 * j + 8 * n + 2 * (lane & 3) + (i & 1);
-        const float2 gs = G[col];
-        const float m = col < t ? p.scale * ex2((gt[i >> 1].x - gs.x) + (gt[i >> 1].y - gs.y)) * (x[n][i] * y[n][i]) : 0.f;
-        own[i >> 1] += m;
-        sum[i & 1] += m;
-      }
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
-        sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], o);
-      }
-      if (lane < 4) *reinterpret_cast<float2*>(cols + 64 * warp + 16 * j + 8 * n + 2 * lane) = make_float2(sum[0], sum[1]);
+    for (int o = 4; o < 32; o <<= 1) {
+      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
+      sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], o);
     }
+    if (lane < 4) *reinterpret_cast<float2*>(cols + 64 * i + 16 * j + 8 * n + 2 * lane) = make_float2(sum[0], sum[1]);
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
     own[0] += __shfl_xor_sync(0xffffffffu, own[0], o);
     own[1] += __shfl_xor_sync(0xffffffffu, own[1], o);
   }
-  const int64_t at = ((int64_t)h * s.B + c.b) * s.T + c.t0;
-  if ((lane & 3) == 0) {
-    if (row < c.len) p.a[at + row] = own[0];
-    if (row + 8 < c.len) p.a[at + row + 8] = own[1];
-  }
+  if ((lane & 3) == 0) { rows[64 * j + row] = own[0]; rows[64 * j + row + 8] = own[1]; }
   __syncthreads();
-  if (threadIdx.x < c.len && threadIdx.x < 64) p.b[at + threadIdx.x] = (cols[threadIdx.x] + cols[64 + threadIdx.x]) + (cols[128 + threadIdx.x] + cols[192 + threadIdx.x]);
+  const int64_t at = ((int64_t)h * s.B + c.b) * s.T + c.t0;
+  const int t = threadIdx.x & 63, block = t >> 4;
+  if (t < c.len && threadIdx.x < 128) {
+    const bool of_row = threadIdx.x < 64;
+    float sum = 0.f;
+    for (int n = of_row ? 0 : block; n <= (of_row ? block : 3); ++n) sum += (of_row ? rows : cols)[64 * n + t];
+    (of_row ? p.a : p.b)[at + t] = sum;
+  }
 }
 
 struct GateGrad {
   const float *inter_a, *intra_a, *inter_b, *intra_b;  // of the scans for dq and dk
-  int parts;                 // of inter: dk / 32
   const float *seg_s, *seg_r;  // states that enter the segments, from the front and from behind
   const float *s0, *ds0;     // null: no initial state
   float* dg;                 // [B, T, Hv], or null
@@ -147,7 +157,8 @@ __device__ __forceinline__ double block_sum(double x, double* sm) {  // 256 thre
   return s;
 }
 
-// One CTA a segment and head: the running sum of B - A from the segment's first token, in 64 bits.
+// One CTA a segment and head: the running sum of B - A from the segment's first token, in 64 bits.  Bound by latencies: the next 256 tokens are read while these are summed.
+template <int PARTS>
 __global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const GateGrad q) {
   __shared__ double sm[8], wsum[8];
   pdl_wait();
@@ -170,20 +181,31 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const Gate
   }
   double dot = 0.0;
   if (x != nullptr)
+#pragma unroll 4
     for (int i = tid * 4; i < size; i += 1024) {
       const float4 u = *reinterpret_cast<const float4*>(x + i), v = *reinterpret_cast<const float4*>(y + i);
       dot += ((double)u.x * v.x + (double)u.y * v.y) + ((double)u.z * v.z + (double)u.w * v.w);
     }
-  double run = block_sum(dot, sm), total = 0.0;  // dg of the next token
   const int64_t base = ((int64_t)h * a.B + seg.b) * a.T + seg.t0, plane = (int64_t)a.Hv * a.B * a.T;
+  float va[PARTS + 1], vb[PARTS + 1];
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      va[p] = t < seg.len ? q.inter_a[p * plane + base + t] : 0.f;
+      vb[p] = t < seg.len ? q.inter_b[p * plane + base + t] : 0.f;
+    }
+    va[PARTS] = t < seg.len ? q.intra_a[base + t] : 0.f;
+    vb[PARTS] = t < seg.len ? q.intra_b[base + t] : 0.f;
+  };
+  fetch(tid);
+  double run = block_sum(dot, sm), total = 0.0;  // dg of the next token
   for (int t0 = 0; t0 < seg.len; t0 += 256) {
     const int t = t0 + tid;
-    double d = 0.0;
-    if (t < seg.len) {
-      float ia = 0.f, ib = 0.f;
-      for (int p = 0; p < q.parts; ++p) { ia += q.inter_a[p * plane + base + t]; ib += q.inter_b[p * plane + base + t]; }
-      d = ((double)ib - (double)ia) + ((double)q.intra_b[base + t] - (double)q.intra_a[base + t]);
-    }
+    float ia = 0.f, ib = 0.f;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) { ia += va[p]; ib += vb[p]; }
+    const double d = ((double)ib - (double)ia) + ((double)vb[PARTS] - (double)va[PARTS]);
+    fetch(t + 256);
     double inc = d;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -374,11 +396,11 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
       const lin::PairSums p{lin_bf(a.q), lin_bf(a.k), lin_bf(a.v), lin_bf(a.d_o), a.q_stride_b, a.q_stride_t, a.q_stride_h, a.k_stride_b, a.k_stride_t, a.k_stride_h,
                             a.v_stride_b, a.v_stride_t, a.v_stride_h, a.do_stride_b, a.do_stride_t, a.do_stride_h, rep, a.scale, f32(l.intra_a), f32(l.intra_b)};
       auto* kernel = lin::pair_sums_kernel<DK, DV>;
-      constexpr int smem = 64 * 4 * (DK + DV) + 64 * 8 + 4 * 64 * 4 + 1024;
+      constexpr int smem = 64 * 4 * (DK + DV) + 64 * 8 + 8 * 64 * 4 + 1024;
       if ((r = lin::allow_smem<DK, DV>(kernel, smem))) return r;
       const int64_t grid = s.plan.slots * a.Hv;
       if (grid > 0x7fffffff) return (int)AVE_GDN_UNSUPPORTED;
-      AVE_CUDA_TRY(launch_after(kernel, (unsigned)grid, 128, smem, stream, s, p));
+      AVE_CUDA_TRY(launch_after(kernel, (unsigned)grid, lin::PAIR_THREADS, smem, stream, s, p));
     }
     return (int)AVE_GDN_OK;
   });
@@ -387,12 +409,12 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
   if (grad) {
     lin::GateGrad q{};
     q.inter_a = f32(l.inter_a); q.inter_b = f32(l.inter_b); q.intra_a = f32(l.intra_a); q.intra_b = f32(l.intra_b);
-    q.parts = a.dk / 32; q.dk = a.dk; q.dv = a.dv;
+    q.dk = a.dk; q.dv = a.dv;
     if (l.plan.cut) { q.seg_s = f32(l.s); q.seg_r = f32(l.r); }
     if (a.initial_state != nullptr) { q.s0 = a.initial_state; q.ds0 = a.d_initial_state; }
     if (by_token) q.dg = a.d_g; else q.sums = f32(l.sums);
     const int64_t grid = l.plan.slots * a.Hv;
-    AVE_CUDA_TRY(launch_after(lin::gate_grad_kernel, (unsigned)grid, 256, 0, stream, base, q));
+    AVE_CUDA_TRY(launch_after(a.dk == 128 ? lin::gate_grad_kernel<4> : lin::gate_grad_kernel<2>, (unsigned)grid, 256, 0, stream, base, q));  // (scans give a sum for each 32 of dk)
     if (!by_token) AVE_CUDA_TRY(launch_after(lin::head_gate_grad_kernel, (unsigned)a.Hv, 256, 0, stream, base, (const float*)q.sums, a.d_g));
   }
   if (a.cu_seqlens != nullptr)
