@@ -1135,6 +1135,19 @@ void check_norm_input(const Tensor& x, const Tensor* w, const Tensor* b) {
   REQ(b == nullptr || b->scalar_type() == w->scalar_type(), "weight and bias must share a dtype");
 }
 
+// Rows of two [rows, n] views with contiguous rows: the same ones, or none in common as far as two row distances tell (views with different distances over one range count as overlapping).
+bool same_or_apart(const Tensor& x, const Tensor& y) {
+  const int64_t n = x.size(1), rows = x.size(0);
+  if (rows == 0 || x.storage().unsafeGetStorageImpl() != y.storage().unsafeGetStorageImpl()) return true;
+  const int64_t sx = rows > 1 ? x.stride(0) : n, sy = rows > 1 ? y.stride(0) : n;
+  const int64_t d = y.storage_offset() - x.storage_offset();
+  if (d >= sx * (rows - 1) + n || -d >= sy * (rows - 1) + n) return true;  // one range behind the other
+  if (sx != sy) return false;
+  if (d == 0) return true;
+  const int64_t r = ((d % sx) + sx) % sx;  // columns of one row beside the other's
+  return r >= n && r + n <= sx;
+}
+
 // layer_norm(x, weight, bias, eps, return_stats, out) -> out or (out, mean, rstd)
 PyObject* layer_norm(PyObject* const* p) {
   const Tensor& x = tensor(p[0], "x");
@@ -1147,6 +1160,8 @@ PyObject* layer_norm(PyObject* const* p) {
   const Tensor y2 = as_rows(y);
   if (x2.stride(1) != 1) x2 = x2.contiguous();
   REQ(y2.is_alias_of(y) && (y2.stride(1) == 1 || y2.size(1) == 1), "out must be viewable as [rows, n] with contiguous rows");
+  REQ(y2.size(0) <= 1 || y2.stride(0) >= y2.size(1), "the rows of out must not overlap");
+  REQ(same_or_apart(x2, y2), "out must be x itself or share no element with it");
   const Tensor wc = w != nullptr ? w->contiguous() : Tensor(), bc = b != nullptr ? b->contiguous() : Tensor();
   const bool stats = truth(p[4]);
   Tensor mean, rstd;

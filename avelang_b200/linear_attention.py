@@ -54,19 +54,21 @@ def linear_attention_backward(q, k, v, g, d_o, scale=None, initial_state=None, d
 
 class LinearAttentionFunction(torch.autograd.Function):
     """``o, final_state = LinearAttentionFunction.apply(q, k, v, g, scale, initial_state, cu_seqlens)``: the chunked forward pass with
-    the chunked backward pass attached (g, scale, initial_state and cu_seqlens may be None)."""
+    the chunked backward pass attached (g, scale, initial_state and cu_seqlens may be None).  A step with its backward pass can be captured
+    into a CUDA graph once the results of eager steps on the same leaves are gone."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, scale, initial_state, cu_seqlens):
         o, final = chunk_linear_attention(q, k, v, g, scale, initial_state, True, cu_seqlens)
         ctx.save_for_backward(q, k, v, g, initial_state, cu_seqlens)
         ctx.scale = scale
+        ctx.set_materialize_grads(False)
         return o, final
 
     @staticmethod
     def backward(ctx, d_o, d_final):
         q, k, v, g, s0, cu = ctx.saved_tensors
-        d_o = d_o.to(torch.bfloat16).contiguous()
+        d_o = torch.zeros_like(v) if d_o is None else d_o.to(torch.bfloat16).contiguous()
         d_final = None if d_final is None else d_final.float().contiguous()
         dq, dk, dv, dg, ds0 = linear_attention_backward(q, k, v, g, d_o, ctx.scale, s0, d_final, cu)
         return dq, dk, dv, dg, None, ds0, None

@@ -20,7 +20,8 @@ _lib.register_operators()
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, *, return_stats=False, out=None):
-    """Returns ``y``, or with ``return_stats`` ``(y, mean, rstd)``, the statistics fp32 in the leading shape of ``x``.  ``out`` may be ``x``."""
+    """Returns ``y``, or with ``return_stats`` ``(y, mean, rstd)``, the statistics fp32 in the leading shape of ``x``.  ``out`` may be ``x``;
+    one that shares some of its elements in another way is refused."""
     return _native.layer_norm(x, weight, bias, eps, return_stats, out)
 
 
@@ -31,7 +32,8 @@ def layer_norm_backward(d_y, x, mean, rstd, weight=None):
 
 
 class LayerNormFunction(torch.autograd.Function):
-    """``y = LayerNormFunction.apply(x, weight, bias, eps)``: ``layer_norm`` with its backward pass attached (weight and bias may be None)."""
+    """``y = LayerNormFunction.apply(x, weight, bias, eps)``: ``layer_norm`` with its backward pass attached (weight and bias may be None).  A step with
+    its backward pass can be captured into a CUDA graph once the results of eager steps on the same leaves are gone."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):

@@ -188,3 +188,20 @@ def test_struct_mirrors(tmp_path):
     subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [x for _, m, f in names for x in (ctypes.sizeof(m), getattr(m, f).offset)]
+
+
+def test_norm_refuses_results_that_overlap_their_input(built_lib):
+    from avelang_b200 import norm as N
+    with FakeTensorMode():
+        buf = bf(9, 64)
+        for x, out in ((buf[:8], buf[1:]), (buf[1:], buf[:8]), (buf[:, :40], buf[:, 20:60]), (buf.view(-1)[:512].view(8, 64), buf.view(-1)[32:544].view(8, 64)),
+                       (buf[:8, :32], buf.view(-1)[:256].view(8, 32)), (buf[:1].expand(8, 64), buf[:8])):
+            with pytest.raises(ValueError, match="itself or share no element"):
+                N.layer_norm(x, out=out)
+        with pytest.raises(ValueError, match="rows of out must not overlap"):
+            N.layer_norm(bf(8, 64), out=buf[:1].expand(8, 64))
+    with FakeTensorMode(), Recorder(run=False) as mode:
+        buf = bf(9, 64)
+        for x, out in ((buf, buf), (buf[:, :32], buf[:, 32:]), (buf[:, 40:], buf[:, :24]), (buf[:4], buf[4:8]), (buf[5:], buf[:4]), (buf[::2], buf[::2]), (buf[0], buf[0])):
+            N.layer_norm(x, out=out)
+    assert mode.seen == ["layer_norm"] * 7
