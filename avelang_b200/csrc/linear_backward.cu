@@ -14,8 +14,42 @@ namespace ave {
 namespace {
 namespace lin {
 
-// The value heads of a key head, summed: out[row][hk][d] = sum over r of part[row][hk rep + r][d]; eight features a thread
-__global__ void __launch_bounds__(256) sum_heads_kernel(const float* part, __nv_bfloat16* out, int64_t pieces, int d8, int hk, int rep) {
+// The scans of one call side by side: their CTAs fill the SMs together, the longest first.
+struct Pass { Args a; Maps m; };
+struct TwoPasses { Pass p[2]; };
+struct ThreePasses { Pass p[3]; };
+// Increments of the segments from the front, and from behind
+template <int DK, int DV>
+__global__ void __launch_bounds__(THREADS, 1) states_kernel(const __grid_constant__ TwoPasses t) {
+  if (blockIdx.y == 0) scan<DK, DV, false, STATE>(t.p[0].a, t.p[0].m);
+  else scan<DK, DV, true, STATE>(t.p[1].a, t.p[1].m);
+}
+template <int DK, int DV>
+__global__ void __launch_bounds__(256) chains_kernel(const Args fwd, const Args rev) {
+  if (blockIdx.y == 0) chain<DK, DV, false>(fwd);
+  else chain<DK, DV, true>(rev);
+}
+// dq, dk, dv (kDq: the mode of the first two, kDv of the last)
+template <int DK, int DV, Mode kDq, Mode kDv>
+__global__ void __launch_bounds__(THREADS, 1) grads_kernel(const __grid_constant__ ThreePasses t) {
+  if (blockIdx.y == 0) scan<DV, DK, false, kDq>(t.p[0].a, t.p[0].m);
+  else if (blockIdx.y == 1) scan<DV, DK, true, kDq>(t.p[1].a, t.p[1].m);
+  else scan<DK, DV, true, kDv>(t.p[2].a, t.p[2].m);
+}
+template <int DK, int DV, Mode kDq, Mode kDv>
+int launch_grads(const ThreePasses& t, cudaStream_t stream) {
+  constexpr auto* kernel = &grads_kernel<DK, DV, kDq, kDv>;
+  constexpr int smem = Cfg<kDq>::SMEM > Cfg<kDv>::SMEM ? Cfg<kDq>::SMEM : Cfg<kDv>::SMEM;
+  const int rc = scan_ready<kernel>(smem);
+  if (rc != AVE_GDN_OK) return rc;
+  AVE_CUDA_TRY(launch_after(kernel, dim3((unsigned)scan_grid(t.p[0].a), 3), THREADS, smem, stream, t));
+  return AVE_GDN_OK;
+}
+
+// The value heads of a key head, summed: out[row][hk][d] = sum over r of part[row][hk rep + r][d]; eight features a thread; dq, and dk
+__global__ void __launch_bounds__(256) sum_heads_kernel(const float* parts, int64_t apart, __nv_bfloat16* dq, __nv_bfloat16* dk, int64_t pieces, int d8, int hk, int rep) {
+  const float* part = parts + blockIdx.y * apart;
+  __nv_bfloat16* out = blockIdx.y == 0 ? dq : dk;
   pdl_wait();
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
     const int64_t head = i / d8;  // row * hk + key head
@@ -146,7 +180,8 @@ struct GateGrad {
   int dk, dv;
 };
 
-__device__ __forceinline__ double block_sum(double x, double* sm) {  // 256 threads, all get it
+template <int THREADS>
+__device__ __forceinline__ double block_sum(double x, double* sm) {  // all threads get it
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   __syncthreads();
@@ -154,17 +189,19 @@ __device__ __forceinline__ double block_sum(double x, double* sm) {  // 256 thre
   __syncthreads();
   double s = 0.0;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) s += sm[w];
+  for (int w = 0; w < THREADS / 32; ++w) s += sm[w];
   return s;
 }
 
 // One CTA a segment and head: the running sum of B - A from the segment's first token, in 64 bits.  Its end is known too, <S, R> of the next segment's beginning or of the final state and
 // its gradient, or 0, and what is open there is spread evenly over the tokens: A and B are sums in 32 bits whose errors a running sum collects like a random walk, and a walk that is
-// tied down at both ends strays 1.7 times less (2 x 4096 tokens in segments of 2048: 1.3e-6 of the gradient's norm without).  Bound by latencies: the next 256 tokens are read while
+// tied down at both ends strays 1.7 times less (2 x 4096 tokens in segments of 2048: 1.3e-6 of the gradient's norm without).  Bound by latencies: the next tokens are read while
 // these are summed.
+constexpr int GATE_THREADS = 512;
 template <int PARTS>
-__global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const GateGrad q) {
-  __shared__ double sm[8], wsum[8];
+__global__ void __launch_bounds__(GATE_THREADS) gate_grad_kernel(const Args a, const GateGrad q) {
+  constexpr int N = GATE_THREADS;
+  __shared__ double sm[N / 32], wsum[N / 32];
   pdl_wait();
   if (!offsets_fit(a, false)) return;
   const int h = blockIdx.x % a.Hv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -195,7 +232,7 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const Gate
     double dot = 0.0;
     if (x != nullptr)
 #pragma unroll 4
-      for (int i = tid * 4; i < size; i += 1024) {
+      for (int i = tid * 4; i < size; i += 4 * N) {
         const float4 u = *reinterpret_cast<const float4*>(x + i), v = *reinterpret_cast<const float4*>(y + i);
         dot += ((double)u.x * v.x + (double)u.y * v.y) + ((double)u.z * v.z + (double)u.w * v.w);
       }
@@ -220,18 +257,18 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const Gate
   };
   fetch(tid);
   double dot = product(x, y), open = product(xe, ye) - dot;  // dg of the first token; what the steps do not come to
-  for (int t = tid; t < seg.len; t += 256) {
+  for (int t = tid; t < seg.len; t += N) {
     open -= step();
-    fetch(t + 256);
+    fetch(t + N);
   }
   fetch(tid);
-  double run = block_sum(dot, sm), total = 0.0;
-  open = block_sum(open, sm) / seg.len;
+  double run = block_sum<N>(dot, sm), total = 0.0;
+  open = block_sum<N>(open, sm) / seg.len;
   if (!isfinite(open)) open = 0.0;
-  for (int t0 = 0; t0 < seg.len; t0 += 256) {
+  for (int t0 = 0; t0 < seg.len; t0 += N) {
     const int t = t0 + tid;
     const double d = step();
-    fetch(t + 256);
+    fetch(t + N);
     double inc = d;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -243,7 +280,7 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const Gate
     __syncthreads();
     double before = 0.0, whole = 0.0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < N / 32; ++w) {
       if (w < warp) before += wsum[w];
       whole += wsum[w];
     }
@@ -255,7 +292,7 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const Args a, const Gate
     run += whole;
   }
   if (q.sums != nullptr) {
-    total = block_sum(total, sm);
+    total = block_sum<N>(total, sm);
     if (tid == 0) q.sums[slot * a.Hv + h] = (float)total;
   }
 }
@@ -266,7 +303,7 @@ __global__ void __launch_bounds__(256) head_gate_grad_kernel(const Args a, const
   if (!offsets_fit(a, false)) return;
   double s = 0.0;
   for (int64_t i = threadIdx.x; i < a.plan.slots; i += 256) s += (double)sums[i * a.Hv + blockIdx.x];
-  s = block_sum(s, sm);
+  s = block_sum<256>(s, sm);
   if (threadIdx.x == 0) dg[blockIdx.x] = (float)s;
 }
 
@@ -307,7 +344,7 @@ Layout layout_of(const AveLinearBwdArgs& a) {
     l.s = take(tiles * a.dk * a.dv * 4); l.s_decay = take(tiles * 4);
     l.r = take(tiles * a.dk * a.dv * 4); l.r_decay = take(tiles * 4);
   }
-  if (a.Hv > a.Hk) l.part = take(rows * a.dk * 4);
+  if (a.Hv > a.Hk) l.part = take(2 * rows * a.dk * 4);
   if (a.g != nullptr) {
     l.inter_a = take(rows * (a.dk / 32) * 4); l.inter_b = take(rows * (a.dk / 32) * 4);
     l.intra_a = take(rows * 4); l.intra_b = take(rows * 4);
@@ -343,6 +380,7 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
   base.g = a.g; base.g_stride_b = a.g_stride_b; base.g_stride_t = a.g_stride_t;
   base.x_div = base.y_div = base.w_div = base.e_div = 1;
   base.plan = l.plan;
+  const int64_t part_floats = (int64_t)a.B * a.T * a.Hv * a.dk;
   lin::Args fwd = base, rev = base;  // states from the front, and their gradients from behind, as [dk][dv]
   fwd.y_div = rep; fwd.w_div = 1; fwd.scale_w = 1.f;
   fwd.state_in = a.initial_state; fwd.st_y = a.dv; fwd.st_w = 1;
@@ -354,71 +392,76 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
     rev.state_out = a.d_initial_state; rev.final_by_chain = a.d_initial_state != nullptr;
   }
   // gradient of q or k: dk features of Hk heads, summed over the value heads
-  auto rows_of = [&](lin::Args& s, lin::Maps& m, void* out) {
+  auto rows_of = [&](lin::Pass& p, void* out, int which) {
+    lin::Args& s = p.a;
     s.o = out; s.o_stride_h = a.dk; s.o_stride_t = (int64_t)a.Hk * a.dk; s.o_stride_b = s.o_stride_t * a.T;
     if (rep == 1) {
-      m.o_ok = lin::result_map(&m.o, out, a.dk, a.Hk, a.B, a.T, s.o_stride_b, s.o_stride_t, s.o_stride_h);
+      p.m.o_ok = lin::result_map(&p.m.o, out, a.dk, a.Hk, a.B, a.T, s.o_stride_b, s.o_stride_t, s.o_stride_h);
       return (int)AVE_GDN_OK;
     }
-    s.o_part = f32(l.part);
+    s.o_part = f32(l.part) + which * part_floats;
     const uint64_t row = (uint64_t)a.Hv * a.dk * 4;
     const uint64_t dims[4] = {(uint64_t)a.dk, (uint64_t)a.Hv, (uint64_t)a.T, (uint64_t)a.B}, str[4] = {4, (uint64_t)a.dk * 4, row, row * a.T};
     const uint32_t box[4] = {32, 1, 64, 1};
-    return make_tmap(&m.o, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, s.o_part, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-  };
-  auto sum_heads = [&](void* out) {
-    if (rep == 1) return (int)AVE_GDN_OK;
-    const int64_t pieces = (int64_t)a.B * a.T * a.Hk * (a.dk / 8), ctas = (pieces + 255) / 256;
-    AVE_CUDA_TRY(launch_after(lin::sum_heads_kernel, (unsigned)(ctas < 148 * 16 ? ctas : 148 * 16), 256, 0, stream, (const float*)f32(l.part),
-                              reinterpret_cast<__nv_bfloat16*>(out), pieces, a.dk / 8, a.Hk, rep));
-    return (int)AVE_GDN_OK;
+    return make_tmap(&p.m.o, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, s.o_part, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   rc = lin::by_dims(a.dk, a.dv, [&](auto dk, auto dv) {
     constexpr int DK = decltype(dk)::value, DV = decltype(dv)::value;
     int r;
+    if (3 * lin::scan_grid(base) > 0x7fffffff) return (int)AVE_GDN_UNSUPPORTED;
     if (l.plan.cut) {
-      lin::Maps m{};
-      m.y = mk; m.w = mv;
-      if ((r = lin::launch_scan<DK, DV, false, lin::STATE>(fwd, m, stream))) return r;
-      m.y = mq; m.w = mo;
-      if ((r = lin::launch_scan<DK, DV, true, lin::STATE>(rev, m, stream))) return r;
-      if ((r = lin::launch_chain<DK, DV, false>(fwd, stream))) return r;
-      if ((r = lin::launch_chain<DK, DV, true>(rev, stream))) return r;
+      lin::TwoPasses t{};
+      t.p[0].a = fwd; t.p[0].m.y = mk; t.p[0].m.w = mv;
+      t.p[1].a = rev; t.p[1].m.y = mq; t.p[1].m.w = mo;
+      constexpr auto* states = &lin::states_kernel<DK, DV>;
+      constexpr int smem = lin::Cfg<lin::STATE>::SMEM;
+      if ((r = lin::scan_ready<states>(smem))) return r;
+      AVE_CUDA_TRY(launch_after(states, dim3((unsigned)lin::scan_grid(base), 2), lin::THREADS, smem, stream, t));
+      const int64_t grid = lin::chain_grid<DK, DV>(base);
+      if (grid > 0x7fffffff) return (int)AVE_GDN_UNSUPPORTED;
+      AVE_CUDA_TRY(launch_after(lin::chains_kernel<DK, DV>, dim3((unsigned)grid, 2), 256, 0, stream, fwd, rev));
+    }
+    lin::ThreePasses t{};
+    {  // dq, and the final state
+      lin::Args& s = t.p[0].a;
+      lin::Maps& m = t.p[0].m;
+      s = fwd;
+      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; lin::set_scale(s, a.scale); s.scale_e = a.scale; s.st_y = 1; s.st_w = a.dv;
+      m.x = mo; m.y = mv; m.w = mk; m.e = mq;
+      if ((r = rows_of(t.p[0], a.d_q, 0))) return r;
+      if (grad) {
+        s.inter = f32(l.inter_a);
+        if (a.d_final_state != nullptr) s.state_out = f32(l.final);
+      }
+    }
+    {  // dk
+      lin::Args& s = t.p[1].a;
+      lin::Maps& m = t.p[1].m;
+      s = rev;
+      s.state_out = nullptr; s.final_by_chain = 0;
+      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; lin::set_scale(s, a.scale); s.scale_e = 1.f; s.st_y = 1; s.st_w = a.dv;
+      m.x = mv; m.y = mo; m.w = mq; m.e = mk;
+      if ((r = rows_of(t.p[1], a.d_k, 1))) return r;
+      if (grad) s.inter = f32(l.inter_b);
     }
     {  // dv, and the gradient of the initial state
-      lin::Args s = rev;
-      lin::Maps m{};
+      lin::Args& s = t.p[2].a;
+      lin::Maps& m = t.p[2].m;
+      s = rev;
       s.x_div = rep; lin::set_scale(s, a.scale); s.scale_e = 1.f;
       s.state_out = a.d_initial_state;
       m.x = mk; m.y = mq; m.w = mo;
       s.o = a.d_v; s.o_stride_h = a.dv; s.o_stride_t = (int64_t)a.Hv * a.dv; s.o_stride_b = s.o_stride_t * a.T;
       m.o_ok = lin::result_map(&m.o, a.d_v, a.dv, a.Hv, a.B, a.T, s.o_stride_b, s.o_stride_t, s.o_stride_h);
-      r = s.state_out != nullptr && !s.final_by_chain ? lin::launch_scan<DK, DV, true, lin::OUT3>(s, m, stream) : lin::launch_scan<DK, DV, true, lin::OUT2>(s, m, stream);
-      if (r) return r;
     }
-    {  // dq
-      lin::Args s = fwd;
-      lin::Maps m{};
-      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; lin::set_scale(s, a.scale); s.scale_e = a.scale; s.st_y = 1; s.st_w = a.dv;
-      m.x = mo; m.y = mv; m.w = mk; m.e = mq;
-      if ((r = rows_of(s, m, a.d_q))) return r;
-      if (grad) {
-        s.inter = f32(l.inter_a);
-        if (a.d_final_state != nullptr) s.state_out = f32(l.final);
-      }
-      r = grad ? lin::launch_scan<DV, DK, false, lin::GRAD>(s, m, stream) : lin::launch_scan<DV, DK, false, lin::OUT2>(s, m, stream);
-      if (r || (r = sum_heads(a.d_q))) return r;
-    }
-    {  // dk
-      lin::Args s = rev;
-      lin::Maps m{};
-      s.state_out = nullptr;
-      s.x_div = s.y_div = 1; s.w_div = s.e_div = rep; lin::set_scale(s, a.scale); s.scale_e = 1.f; s.st_y = 1; s.st_w = a.dv;
-      m.x = mv; m.y = mo; m.w = mq; m.e = mk;
-      if ((r = rows_of(s, m, a.d_k))) return r;
-      if (grad) s.inter = f32(l.inter_b);
-      r = grad ? lin::launch_scan<DV, DK, true, lin::GRAD>(s, m, stream) : lin::launch_scan<DV, DK, true, lin::OUT2>(s, m, stream);
-      if (r || (r = sum_heads(a.d_k))) return r;
+    const bool exact = t.p[2].a.state_out != nullptr && !t.p[2].a.final_by_chain;
+    if (grad) r = exact ? lin::launch_grads<DK, DV, lin::GRAD, lin::OUT3>(t, stream) : lin::launch_grads<DK, DV, lin::GRAD, lin::OUT2>(t, stream);
+    else r = exact ? lin::launch_grads<DK, DV, lin::OUT2, lin::OUT3>(t, stream) : lin::launch_grads<DK, DV, lin::OUT2, lin::OUT2>(t, stream);
+    if (r) return r;
+    if (rep > 1) {
+      const int64_t pieces = (int64_t)a.B * a.T * a.Hk * (a.dk / 8), ctas = (pieces + 255) / 256;
+      AVE_CUDA_TRY(launch_after(lin::sum_heads_kernel, dim3((unsigned)(ctas < 148 * 8 ? ctas : 148 * 8), 2), 256, 0, stream, (const float*)f32(l.part), part_floats,
+                                reinterpret_cast<__nv_bfloat16*>(a.d_q), reinterpret_cast<__nv_bfloat16*>(a.d_k), pieces, a.dk / 8, a.Hk, rep));
     }
     if (grad) {
       lin::Args s = base;
@@ -445,7 +488,7 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
     if (a.d_final_state != nullptr) { q.sT = f32(l.final); q.dsT = a.d_final_state; }
     if (by_token) q.dg = a.d_g; else q.sums = f32(l.sums);
     const int64_t grid = l.plan.slots * a.Hv;
-    AVE_CUDA_TRY(launch_after(a.dk == 128 ? lin::gate_grad_kernel<4> : lin::gate_grad_kernel<2>, (unsigned)grid, 256, 0, stream, base, q));  // (scans give a sum for each 32 of dk)
+    AVE_CUDA_TRY(launch_after(a.dk == 128 ? lin::gate_grad_kernel<4> : lin::gate_grad_kernel<2>, (unsigned)grid, lin::GATE_THREADS, 0, stream, base, q));  // (scans give a sum for each 32 of dk)
     if (!by_token) AVE_CUDA_TRY(launch_after(lin::head_gate_grad_kernel, (unsigned)a.Hv, 256, 0, stream, base, (const float*)q.sums, a.d_g));
   }
   if (a.cu_seqlens != nullptr)

@@ -31,11 +31,13 @@ int launch_linear_prefill(const AveLinearArgs& a, cudaStream_t stream) {
   m.o_ok = lin::result_map(&m.o, a.o, a.dv, a.Hv, a.B, a.T, a.o_stride_b, a.o_stride_t, a.o_stride_h);
   return lin::by_dims(a.dk, a.dv, [&](auto dk, auto dv) {
     if (s.plan.cut) {
-      int r = lin::launch_scan<dk, dv, false, lin::STATE>(s, m, stream);
-      if (r == AVE_GDN_OK) r = lin::launch_chain<dk, dv, false>(s, stream);
+      const int r = lin::launch_scan<dk, dv, lin::STATE>(s, m, stream);
       if (r != AVE_GDN_OK) return r;
+      const int64_t grid = lin::chain_grid<dk, dv>(s);
+      if (grid > 0x7fffffff) return (int)AVE_GDN_UNSUPPORTED;
+      AVE_CUDA_TRY(launch_after(lin::chain_kernel<dk, dv>, (unsigned)grid, 256, 0, stream, s));
     }
-    return s.state_out != nullptr && !s.final_by_chain ? lin::launch_scan<dk, dv, false, lin::OUT3>(s, m, stream) : lin::launch_scan<dk, dv, false, lin::OUT2>(s, m, stream);
+    return s.state_out != nullptr && !s.final_by_chain ? lin::launch_scan<dk, dv, lin::OUT3>(s, m, stream) : lin::launch_scan<dk, dv, lin::OUT2>(s, m, stream);
   });
 }
 

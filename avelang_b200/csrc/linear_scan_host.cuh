@@ -14,14 +14,15 @@ constexpr int MAX_DEVICES = 64;
 // One CTA walks a segment of one (sequence, value head).  Whole sequences need one pass; segments need their own increments first (a pass that reads Y and W alone) and the chain
 // of them, so they pay where there are too few sequences and heads for the SMs, or where one sequence is so long that the others wait for it.  The lengths of packed sequences are
 // not known here: the longest is taken to be four times the mean.  Unit: a chunk of the scan, 2.2 us on every SM; a chunk of the first pass takes 0.45 of that, a CTA's
-// beginning and end 3 and 2.5, the chain and its launches 2.5 (2 x 4096 tokens x 32 heads, forward: whole 220 us, segments of 2048 tokens 127, of 256 221).
+// beginning and end 3 and 2.5, the chain and its launches 2.5 (8192 tokens x 32 heads, forward: whole 304 us, segments of 4096 tokens
+// 212, of 2048 123; 24 prompts of 65536 tokens x 32 heads: whole 568, segments of 5504 908.)
 inline Plan plan_of(int B, int64_t T, int n_seqs, bool packed, int heads) {
   constexpr double SMS = 148;
   const double chunks = (double)((T * B + C - 1) / C);
   const double longest = packed ? (n_seqs > 1 ? fmin((double)T, 4.0 * T / n_seqs) : (double)T) / C : (double)((T + C - 1) / C);
   auto waves = [&](double units) { return packed ? units / SMS + 0.5 : (double)(int64_t)(units / SMS + 0.999999); };
   const double seqs = packed ? (double)n_seqs : (double)B;
-  double best = packed ? fmax((chunks + 3.0 * seqs) * heads / SMS, longest + 3.0) + 0.25 * longest : waves(seqs * heads) * (longest + 3.0);
+  double best = packed ? fmax((chunks + 3.0 * seqs) * heads / SMS, longest + 3.0) + (n_seqs > MOST_IN_ORDER ? 0.25 * longest : 0.0) : waves(seqs * heads) * (longest + 3.0);
   int64_t len = 0;
   for (int parts = 2; parts <= 256; ++parts) {
     const int64_t each = (int64_t)((longest + parts - 1) / parts);
@@ -84,10 +85,8 @@ int allow_smem(K* kernel, int smem) {
 }
 
 // The register split of the roles counts on the registers that the kernel is launched with.
-template <int DK, int DV, bool kRev, Mode kMode>
-int launch_scan(const Args& a, const Maps& maps, cudaStream_t stream) {
-  auto* kernel = scan_kernel<DK, DV, kRev, kMode>;
-  constexpr int smem = Cfg<kMode>::SMEM;
+template <auto* kernel>
+int scan_ready(int smem) {
   static std::atomic<bool> ready[MAX_DEVICES];
   int dev = 0;
   AVE_CUDA_TRY(cudaGetDevice(&dev));
@@ -99,18 +98,21 @@ int launch_scan(const Args& a, const Maps& maps, cudaStream_t stream) {
     AVE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ready[dev].store(true, std::memory_order_release);
   }
-  const int64_t grid = a.plan.slots * a.Hv;
-  if (grid > 0x7fffffff) return AVE_GDN_UNSUPPORTED;
-  AVE_CUDA_TRY(launch_after(kernel, (unsigned)grid, THREADS, smem, stream, a, maps));
   return AVE_GDN_OK;
 }
-template <int DK, int DV, bool kRev>
-int launch_chain(const Args& a, cudaStream_t stream) {
-  const int64_t grid = (int64_t)a.n_seqs * a.Hv * (DK * DV / 1024);
-  if (grid > 0x7fffffff) return AVE_GDN_UNSUPPORTED;
-  AVE_CUDA_TRY(launch_after(chain_kernel<DK, DV, kRev>, (unsigned)grid, 256, 0, stream, a));
+inline int64_t scan_grid(const Args& a) { return a.plan.slots * a.Hv; }
+template <int DK, int DV, Mode kMode>
+int launch_scan(const Args& a, const Maps& maps, cudaStream_t stream) {
+  constexpr auto* kernel = &scan_kernel<DK, DV, false, kMode>;
+  constexpr int smem = Cfg<kMode>::SMEM;
+  const int rc = scan_ready<kernel>(smem);
+  if (rc != AVE_GDN_OK) return rc;
+  if (scan_grid(a) > 0x7fffffff) return AVE_GDN_UNSUPPORTED;
+  AVE_CUDA_TRY(launch_after(kernel, (unsigned)scan_grid(a), THREADS, smem, stream, a, maps));
   return AVE_GDN_OK;
 }
+template <int DK, int DV>
+int64_t chain_grid(const Args& a) { return (int64_t)a.n_seqs * a.Hv * (DK * DV / 1024); }
 
 template <class F>
 int by_dims(int dk, int dv, F f) {

@@ -187,3 +187,16 @@ def test_streams_and_captured_calls(built_lib):
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, r) for g, w in zip(outs, want) for p, r in zip(g, w))
+
+
+@pytest.mark.parametrize("n", [2, 256, 257])
+def test_many_sequences_of_unequal_length(built_lib, n):
+    """More work than SMs: up to 256 sequences run in the order of their lengths, ties in the batch's."""
+    from avelang_b200 import gdn, linear_attention as L
+    lens = torch.randint(0, 40, (n,), generator=torch.Generator().manual_seed(n)).tolist()
+    lens[n // 2] = 200
+    cu = torch.tensor([sum(lens[:i]) for i in range(n + 1)], dtype=torch.int32)
+    q, k, v, g, s0 = make(1, int(cu[-1]), 1, 2, 64, 64, "token", 13, n, 0.1)
+    o, s = L.chunk_linear_attention(*cuda(q, k, v, g, None, s0), True, cu.cuda())
+    assert gdn.read_status() == 0
+    check(o, s, q, k, v, g, 64 ** -0.5, s0, cu)
