@@ -54,8 +54,8 @@ def linear_attention_backward(q, k, v, g, d_o, scale=None, initial_state=None, d
 
 class LinearAttentionFunction(torch.autograd.Function):
     """``o, final_state = LinearAttentionFunction.apply(q, k, v, g, scale, initial_state, cu_seqlens)``: the chunked forward pass with
-    the chunked backward pass attached (g, scale, initial_state and cu_seqlens may be None).  A step with its backward pass can be captured
-    into a CUDA graph once the results of eager steps on the same leaves are gone."""
+    the chunked backward pass attached (g, scale, initial_state and cu_seqlens may be None).  It can be differentiated once.  A step with
+    its backward pass can be captured into a CUDA graph once the results of eager steps on the same leaves are gone."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, scale, initial_state, cu_seqlens):
@@ -66,6 +66,7 @@ class LinearAttentionFunction(torch.autograd.Function):
         return o, final
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_final):
         q, k, v, g, s0, cu = ctx.saved_tensors
         d_o = torch.zeros_like(v) if d_o is None else d_o.to(torch.bfloat16).contiguous()

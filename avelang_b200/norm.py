@@ -32,8 +32,8 @@ def layer_norm_backward(d_y, x, mean, rstd, weight=None):
 
 
 class LayerNormFunction(torch.autograd.Function):
-    """``y = LayerNormFunction.apply(x, weight, bias, eps)``: ``layer_norm`` with its backward pass attached (weight and bias may be None).  A step with
-    its backward pass can be captured into a CUDA graph once the results of eager steps on the same leaves are gone."""
+    """``y = LayerNormFunction.apply(x, weight, bias, eps)``: ``layer_norm`` with its backward pass attached (weight and bias may be None).
+    It can be differentiated once.  A step with its backward pass can be captured into a CUDA graph once the results of eager steps on the same leaves are gone."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -43,6 +43,7 @@ class LayerNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, d_y):
         x, mean, rstd, weight = ctx.saved_tensors
         dx, dw, db = layer_norm_backward(d_y, x, mean, rstd, weight)

@@ -161,3 +161,27 @@ def test_two_streams_at_once(built_lib):
     for i in range(2):
         for run in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(run, alone[i]))
+
+
+def test_gradients_have_no_gradients(built_lib):
+    from avelang_b200 import linear_attention as L, norm
+    q, k, v, g, _ = [t.cuda().requires_grad_() if t is not None else None for t in P.make(1, 70, 1, 1, 64, 64, "token", 11)]
+    o, _ = L.LinearAttentionFunction.apply(q, k, v, g, None, None, None)
+    first = torch.autograd.grad(o.float().square().sum(), (q, k, v, g), create_graph=True)
+    for t in first:
+        with pytest.raises(RuntimeError, match="twice"):
+            t.float().sum().backward(retain_graph=True)
+    x = torch.randn(3, 64, device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(norm.LayerNormFunction.apply(x, None, None, 1e-5).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        dx.sum().backward()
+
+
+def test_refusals_of_the_differentiable_call(built_lib):
+    from avelang_b200 import linear_attention as L
+    q, k, v, g, s0 = P.cuda(*P.make(1, 70, 1, 1, 64, 64, "token", 12, 1))
+    f = L.LinearAttentionFunction.apply
+    for match, args in (("q must have dtype", (q.float(), k, v, g)), ("k must have shape", (q, k[:, :50], v, g)), ("g must have dtype", (q, k, v, g.double())),
+                        ("one state per sequence", (q, k, v, g, None, s0.expand(2, -1, -1, -1).contiguous()))):
+        with pytest.raises(ValueError, match=match):
+            f(*args, *[None] * (7 - len(args)))
