@@ -871,21 +871,25 @@ int by_element(int64_t n, F f) {
   }
   return AVE_GDN_UNSUPPORTED;
 }
+// Few rows: a row a CTA, two at most one behind the other.  (bf16 rows of 2048, forward and backward us: 37 rows 2.2 and 4.9, with a row a warp or two 4.1 and 6.0; 296 rows
+// 3.1 and 6.3, 4.3 and 7.1; 592 rows 4.6 and 7.7, 4.3 and 7.6; 8192 rows 48 and 46, 14 and 25.)
+bool few_rows(int64_t rows) { return rows <= 2 * 148; }
 bool on16(int64_t stride, int size) { return (stride * size) % 16 == 0; }
 
 template <class T>
 int forward_t(const AveLayerNormArgs& a, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   const bool wide = a.n % V == 0 && aligned16(a.x) && aligned16(a.y) && on16(a.x_stride, sizeof(T)) && on16(a.y_stride, sizeof(T));
-  // The ring from 513 columns on, 64 a thread, however few the rows (bf16, 64 rows of 2048: 8.2 us either way; 16384 rows of 512: 20.4 us, 14.4 with rows in
+  // The ring from 513 columns on, 64 a thread or, with few rows, fewer (bf16, 16384 rows of 512: 20.4 us, 14.4 with rows in
   // registers; of 1024: 22.5 and 36.9; of 8192: 108 and 137)
   if (wide) {
     constexpr int P = 64 / V;
     if (a.n <= 512) return short_rows<V>(a.n, [&](auto f) { return run_forward<T, V, f.tpr, f.p, f.u>(a, stream); });
-    if (a.n <= 1024) return run_forward_ring<T, P / 2, 1>(a, stream);
-    if (a.n <= 2048) return run_forward_ring<T, P, 1>(a, stream);
-    if (a.n <= 4096) return run_forward_ring<T, P, 2>(a, stream);
-    if (a.n <= 8192) return run_forward_ring<T, P, 4>(a, stream);
+    const bool few = few_rows(a.rows);
+    if (a.n <= 1024) return few ? run_forward_ring<T, P / 8, 8>(a, stream) : run_forward_ring<T, P / 2, 1>(a, stream);
+    if (a.n <= 2048) return few ? run_forward_ring<T, P / 8, 8>(a, stream) : run_forward_ring<T, P, 1>(a, stream);
+    if (a.n <= 4096) return few ? run_forward_ring<T, P / 4, 8>(a, stream) : run_forward_ring<T, P, 2>(a, stream);
+    if (a.n <= 8192) return few ? run_forward_ring<T, P / 2, 8>(a, stream) : run_forward_ring<T, P, 4>(a, stream);
     if (a.n <= 16384) return run_forward_ring<T, P, 8>(a, stream);
     return run_forward<T, V, 1024, (MAX_N / V + 1023) / 1024, 1>(a, stream);
   }
@@ -900,10 +904,11 @@ int backward_t(const AveLayerNormBwdArgs& a, cudaStream_t stream) {
     // The ring from 257 columns on, 32 a thread (bf16, 16384 rows of 256: 20.5 us, 19.5 with rows in registers; of 512: 24.6 and 27.5; of 8192: 145 and 347)
     constexpr int P = 32 / V;
     if (a.n <= 256) return short_rows<V>(a.n, [&](auto f) { return run_backward<T, V, f.tpr, f.p, f.u>(a, stream); });
-    if (a.n <= 512) return run_backward_ring<T, P / 2, 1>(a, stream);
-    if (a.n <= 1024) return run_backward_ring<T, P, 1>(a, stream);
-    if (a.n <= 2048) return run_backward_ring<T, P, 2>(a, stream);
-    if (a.n <= 4096) return run_backward_ring<T, P, 4>(a, stream);
+    const bool few = few_rows(a.rows);
+    if (a.n <= 512) return few ? run_backward_ring<T, P / 4, 8>(a, stream) : run_backward_ring<T, P / 2, 1>(a, stream);
+    if (a.n <= 1024) return few ? run_backward_ring<T, P / 4, 8>(a, stream) : run_backward_ring<T, P, 1>(a, stream);
+    if (a.n <= 2048) return few ? run_backward_ring<T, P / 4, 8>(a, stream) : run_backward_ring<T, P, 2>(a, stream);
+    if (a.n <= 4096) return few ? run_backward_ring<T, P / 2, 8>(a, stream) : run_backward_ring<T, P, 4>(a, stream);
     if (a.n <= 8192) return run_backward_ring<T, P, 8>(a, stream);
     if (a.n <= 16384) return run_backward_long<T, V, 16 / V>(a, stream);
     if (a.n <= 24576) return run_backward_long<T, V, 24 / V>(a, stream);
