@@ -497,7 +497,8 @@ __device__ __forceinline__ void scan(const Args& a, const Maps& maps) {
     const bool mine = d < DV;
     float2 S[HC / 2];
     {
-      const float* src = kState ? nullptr : seg.count > 1 ? a.seg_state + seg_tile : a.state_in != nullptr ? a.state_in + state_tile : nullptr;
+      // (with the chain, which may have put the final state in the place of the initial one, every segment's)
+      const float* src = kState ? nullptr : seg.count > 1 || a.final_by_chain ? a.seg_state + seg_tile : a.state_in != nullptr ? a.state_in + state_tile : nullptr;
       asm volatile("" : "+l"(src));
 #pragma unroll
       for (int i = 0; i < HC / 2; ++i) {
@@ -883,7 +884,7 @@ __device__ __forceinline__ void chain(const Args& a) {
     for (int u = 0; u < 4; ++u)
       if (i0 + u < count) {
         const int64_t sl = s0 + (kRev ? count - 1 - i0 - u : i0 + u);
-        if (count > 1) *reinterpret_cast<float4*>(base + sl * step) = cur;
+        *reinterpret_cast<float4*>(base + sl * step) = cur;
         if (i0 + u < own_until) {
           cur.x = fmaf(decay[u], cur.x, own[u].x); cur.y = fmaf(decay[u], cur.y, own[u].y);
           cur.z = fmaf(decay[u], cur.z, own[u].z); cur.w = fmaf(decay[u], cur.w, own[u].w);

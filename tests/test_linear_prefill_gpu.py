@@ -200,3 +200,20 @@ def test_many_sequences_of_unequal_length(built_lib, n):
     o, s = L.chunk_linear_attention(*cuda(q, k, v, g, None, s0), True, cu.cuda())
     assert gdn.read_status() == 0
     check(o, s, q, k, v, g, 64 ** -0.5, s0, cu)
+
+
+def test_pool_in_place_where_some_sequences_are_cut_into_segments(built_lib):
+    """A sequence of one segment beside longer ones: its state is read before the final one takes its place."""
+    from avelang_b200 import gdn, linear_attention as L
+    lens = [1500, 3, 0, 700, 64]
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32)
+    q, k, v, g, pool = make(1, sum(lens), 1, 2, 128, 128, "token", 14, 7, 0.05)
+    idx = torch.tensor([4, 0, 6, 2, 5], dtype=torch.int32)
+    args, pd = cuda(q, k, v, g), pool.cuda()
+    apart = L.chunk_linear_attention(*args, None, pd, True, cu.cuda(), state_indices=idx.cuda(), inplace_state=False)
+    assert torch.equal(pd.cpu(), pool)
+    o, s = L.chunk_linear_attention(*args, None, pd, True, cu.cuda(), state_indices=idx.cuda())
+    assert gdn.read_status() == 0 and s.data_ptr() == pd.data_ptr()
+    assert torch.equal(o, apart[0]) and torch.equal(s, apart[1])
+    check(o, s[idx.long().cuda()], q, k, v, g, 128 ** -0.5, pool[idx.long()], cu)
+    assert torch.equal(s.cpu()[[1, 3]], pool[[1, 3]])
