@@ -347,7 +347,7 @@ typedef struct AveLinearArgs {
   const int32_t* cu_seqlens;    /* optional int32 [n_seqs+1]; requires B == 1 */
   const int32_t* state_indices; /* optional int32 [n_seqs], as in AveGdnArgs */
   uint32_t* status;           /* optional device status word */
-  void* workspace;            /* prefill only: ave_linear_prefill_workspace_bytes(), 16-byte aligned */
+  void* workspace;            /* prefill only: ave_linear_prefill_workspace_bytes() of this very call (a shorter one may need more), 16-byte aligned */
   uint64_t workspace_bytes;
   int32_t B, T, Hk, Hv, dk, dv;
   int32_t n_seqs;             /* B when cu_seqlens is null */
