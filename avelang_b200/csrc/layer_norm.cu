@@ -6,7 +6,7 @@
 // Both are bound by HBM: the forward pass reads x and writes y, the backward pass reads x and dy and writes dx.  A row belongs to a group of threads, each of which keeps the same
 // columns for every row it meets: the weights are read once a CTA, and the sums of the weight's gradient are registers too.  A CTA's sums go to scratch and a second kernel adds them
 // in a fixed order.  Three forms by the row's length, figures for bf16 rows with fp32 weights, copy rate 6549 GB/s: rings of rows in shared memory for aligned rows of middle length
-// (131072 x 2048: forward 179 us, 5.98 TB/s, backward 267 us, 6.03 TB/s; 32768 x 8192: 203 and 262 us); rows in registers, U of them in flight a group, for short ones and for those
+// (131072 x 2048: forward 179 to 187 us, 5.7 to 6.0 TB/s, backward 267 to 272 us, 5.9 to 6.0 TB/s; 32768 x 8192: 203 and 262 us); rows in registers, U of them in flight a group, for short ones and for those
 // that do not lie on 16 bytes (131072 x 64: 8.7 and 12.9 us; 30000 x 2047: 89 and 103 us, bound by the loads of single elements); and CTAs of 1024 threads for long ones
 // (16384 x 16384 backward 567 us).
 #include <cuda_fp16.h>
