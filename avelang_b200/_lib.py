@@ -105,14 +105,14 @@ class LinearBwdArgs(ctypes.Structure):
 class LayerNormArgs(ctypes.Structure):
     _fields_ = ([("struct_size", U32), ("flags", U32)] + [(n, P) for n in ("x", "weight", "bias", "y", "mean", "rstd")]
                 + [(n, I64) for n in ("rows", "n", "x_stride", "y_stride")]
-                + [("x_dtype", I32), ("w_dtype", I32), ("eps", F32), ("reserved0", F32)])
+                + [("x_dtype", I32), ("w_dtype", I32), ("eps", F32), ("reserved0", F32), ("status", P)])
 
 
 class LayerNormBwdArgs(ctypes.Structure):
     _fields_ = ([("struct_size", U32), ("flags", U32)]
                 + [(n, P) for n in ("d_y", "x", "mean", "rstd", "weight", "d_x", "d_weight", "d_bias", "workspace")]
                 + [("workspace_bytes", U64)] + [(n, I64) for n in ("rows", "n", "dy_stride", "x_stride", "dx_stride")]
-                + [("x_dtype", I32), ("w_dtype", I32)])
+                + [("x_dtype", I32), ("w_dtype", I32), ("status", P)])
 
 
 # every symbol include/ave_gdn.h declares: name -> (restype, argtypes)

@@ -1,5 +1,8 @@
 // extern "C" boundary of linear attention with a decay for each head and of layer norm: argument validation and dispatch.  No device
 // allocation, no synchronisation, nothing thrown across the boundary.
+#include <stddef.h>
+#include <string.h>
+
 #include "common.cuh"
 
 namespace ave {
@@ -59,6 +62,15 @@ int validate_linear_bwd(const AveLinearBwdArgs* a) {
 }
 
 bool dtype_ok(int x, int w) { return x >= AVE_DTYPE_BF16 && x <= AVE_DTYPE_FP32 && (w == x || w == AVE_DTYPE_FP32); }
+// Arguments whose status word, the last field, may be missing
+template <class Args>
+const Args* with_status(const Args* a, Args& own) {
+  if (a == nullptr || a->struct_size == sizeof(Args)) return a;
+  if (a->struct_size != offsetof(Args, status)) return nullptr;
+  own = Args{};
+  memcpy(&own, a, offsetof(Args, status));
+  return &own;
+}
 bool on_elem(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == AVE_DTYPE_FP32 ? 3u : 1u)) == 0; }
 
 }  // namespace
@@ -105,8 +117,10 @@ int ave_linear_backward(const AveLinearBwdArgs* a, void* stream) {
   return launch_linear_backward(*a, reinterpret_cast<cudaStream_t>(stream));
 }
 
-int ave_layer_norm(const AveLayerNormArgs* a, void* stream) {
-  if (a == nullptr || a->struct_size != sizeof(AveLayerNormArgs) || a->rows < 0 || a->n <= 0 || !dtype_ok(a->x_dtype, a->w_dtype)) return AVE_GDN_INVALID_ARGUMENT;
+int ave_layer_norm(const AveLayerNormArgs* args, void* stream) {
+  AveLayerNormArgs own;
+  const AveLayerNormArgs* a = with_status(args, own);
+  if (a == nullptr || a->rows < 0 || a->n <= 0 || !dtype_ok(a->x_dtype, a->w_dtype)) return AVE_GDN_INVALID_ARGUMENT;
   if (a->n > layer_norm_max_n()) return AVE_GDN_UNSUPPORTED;
   if (a->rows == 0) return AVE_GDN_OK;
   if (!a->x || !a->y || (a->bias && !a->weight)) return AVE_GDN_INVALID_ARGUMENT;
@@ -114,13 +128,17 @@ int ave_layer_norm(const AveLayerNormArgs* a, void* stream) {
   return launch_layer_norm(*a, reinterpret_cast<cudaStream_t>(stream));
 }
 
-size_t ave_layer_norm_backward_workspace_bytes(const AveLayerNormBwdArgs* a) {
-  if (a == nullptr || a->struct_size != sizeof(AveLayerNormBwdArgs) || a->rows <= 0 || a->n <= 0 || a->n > layer_norm_max_n()) return 0;
+size_t ave_layer_norm_backward_workspace_bytes(const AveLayerNormBwdArgs* args) {
+  AveLayerNormBwdArgs own;
+  const AveLayerNormBwdArgs* a = with_status(args, own);
+  if (a == nullptr || a->rows <= 0 || a->n <= 0 || a->n > layer_norm_max_n()) return 0;
   return layer_norm_backward_workspace_bytes(*a);
 }
 
-int ave_layer_norm_backward(const AveLayerNormBwdArgs* a, void* stream) {
-  if (a == nullptr || a->struct_size != sizeof(AveLayerNormBwdArgs) || a->rows < 0 || a->n <= 0 || !dtype_ok(a->x_dtype, a->w_dtype)) return AVE_GDN_INVALID_ARGUMENT;
+int ave_layer_norm_backward(const AveLayerNormBwdArgs* args, void* stream) {
+  AveLayerNormBwdArgs own;
+  const AveLayerNormBwdArgs* a = with_status(args, own);
+  if (a == nullptr || a->rows < 0 || a->n <= 0 || !dtype_ok(a->x_dtype, a->w_dtype)) return AVE_GDN_INVALID_ARGUMENT;
   if (a->n > layer_norm_max_n()) return AVE_GDN_UNSUPPORTED;
   if (a->rows == 0) return AVE_GDN_OK;  // (sums over no rows: the caller's)
   if (!a->d_y || !a->x || !a->mean || !a->rstd || !a->d_x) return AVE_GDN_INVALID_ARGUMENT;

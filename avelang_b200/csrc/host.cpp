@@ -756,6 +756,7 @@ void op_layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bi
   a.rows = x.size(0); a.n = x.size(1); a.x_stride = x.stride(0); a.y_stride = out.stride(0);
   a.x_dtype = dtype_code(x, "x"); a.w_dtype = some(weight) != nullptr ? dtype_code(*some(weight), "weight") : a.x_dtype;
   a.eps = (float)eps;
+  a.status = reinterpret_cast<uint32_t*>(status_word(x.device()).data_ptr());
   Launch launch(x);
   check(launch([&] { return api.layer_norm(&a, launch.stream); }), "layer_norm");
 }
@@ -769,6 +770,7 @@ void op_layer_norm_backward(const Tensor& d_y, const Tensor& x, const Tensor& me
   a.d_x = const_cast<void*>(ptr(&d_x)); a.d_weight = const_cast<void*>(ptr(some(d_weight))); a.d_bias = const_cast<void*>(ptr(some(d_bias)));
   a.rows = x.size(0); a.n = x.size(1); a.dy_stride = d_y.stride(0); a.x_stride = x.stride(0); a.dx_stride = d_x.stride(0);
   a.x_dtype = dtype_code(x, "x"); a.w_dtype = some(weight) != nullptr ? dtype_code(*some(weight), "weight") : a.x_dtype;
+  a.status = reinterpret_cast<uint32_t*>(status_word(x.device()).data_ptr());
   Launch launch(x);
   const Scratch ws(x, launch.stream, api.layer_norm_backward_workspace_bytes(&a));
   a.workspace = ws.data(); a.workspace_bytes = ws.size();

@@ -289,6 +289,7 @@ struct Ring {
   bool leader, dead = false;
   int issued = 0, waited = 0, slot = 0;
   uint32_t phase = 0;
+  __device__ __forceinline__ float own(float sum) const { return dead ? __int_as_float(0x7fffffff) : sum; }  // what the thread adds to its row's sum
   __device__ __forceinline__ void issue(const T* a, const T* b) {  // into the slot that is free next
     if (leader && !dead) {
       const int s = issued % depth;
@@ -299,10 +300,12 @@ struct Ring {
     }
     ++issued;
   }
-  // A wait that expires leaves the thread `dead`: its rows become NaN, it issues nothing more, and the copies on their way are waited for once more, with a limit.
-  __device__ __forceinline__ const uint8_t* wait() {
+  // A wait that expires leaves the thread `dead` and is noted in the status word: from then on the thread adds NaN to its rows' sums, which makes them NaN for the whole group, it issues
+  // nothing more, and the copies on their way are waited for once more, with a limit.
+  __device__ __forceinline__ const uint8_t* wait(uint32_t* status) {
     if (!dead && !tc::mbar_wait(bars + slot, phase, flag)) {
       dead = true;
+      if (status != nullptr) atomicOr(status, AVE_GDN_DEV_WAIT_EXPIRED);
       if (leader)
         for (int i = 0; i < issued - waited; ++i) tc::drain(bars + (slot + i) % depth, slot + i < depth ? phase : phase ^ 1u);
     }
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(256, 1) layer_norm_ring_kernel(const AveLayerN
   const float inv_n = 1.f / (float)a.n;
   const int n = (int)a.n;
   for (int64_t r = first; r < a.rows; r += step) {
-    const T* row = reinterpret_cast<const T*>(ring.wait());
+    const T* row = reinterpret_cast<const T*>(ring.wait(a.status));
     Pairs<N> f;
     f.fill(0.f);
 #pragma unroll
@@ -370,12 +373,12 @@ __global__ void __launch_bounds__(256, 1) layer_norm_ring_kernel(const AveLayerN
     float2 t = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < H; ++i) t = __fadd2_rn(t, f.v[i]);
-    float s[1] = {t.x + t.y};
+    float s[1] = {ring.own(t.x + t.y)};
     ring_sum<G, 1>(s, sums[0][0]);
     __syncwarp();  // the whole group has read the row
     if (ahead < a.rows) { ring.issue(x + ahead * a.x_stride, nullptr); ahead += step; }
     ring.next();
-    const float mean = ring.dead ? __int_as_float(0x7fffffff) : s[0] * inv_n;
+    const float mean = s[0] * inv_n;
     t = make_float2(0.f, 0.f);
 #pragma unroll
     for (int p = 0; p < P; ++p)  // the squares are of differences from the mean: the sum of x^2 would lose what a large mean hides
@@ -554,11 +557,10 @@ __global__ void __launch_bounds__(256, 1) layer_norm_backward_ring_kernel(const 
   float mean_next = first < a.rows ? a.mean[first] : 0.f, rstd_next = first < a.rows ? a.rstd[first] : 0.f;
   int turn = 0;
   for (int64_t r = first; r < a.rows; r += step, turn ^= 1) {
-    const float mean_r = mean_next, rstd = rstd_next;
+    const float mean = mean_next, rstd = rstd_next;
     if (r + step < a.rows) { mean_next = a.mean[r + step]; rstd_next = a.rstd[r + step]; }
-    const uint8_t* slot = ring.wait();
+    const uint8_t* slot = ring.wait(a.status);
     const T *row = reinterpret_cast<const T*>(slot), *grow = reinterpret_cast<const T*>(slot + ring.slot_bytes / 2);
-    const float mean = ring.dead ? __int_as_float(0x7fffffff) : mean_r;
     Pairs<N> xh, d;
     xh.fill(0.f); d.fill(0.f);
     float2 s0 = make_float2(0.f, 0.f), s1 = s0;
@@ -580,7 +582,7 @@ __global__ void __launch_bounds__(256, 1) layer_norm_backward_ring_kernel(const 
         d.v[i] = gw;
       }
     }
-    float s[2] = {s0.x + s0.y, s1.x + s1.y};
+    float s[2] = {ring.own(s0.x + s0.y), ring.own(s1.x + s1.y)};
     ring_sum<G, 2>(s, sums[turn][0]);
     __syncwarp();  // the whole group has read the rows
     if (ahead < a.rows) { ring.issue(x + ahead * a.x_stride, dy + ahead * a.dy_stride); ahead += step; }
@@ -597,6 +599,7 @@ __global__ void __launch_bounds__(256, 1) layer_norm_backward_ring_kernel(const 
     }
   }
   if (partial == nullptr) return;
+  if (ring.dead) { dw.fill(__int_as_float(0x7fffffff)); db.fill(__int_as_float(0x7fffffff)); }
   __syncthreads();  // all rows are done: the ring's memory takes the groups' sums, [GROUPS][2][n]
   float* cols = reinterpret_cast<float*>(ring_mem);
 #pragma unroll

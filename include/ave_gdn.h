@@ -403,7 +403,8 @@ typedef struct AveLinearBwdArgs {
 int ave_linear_backward(const AveLinearBwdArgs* args, void* stream);
 size_t ave_linear_backward_workspace_bytes(const AveLinearBwdArgs* args);
 
-/* y = (x - mean) * rstd * weight + bias over rows of n elements, 1 <= n <= 28672, rstd = 1 / sqrt(var + eps). */
+/* y = (x - mean) * rstd * weight + bias over rows of n elements, 1 <= n <= 28672, rstd = 1 / sqrt(var + eps).
+ * Rows that a bounded wait has given up on are NaN in all their results, and AVE_GDN_DEV_WAIT_EXPIRED is set in the status word. */
 #define AVE_DTYPE_BF16 0
 #define AVE_DTYPE_FP16 1
 #define AVE_DTYPE_FP32 2
@@ -420,6 +421,7 @@ typedef struct AveLayerNormArgs {
   int32_t x_dtype, w_dtype; /* w_dtype: x_dtype or AVE_DTYPE_FP32 */
   float eps;
   float reserved0;
+  uint32_t* status;         /* optional device status word; a struct_size that ends in front of it is accepted too */
 } AveLayerNormArgs;
 int ave_layer_norm(const AveLayerNormArgs* args, void* stream);
 
@@ -439,6 +441,7 @@ typedef struct AveLayerNormBwdArgs {
   uint64_t workspace_bytes;
   int64_t rows, n, dy_stride, x_stride, dx_stride;
   int32_t x_dtype, w_dtype;
+  uint32_t* status;       /* as in AveLayerNormArgs; with it the columns of d_weight and d_bias that the lost rows reach are NaN */
 } AveLayerNormBwdArgs;
 int ave_layer_norm_backward(const AveLayerNormBwdArgs* args, void* stream);
 size_t ave_layer_norm_backward_workspace_bytes(const AveLayerNormBwdArgs* args);
