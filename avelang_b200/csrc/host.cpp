@@ -694,9 +694,10 @@ AveLinearArgs fill_linear(const Tensor& q, const Tensor& k, const Tensor& v, con
 }
 
 void op_linear_prefill(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g, const Tensor& out, double scale, const OptTensor& initial_state,
-                       const OptTensor& final_state, const OptTensor& cu_seqlens, const OptTensor& state_indices) {
+                       const OptTensor& final_state, const OptTensor& cu_seqlens, const OptTensor& state_indices, bool zero_outside) {
   loaded();
   AveLinearArgs a = fill_linear(q, k, v, some(g), out, scale, some(initial_state), some(final_state), some(cu_seqlens), some(state_indices));
+  if (zero_outside) a.flags |= AVE_LINEAR_FLAG_ZERO_OUTSIDE;
   Launch launch(q);
   const Scratch ws(q, launch.stream, api.linear_prefill_workspace_bytes(&a));
   a.workspace = ws.data(); a.workspace_bytes = ws.size();
@@ -1087,7 +1088,7 @@ Shape check_linear(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   return s;
 }
 
-// linear_prefill / linear_decode(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, state_indices, inplace_state, out, chunk_size)
+// linear_prefill / linear_decode(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, state_indices, inplace_state, out, chunk_size[, zero_outside])
 //   -> (o, final or None)
 template <bool kPrefill>
 PyObject* linear_forward(PyObject* const* p) {
@@ -1099,10 +1100,13 @@ PyObject* linear_forward(PyObject* const* p) {
   REQ(chunk == 64, "chunk_size must be 64, got ", chunk, ".");
   const Tensor o = prep_out(out, v);
   const Tensor final = prep_states(s0, idx, s, q, truth(p[6]), truth(p[9]));
-  if constexpr (kPrefill)
-    call<op_linear_prefill>("avelang_gdn::linear_prefill", spread(q), spread(k), spread(v), opt(g), o, scale_or(p[4], s.dk), opt(s0), opt(final), opt(cu), opt(idx));
-  else
+  if constexpr (kPrefill) {
+    const bool zero_outside = truth(p[12]);
+    if (zero_outside && s.n == 0) o.zero_();  // no kernel runs
+    call<op_linear_prefill>("avelang_gdn::linear_prefill", spread(q), spread(k), spread(v), opt(g), o, scale_or(p[4], s.dk), opt(s0), opt(final), opt(cu), opt(idx), zero_outside);
+  } else {
     call<op_linear_decode>("avelang_gdn::linear_decode", q, k, v, opt(g), o, scale_or(p[4], s.dk), opt(s0), opt(final), opt(cu), opt(idx));
+  }
   return wrap_pair(o, final);
 }
 
@@ -1281,7 +1285,7 @@ PyMethodDef methods[] = {
     ENTRY("gate", gate, 4),
     ENTRY("gemm", gemm, 3),
     ENTRY("backward", backward, 10),
-    ENTRY("linear_prefill", linear_forward<true>, 12),
+    ENTRY("linear_prefill", linear_forward<true>, 13),
     ENTRY("linear_decode", linear_forward<false>, 12),
     ENTRY("linear_backward", linear_backward, 9),
     ENTRY("layer_norm", layer_norm, 6),

@@ -18,6 +18,7 @@ int launch_linear_prefill(const AveLinearArgs& a, cudaStream_t stream) {
   lin::set_scale(s, a.scale);
   s.scale_e = a.scale; s.scale_w = 1.f;
   s.o = a.o; s.o_stride_b = a.o_stride_b; s.o_stride_t = a.o_stride_t; s.o_stride_h = a.o_stride_h;
+  s.zero_outside = a.cu_seqlens != nullptr && (a.flags & AVE_LINEAR_FLAG_ZERO_OUTSIDE) != 0;
   s.state_in = a.initial_state; s.state_out = a.final_state; s.st_y = a.dv; s.st_w = 1;
   s.plan = prefill_plan(a);
   if (s.plan.cut) {

@@ -49,6 +49,7 @@ struct Args {
   float scale_e, scale_w;
   void* o;                         // bf16
   int64_t o_stride_b, o_stride_t, o_stride_h;
+  int zero_outside;                // rows of no sequence become zero
   float* o_part;                   // fp32 [B, T, Hv, dv] instead, for a sum over heads behind the scan
   const float* state_in;           // [slot, Hv, ..]: element (y feature, w feature) at y * st_y + w * st_w
   float* state_out;
@@ -210,6 +211,18 @@ __device__ __forceinline__ float pow2(Two x) {
   return n > 127.f ? p * __int_as_float(0x7f800000) : p * __int_as_float(((int)n + 127) << 23);  // (a NaN stays one)
 }
 
+// Rows of a packed batch in front of its first offset and behind its last, or all where the offsets are not monotone: the CTAs of a head share them out.
+template <int D>
+__device__ __forceinline__ void zero_outside(const Args& a, bool fit) {
+  const int lo = fit ? a.cu_seqlens[0] : a.T, hi = fit ? a.cu_seqlens[a.n_seqs] : a.T;
+  __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.o) + (int64_t)(blockIdx.x % a.Hv) * a.o_stride_h;
+  const int64_t pieces = (int64_t)(lo + (a.T - hi)) * (D / 8), step = (int64_t)(gridDim.x / a.Hv) * THREADS;
+  for (int64_t i = (int64_t)(blockIdx.x / a.Hv) * THREADS + threadIdx.x; i < pieces; i += step) {
+    const int64_t r = i / (D / 8), t = r < lo ? r : hi + (r - lo);
+    *reinterpret_cast<uint4*>(o + t * a.o_stride_t + 8 * (i % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 template <int DK, int DV, bool kRev, Mode kMode>
 __device__ __forceinline__ void scan(const Args& a, const Maps& maps) {
   using K = Cfg<kMode>;
@@ -256,7 +269,10 @@ __device__ __forceinline__ void scan(const Args& a, const Maps& maps) {
     tc::fence_barrier_init();
   }
   pdl_wait();
-  if (!offsets_fit(a, true)) return;
+  const bool fit = offsets_fit(a, true);
+  if constexpr (!kState && !kGrad && !kRev)
+    if (a.zero_outside) zero_outside<DV>(a, fit);
+  if (!fit) return;
   const int h = blockIdx.x % a.Hv;
   const int64_t seg_slot = longest_first(a, blockIdx.x / a.Hv);
   const Seg seg = seg_of_slot(a, seg_slot);

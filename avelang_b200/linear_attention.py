@@ -30,10 +30,10 @@ def chunk_linear_attention(q, k, v, g=None, scale=None, initial_state=None, outp
 
     With ``state_indices`` (int32 ``[N]``) the initial states are read from, and the final states written to, slots of the
     ``initial_state`` pool (in place unless ``inplace_state=False``); a negative slot skips the sequence (zero output, no state
-    access).  Sequences that share a slot race for it.  A sequence of no tokens hands its initial state on.  Rows behind the last
-    offset of a packed batch are left as they were."""
+    access).  Sequences that share a slot race for it.  A sequence of no tokens hands its initial state on.  Rows in front of
+    the first offset of a packed batch and behind its last are left as they were."""
     return _native.linear_prefill(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, state_indices, inplace_state, out,
-                                  chunk_size)
+                                  chunk_size, False)
 
 
 def fused_recurrent_linear_attention(q, k, v, g=None, scale=None, initial_state=None, output_final_state=True, cu_seqlens=None, *,
@@ -54,12 +54,12 @@ def linear_attention_backward(q, k, v, g, d_o, scale=None, initial_state=None, d
 
 class LinearAttentionFunction(torch.autograd.Function):
     """``o, final_state = LinearAttentionFunction.apply(q, k, v, g, scale, initial_state, cu_seqlens)``: the chunked forward pass with
-    the chunked backward pass attached (g, scale, initial_state and cu_seqlens may be None).  It can be differentiated once.  A step with
+    the chunked backward pass attached (g, scale, initial_state and cu_seqlens may be None).  Rows of a packed batch that belong to no sequence are zero, in the result and in the gradients.  It can be differentiated once.  A step with
     its backward pass can be captured into a CUDA graph once the results of eager steps on the same leaves are gone."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, scale, initial_state, cu_seqlens):
-        o, final = chunk_linear_attention(q, k, v, g, scale, initial_state, True, cu_seqlens)
+        o, final = _native.linear_prefill(q, k, v, g, scale, initial_state, True, cu_seqlens, None, True, None, 64, True)
         ctx.save_for_backward(q, k, v, g, initial_state, cu_seqlens)
         ctx.scale = scale
         ctx.set_materialize_grads(False)

@@ -36,7 +36,7 @@ SCHEMAS = {
                          "Tensor? norm_weight, Tensor(b!) state_pool, Tensor? state_indices, Tensor(c!) out, int Hk, int Hv, "
                          "float scale, float norm_eps, bool gate_first) -> ()",
     "linear_prefill": "(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor(a!) out, float scale, Tensor? initial_state, "
-                      "Tensor(b!)? final_state, Tensor? cu_seqlens, Tensor? state_indices) -> ()",
+                      "Tensor(b!)? final_state, Tensor? cu_seqlens, Tensor? state_indices, bool zero_outside=False) -> ()",
     "linear_decode": "(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor(a!) out, float scale, Tensor? initial_state, "
                      "Tensor(b!)? final_state, Tensor? cu_seqlens, Tensor? state_indices) -> ()",
     "linear_backward": "(Tensor q, Tensor k, Tensor v, Tensor? g, Tensor d_o, float scale, Tensor? initial_state, Tensor? d_final_state, "

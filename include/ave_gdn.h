@@ -334,9 +334,10 @@ int ave_gdn_gate_beta(const AveGateArgs* args, void* stream);
  * in the layouts of the recurrences above, for dk and dv of 64 or 128 each.  g (the decay's logarithm) is fp32 [B,T,Hv], or one
  * number a head with both strides zero, or null (no decay).  g is meant to be <= 0: minus infinity empties the state (values below
  * -1e6 are taken as -1e6, whose exponential is zero too); positive values let it grow. */
+#define AVE_LINEAR_FLAG_ZERO_OUTSIDE 2u
 typedef struct AveLinearArgs {
   uint32_t struct_size;
-  uint32_t flags;             /* 0 */
+  uint32_t flags;             /* AVE_LINEAR_FLAG_ZERO_OUTSIDE (prefill) */
   const void* q;              /* bf16 */
   const void* k;              /* bf16 */
   const void* v;              /* bf16 */
@@ -361,7 +362,8 @@ typedef struct AveLinearArgs {
   float reserved0;
 } AveLinearArgs;
 /* Whole sequences, dense [B,T] or packed via cu_seqlens.  A packed batch whose offsets are not monotone inside [0, T] is skipped as a
- * whole (AVE_GDN_DEV_BAD_SEQLEN); rows behind the last offset are left as they were. */
+ * whole (AVE_GDN_DEV_BAD_SEQLEN); rows in front of the first offset and behind the last are left as they were, or, with AVE_LINEAR_FLAG_ZERO_OUTSIDE, become
+ * zero, all rows with bad offsets (n_seqs == 0: no row is touched). */
 int ave_linear_chunk_prefill(const AveLinearArgs* args, void* stream);
 size_t ave_linear_prefill_workspace_bytes(const AveLinearArgs* args);
 /* Token by token; T == 1 with state_indices is the continuous-batching decode step.  A sequence with bad offsets is skipped. */
