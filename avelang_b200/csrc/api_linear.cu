@@ -19,7 +19,11 @@ int launch_layer_norm_backward(const AveLayerNormBwdArgs& a, cudaStream_t stream
 namespace {
 
 bool head_dim(int d) { return d == 64 || d == 128; }
-bool rows_on16(const void* p, int64_t sb, int64_t st, int64_t sh) { return aligned16(p) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0; }
+// (The distance of a dimension's elements says nothing where it has one only.)
+template <class Args>
+bool rows_on16(const Args& a, const void* p, int heads, int64_t sb, int64_t st, int64_t sh) {
+  return aligned16(p) && (a.B <= 1 || sb % 8 == 0) && (a.T <= 1 || st % 8 == 0) && (heads <= 1 || sh % 8 == 0);
+}
 
 template <class Args>
 int validate_shape(const Args* a) {
@@ -39,8 +43,8 @@ int validate_linear(const AveLinearArgs* a) {
   if (a->state_indices == nullptr && (a->initial_state || a->final_state) && a->num_slots < a->n_seqs) return AVE_GDN_INVALID_ARGUMENT;
   if (nothing_to_do(*a)) return AVE_GDN_OK;
   if (!a->q || !a->k || !a->v || !a->o) return AVE_GDN_INVALID_ARGUMENT;
-  if (!rows_on16(a->q, a->q_stride_b, a->q_stride_t, a->q_stride_h) || !rows_on16(a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h) ||
-      !rows_on16(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h) || !rows_on16(a->o, a->o_stride_b, a->o_stride_t, a->o_stride_h))
+  if (!rows_on16(*a, a->q, a->Hk, a->q_stride_b, a->q_stride_t, a->q_stride_h) || !rows_on16(*a, a->k, a->Hk, a->k_stride_b, a->k_stride_t, a->k_stride_h) ||
+      !rows_on16(*a, a->v, a->Hv, a->v_stride_b, a->v_stride_t, a->v_stride_h) || !rows_on16(*a, a->o, a->Hv, a->o_stride_b, a->o_stride_t, a->o_stride_h))
     return AVE_GDN_MISALIGNED;
   if (!aligned16(a->initial_state) || !aligned16(a->final_state) || (reinterpret_cast<uintptr_t>(a->g) & 3u)) return AVE_GDN_MISALIGNED;
   return AVE_GDN_OK;
@@ -52,8 +56,8 @@ int validate_linear_bwd(const AveLinearBwdArgs* a) {
   if (nothing_to_do(*a)) return AVE_GDN_OK;
   if (!a->q || !a->k || !a->v || !a->d_o || !a->d_q || !a->d_k || !a->d_v || (a->g && !a->d_g) || (a->initial_state && !a->d_initial_state)) return AVE_GDN_INVALID_ARGUMENT;
   if ((a->flags & AVE_LINEAR_FLAG_HEAD_GATE) && (a->g_stride_b != 0 || a->g_stride_t != 0)) return AVE_GDN_INVALID_ARGUMENT;
-  if (!rows_on16(a->q, a->q_stride_b, a->q_stride_t, a->q_stride_h) || !rows_on16(a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h) ||
-      !rows_on16(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h) || !rows_on16(a->d_o, a->do_stride_b, a->do_stride_t, a->do_stride_h))
+  if (!rows_on16(*a, a->q, a->Hk, a->q_stride_b, a->q_stride_t, a->q_stride_h) || !rows_on16(*a, a->k, a->Hk, a->k_stride_b, a->k_stride_t, a->k_stride_h) ||
+      !rows_on16(*a, a->v, a->Hv, a->v_stride_b, a->v_stride_t, a->v_stride_h) || !rows_on16(*a, a->d_o, a->Hv, a->do_stride_b, a->do_stride_t, a->do_stride_h))
     return AVE_GDN_MISALIGNED;
   if (!aligned16(a->d_q) || !aligned16(a->d_k) || !aligned16(a->d_v) || !aligned16(a->initial_state) || !aligned16(a->d_final_state) || !aligned16(a->d_initial_state) ||
       ((reinterpret_cast<uintptr_t>(a->g) | reinterpret_cast<uintptr_t>(a->d_g)) & 3u))

@@ -28,3 +28,35 @@ def test_only_the_differentiable_call_clears_rows_of_no_sequence(built_lib):
         L.chunk_linear_attention(*x, cu_seqlens=i32(3))
         L.LinearAttentionFunction.apply(*x, None, None, None, i32(3))
     assert [(n, a.get("zero_outside", False)) for n, a in mode.made] == [("linear_prefill", False), ("linear_prefill", True)]
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "o"])
+def test_distances_in_dimensions_of_one_element_may_be_anything(built_lib, name):
+    """A batch of one cut out of a wider buffer, or a single token, or a single head.  (No call gets as far as a launch: scratch is missing.)"""
+    import ctypes
+
+    from avelang_b200 import _lib
+    lib = _lib.load()
+
+    def rc(dim, one):
+        a, b = _lib.LinearArgs(), _lib.LinearBwdArgs()
+        for args in (a, b):
+            args.struct_size = ctypes.sizeof(args)
+            args.B, args.T, args.Hk, args.Hv, args.dk, args.dv = 2, 8192, 2, 2, 64, 64
+            if one:
+                for field in {"b": ("B",), "t": ("T",), "h": ("Hk", "Hv")}[dim]:
+                    setattr(args, field, 1)
+            args.n_seqs, args.g = args.B, 0x1000
+            for t in ("q", "k", "v", "o", "d_o", "d_q", "d_k", "d_v", "d_g"):
+                if hasattr(args, t):
+                    setattr(args, t, 0x1000)
+                for d in "bth":
+                    if hasattr(args, f"{t.replace('d_', 'd')}_stride_{d}"):
+                        setattr(args, f"{t.replace('d_', 'd')}_stride_{d}", 1001 if d == dim and t.replace("d_", "") == name else 512)
+        a.num_slots = a.n_seqs
+        return lib.ave_linear_chunk_prefill(ctypes.byref(a), None) if dim != "t" or not one else None, lib.ave_linear_backward(ctypes.byref(b), None)
+
+    for dim in "bth":
+        assert rc(dim, False) == (_lib.MISALIGNED, _lib.MISALIGNED)
+        forward, backward = rc(dim, True)
+        assert backward == _lib.INVALID_ARGUMENT and forward in (None, _lib.INVALID_ARGUMENT)
