@@ -712,17 +712,25 @@ void op_linear_decode(const Tensor& q, const Tensor& k, const Tensor& v, const O
   check(launch([&] { return api.linear_decode(&a, launch.stream); }), "fused_recurrent_linear_attention");
 }
 
+// A gradient's layout is nobody's choice: one that is a view into a larger gradient may lie off 16-byte boundaries and is copied then.
+Tensor on16(const Tensor& t) {
+  bool fits = reinterpret_cast<uintptr_t>(ptr(&t)) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) fits = fits && (t.size(i) <= 1 || t.stride(i) * t.element_size() % 16 == 0);
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 // dq, dk, dv, dg, d_initial_state: contiguous
-void op_linear_backward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g_in, const Tensor& d_o, double scale, const OptTensor& initial_state,
-                        const OptTensor& d_final_state, const OptTensor& cu_seqlens, const Tensor& dq, const Tensor& dk, const Tensor& dv, const OptTensor& dg,
+void op_linear_backward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g_in, const Tensor& d_o_in, double scale, const OptTensor& initial_state,
+                        const OptTensor& d_final_in, const OptTensor& cu_seqlens, const Tensor& dq, const Tensor& dk, const Tensor& dv, const OptTensor& dg,
                         const OptTensor& d_initial_state) {
   loaded();
   const Tensor *g = some(g_in), *cu = some(cu_seqlens);
+  const Tensor d_o = on16(d_o_in), d_final = some(d_final_in) != nullptr ? on16(*some(d_final_in)) : Tensor();
   AveLinearBwdArgs a{};
   a.struct_size = sizeof(a);
   a.flags = g != nullptr && g->dim() == 1 ? AVE_LINEAR_FLAG_HEAD_GATE : 0;
   a.q = ptr(&q); a.k = ptr(&k); a.v = ptr(&v); a.g = ptr_as<float>(g); a.d_o = ptr(&d_o);
-  a.initial_state = ptr_as<float>(some(initial_state)); a.d_final_state = ptr_as<float>(some(d_final_state)); a.cu_seqlens = ptr_as<int32_t>(cu);
+  a.initial_state = ptr_as<float>(some(initial_state)); a.d_final_state = ptr_as<float>(some(d_final)); a.cu_seqlens = ptr_as<int32_t>(cu);
   a.d_q = ptr_as<void>(&dq); a.d_k = ptr_as<void>(&dk); a.d_v = ptr_as<void>(&dv);
   a.d_g = ptr_as<float>(some(dg)); a.d_initial_state = ptr_as<float>(some(d_initial_state));
   a.status = reinterpret_cast<uint32_t*>(status_word(q.device()).data_ptr());

@@ -46,7 +46,7 @@ def fused_recurrent_linear_attention(q, k, v, g=None, scale=None, initial_state=
 
 def linear_attention_backward(q, k, v, g, d_o, scale=None, initial_state=None, d_final_state=None, cu_seqlens=None):
     """Gradients of ``chunk_linear_attention`` / ``fused_recurrent_linear_attention``.  ``d_o``: bf16, shaped like ``v``; ``d_final_state``:
-    optional fp32 gradient of the final states.  Returns ``(dq, dk, dv, dg, d_initial_state)``: dq, dk bf16 in the shape of q, k (the
+    optional fp32 gradient of the final states; neither needs to lie on 16-byte boundaries.  Returns ``(dq, dk, dv, dg, d_initial_state)``: dq, dk bf16 in the shape of q, k (the
     value heads sharing a key head are summed in fp32), dv bf16, dg fp32 in the shape of g (None without one), ``d_initial_state``
     fp32 (None when no initial state was given).  Rows of a packed batch that belong to no sequence get zeros."""
     return _native.linear_backward(q, k, v, g, d_o, scale, initial_state, d_final_state, cu_seqlens)
