@@ -1096,6 +1096,11 @@ Shape check_linear(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   return s;
 }
 
+// Whether two tensors begin with the same element
+bool same_place(const Tensor& a, const Tensor& b) {
+  return a.numel() > 0 && b.numel() > 0 && a.storage().unsafeGetStorageImpl() == b.storage().unsafeGetStorageImpl() && a.storage_offset() == b.storage_offset();
+}
+
 // linear_prefill / linear_decode(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, state_indices, inplace_state, out, chunk_size[, zero_outside])
 //   -> (o, final or None)
 template <bool kPrefill>
@@ -1107,6 +1112,11 @@ PyObject* linear_forward(PyObject* const* p) {
   const int64_t chunk = integer(p[11]);
   REQ(chunk == 64, "chunk_size must be 64, got ", chunk, ".");
   const Tensor o = prep_out(out, v);
+  if (out != nullptr) {
+    for (int64_t i = 0; i < 3; ++i) REQ(o.size(i) <= 1 || o.stride(i) != 0, "the rows of out must not share memory");
+    // (a state's columns are shared out among CTAs, each of which reads all of q and k)
+    REQ(kPrefill || !(same_place(o, q) || same_place(o, k)), "out must not lie in the place of q or k");
+  }
   const Tensor final = prep_states(s0, idx, s, q, truth(p[6]), truth(p[9]));
   if constexpr (kPrefill) {
     const bool zero_outside = truth(p[12]);

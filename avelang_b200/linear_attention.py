@@ -31,7 +31,7 @@ def chunk_linear_attention(q, k, v, g=None, scale=None, initial_state=None, outp
     With ``state_indices`` (int32 ``[N]``) the initial states are read from, and the final states written to, slots of the
     ``initial_state`` pool (in place unless ``inplace_state=False``); a negative slot skips the sequence (zero output, no state
     access).  Sequences that share a slot race for it.  A sequence of no tokens hands its initial state on.  Rows in front of
-    the first offset of a packed batch and behind its last are left as they were."""
+    the first offset of a packed batch and behind its last are left as they were.  ``out`` may be q, k or v."""
     return _native.linear_prefill(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, state_indices, inplace_state, out,
                                   chunk_size, False)
 
@@ -40,7 +40,7 @@ def fused_recurrent_linear_attention(q, k, v, g=None, scale=None, initial_state=
                                      state_indices=None, inplace_state=True, out=None):
     """Token by token with the state on chip; ``T == 1`` with ``state_indices`` is the continuous-batching decode step: each state is
     read once from its slot of the ``initial_state`` pool and written once, in place unless ``inplace_state=False``.  A negative
-    slot skips the sequence.  Returns ``(o, state)``."""
+    slot skips the sequence.  ``out`` may be v, not q or k.  Returns ``(o, state)``."""
     return _native.linear_decode(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, state_indices, inplace_state, out, 64)
 
 

@@ -60,3 +60,27 @@ def test_distances_in_dimensions_of_one_element_may_be_anything(built_lib, name)
         assert rc(dim, False) == (_lib.MISALIGNED, _lib.MISALIGNED)
         forward, backward = rc(dim, True)
         assert backward == _lib.INVALID_ARGUMENT and forward in (None, _lib.INVALID_ARGUMENT)
+
+
+@pytest.mark.parametrize("entry", ["chunk_linear_attention", "fused_recurrent_linear_attention"])
+def test_results_that_lie_badly(built_lib, entry):
+    """A result whose rows share memory; one in the place of q or k, which the recurrent form's CTAs read while others write."""
+    from avelang_b200 import linear_attention as L
+    f = getattr(L, entry)
+    with FakeTensorMode(), Calls() as mode:
+        q, k, v = bf(2, 9, 4, 128), bf(2, 9, 4, 128), bf(2, 9, 4, 128)
+        for out in (bf(1, 9, 4, 128).expand(2, 9, 4, 128), bf(2, 1, 4, 128).expand(2, 9, 4, 128), bf(2, 9, 1, 128).expand(2, 9, 4, 128)):
+            with pytest.raises(ValueError, match="rows of out must not share memory"):
+                f(q, k, v, out=out)
+        assert not mode.made
+        for out in (q, k, q.view(2, 9, 4, 128)):
+            if entry == "chunk_linear_attention":
+                f(q, k, v, out=out)
+            else:
+                with pytest.raises(ValueError, match="out must not lie in the place of q or k"):
+                    f(q, k, v, out=out)
+        wide = bf(2, 9, 16, 128)
+        f(wide[:, :, :4], wide[:, :, 4:8], wide[:, :, 8:12], out=wide[:, :, 12:])
+        f(q, k, v, out=v)
+        f(q[:1, :1, :1], k[:1, :1, :1], v[:1, :1, :1], out=bf(1, 1, 1, 128).expand(1, 1, 1, 128))
+    assert len(mode.made) == (6 if entry == "chunk_linear_attention" else 3)
