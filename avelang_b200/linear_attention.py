@@ -11,6 +11,9 @@ convention of the reference's kernel library, python/avelang_kernels/amdgpu_gemm
 
 ``g``, the logarithm of the decay, is fp32: ``[B, T, Hv]`` (one for every token and head), ``[Hv]`` (one a head) or None (no
 decay).  It is meant to be <= 0; minus infinity empties the state.
+
+A NaN or an infinity in a token of v reaches the outputs from that token on, and in the whole-sequence form also those of the tokens in front of it among its sixteen (counted from
+the sequence's first): a masked score is an exact zero, but zero times a NaN is none.  In the gradients the same holds for k, q and d_o, on either side.  Other sequences are never reached.
 """
 from __future__ import annotations
 

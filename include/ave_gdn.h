@@ -333,7 +333,8 @@ int ave_gdn_gate_beta(const AveGateArgs* args, void* stream);
  *   M <- exp(g_t) M + k_t v_t^T,   o_t = scale * M^T q_t,
  * in the layouts of the recurrences above, for dk and dv of 64 or 128 each.  g (the decay's logarithm) is fp32 [B,T,Hv], or one
  * number a head with both strides zero, or null (no decay).  g is meant to be <= 0: minus infinity empties the state (values below
- * -1e6 are taken as -1e6, whose exponential is zero too); positive values let it grow. */
+ * -1e6 are taken as -1e6, whose exponential is zero too); positive values let it grow.  In the whole-sequence form a NaN or an infinity in a token of v also reaches
+ * the outputs of the tokens in front of it among its sixteen, counted from the sequence's first. */
 #define AVE_LINEAR_FLAG_ZERO_OUTSIDE 2u
 typedef struct AveLinearArgs {
   uint32_t struct_size;
