@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 #include "ave_gdn.h"
@@ -85,6 +86,21 @@ inline cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block
   cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = stream;
   cfg.attrs = at; cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Dynamic shared memory beyond the default, asked for once a device and kernel
+constexpr int MAX_DEVICES = 64;
+template <auto* kernel>
+int allow_smem(int bytes) {
+  static std::atomic<bool> ready[MAX_DEVICES];
+  int dev = 0;
+  AVE_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= MAX_DEVICES) return AVE_GDN_UNSUPPORTED;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    AVE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    ready[dev].store(true, std::memory_order_release);
+  }
+  return AVE_GDN_OK;
 }
 
 // Sequence n of a dense [B,T] batch or of a packed varlen batch: batch row, first token, length.

@@ -11,8 +11,6 @@
 // (16384 x 16384 backward 567 us).
 #include <cuda_fp16.h>
 
-#include <atomic>
-
 #include "common.cuh"
 #include "tc.cuh"
 
@@ -777,18 +775,6 @@ inline RingShape ring_shape(int64_t rows, int64_t row_bytes, int arrays, int gro
   depth = depth < 8 ? depth : 8;
   depth = depth < turns ? depth : turns;
   return {(int)grid, (int)depth, (int)(depth * slot * groups)};
-}
-template <auto* kernel>
-int allow_smem(int smem) {  // more shared memory than the default, asked for once a device
-  static std::atomic<bool> ready[64];
-  int dev = 0;
-  AVE_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) return AVE_GDN_UNSUPPORTED;
-  if (!ready[dev].load(std::memory_order_acquire)) {
-    AVE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    ready[dev].store(true, std::memory_order_release);
-  }
-  return AVE_GDN_OK;
 }
 template <class T, int P, int G>
 int run_forward_ring(const AveLayerNormArgs& a, cudaStream_t stream) {

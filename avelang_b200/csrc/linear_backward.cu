@@ -471,9 +471,9 @@ int launch_linear_backward(const AveLinearBwdArgs& a, cudaStream_t stream) {
       s.plan = lin::Plan{lin::C, 1, (int64_t)a.B * a.T / lin::C + a.n_seqs + 1};
       const lin::PairSums p{lin_bf(a.q), lin_bf(a.k), lin_bf(a.v), lin_bf(a.d_o), a.q_stride_b, a.q_stride_t, a.q_stride_h, a.k_stride_b, a.k_stride_t, a.k_stride_h,
                             a.v_stride_b, a.v_stride_t, a.v_stride_h, a.do_stride_b, a.do_stride_t, a.do_stride_h, rep, a.scale, f32(l.intra_a), f32(l.intra_b)};
-      auto* kernel = lin::pair_sums_kernel<DK, DV>;
+      constexpr auto* kernel = &lin::pair_sums_kernel<DK, DV>;
       constexpr int smem = 64 * 4 * (DK + DV) + 64 * 8 + 8 * 64 * 4 + 1024;
-      if ((r = lin::allow_smem<DK, DV>(kernel, smem))) return r;
+      if ((r = allow_smem<kernel>(smem))) return r;
       const int64_t grid = s.plan.slots * a.Hv;
       if (grid > 0x7fffffff) return (int)AVE_GDN_UNSUPPORTED;
       AVE_CUDA_TRY(launch_after(kernel, (unsigned)grid, lin::PAIR_THREADS, smem, stream, s, p));

@@ -1,6 +1,5 @@
 // Host side of the scans of linear attention: how a batch is cut into segments, tensor maps, launches.
 #pragma once
-#include <atomic>
 #include <cmath>
 
 #include "linear_scan.cuh"
@@ -8,8 +7,6 @@
 namespace ave {
 namespace {
 namespace lin {
-
-constexpr int MAX_DEVICES = 64;
 
 // One CTA walks a segment of one (sequence, value head).  Whole sequences need one pass; segments need their own increments first (a pass that reads Y and W alone) and the chain
 // of them, so they pay where there are too few sequences and heads for the SMs, or where one sequence is so long that the others wait for it.  The lengths of packed sequences are
@@ -70,35 +67,17 @@ inline bool result_map(CUtensorMap* m, void* p, int d, int heads, int B, int T, 
   return ok;
 }
 
-// More shared memory than the default, asked for once a device
-template <int DK, int DV, class K>
-int allow_smem(K* kernel, int smem) {
-  static std::atomic<bool> ready[MAX_DEVICES];
-  int dev = 0;
-  AVE_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= MAX_DEVICES) return AVE_GDN_UNSUPPORTED;
-  if (!ready[dev].load(std::memory_order_acquire)) {
-    AVE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    ready[dev].store(true, std::memory_order_release);
-  }
-  return AVE_GDN_OK;
-}
-
 // The register split of the roles counts on the registers that the kernel is launched with.
 template <auto* kernel>
 int scan_ready(int smem) {
-  static std::atomic<bool> ready[MAX_DEVICES];
-  int dev = 0;
-  AVE_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= MAX_DEVICES) return AVE_GDN_UNSUPPORTED;
-  if (!ready[dev].load(std::memory_order_acquire)) {
+  static std::atomic<bool> looked{false};
+  if (!looked.load(std::memory_order_acquire)) {
     cudaFuncAttributes at;
     AVE_CUDA_TRY(cudaFuncGetAttributes(&at, kernel));
     if (at.numRegs != REGS_LAUNCH) return cuda_fail(cudaErrorInvalidKernelImage);
-    AVE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    ready[dev].store(true, std::memory_order_release);
+    looked.store(true, std::memory_order_release);
   }
-  return AVE_GDN_OK;
+  return allow_smem<kernel>(smem);
 }
 inline int64_t scan_grid(const Args& a) { return a.plan.slots * a.Hv; }
 template <int DK, int DV, Mode kMode>

@@ -674,7 +674,7 @@ struct SideSet {
   cudaEvent_t done[SEG_MAX] = {}, scanned[SEG_MAX] = {};
   bool ready = false;
 };
-constexpr int SIDE_SETS = 4, MAX_DEVICES = 64;
+constexpr int SIDE_SETS = 4;
 struct DeviceSide {
   std::mutex mu;
   SideSet sets[SIDE_SETS];
