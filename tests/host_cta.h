@@ -21,18 +21,23 @@
 #include "ave_gdn.h"
 
 #undef __global__
+#undef __host__
 #undef __device__
 #undef __shared__
 #undef __forceinline__
 #undef __launch_bounds__
 #define __global__
+#define __host__
 #define __device__
 #define __shared__ static
 #define __forceinline__ inline
 #define __launch_bounds__(...)
 
 namespace cta {
-constexpr int THREADS = 256;
+#ifndef CTA_THREADS
+#define CTA_THREADS 256
+#endif
+constexpr int THREADS = CTA_THREADS;
 struct Copy { void* dst; const void* src; uint32_t bytes; uint64_t* bar; bool late; long due; };  // a turn, or a number of polls
 struct Phase { int count, pending; long tx; uint32_t phase; long polls; };
 struct Meeting { int here = 0; long turn = 0; };
@@ -51,7 +56,7 @@ struct Index { unsigned x; } thread, block, grid, size{THREADS};
 ucontext_t contexts[THREADS];  // a thread's first turn; from then on by jumps, which save no signal masks
 jmp_buf back, at[THREADS];
 std::function<void()> body;
-alignas(128) uint8_t memory[204800];
+alignas(1024) uint8_t memory[232448];
 
 inline void yield() {
   if (_setjmp(at[thread.x]) == 0) _longjmp(back, 1);
@@ -71,8 +76,9 @@ inline void entry() {
   s.done[thread.x] = true;
   _longjmp(back, 1);
 }
+inline int slow() { const int among[] = {1, 1, 4, 30}; return among[s.rng() % 4]; }  // turns of a warp's that are passed over
 // Runs CTA b of n; returns what went wrong, or nothing.
-inline const char* run(int b, int n, unsigned seed, int limit, int late, int pollers, std::function<void()> kernel) {
+inline const char* run(int b, int n, unsigned seed, int limit, int late, int pollers, std::function<void()> kernel, std::function<bool()> step = nullptr) {
   s = State();
   s.rng.seed(seed); s.limit = limit; s.late = late; s.pollers = pollers;
   block.x = b; grid.x = n;
@@ -88,9 +94,13 @@ inline const char* run(int b, int n, unsigned seed, int limit, int late, int pol
   static bool begun[THREADS];
   left = THREADS;
   for (int i = 0; i < THREADS; ++i) { order[i] = i; begun[i] = false; }
+  int speed[THREADS / 32];
+  for (int& x : speed) x = step ? slow() : 1;
   while (left > 0) {
+    if (step && s.rng() % 4096 == 0) speed[s.rng() % (THREADS / 32)] = slow();
     next = (int)(s.rng() % left);
     thread.x = order[next];
+    if (speed[thread.x >> 5] > 1 && s.rng() % speed[thread.x >> 5] != 0) { ++s.now; continue; }
     if (_setjmp(back) == 0) {
       if (begun[thread.x]) _longjmp(at[thread.x], 1);
       begun[thread.x] = true;
@@ -107,8 +117,10 @@ inline const char* run(int b, int n, unsigned seed, int limit, int late, int pol
       complete(p);
       s.copies.erase(s.copies.begin() + i);
     }
-    if (s.now > 400000000) return "the CTA does not end";
+    if (step) step();
+    if (s.now > 25000000) return s.fault ? s.fault : "the CTA does not end";
   }
+  if (step && step()) return "copies or products on their way in a CTA that has ended";
   if (!s.copies.empty()) return "copies on their way into a CTA that has ended";
   return s.fault;
 }

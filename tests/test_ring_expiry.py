@@ -94,7 +94,7 @@ int whole(int rows, int n, int depth, int seeds) {
   printf("right %d NaN %d runs with an expiry %d of %d\n", all_right, all_nan, expired, 2 * seeds);
   return all_right > 0 && all_nan > 0 && expired > 0 && expired < 2 * seeds ? 0 : 1;
 }
-int main() { return whole<TYPE, PIECES, GROUP>(ROWS, COLUMNS, DEPTH, 60); }
+int main() { return whole<TYPE, PIECES, GROUP>(ROWS, COLUMNS, DEPTH, 30); }
 """
 
 
