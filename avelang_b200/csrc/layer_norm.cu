@@ -6,7 +6,7 @@
 // Both are bound by HBM: the forward pass reads x and writes y, the backward pass reads x and dy and writes dx.  A row belongs to a group of threads, each of which keeps the same
 // columns for every row it meets: the weights are read once a CTA, and the sums of the weight's gradient are registers too.  A CTA's sums go to scratch and a second kernel adds them
 // in a fixed order.  Three forms by the row's length, figures for bf16 rows with fp32 weights, copy rate 6549 GB/s: rings of rows in shared memory for aligned rows of middle length
-// (131072 x 2048: forward 179 to 187 us, 5.7 to 6.0 TB/s, backward 267 to 272 us, 5.9 to 6.0 TB/s; 32768 x 8192: 203 and 262 us); rows in registers, U of them in flight a group, for short ones and for those
+// (131072 x 2048: forward 179 to 187 us, 5.7 to 6.0 TB/s, through the public call 187 to 197, backward 267 to 272 us, 5.9 to 6.0 TB/s; 32768 x 8192: 203 and 262 us); rows in registers, U of them in flight a group, for short ones and for those
 // that do not lie on 16 bytes (131072 x 64: 8.7 and 12.9 us; 30000 x 2047: 89 and 103 us, bound by the loads of single elements); and CTAs of 1024 threads for long ones
 // (16384 x 16384 backward 567 us).
 #include <cuda_fp16.h>
@@ -624,7 +624,8 @@ __global__ void __launch_bounds__(256, 1) layer_norm_backward_ring_kernel(const 
 }
 
 // Long rows: five numbers a column are more than the register file holds, so the column sums lie in shared memory (each thread's own place), the weights are read for every row, and the row
-// stays as it was read.  (16384 rows of 16384 bf16: 567 us; 7.6 ms with everything in registers, which spill.)
+// stays as it was read.  (16384 rows of 16384 bf16: 567 us; 7.6 ms with everything in registers, which spill.  The longest still do, at 1024 threads: up to 184 bytes stored a thread above 24576 columns, up to
+// 432 above 16384 off 16 bytes.  8192 rows, forward and backward us: of 20480 bf16 283 and 412, of 28672 334 and 590, fp32 369 and 882; off 16 bytes of 16383 250 and 602, 4096 of 28671 264 and 825.)
 template <class T, int VEC, int P>
 __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(const AveLayerNormBwdArgs a, float* partial, bool aligned) {
   constexpr int TPR = 1024, HV = Pairs<VEC>::H;

@@ -1,6 +1,6 @@
 // Chunked form of linear attention with a decay for each head over whole sequences: one scan, or, where sequences are cut into segments that
-// run side by side, the segments' increments, their chain, and the scan from the states that enter them.  (32 heads of 128 over 16 key heads: 8192 tokens 122 us, of which
-// increments 42, chain 7, scan 70; 203 tokens 15 us; 24 prompts of 65536 tokens 568 us = 3.0 TB/s.)
+// run side by side, the segments' increments, their chain, and the scan from the states that enter them.  (32 heads of 128 over 16 key heads: 8192 tokens 118 to 129 us, of which
+// increments 43, chain 6, scan 70 to 77; 203 tokens 13.5 us; 24 prompts of 65536 tokens 568 to 690 us by the draw of their lengths, 2.5 to 3.0 TB/s.)
 #include "linear_scan_host.cuh"
 
 namespace ave {

@@ -11,7 +11,8 @@
 // one would leave 2^-9 of each number in a sum.  Tokens of a chunk come as one TMA copy an operand, three or four chunks ahead.  The state stays on chip from a segment's first chunk
 // to its last, so HBM sees each input and output once; one CTA fills an SM.  What bounds a chunk is the chain of hand-overs between the roles (products, masking and decaying P, the
 // state's update and its image for the next chunk), not the tensor pipe and not HBM: 2.3 us of outputs and state, 1.4 of the state alone, 3.9 with the gate gradient's terms.
-// (d = 128, 148 heads x 2048 tokens: 75 us, 4.1 TB/s of the copy rate's 6.5; the scans of a 2 x 4096 token, 32 head backward 335 us.)  64 tokens a chunk: with 128
+// (d = 128, 148 heads x 2048 tokens: 72 us, 4.3 TB/s of the copy rate's 6.5,
+// tensor pipe busy 0.42 of the cycles, DRAM 0.49, issue slots 0.52; the scans of a 2 x 4096 token, 32 head backward 335 us, of 49 heads x 2048 tokens 0.21, 0.26 and 0.33.)  64 tokens a chunk: with 128
 // P is four times as large for twice the tokens, half of it masked, and two chunks' terms of it would not fit beside the stages.
 #pragma once
 #include "common.cuh"
@@ -105,7 +106,7 @@ __device__ __forceinline__ bool offsets_fit(const Args& a, bool flag) {
 }
 
 // Whole sequences of a packed batch, the longest first, so that the SMs end together: the sequence whose turn it is.  Called by the whole CTA.  (24 prompts of 65536 tokens in all,
-// 2 to 161 chunks each, 32 heads: 568 us, in the batch's order 777.)  Each sequence counts those in front of it, which takes a thread as many steps as there are sequences; where there are
+// 2 to 161 chunks each, 32 heads: 568 us, in the batch's order 777; other draws of the lengths take up to 690.)  Each sequence counts those in front of it, which takes a thread as many steps as there are sequences; where there are
 // many, each is a small part of an SM's work and the batch's order serves.
 constexpr int MOST_IN_ORDER = 256;
 __device__ __forceinline__ int64_t longest_first(const Args& a, int64_t turn) {
@@ -154,6 +155,8 @@ struct Cfg {
 
 constexpr int THREADS = 640;  // warpgroups: loader, gate vectors and two issuers; two for the state and P'; outputs; images of W^T
 constexpr int REGS_LAUNCH = 96, REGS_CTRL = 56, REGS_STATE = 128, REGS_OUT = 96, REGS_PREP = 72;
+// (At 96 registers some roles spill: bytes stored and loaded a thread at d = 128, outputs 32 and 32, with an exact final state 32 and 32, the state alone 24 and 44; the backward's kernel of three
+// scans 320 and 988, 116 and 508 without the gate gradient.)
 static_assert(REGS_CTRL + 2 * REGS_STATE + REGS_OUT + REGS_PREP <= 5 * REGS_LAUNCH, "register redistribution exceeds the launch allocation");
 static_assert(THREADS * REGS_LAUNCH <= 65536, "launch allocation exceeds the register file");
 
@@ -865,7 +868,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(const Args a, const __
   scan<DK, DV, kRev, kMode>(a, maps);
 }
 
-// Four numbers a thread, the next four segments read ahead; bound by their latency (8192 tokens x 32 heads in four segments: 7 us, 34 MB through L2).
+// Four numbers a thread, the next four segments read ahead; bound by their latency (8192 tokens x 32 heads in four segments: 6 us for 17 to 21 MB through L2).
 // Between the two passes: seg_state goes from each segment's own increment to the state that enters it, and the last one's is the final state.
 template <int DK, int DV, bool kRev>
 __device__ __forceinline__ void chain(const Args& a) {

@@ -12,7 +12,8 @@ namespace lin {
 // of them, so they pay where there are too few sequences and heads for the SMs, or where one sequence is so long that the others wait for it.  The lengths of packed sequences are
 // not known here: the longest is taken to be four times the mean.  Unit: a chunk of the scan, 2.2 us on every SM; a chunk of the first pass takes 0.45 of that, a CTA's
 // beginning and end 3 and 2.5, the chain and its launches 2.5 (8192 tokens x 32 heads, forward: whole 304 us, segments of 4096 tokens
-// 212, of 2048 123; 24 prompts of 65536 tokens x 32 heads: whole 568, segments of 5504 908.)
+// 212, of 2048 123; 24 prompts of 65536 tokens x 32 heads, one draw of their lengths: whole 568, segments of 5504 908;
+// other draws, whole, up to 690.)
 inline Plan plan_of(int B, int64_t T, int n_seqs, bool packed, int heads) {
   constexpr double SMS = 148;
   const double chunks = (double)((T * B + C - 1) / C);
