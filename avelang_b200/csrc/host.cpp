@@ -167,20 +167,24 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType dt, const Tensor& like) {
 Tensor f32(const Tensor& t) { return (t.requires_grad() ? t.detach() : t).to(at::kFloat).contiguous(); }
 
 // ---------------------------------------------------------------------------------------------- scratch and status word
-// In memory of its own, cleared on a stream of its own, whatever the caller's stream is being captured into: as part of a graph the word would hold nothing before the first
-// replay, and each replay would clear what other calls have left in it.
+// In memory of its own, cleared on a stream of its own and before anybody has it.  Cleared on the caller's stream, it would lose what calls on other streams flag until then; captured there, it
+// would hold nothing before the first replay, and each replay would clear what other calls have left in it.  (Where torch holds all memory, it comes from torch.)
 Tensor make_status_word(int device) {
   const c10::InferenceMode ordinary(false);  // a word made in inference mode could not be reset outside it
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  const auto options = at::TensorOptions().dtype(at::kInt).device(at::Device(at::kCUDA, (c10::DeviceIndex)device));
   const c10::cuda::CUDAStreamCaptureModeGuard apart(cudaStreamCaptureModeRelaxed);
   void* word = nullptr;
   cudaStream_t stream;
-  C10_CUDA_CHECK(cudaMalloc(&word, sizeof(int32_t)));
+  if (cudaMalloc(&word, sizeof(int32_t)) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return at::zeros({1}, options);
+  }
   C10_CUDA_CHECK(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking));
   C10_CUDA_CHECK(cudaMemsetAsync(word, 0, sizeof(int32_t), stream));
   C10_CUDA_CHECK(cudaStreamSynchronize(stream));
   C10_CUDA_CHECK(cudaStreamDestroy(stream));
-  return at::from_blob(word, {1}, at::TensorOptions().dtype(at::kInt).device(at::Device(at::kCUDA, (c10::DeviceIndex)device)));
+  return at::from_blob(word, {1}, options);
 }
 const Tensor& status_word(const at::Device& dev) {  // one a device, never destroyed: the CUDA context may be gone at exit
   static std::atomic<Tensor*> words[C10_COMPILE_TIME_MAX_GPUS];
