@@ -1118,8 +1118,6 @@ PyObject* linear_forward(PyObject* const* p) {
   const Tensor o = prep_out(out, v);
   if (out != nullptr) {
     for (int64_t i = 0; i < 3; ++i) REQ(o.size(i) <= 1 || o.stride(i) != 0, "the rows of out must not share memory");
-    // (a state's columns are shared out among CTAs, each of which reads all of q and k)
-    REQ(kPrefill || !(same_place(o, q) || same_place(o, k)), "out must not lie in the place of q or k");
   }
   const Tensor final = prep_states(s0, idx, s, q, truth(p[6]), truth(p[9]));
   if constexpr (kPrefill) {
@@ -1127,7 +1125,8 @@ PyObject* linear_forward(PyObject* const* p) {
     if (zero_outside && s.n == 0) o.zero_();  // no kernel runs
     call<op_linear_prefill>("avelang_gdn::linear_prefill", spread(q), spread(k), spread(v), opt(g), o, scale_or(p[4], s.dk), opt(s0), opt(final), opt(cu), opt(idx), zero_outside);
   } else {
-    call<op_linear_decode>("avelang_gdn::linear_decode", q, k, v, opt(g), o, scale_or(p[4], s.dk), opt(s0), opt(final), opt(cu), opt(idx));
+    // (a state's columns are shared out among CTAs, each of which reads all of q and k: neither may be written over while they do)
+    call<op_linear_decode>("avelang_gdn::linear_decode", same_place(o, q) ? q.clone() : q, same_place(o, k) ? k.clone() : k, v, opt(g), o, scale_or(p[4], s.dk), opt(s0), opt(final), opt(cu), opt(idx));
   }
   return wrap_pair(o, final);
 }

@@ -43,7 +43,7 @@ def fused_recurrent_linear_attention(q, k, v, g=None, scale=None, initial_state=
                                      state_indices=None, inplace_state=True, out=None):
     """Token by token with the state on chip; ``T == 1`` with ``state_indices`` is the continuous-batching decode step: each state is
     read once from its slot of the ``initial_state`` pool and written once, in place unless ``inplace_state=False``.  A negative
-    slot skips the sequence.  ``out`` may be v, not q or k.  Returns ``(o, state)``."""
+    slot skips the sequence.  ``out`` may be q, k or v.  Returns ``(o, state)``."""
     return _native.linear_decode(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, state_indices, inplace_state, out, 64)
 
 

@@ -64,7 +64,7 @@ def test_distances_in_dimensions_of_one_element_may_be_anything(built_lib, name)
 
 @pytest.mark.parametrize("entry", ["chunk_linear_attention", "fused_recurrent_linear_attention"])
 def test_results_that_lie_badly(built_lib, entry):
-    """A result whose rows share memory; one in the place of q or k, which the recurrent form's CTAs read while others write."""
+    """A result whose rows share memory is refused; where one takes the place of q or k, which the recurrent form's CTAs read while others write, that form reads a copy."""
     from avelang_b200 import linear_attention as L
     f = getattr(L, entry)
     with FakeTensorMode(), Calls() as mode:
@@ -73,14 +73,14 @@ def test_results_that_lie_badly(built_lib, entry):
             with pytest.raises(ValueError, match="rows of out must not share memory"):
                 f(q, k, v, out=out)
         assert not mode.made
-        for out in (q, k, q.view(2, 9, 4, 128)):
-            if entry == "chunk_linear_attention":
-                f(q, k, v, out=out)
-            else:
-                with pytest.raises(ValueError, match="out must not lie in the place of q or k"):
-                    f(q, k, v, out=out)
+        apart = lambda a: tuple(a[n].untyped_storage()._cdata != a["out"].untyped_storage()._cdata for n in "qk")
+        for out, copied in ((q, (True, False)), (k, (False, True)), (q.view(2, 9, 4, 128), (True, False))):
+            f(q, k, v, out=out)
+            assert mode.made[-1][1]["out"] is out
+            assert apart(mode.made[-1][1]) == ((True, True) if entry != "chunk_linear_attention" else tuple(not c for c in copied))
         wide = bf(2, 9, 16, 128)
         f(wide[:, :, :4], wide[:, :, 4:8], wide[:, :, 8:12], out=wide[:, :, 12:])
         f(q, k, v, out=v)
+        assert mode.made[-1][1]["q"] is q and mode.made[-1][1]["k"] is k
         f(q[:1, :1, :1], k[:1, :1, :1], v[:1, :1, :1], out=bf(1, 1, 1, 128).expand(1, 1, 1, 128))
-    assert len(mode.made) == (6 if entry == "chunk_linear_attention" else 3)
+    assert len(mode.made) == 6

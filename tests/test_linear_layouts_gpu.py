@@ -62,7 +62,7 @@ def test_one_of_a_kind_with_an_odd_distance(built_lib):
 
 @pytest.mark.parametrize("T", [90, 2100])
 def test_results_in_the_place_of_inputs(built_lib, T):
-    """Whole sequences, cut into segments or not, in the place of q, k or v; the recurrent form in the place of v."""
+    """Whole sequences, cut into segments or not, and the recurrent form, in the place of q, k or v."""
     from avelang_b200 import linear_attention as L
     q, k, v, g, s0 = P.cuda(*P.make(1, T, 2, 2, 128, 128, "token", 9, 1, 0.05))
     want = L.chunk_linear_attention(q, k, v, g, None, s0, True)
@@ -73,5 +73,7 @@ def test_results_in_the_place_of_inputs(built_lib, T):
     n = min(T, 90)
     x = [t[:, :n].contiguous() for t in (q, k, v)]
     want = L.fused_recurrent_linear_attention(*x, g[:, :n], None, s0)
-    o, s = L.fused_recurrent_linear_attention(*x, g[:, :n], None, s0, out=x[2])
-    assert o.data_ptr() == x[2].data_ptr() and torch.equal(o, want[0]) and torch.equal(s, want[1])
+    for i in range(3):
+        y = [t.clone() for t in x]
+        o, s = L.fused_recurrent_linear_attention(*y, g[:, :n], None, s0, out=y[i])
+        assert o.data_ptr() == y[i].data_ptr() and torch.equal(o, want[0]) and torch.equal(s, want[1])
