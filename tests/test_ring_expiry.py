@@ -52,7 +52,7 @@ struct Run {
   }
 };
 static int all_nan, all_right, wrong;
-template <class F> void judge(int count, F same) {  // same(i): 1 the right bits, 0 NaN, -1 neither
+template <class F> void tally(int count, F same) {  // same(i): 1 the right bits, 0 NaN, -1 neither
   int right = 0, nan = 0;
   for (int i = 0; i < count; ++i) { const int s = same(i); right += s == 1; nan += s == 0; }
   if (right == count) ++all_right; else if (nan == count) ++all_nan; else ++wrong;
@@ -79,12 +79,12 @@ int whole(int rows, int n, int depth, int seeds) {
       fault = pass == 0 ? got.template forward<P, G>(seed, depth, 8, 30) : got.template backward<P, G>(seed, depth, 6, 100);
       if (fault != nullptr) { printf("seed %d: %s\n", seed, fault); return 1; }
       for (int r = 0; r < rows; ++r)
-        judge(pass == 0 ? n + 2 : n, [&](int i) {
+        tally(pass == 0 ? n + 2 : n, [&](int i) {
           if (pass == 1) return compare(get(got.dx[r * n + i]), get(ref.dx[r * n + i]));
           return i < n ? compare(get(got.y[r * n + i]), get(ref.y[r * n + i])) : i == n ? compare(got.mean[r], ref.mean[r]) : compare(got.rstd[r], ref.rstd[r]);
         });
       if (pass == 1)
-        for (int c = 0; c < 2 * n; ++c) judge(1, [&](int) { return compare(got.partial[c], ref.partial[c]); });
+        for (int c = 0; c < 2 * n; ++c) tally(1, [&](int) { return compare(got.partial[c], ref.partial[c]); });
       const bool nan = all_nan > before;
       if (got.status != (nan ? AVE_GDN_DEV_WAIT_EXPIRED : 0u)) { printf("seed %d, pass %d: status %u with %s\n", seed, pass, got.status, nan ? "NaN" : "no NaN"); return 1; }
       expired += nan;
