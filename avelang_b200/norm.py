@@ -5,8 +5,8 @@
 over the last dimension (1 to 28672 elements).  ``x`` is bf16, fp16 or fp32; ``weight`` and ``bias`` have its dtype or fp32.  Sums and
 statistics are fp32, results are rounded once.  Rows that are evenly spaced and contiguous are read as they are; others are copied first.
 Rows of a whole number of 16-byte pieces on 16-byte boundaries take wide loads, others go element by element.  Errors are ValueError, as
-in the reference's kernel library (python/avelang_kernels/amdgpu_gemm.py:463-486).  Rows that a bounded wait on the device has given up on are NaN in all their results, and so is what they reach in
-the gradients of weight and bias; ``gdn.read_status()`` says so.
+in the reference's kernel library (python/avelang_kernels/amdgpu_gemm.py:463-486).  Rows that a bounded wait on the device has given up on are NaN in all their results, and so are
+the columns of the gradients of weight and bias that miss elements of them; ``gdn.read_status()`` says so.
 """
 from __future__ import annotations
 

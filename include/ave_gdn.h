@@ -444,7 +444,7 @@ typedef struct AveLayerNormBwdArgs {
   uint64_t workspace_bytes;
   int64_t rows, n, dy_stride, x_stride, dx_stride;
   int32_t x_dtype, w_dtype;
-  uint32_t* status;       /* as in AveLayerNormArgs; with it the columns of d_weight and d_bias that the lost rows reach are NaN */
+  uint32_t* status;       /* as in AveLayerNormArgs; columns of d_weight and d_bias that miss elements of such a row are NaN too */
 } AveLayerNormBwdArgs;
 int ave_layer_norm_backward(const AveLayerNormBwdArgs* args, void* stream);
 size_t ave_layer_norm_backward_workspace_bytes(const AveLayerNormBwdArgs* args);
