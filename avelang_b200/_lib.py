@@ -115,6 +115,29 @@ class LayerNormBwdArgs(ctypes.Structure):
                 + [("x_dtype", I32), ("w_dtype", I32), ("status", P)])
 
 
+class RmsNormArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", U32), ("flags", U32)] + [(n, P) for n in ("x", "residual", "weight", "sum", "y", "scale", "rstd")]
+                + [(n, I64) for n in ("rows", "n", "x_stride", "residual_stride", "sum_stride", "y_stride")]
+                + [("x_dtype", I32), ("w_dtype", I32), ("eps", F32), ("reserved0", F32)])
+
+
+class RmsNormBwdArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", U32), ("flags", U32)]
+                + [(n, P) for n in ("d_y", "x", "rstd", "weight", "d_sum", "d_x", "d_weight", "workspace")]
+                + [("workspace_bytes", U64)] + [(n, I64) for n in ("rows", "n", "dy_stride", "x_stride", "ds_stride", "dx_stride")]
+                + [("x_dtype", I32), ("w_dtype", I32)])
+
+
+class QuantRowsArgs(ctypes.Structure):
+    _fields_ = [("struct_size", U32), ("flags", U32), ("x", P), ("q", P), ("scale", P), ("rows", I64), ("n", I64), ("x_stride", I64), ("q_stride", I64),
+                ("x_dtype", I32), ("reserved0", I32)]
+
+
+class GemmInt8Args(ctypes.Structure):
+    _fields_ = ([("struct_size", U32), ("flags", U32)] + [(n, P) for n in ("a", "b", "c", "a_scale", "b_scale", "bias")]
+                + [(n, I64) for n in ("M", "N", "K", "lda", "ldb", "ldc")] + [("c_dtype", I32), ("bias_dtype", I32), ("status", P)])
+
+
 # every symbol include/ave_gdn.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "ave_gdn_chunk_prefill": (ctypes.c_int, [ctypes.POINTER(GdnArgs), P]),
@@ -142,6 +165,12 @@ SYMBOLS = {
     "ave_layer_norm": (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), P]),
     "ave_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(LayerNormBwdArgs), P]),
     "ave_layer_norm_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LayerNormBwdArgs)]),
+    "ave_rms_norm": (ctypes.c_int, [ctypes.POINTER(RmsNormArgs), P]),
+    "ave_rms_norm_backward": (ctypes.c_int, [ctypes.POINTER(RmsNormBwdArgs), P]),
+    "ave_rms_norm_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(RmsNormBwdArgs)]),
+    "ave_quantize_rows_int8": (ctypes.c_int, [ctypes.POINTER(QuantRowsArgs), P]),
+    "ave_dequantize_rows_int8": (ctypes.c_int, [ctypes.POINTER(QuantRowsArgs), P]),
+    "ave_gemm_int8_nt": (ctypes.c_int, [ctypes.POINTER(GemmInt8Args), P]),
     "ave_gdn_abi_version": (ctypes.c_int, []),
     "ave_gdn_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ave_gdn_last_cuda_error": (ctypes.c_int, []),

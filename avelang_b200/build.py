@@ -16,7 +16,8 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libave_gdn_b200.so")
 HOST = os.path.join(HERE, "_host.so")  # Python module: the host side of the public functions (csrc/host.cpp)
 SOURCES = ["api.cu", "decode.cu", "decode_layer.cu", "backward.cu", "rmsnorm.cu", "prefill_d64.cu", "elementwise.cu", "gemm.cu", "tmap.cu", "prefill_tc.cu",
-           "api_linear.cu", "linear_decode.cu", "linear_prefill.cu", "linear_backward.cu", "layer_norm.cu"]
+           "api_linear.cu", "linear_decode.cu", "linear_prefill.cu", "linear_backward.cu", "layer_norm.cu",
+           "api_int8.cu", "rms_norm.cu", "rms_norm_backward.cu", "gemm_int8.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-I" + INCLUDE,
               "-I" + CSRC]

@@ -20,6 +20,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
@@ -99,6 +100,12 @@ struct Api {
   decltype(&ave_layer_norm) layer_norm = nullptr;
   decltype(&ave_layer_norm_backward) layer_norm_backward = nullptr;
   decltype(&ave_layer_norm_backward_workspace_bytes) layer_norm_backward_workspace_bytes = nullptr;
+  decltype(&ave_rms_norm) rms_norm = nullptr;
+  decltype(&ave_rms_norm_backward) rms_norm_backward = nullptr;
+  decltype(&ave_rms_norm_backward_workspace_bytes) rms_norm_backward_workspace_bytes = nullptr;
+  decltype(&ave_quantize_rows_int8) quantize_rows = nullptr;
+  decltype(&ave_dequantize_rows_int8) dequantize_rows = nullptr;
+  decltype(&ave_gemm_int8_nt) gemm_int8_nt = nullptr;
   decltype(&ave_gdn_status_string) status_string = nullptr;
   decltype(&ave_gdn_last_cuda_error) last_cuda_error = nullptr;
 } api;
@@ -790,13 +797,86 @@ void op_layer_norm_backward(const Tensor& d_y, const Tensor& x, const Tensor& me
   check(launch([&] { return api.layer_norm_backward(&a, launch.stream); }), "layer_norm_backward");
 }
 
+// x, residual, out, sum: [rows, n] views with contiguous rows; with a scale out holds int8
+void op_rms_norm(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps, bool zero_centered, const Tensor& out, const OptTensor& sum,
+                 const OptTensor& scale, const OptTensor& rstd) {
+  loaded();
+  const Tensor *r = some(residual), *w = some(weight), *h = some(sum);
+  AveRmsNormArgs a{};
+  a.struct_size = sizeof(a);
+  a.flags = (zero_centered ? AVE_RMS_FLAG_ZERO_CENTERED : 0) | (some(scale) != nullptr ? AVE_RMS_FLAG_INT8 : 0);
+  a.x = ptr(&x); a.residual = ptr(r); a.weight = ptr(w); a.sum = const_cast<void*>(ptr(h)); a.y = const_cast<void*>(ptr(&out));
+  a.scale = ptr_as<float>(some(scale)); a.rstd = ptr_as<float>(some(rstd));
+  a.rows = x.size(0); a.n = x.size(1); a.x_stride = x.stride(0); a.y_stride = out.stride(0);
+  if (r != nullptr) a.residual_stride = r->stride(0);
+  if (h != nullptr) a.sum_stride = h->stride(0);
+  a.x_dtype = dtype_code(x, "x"); a.w_dtype = w != nullptr ? dtype_code(*w, "weight") : a.x_dtype;
+  a.eps = (float)eps;
+  Launch launch(x);
+  check(launch([&] { return api.rms_norm(&a, launch.stream); }), "rms_norm");
+}
+
+void op_rms_norm_backward(const Tensor& d_y, const Tensor& x, const Tensor& rstd, const OptTensor& weight, const OptTensor& d_sum, bool zero_centered,
+                          const Tensor& d_x, const OptTensor& d_weight) {
+  loaded();
+  const Tensor *w = some(weight), *ds = some(d_sum);
+  AveRmsNormBwdArgs a{};
+  a.struct_size = sizeof(a);
+  a.flags = zero_centered ? AVE_RMS_FLAG_ZERO_CENTERED : 0;
+  a.d_y = ptr(&d_y); a.x = ptr(&x); a.rstd = ptr_as<float>(&rstd); a.weight = ptr(w); a.d_sum = ptr(ds);
+  a.d_x = const_cast<void*>(ptr(&d_x)); a.d_weight = const_cast<void*>(ptr(some(d_weight)));
+  a.rows = x.size(0); a.n = x.size(1); a.dy_stride = d_y.stride(0); a.x_stride = x.stride(0); a.dx_stride = d_x.stride(0);
+  if (ds != nullptr) a.ds_stride = ds->stride(0);
+  a.x_dtype = dtype_code(x, "x"); a.w_dtype = w != nullptr ? dtype_code(*w, "weight") : a.x_dtype;
+  Launch launch(x);
+  const Scratch ws(x, launch.stream, api.rms_norm_backward_workspace_bytes(&a));
+  a.workspace = ws.data(); a.workspace_bytes = ws.size();
+  check(launch([&] { return api.rms_norm_backward(&a, launch.stream); }), "rms_norm_backward");
+}
+
+AveQuantRowsArgs quant_args(const Tensor& x, const Tensor& q, const Tensor& scale) {  // [rows, n] views with contiguous rows
+  AveQuantRowsArgs a{};
+  a.struct_size = sizeof(a);
+  a.x = const_cast<void*>(ptr(&x)); a.q = const_cast<void*>(ptr(&q)); a.scale = ptr_as<float>(&scale);
+  a.rows = x.size(0); a.n = x.size(1); a.x_stride = x.stride(0); a.q_stride = q.stride(0);
+  a.x_dtype = dtype_code(x, "x");
+  return a;
+}
+void op_quantize_rows(const Tensor& x, const Tensor& q, const Tensor& scale) {
+  loaded();
+  const AveQuantRowsArgs a = quant_args(x, q, scale);
+  Launch launch(x);
+  check(launch([&] { return api.quantize_rows(&a, launch.stream); }), "quantize_rows_int8");
+}
+void op_dequantize_rows(const Tensor& q, const Tensor& scale, const Tensor& x) {
+  loaded();
+  const AveQuantRowsArgs a = quant_args(x, q, scale);
+  Launch launch(x);
+  check(launch([&] { return api.dequantize_rows(&a, launch.stream); }), "dequantize_rows_int8");
+}
+
+void op_gemm_int8(const Tensor& A, const Tensor& B, const Tensor& a_scale, const Tensor& b_scale, const OptTensor& bias, const Tensor& out) {
+  loaded();
+  AveGemmInt8Args a{};
+  a.struct_size = sizeof(a);
+  a.a = ptr(&A); a.b = ptr(&B); a.c = const_cast<void*>(ptr(&out)); a.a_scale = ptr_as<float>(&a_scale); a.b_scale = ptr_as<float>(&b_scale);
+  a.bias = ptr(some(bias));
+  a.M = A.size(0); a.N = B.size(0); a.K = A.size(1); a.lda = A.stride(0); a.ldb = B.stride(0); a.ldc = out.stride(0);
+  a.c_dtype = dtype_code(out, "out"); a.bias_dtype = some(bias) != nullptr ? dtype_code(*some(bias), "bias") : a.c_dtype;
+  a.status = reinterpret_cast<uint32_t*>(status_word(A.device()).data_ptr());
+  Launch launch(A);
+  check(launch([&] { return api.gemm_int8_nt(&a, launch.stream); }), "gemm_int8_transposed_b");
+}
+
 #define OPERATORS(X)                                                                                                        \
   X("chunk_prefill", op_prefill) X("decode_step", op_decode) X("mixed_step", op_mixed) X("decode_layer_step", op_decode_layer) \
   X("gated_rmsnorm", op_rmsnorm) X("conv1d_silu", op_conv) X("conv1d_update", op_conv_update) X("gate_beta", op_gate)          \
   X("gemm_bf16_nt", op_gemm) X("recurrent_backward", op_backward)                                                           \
   X("linear_prefill", op_linear_prefill) X("linear_decode", op_linear_decode)                                               \
   X("linear_backward", op_linear_backward)                                                                                  \
-  X("layer_norm", op_layer_norm) X("layer_norm_backward", op_layer_norm_backward)
+  X("layer_norm", op_layer_norm) X("layer_norm_backward", op_layer_norm_backward)                                           \
+  X("rms_norm", op_rms_norm) X("rms_norm_backward", op_rms_norm_backward) X("quantize_rows_int8", op_quantize_rows)         \
+  X("dequantize_rows_int8", op_dequantize_rows) X("gemm_int8_nt", op_gemm_int8)
 TORCH_LIBRARY_IMPL(avelang_gdn, CUDA, m) {
 #define CUDA_KERNEL(name, f) m.impl(name, f);
   OPERATORS(CUDA_KERNEL)
@@ -1189,6 +1269,20 @@ bool same_or_apart(const Tensor& x, const Tensor& y) {
   return r >= n && r + n <= sx;
 }
 
+// Whether the bytes from the first to the last element of two tensors have any in common
+bool ranges_meet(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0 || a.storage().unsafeGetStorageImpl() != b.storage().unsafeGetStorageImpl()) return false;
+  auto range = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    const int64_t size = (int64_t)t.element_size();
+    return std::pair<int64_t, int64_t>(t.storage_offset() * size, (t.storage_offset() + last + 1) * size);
+  };
+  const auto [a0, a1] = range(a);
+  const auto [b0, b1] = range(b);
+  return a0 < b1 && b0 < a1;
+}
+
 // layer_norm(x, weight, bias, eps, return_stats, out) -> out or (out, mean, rstd)
 PyObject* layer_norm(PyObject* const* p) {
   const Tensor& x = tensor(p[0], "x");
@@ -1241,6 +1335,174 @@ PyObject* layer_norm_backward(PyObject* const* p) {
   return wrap_all({&dx, &dw, &db});
 }
 
+// The results of a row-wise call, as [rows, n] views of what the caller has named `name`, or gets
+Tensor result_rows(const Tensor& y, const char* name) {
+  const Tensor y2 = as_rows(y);
+  REQ(y2.is_alias_of(y) && (y2.stride(1) == 1 || y2.size(1) == 1), name, " must be viewable as [rows, n] with contiguous rows");
+  REQ(y2.size(0) <= 1 || y2.stride(0) >= y2.size(1), "the rows of ", name, " must not overlap");
+  return y2;
+}
+Tensor input_rows(const Tensor& x) {
+  const Tensor x2 = as_rows(x);
+  return x2.stride(1) == 1 ? x2 : x2.contiguous();
+}
+bool same_rows(const Tensor& a, const Tensor& b) {
+  return a.numel() > 0 && a.storage().unsafeGetStorageImpl() == b.storage().unsafeGetStorageImpl() && a.storage_offset() == b.storage_offset();
+}
+void check_like(const Tensor& t, const char* name, const Tensor& x) {
+  REQ(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device(), name, " must be a ", dtype_name(x), " tensor of shape ",
+      shape_of(x.sizes()), " on ", x.device());
+}
+// 8-bit rows in the shape of x, a whole number of 16 bytes apart, and a place for their scales
+std::pair<Tensor, Tensor> empty_int8(const Tensor& x) {
+  const int64_t n = x.size(-1);
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = (n + 15) / 16 * 16;
+  return {empty(shape, at::kChar, x).narrow(-1, 0, n), empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x)};
+}
+
+// rms_norm(x, weight, eps, residual, zero_centered, return_stats, out, sum_out) -> out, or a tuple of out[, sum][, rstd]
+// rms_norm_int8(x, weight, eps, residual, zero_centered, sum_out) -> (q, scale[, sum])
+template <bool kInt8>
+PyObject* rms_norm(PyObject* const* p) {
+  const Tensor& x = tensor(p[0], "x");
+  const Tensor *w = opt_tensor(p[1], "weight"), *res = opt_tensor(p[3], "residual"), *out = kInt8 ? nullptr : opt_tensor(p[6], "out"),
+               *sum_out = opt_tensor(p[kInt8 ? 5 : 7], "sum_out");
+  check_norm_input(x, w, nullptr);
+  if (res != nullptr) check_like(*res, "residual", x);
+  REQ(sum_out == nullptr || res != nullptr, "sum_out needs residual");
+  if (out != nullptr) check_like(*out, "out", x);
+  if (sum_out != nullptr) check_like(*sum_out, "sum_out", x);
+  const Tensor x2 = input_rows(x), r2 = res != nullptr ? input_rows(*res) : Tensor(), wc = w != nullptr ? w->contiguous() : Tensor();
+  Tensor h, h2;
+  if (res != nullptr) {
+    h = sum_out != nullptr ? *sum_out : empty(x.sizes(), x.scalar_type(), x);
+    h2 = result_rows(h, "sum_out");
+  }
+  if (sum_out != nullptr) REQ(same_or_apart(x2, h2) && same_or_apart(r2, h2), "sum_out must be x or residual themselves or share no element with them");
+  const bool zero_centered = truth(p[4]);
+  if constexpr (kInt8) {
+    const auto [q, scale] = empty_int8(x);
+    call<op_rms_norm>("avelang_gdn::rms_norm", x2, opt(r2), opt(wc), number(p[2]), zero_centered, as_rows(q), opt(h2), opt(scale), OptTensor());
+    return h.defined() ? wrap_all({&q, &scale, &h}) : wrap_all({&q, &scale});
+  } else {
+    const Tensor y = out != nullptr ? *out : empty(x.sizes(), x.scalar_type(), x);
+    const Tensor y2 = result_rows(y, "out");
+    if (out != nullptr) {
+      REQ(same_or_apart(x2, y2) && (res == nullptr || same_or_apart(r2, y2)), "out must be x or residual themselves or share no element with them");
+      REQ(!h.defined() || (same_or_apart(h2, y2) && !same_rows(h2, y2)), "out and sum_out must share no element");
+    }
+    const bool stats = truth(p[5]);
+    Tensor rstd;
+    if (stats) rstd = empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+    call<op_rms_norm>("avelang_gdn::rms_norm", x2, opt(r2), opt(wc), number(p[2]), zero_centered, y2, opt(h2), OptTensor(), opt(rstd));
+    if (h.defined()) return stats ? wrap_all({&y, &h, &rstd}) : wrap_all({&y, &h});
+    return stats ? wrap_all({&y, &rstd}) : wrap(y);
+  }
+}
+
+// rms_norm_backward(d_y, x, rstd, weight, d_sum, zero_centered) -> (dx, dweight or None)
+PyObject* rms_norm_backward(PyObject* const* p) {
+  const Tensor &d_y = tensor(p[0], "d_y"), &x = tensor(p[1], "x"), &rstd = tensor(p[2], "rstd");
+  const Tensor *w = opt_tensor(p[3], "weight"), *d_sum = opt_tensor(p[4], "d_sum");
+  check_norm_input(x, w, nullptr);
+  check_like(d_y, "d_y", x);
+  if (d_sum != nullptr) check_like(*d_sum, "d_sum", x);
+  const int64_t n = x.size(-1), rows = x.numel() / n;
+  REQ(rstd.scalar_type() == at::kFloat && rstd.numel() == rows && rstd.is_contiguous() && rstd.device() == x.device(), "rstd must be a contiguous fp32 tensor of ",
+      rows, " elements on ", x.device());
+  const Tensor dx = empty(x.sizes(), x.scalar_type(), x);
+  Tensor wc, dw;
+  if (w != nullptr) {
+    wc = w->contiguous();
+    dw = empty({n}, w->scalar_type(), x);
+    if (rows == 0) dw.zero_();  // no kernel runs
+  }
+  const Tensor ds2 = d_sum != nullptr ? input_rows(*d_sum) : Tensor();
+  call<op_rms_norm_backward>("avelang_gdn::rms_norm_backward", input_rows(d_y), input_rows(x), rstd, opt(wc), opt(ds2), truth(p[5]), as_rows(dx), opt(dw));
+  return wrap_all({&dx, &dw});
+}
+
+// quantize_rows(x) -> (q, scale)
+PyObject* quantize_rows(PyObject* const* p) {
+  const Tensor& x = tensor(p[0], "x");
+  check_norm_input(x, nullptr, nullptr);
+  const auto [q, scale] = empty_int8(x);
+  call<op_quantize_rows>("avelang_gdn::quantize_rows_int8", input_rows(x), as_rows(q), scale);
+  return wrap_all({&q, &scale});
+}
+
+// 8-bit rows as the kernels take them: on 16 bytes, others are copied
+Tensor int8_rows(const Tensor& q) {
+  const Tensor q2 = as_rows(q);
+  const bool apart = q2.size(0) <= 1 || (q2.stride(0) % 16 == 0 && q2.stride(0) >= q2.size(1));
+  if (q2.stride(1) == 1 && apart && q2.storage_offset() % 16 == 0) return q2;
+  const Tensor own = empty_int8(q2).first;
+  own.copy_(q2);
+  return own;
+}
+at::ScalarType float_type(PyObject* o, const char* name) {  // None: bf16
+  if (o == Py_None) return at::kBFloat16;
+  REQ(THPDtype_Check(o), name, " must be a dtype");
+  const at::ScalarType t = reinterpret_cast<THPDtype*>(o)->scalar_type;
+  REQ(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat, name, " must be torch.bfloat16, torch.float16 or torch.float32");
+  return t;
+}
+
+// dequantize_rows(q, scale, dtype) -> x
+PyObject* dequantize_rows(PyObject* const* p) {
+  const Tensor &q = tensor(p[0], "q"), &scale = tensor(p[1], "scale");
+  REQ(q.scalar_type() == at::kChar, "q must have dtype torch.int8, got ", dtype_name(q), ".");
+  REQ(q.is_cuda(), "q must be a CUDA tensor");
+  REQ(q.dim() >= 1 && q.size(-1) >= 1 && q.size(-1) <= 28672, "the last dimension of q must lie in [1, 28672], got ", q.dim() > 0 ? q.size(-1) : 0, ".");
+  REQ(scale.scalar_type() == at::kFloat && scale.sizes() == q.sizes().slice(0, q.dim() - 1) && scale.device() == q.device(), "scale must be a fp32 tensor of shape ",
+      shape_of(q.sizes().slice(0, q.dim() - 1)), " on ", q.device());
+  const Tensor x = empty(q.sizes(), float_type(p[2], "dtype"), q);
+  call<op_dequantize_rows>("avelang_gdn::dequantize_rows_int8", int8_rows(q), scale.contiguous(), as_rows(x));
+  return wrap(x);
+}
+
+// gemm_int8(A, B, a_scale, b_scale, bias, out, out_dtype) -> out
+PyObject* gemm_int8(PyObject* const* p) {
+  const Tensor &A = tensor(p[0], "A"), &B = tensor(p[1], "B"), &a_scale = tensor(p[2], "a_scale"), &b_scale = tensor(p[3], "b_scale");
+  const Tensor *bias = opt_tensor(p[4], "bias"), *out = opt_tensor(p[5], "out");
+  REQ(A.scalar_type() == at::kChar, "A must have dtype torch.int8, got ", dtype_name(A), ".");
+  REQ(B.scalar_type() == at::kChar, "B must have dtype torch.int8, got ", dtype_name(B), ".");
+  REQ(A.dim() == 2 && B.dim() == 2 && A.size(1) == B.size(1), "A [M, K] and B [N, K] must share K, got ", shape_of(A.sizes()), " and ", shape_of(B.sizes()), ".");
+  REQ(A.is_cuda() && B.device() == A.device(), "A and B must be CUDA tensors on one device, got ", A.device(), " and ", B.device(), ".");
+  const int64_t m = A.size(0), k = A.size(1), n = B.size(0);
+  REQ(k >= 1 && k <= 131071, "K must lie in [1, 131071], got ", k, ".");
+  const std::pair<const char*, const Tensor*> ab[] = {{"A", &A}, {"B", &B}};
+  for (const auto& [name, t] : ab)
+    REQ((t->stride(1) == 1 || k == 1) && (t->size(0) <= 1 || (t->stride(0) % 16 == 0 && t->stride(0) >= k)), name,
+        " must be contiguous in its last dimension, with rows a multiple of 16 bytes apart, got strides ", shape_of(t->strides()), ".");
+  const std::pair<const char*, const Tensor*> scales[] = {{"a_scale", &a_scale}, {"b_scale", &b_scale}};
+  for (const auto& [name, t] : scales)
+    REQ(t->scalar_type() == at::kFloat && t->numel() == (t == &a_scale ? m : n) && t->is_contiguous() && t->device() == A.device(), name,
+        " must be a contiguous fp32 tensor of ", t == &a_scale ? m : n, " elements on ", A.device());
+  at::ScalarType dt = float_type(p[6], "out_dtype");
+  if (out != nullptr) {
+    REQ(out->dim() == 2 && out->size(0) == m && out->size(1) == n, "out must have shape ", shape_of({m, n}), ", got ", shape_of(out->sizes()), ".");
+    REQ(p[6] == Py_None || out->scalar_type() == dt, "out must have dtype out_dtype, got ", dtype_name(*out), ".");
+    dtype_code(*out, "out");
+    dt = out->scalar_type();
+    REQ(out->device() == A.device(), "out must be on device ", A.device(), ", got ", out->device(), ".");
+    REQ((out->stride(1) == 1 || n == 1) && (m <= 1 || out->stride(0) >= n), "out must be contiguous in its last dimension, its rows apart.");
+    const std::pair<const char*, const Tensor*> all[] = {{"A", &A}, {"B", &B}, {"a_scale", &a_scale}, {"b_scale", &b_scale}, {"bias", bias}};
+    for (const auto& [name, t] : all) REQ(t == nullptr || !ranges_meet(*out, *t), "out must not share memory with ", name);
+  }
+  Tensor bc;
+  if (bias != nullptr) {
+    REQ(bias->dim() == 1 && bias->size(0) == n, "bias must have shape ", shape_of({n}), ", got ", shape_of(bias->sizes()), ".");
+    REQ(bias->scalar_type() == dt || bias->scalar_type() == at::kFloat, "bias must have the dtype of the result or torch.float32, got ", dtype_name(*bias), ".");
+    REQ(bias->device() == A.device(), "bias must be on device ", A.device(), ", got ", bias->device(), ".");
+    bc = bias->contiguous();
+  }
+  const Tensor c = out != nullptr ? *out : empty({m, n}, dt, A);
+  call<op_gemm_int8>("avelang_gdn::gemm_int8_nt", A, B, a_scale, b_scale, opt(bc), c);
+  return wrap(c);
+}
+
 PyObject* none() { Py_RETURN_NONE; }
 // status_word(device_index) -> the device status word; workspace-independent
 PyObject* py_status_word(PyObject* const* p) { return wrap(status_word(at::Device(at::kCUDA, (c10::DeviceIndex)integer(p[0])))); }
@@ -1274,6 +1536,12 @@ PyObject* bind(PyObject* const* p) {
   RESOLVE(layer_norm, ave_layer_norm);
   RESOLVE(layer_norm_backward, ave_layer_norm_backward);
   RESOLVE(layer_norm_backward_workspace_bytes, ave_layer_norm_backward_workspace_bytes);
+  RESOLVE(rms_norm, ave_rms_norm);
+  RESOLVE(rms_norm_backward, ave_rms_norm_backward);
+  RESOLVE(rms_norm_backward_workspace_bytes, ave_rms_norm_backward_workspace_bytes);
+  RESOLVE(quantize_rows, ave_quantize_rows_int8);
+  RESOLVE(dequantize_rows, ave_dequantize_rows_int8);
+  RESOLVE(gemm_int8_nt, ave_gemm_int8_nt);
   RESOLVE(status_string, ave_gdn_status_string);
   RESOLVE(last_cuda_error, ave_gdn_last_cuda_error);
 #undef RESOLVE
@@ -1311,6 +1579,12 @@ PyMethodDef methods[] = {
     ENTRY("linear_backward", linear_backward, 9),
     ENTRY("layer_norm", layer_norm, 6),
     ENTRY("layer_norm_backward", layer_norm_backward, 5),
+    ENTRY("rms_norm", rms_norm<false>, 8),
+    ENTRY("rms_norm_int8", rms_norm<true>, 6),
+    ENTRY("rms_norm_backward", rms_norm_backward, 6),
+    ENTRY("quantize_rows", quantize_rows, 1),
+    ENTRY("dequantize_rows", dequantize_rows, 3),
+    ENTRY("gemm_int8", gemm_int8, 7),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

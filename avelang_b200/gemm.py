@@ -3,7 +3,11 @@
 Same name, operand convention and error behaviour as the reference's
 ``gemm_pipeline_transposed_b`` (python/avelang_kernels/amdgpu_gemm.py:458-494): ``A [M, K]`` and ``B [N, K]``
 (the layout of ``nn.Linear.weight``) in bf16, fp32 accumulation, bf16 result, optional ``out=``.  The reference
-requires M % 128 == N % 128 == K % 64 == 0; here only K % 8 == 0 and 16-byte aligned rows are required."""
+requires M % 128 == N % 128 == K % 64 == 0; here only K % 8 == 0 and 16-byte aligned rows are required.
+
+Its form in 8 bits is ``gemm_int8_transposed_b``: int8 operands whose rows (tokens of A, output channels of B) each have a scale, exact int32
+sums, one rounding of the scaled result.  ``quantize_rows_int8`` makes such rows (``norm.rms_norm_int8`` those behind a norm) and
+``dequantize_rows_int8`` gives the values they stand for."""
 from __future__ import annotations
 
 import ctypes
@@ -12,11 +16,33 @@ import torch
 
 from . import _lib, gdn, torch_ops
 
-__all__ = ["gemm_pipeline_transposed_b", "gemm_scatter_to_owners", "reduce_push_to_all"]
+__all__ = ["gemm_pipeline_transposed_b", "gemm_int8_transposed_b", "quantize_rows_int8", "dequantize_rows_int8", "gemm_scatter_to_owners", "reduce_push_to_all"]
 
 
 def gemm_pipeline_transposed_b(A: torch.Tensor, B: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     return gdn._native.gemm(A, B, out)
+
+
+# ---------------------------------------------------------------- 8 bits
+def gemm_int8_transposed_b(A, B, a_scale, b_scale, bias=None, out=None, *, out_dtype=None):
+    """``C[m, n] = (sum_k A[m, k] B[n, k]) * a_scale[m] * b_scale[n] + bias[n]``: int8 ``A [M, K]`` and ``B [N, K]`` with rows a multiple of 16 bytes
+    apart (K itself may be odd, 131071 at most), fp32 scales of M and of N elements.  The sums are exact; they are scaled, in this order, and
+    the bias (in the dtype of the result or fp32) is added in fp32, behind one rounding of sums of more than 24 bits.  The result is bf16, or
+    ``out_dtype``, or of the dtype of ``out`` (bf16, fp16 or fp32), which shares no memory with the operands.  A row or column whose scale is NaN
+    is NaN."""
+    return gdn._native.gemm_int8(A, B, a_scale, b_scale, bias, out, out_dtype)
+
+
+def quantize_rows_int8(x):
+    """``(q, scale)``: the rows of ``x`` (bf16, fp16 or fp32, last dimension up to 28672) in 8 bits.  ``scale`` (fp32, in the leading shape of ``x``) is
+    the row's largest ``|x|`` / 127, ``q`` (int8, rows a multiple of 16 bytes apart) is ``x / scale`` to nearest, ties to even.  A row that holds a NaN
+    or an infinity has a NaN as its scale and zeros in ``q``; one whose scale would be below the smallest normal number has zeros in both."""
+    return gdn._native.quantize_rows(x)
+
+
+def dequantize_rows_int8(q, scale, dtype=None):
+    """The values ``q * scale``, rounded to ``dtype`` (bf16 where it is None, fp16 or fp32)."""
+    return gdn._native.dequantize_rows(q, scale, dtype)
 
 
 # ---------------------------------------------------------------- row-parallel linear with the cross-rank sum fused in

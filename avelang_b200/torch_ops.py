@@ -44,6 +44,13 @@ SCHEMAS = {
     "layer_norm": "(Tensor x, Tensor? weight, Tensor? bias, float eps, Tensor(a!) out, Tensor(b!)? mean, Tensor(c!)? rstd) -> ()",
     "layer_norm_backward": "(Tensor d_y, Tensor x, Tensor mean, Tensor rstd, Tensor? weight, Tensor(a!) d_x, Tensor(b!)? d_weight, "
                            "Tensor(c!)? d_bias) -> ()",
+    "rms_norm": "(Tensor x, Tensor? residual, Tensor? weight, float eps, bool zero_centered, Tensor(a!) out, Tensor(b!)? sum, Tensor(c!)? scale, "
+                "Tensor(d!)? rstd) -> ()",
+    "rms_norm_backward": "(Tensor d_y, Tensor x, Tensor rstd, Tensor? weight, Tensor? d_sum, bool zero_centered, Tensor(a!) d_x, "
+                         "Tensor(b!)? d_weight) -> ()",
+    "quantize_rows_int8": "(Tensor x, Tensor(a!) q, Tensor(b!) scale) -> ()",
+    "dequantize_rows_int8": "(Tensor q, Tensor scale, Tensor(a!) x) -> ()",
+    "gemm_int8_nt": "(Tensor A, Tensor B, Tensor a_scale, Tensor b_scale, Tensor? bias, Tensor(a!) out) -> ()",
 }
 for _name, _schema in SCHEMAS.items():
     _library.define(_name + _schema)

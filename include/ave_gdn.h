@@ -449,6 +449,79 @@ typedef struct AveLayerNormBwdArgs {
 int ave_layer_norm_backward(const AveLayerNormBwdArgs* args, void* stream);
 size_t ave_layer_norm_backward_workspace_bytes(const AveLayerNormBwdArgs* args);
 
+/* RMS norm over rows of n elements, 1 <= n <= 28672: h = round(x + residual) (x itself without a residual), y = h * rstd * weight,
+ * rstd = 1 / sqrt(mean(h^2) + eps); with AVE_RMS_FLAG_ZERO_CENTERED the weight is 1 + weight.  With AVE_RMS_FLAG_INT8 y is held as
+ * q * scale: scale = max|y| / 127 of the row, q = y / scale to nearest, ties to even.  A row that holds a NaN or an infinity then has a NaN as
+ * its scale, one whose scale would be below the smallest normal number (or whose largest |h * weight| is below 3.8e-37) zero, both with q = 0. */
+#define AVE_RMS_FLAG_ZERO_CENTERED 1u
+#define AVE_RMS_FLAG_INT8 2u
+typedef struct AveRmsNormArgs {
+  uint32_t struct_size;
+  uint32_t flags;        /* AVE_RMS_FLAG_* */
+  const void* x;         /* [rows, n], row stride x_stride elements */
+  const void* residual;  /* [rows, n] of x_dtype, optional */
+  const void* weight;    /* [n] of w_dtype, optional */
+  void* sum;             /* h, [rows, n] of x_dtype; needed with a residual, else null; may be x or residual */
+  void* y;               /* [rows, n] of x_dtype, may be x or residual; with AVE_RMS_FLAG_INT8 int8, rows on 16 bytes */
+  float* scale;          /* fp32 [rows], with AVE_RMS_FLAG_INT8 */
+  float* rstd;           /* fp32 [rows], optional */
+  int64_t rows, n, x_stride, residual_stride, sum_stride, y_stride;
+  int32_t x_dtype, w_dtype; /* AVE_DTYPE_*; w_dtype: x_dtype or AVE_DTYPE_FP32 */
+  float eps;
+  float reserved0;
+} AveRmsNormArgs;
+int ave_rms_norm(const AveRmsNormArgs* args, void* stream);
+
+/* Its gradients: xh = x * rstd, d_x = rstd * (w d_y - xh mean(w d_y xh)) + d_sum, d_weight the sum over the rows of d_y xh, formed in fp32 in a
+ * fixed order and rounded once.  x is the h of the forward pass; d_x is the gradient of x and of the residual alike. */
+typedef struct AveRmsNormBwdArgs {
+  uint32_t struct_size;
+  uint32_t flags;         /* AVE_RMS_FLAG_ZERO_CENTERED */
+  const void* d_y;        /* [rows, n] of x_dtype */
+  const void* x;          /* [rows, n] */
+  const float* rstd;      /* fp32 [rows] */
+  const void* weight;     /* [n] of w_dtype, optional */
+  const void* d_sum;      /* [rows, n] of x_dtype, optional: the gradient that reaches h beside the norm */
+  void* d_x;              /* [rows, n] of x_dtype */
+  void* d_weight;         /* [n] of w_dtype, optional */
+  void* workspace;        /* ave_rms_norm_backward_workspace_bytes(), 16-byte aligned; needed with d_weight */
+  uint64_t workspace_bytes;
+  int64_t rows, n, dy_stride, x_stride, ds_stride, dx_stride;
+  int32_t x_dtype, w_dtype;
+} AveRmsNormBwdArgs;
+int ave_rms_norm_backward(const AveRmsNormBwdArgs* args, void* stream);
+size_t ave_rms_norm_backward_workspace_bytes(const AveRmsNormBwdArgs* args);
+
+/* Rows in 8 bits, as above, and the values they stand for (q * scale, rounded to x_dtype). */
+typedef struct AveQuantRowsArgs {
+  uint32_t struct_size;
+  uint32_t flags;   /* 0 */
+  void* x;          /* [rows, n] of x_dtype; read when quantising, written when dequantising */
+  void* q;          /* int8 [rows, n], rows on 16 bytes, each with room for a whole number of 16 */
+  float* scale;     /* fp32 [rows] */
+  int64_t rows, n, x_stride, q_stride;
+  int32_t x_dtype, reserved0;
+} AveQuantRowsArgs;
+int ave_quantize_rows_int8(const AveQuantRowsArgs* args, void* stream);
+int ave_dequantize_rows_int8(const AveQuantRowsArgs* args, void* stream);
+
+/* C[m][n] = sum_k A[m][k] B[n][k] * a_scale[m] * b_scale[n] + bias[n]: int8 A and B, exact sums (1 <= K <= 131071), (sum * a_scale) * b_scale + bias in
+ * fp32 and one rounding.  Rows of A and B lie on 16 bytes; K need not be a multiple of anything.  An expired wait sets AVE_GDN_DEV_WAIT_EXPIRED. */
+typedef struct AveGemmInt8Args {
+  uint32_t struct_size;
+  uint32_t flags;           /* 0 */
+  const void* a;            /* int8 [M, K], row stride lda */
+  const void* b;            /* int8 [N, K], row stride ldb */
+  void* c;                  /* [M, N] of c_dtype, row stride ldc elements */
+  const float* a_scale;     /* fp32 [M] */
+  const float* b_scale;     /* fp32 [N] */
+  const void* bias;         /* [N] of bias_dtype, optional */
+  int64_t M, N, K, lda, ldb, ldc;
+  int32_t c_dtype, bias_dtype; /* AVE_DTYPE_*; bias_dtype: c_dtype or AVE_DTYPE_FP32 */
+  uint32_t* status;         /* optional device status word */
+} AveGemmInt8Args;
+int ave_gemm_int8_nt(const AveGemmInt8Args* args, void* stream);
+
 int ave_gdn_abi_version(void);
 const char* ave_gdn_status_string(int status);
 /* cudaError_t of the most recent failing CUDA call made by this thread through the library (0 if none). */
