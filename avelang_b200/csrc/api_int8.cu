@@ -14,6 +14,7 @@ int launch_gemm_int8_nt(const AveGemmInt8Args& a, cudaStream_t stream);
 namespace {
 
 constexpr int64_t MAX_K = 131071;  // 128 * 128 * K below 2^31
+constexpr int64_t MAX_ROWS = (1ll << 31) - 1024;  // a tile's coordinates are 32-bit
 
 bool dtype_ok(int x) { return x >= AVE_DTYPE_BF16 && x <= AVE_DTYPE_FP32; }
 bool param_ok(int x, int w) { return dtype_ok(x) && (w == x || w == AVE_DTYPE_FP32); }
@@ -85,7 +86,7 @@ int ave_dequantize_rows_int8(const AveQuantRowsArgs* a, void* stream) {
 
 int ave_gemm_int8_nt(const AveGemmInt8Args* a, void* stream) {
   if (a == nullptr || a->struct_size != sizeof(AveGemmInt8Args) || a->M < 0 || a->N < 0 || a->K <= 0 || !param_ok(a->c_dtype, a->bias_dtype)) return AVE_GDN_INVALID_ARGUMENT;
-  if (a->K > MAX_K || a->M > INT32_MAX || a->N > INT32_MAX) return AVE_GDN_UNSUPPORTED;
+  if (a->K > MAX_K || a->M > MAX_ROWS || a->N > MAX_ROWS) return AVE_GDN_UNSUPPORTED;
   if (a->M == 0 || a->N == 0) return AVE_GDN_OK;
   if (!a->a || !a->b || !a->c || !a->a_scale || !a->b_scale) return AVE_GDN_INVALID_ARGUMENT;
   if (a->ldc < a->N && a->M > 1) return AVE_GDN_INVALID_ARGUMENT;

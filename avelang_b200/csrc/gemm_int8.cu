@@ -1,8 +1,9 @@
 // C[M,N] = (A[M,K] * B[N,K]^T) a_scale[m] b_scale[n] + bias[n]: int8 operands, exact int32 sums in tensor memory (kind::i8), one rounding to bf16, fp16
 // or fp32 behind fp32 scaling.  K is at most 131071, so that |sum| <= 128 * 128 * K stays below 2^31.
 //
-// One tile a cluster of `split` CTAs, each of which takes a contiguous share of K (split == 1 where there are tiles enough); the partial sums meet over
-// distributed shared memory.  They are whole numbers: the result does not depend on the split.
+// Two forms.  Many tiles: persistent pairs of CTAs on tiles of 256 x bn (gemm_int8_pair_kernel).  Few tiles: one tile a cluster of `split` CTAs, each of
+// which takes a contiguous share of K; the partial sums meet over distributed shared memory (gemm_int8_cluster_kernel).  Sums are whole numbers and all forms
+// finish them in the same way: a result depends neither on the form nor on the split.
 #include <mutex>
 
 #include "rows.cuh"
@@ -26,6 +27,12 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_
                : "memory");
 }
 
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc),
+               "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+
 struct Epilogue {  // what a sum becomes
   const float *a_scale, *b_scale;
   const void* bias;
@@ -39,6 +46,201 @@ __device__ __forceinline__ float bias_at(const Epilogue& e, int64_t n) { return 
 // (sum * a_scale) * b_scale + bias: a sum of 24 bits and more is rounded to fp32 first, 2^-24 of its value
 __device__ __forceinline__ float finish(int32_t sum, float a_scale, float b_scale, float bias) { return fmaf(__fmul_rn((float)sum, a_scale), b_scale, bias); }
 
+// ------------------------------------------------------------------------------------------------ many tiles
+// A pair of CTAs works on a tile of 256 rows x bn columns (whole chunks of 128 bytes of the result, at most 256): each loads its 128 rows of A and bn / 2 rows of B, the leader issues
+// MMAs of 256 x bn x 32 for both, and each finishes the 128 rows whose sums lie in its tensor memory, in one of two accumulators, while the next tile's products run.
+//   warp 0      TMA producer: a ring of 6 stages of 32 KB; the bytes of both CTAs are counted at the leader's barrier
+//   warp 1      of the leader: MMAs; a stage is free in both CTAs when its products are done
+//   warps 2..5  sums -> fp32 -> result: 32 rows x 128 bytes a warp through shared memory and out as one TMA store, or element by element where the rows of C
+//               do not lie on 16 bytes
+constexpr int PAIR_STAGES = 6, PAIR_STAGE = 2 * BM * BK, PAIR_THREADS = 192, PAIR_ROWS = 2 * BM;
+constexpr int GROUP_M = 8;  // row tiles that are swept together, so that their rows of A stay in L2
+constexpr int PAIR_OUT = PAIR_STAGES * PAIR_STAGE, PAIR_COLS = PAIR_OUT + 4 * 4096, PAIR_SMEM = PAIR_COLS + 4 * 2048 + 1024;
+
+template <class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC, const Epilogue e,
+                      int64_t M, int64_t N, int64_t K, uint32_t* status, int bn) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = tc::align1024(smem_raw);
+  __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile uint32_t abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = tc::cluster_rank();
+  const int mt = (int)((M + PAIR_ROWS - 1) / PAIR_ROWS), nt = (int)((N + bn - 1) / bn), kb_count = (int)((K + BK - 1) / BK);
+  const int64_t tiles = (int64_t)mt * nt, first = blockIdx.x / 2, step = gridDim.x / 2;
+  auto tile_m = [&](int64_t tile, int& m, int& n) {
+    const int64_t group = tile / ((int64_t)GROUP_M * nt);
+    const int r = (int)(tile - group * GROUP_M * nt), rows = min(GROUP_M, mt - (int)group * GROUP_M);
+    m = (int)group * GROUP_M + r % rows;
+    n = r / rows;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < PAIR_STAGES; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], 8); }
+    tc::mbar_init(&drained, 1);
+    abort_flag = 0;
+    tc::fence_barrier_init();
+    tc::prefetch_tmap(&tmA);
+    tc::prefetch_tmap(&tmB);
+  }
+  if (warp == 1) tc::tmem_alloc_pair(&tmem_slot, 512);
+  tc::tc_fence_before_sync();
+  __syncthreads();
+  tc::cluster_sync();  // both CTAs' barriers are there
+  tc::tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    const uint32_t stage_bytes = (uint32_t)((BM + bn / 2) * BK);
+    int s = 0; uint32_t ph = 0;
+    int64_t turns = 0;
+    bool ok = true;
+    for (int64_t tile = first; tile < tiles && ok; tile += step) {
+      int m, n;
+      tile_m(tile, m, n);
+      for (int kb = 0; kb < kb_count; ++kb) {
+        if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+        if (tc::elect_one()) {
+          uint8_t* st = smem + s * PAIR_STAGE;
+          const uint32_t bar = tc::mapa(tc::smem_u32(&full[s]), 0);
+          if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * stage_bytes);
+          tc::tma_load_2d_pair(st, &tmA, bar, kb * BK, m * PAIR_ROWS + (int)rank * BM);
+          tc::tma_load_2d_pair(st + BM * BK, &tmB, bar, kb * BK, n * bn + (int)rank * (bn / 2));
+        }
+        __syncwarp();
+        ++turns;
+        if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (ok)  // the leader's last arrivals at this CTA's barriers
+      for (int i = 0; i < PAIR_STAGES && i < turns; ++i) {
+        if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) break;
+        if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+      }
+    else if (rank == 0)  // copies may be on their way: those of both CTAs are counted here
+      for (int64_t i = turns > PAIR_STAGES ? turns - PAIR_STAGES : 0; i < turns; ++i) tc::drain(&full[i % PAIR_STAGES], (uint32_t)(i / PAIR_STAGES) & 1u);
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint32_t idesc = idesc_i8(PAIR_ROWS, bn);
+      int s = 0, local = 0; uint32_t ph = 0;
+      bool ok = true;
+      for (int64_t tile = first; tile < tiles; tile += step, ++local) {
+        const int buf = local & 1;
+        if (!tc::mbar_wait_cluster(&acc_empty[buf], ((uint32_t)(local >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
+        tc::tc_fence_after_sync();
+        const uint32_t d = tmem_base + (uint32_t)buf * BN;
+        for (int kb = 0; kb < kb_count; ++kb) {
+          if (!tc::mbar_wait_unrolled(&full[s], ph, &abort_flag)) { ok = false; break; }
+          tc::tc_fence_after_sync();
+          if (tc::elect_one()) {
+            const uint32_t a_addr = tc::smem_u32(smem + s * PAIR_STAGE);
+            const uint64_t da = tc::smem_desc_sw128(a_addr, 16, 1024), db = tc::smem_desc_sw128(a_addr + BM * BK, 16, 1024);
+#pragma unroll
+            for (int k = 0; k < BK / 32; ++k) mma_i8_pair(d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (kb | k) != 0 ? 1u : 0u);
+            tc::mma_commit_pair(&empty[s]);
+          }
+          __syncwarp();
+          if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+        }
+        if (!ok) break;
+        if (tc::elect_one()) tc::mma_commit_pair(&acc_full[buf]);
+        __syncwarp();
+      }
+      if (!ok) {
+        if (tc::elect_one()) tc::mma_commit_pair(&drained);
+        __syncwarp();
+        tc::drain(&drained, 0u);
+      }
+    }
+  } else {
+    const int quarter = warp & 3;  // tensor memory lanes this warp may touch
+    constexpr int V = rows::kVec<T>, CW = 128 / (int)sizeof(T);  // columns a chunk
+    uint8_t* out = smem + PAIR_OUT + quarter * 4096;
+    float* cols = reinterpret_cast<float*>(smem + PAIR_COLS) + quarter * 512;  // [256] scales, [256] bias
+    int local = 0;
+    for (int64_t tile = first; tile < tiles; tile += step, ++local) {
+      int m, n;
+      tile_m(tile, m, n);
+      const int buf = local & 1;
+      const int64_t row0 = (int64_t)m * PAIR_ROWS + rank * BM + quarter * 32, col0 = (int64_t)n * bn;
+      const int n_left = (int)min((int64_t)bn, N - col0);
+      __syncwarp();
+      for (int c = lane; c < n_left; c += 32) {
+        cols[c] = e.b_scale[col0 + c];
+        cols[256 + c] = bias_at<T>(e, col0 + c);
+      }
+      const float a_scale = row0 + lane < M ? e.a_scale[row0 + lane] : 0.f;
+      __syncwarp();
+      if (!tc::mbar_wait_unrolled(&acc_full[buf], (uint32_t)(local >> 1) & 1u, &abort_flag)) break;
+      tc::tc_fence_after_sync();
+#pragma unroll 1
+      for (int c = 0; c < n_left; c += CW) {
+        uint4 packed[8];  // a row's 128 bytes
+#pragma unroll
+        for (int part = 0; part < CW; part += 32) {
+          uint32_t r[32];
+          tc::tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + c + part), r);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int v = 0; v < 32; v += V) {
+            float2 f[V / 2];
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+              const float4 sc = *reinterpret_cast<const float4*>(cols + c + part + v + i), bi = *reinterpret_cast<const float4*>(cols + 256 + c + part + v + i);
+              f[i / 2] = make_float2(finish((int32_t)r[v + i], a_scale, sc.x, bi.x), finish((int32_t)r[v + i + 1], a_scale, sc.y, bi.y));
+              f[i / 2 + 1] = make_float2(finish((int32_t)r[v + i + 2], a_scale, sc.z, bi.z), finish((int32_t)r[v + i + 3], a_scale, sc.w, bi.w));
+            }
+            packed[(part + v) / V] = rows::narrow<T>(f);
+          }
+        }
+        if (c + CW >= n_left) {  // the accumulator is out of tensor memory
+          tc::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_cluster(tc::mapa(tc::smem_u32(&acc_empty[buf]), 0));
+        }
+        if (lane == 0) tc::bulk_wait_read<0>();  // the chunk before has left
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(out + lane * 128 + ((j ^ (lane & 7)) << 4)) = packed[j];
+        if (e.vector != 0 && (c + CW <= n_left || n_left % V == 0)) {  // (a store writes whole 16 bytes: also those that begin inside the tensor and end behind it)
+          tc::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < M) {
+            tc::tma_store_2d(&tmC, out, (int)col0 + c, (int)row0);
+            tc::bulk_commit();
+          }
+        } else {
+          __syncwarp();
+          const int live = (int)max((int64_t)0, min((int64_t)32, M - row0)), width = min(CW, n_left - c);
+          T* dst = reinterpret_cast<T*>(e.c) + row0 * e.ldc + col0 + c;
+#pragma unroll 4
+          for (int i = 0; i < live; ++i)
+#pragma unroll
+            for (int k = lane; k < CW; k += 32)
+              if (k < width) dst[i * e.ldc + k] = *reinterpret_cast<const T*>(out + i * 128 + (((k / V) ^ (i & 7)) << 4) + (k % V) * (int)sizeof(T));
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) tc::bulk_wait_all();
+  }
+
+  __syncwarp();
+  tc::tc_fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0 && abort_flag != 0u && status != nullptr) atomicOr(status, AVE_GDN_DEV_WAIT_EXPIRED);
+  tc::cluster_sync();  // neither CTA ends, or gives tensor memory back, while the other may reach it
+  if (warp == 1) {
+    tc::tc_fence_after_sync();
+    tc::tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ few tiles
 struct Plan { int bn, split, stages, ks, a_rows; };  // tile width, CTAs a tile, ring depth, blocks of 128 a stage, rows of A
 
 template <class T>
@@ -256,6 +458,40 @@ int operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int
   return make_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, const_cast<void*>(base), 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Width of the pairs' column tiles, whole chunks of the results' 128 bytes: the one with the least time, in columns, of the busiest pair
+int pair_width(int64_t M, int64_t N, int pairs, int chunk) {
+  const int64_t mt = (M + PAIR_ROWS - 1) / PAIR_ROWS;
+  int best = BN;
+  int64_t best_cost = INT64_MAX;
+  for (int bn = BN; bn >= 128; bn -= chunk) {
+    const int64_t nt = (N + bn - 1) / bn, cost = (mt * nt + pairs - 1) / pairs * bn;
+    if (cost < best_cost) { best_cost = cost; best = bn; }
+  }
+  return best;
+}
+template <class T>
+int launch_pairs(const AveGemmInt8Args& a, const Epilogue& e, int pairs, cudaStream_t stream) {
+  const int bn = pair_width(a.M, a.N, pairs, 128 / (int)sizeof(T));
+  CUtensorMap tmA, tmB, tmC{};
+  int rc = operand_map(&tmA, a.a, a.M, a.K, a.lda, BM);
+  if (rc != AVE_GDN_OK) return rc;
+  rc = operand_map(&tmB, a.b, a.N, a.K, a.ldb, bn / 2);
+  if (rc != AVE_GDN_OK) return rc;
+  if (e.vector != 0) {
+    const uint64_t size = sizeof(T), dims[2] = {(uint64_t)a.N, (uint64_t)a.M}, strides[2] = {size, (uint64_t)a.ldc * size};
+    const uint32_t box[2] = {128 / (uint32_t)sizeof(T), 32};
+    const CUtensorMapDataType dt = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    rc = make_tmap(&tmC, dt, (int)size, a.c, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != AVE_GDN_OK) return rc;
+  }
+  constexpr auto* kernel = &gemm_int8_pair_kernel<T>;
+  rc = allow_smem<kernel>(PAIR_SMEM);
+  if (rc != AVE_GDN_OK) return rc;
+  const int64_t tiles = ((a.M + PAIR_ROWS - 1) / PAIR_ROWS) * ((a.N + bn - 1) / bn);
+  AVE_CUDA_TRY(launch_after(kernel, (unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, PAIR_SMEM, stream, tmA, tmB, tmC, e, a.M, a.N, a.K, a.status, bn));
+  return AVE_GDN_OK;
+}
+
 template <class T>
 int launch_t(const AveGemmInt8Args& a, cudaStream_t stream) {
   int dev = 0, sms = 148;
@@ -265,6 +501,9 @@ int launch_t(const AveGemmInt8Args& a, cudaStream_t stream) {
   const Epilogue e{a.a_scale, a.b_scale, a.bias, a.c, a.ldc, a.bias_dtype == AVE_DTYPE_FP32, aligned16(a.c) && rows::on16(a.ldc, size)};
   const int* clusters = cluster_counts(dev, sms);
   if (clusters == nullptr) return AVE_GDN_UNSUPPORTED;
+  const int pairs = clusters[2];
+  const int64_t mt = (a.M + PAIR_ROWS - 1) / PAIR_ROWS, nt = (a.N + BN - 1) / BN;
+  if (a.M > BM && mt * nt >= pairs) return launch_pairs<T>(a, e, pairs, stream);
   const Plan plan = make_plan(a.M, a.N, a.K, sms, clusters);
   CUtensorMap tmA, tmB;
   int rc = operand_map(&tmA, a.a, a.M, a.K, a.lda, plan.a_rows);

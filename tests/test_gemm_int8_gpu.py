@@ -40,7 +40,8 @@ def make(m, n, k, seed, dt, bias):
 
 
 SIZES = [(1, 1, 1), (1, 16, 16), (1, 12352, 2048), (2, 130, 33), (3, 1544, 2048), (4, 100, 8192), (5, 7, 100), (8, 2048, 4096), (9, 257, 640), (16, 4096, 512), (17, 12352, 256), (33, 48, 1000),
-         (64, 2048, 4096), (100, 1544, 127), (128, 256, 128), (129, 255, 129), (200, 12352, 384), (256, 512, 2048), (300, 1000, 1999), (1000, 1544, 200), (1003, 4104, 96), (2500, 300, 72), (4096, 2048, 256)]
+         (64, 2048, 4096), (100, 1544, 127), (128, 256, 128), (129, 255, 129), (200, 12352, 384), (256, 512, 2048), (300, 1000, 1999), (1000, 1544, 200), (1003, 4104, 96), (2500, 300, 72), (4096, 2048, 256), (2900, 2571, 100),
+         (5000, 1032, 513), (257, 20000, 64), (130, 19003, 1000), (10000, 1540, 33)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -62,7 +63,7 @@ def test_product(built_lib, m, n, k):
 def test_largest_sums(built_lib):
     """All operands at their lowest value, K at its limit: sums of 128 * 128 * 131071, just below 2^31."""
     from avelang_b200 import gemm
-    for m, n, k in ((3, 20, 131071), (130, 40, 131071), (20, 600, 100003)):
+    for m, n, k in ((3, 20, 131071), (130, 40, 131071), (20, 600, 100003), (1030, 4000, 131071)):
         pitch = -(-k // 16) * 16
         aq, bq = torch.full((m, pitch), -128, dtype=torch.int8), torch.full((n, pitch), -128, dtype=torch.int8)
         bq[n // 2] = 127
@@ -76,15 +77,15 @@ def test_largest_sums(built_lib):
 def test_rows_are_the_same_in_any_batch(built_lib):
     """A token's result does not depend on the batch that it is in."""
     from avelang_b200 import gemm
-    aq, a, bq, b, sa, sb, bb = make(2000, 1544, 1000, 3, "bf16", "wide")
+    aq, a, bq, b, sa, sb, bb = make(4000, 1544, 1000, 3, "bf16", "wide")
     A, B, sa, sb, bb = device_rows(aq, 1000), device_rows(bq, 1000), sa.cuda(), sb.cuda(), bb.cuda()
     whole = gemm.gemm_int8_transposed_b(A, B, sa, sb, bb)
-    for lo, hi in ((0, 1), (5, 7), (100, 103), (300, 308), (17, 33), (1000, 1064), (700, 828), (60, 360), (1, 1100)):
+    for lo, hi in ((0, 1), (5, 7), (100, 103), (300, 308), (17, 33), (1000, 1064), (700, 828), (60, 360), (1, 1100), (0, 3000)):
         assert torch.equal(gemm.gemm_int8_transposed_b(A[lo:hi], B, sa[lo:hi], sb, bb), whole[lo:hi])
 
 
 @pytest.mark.parametrize("dt", list(DT))
-@pytest.mark.parametrize("m,n", [(1, 100), (5, 333), (70, 264), (300, 1000), (3000, 520)])
+@pytest.mark.parametrize("m,n", [(1, 100), (5, 333), (70, 264), (300, 1000), (3000, 520), (9000, 600), (3000, 2001)])
 def test_results_in_a_wider_tensor(built_lib, m, n, dt):
     """Results whose rows lie apart, on 16 bytes and off them; what lies beside them stays as it was."""
     from avelang_b200 import gemm
@@ -102,7 +103,7 @@ def test_results_in_a_wider_tensor(built_lib, m, n, dt):
 def test_what_lies_behind_a_row_is_not_read_into_it(built_lib):
     """Rows of 33 of 48 bytes: the 15 behind them hold something else, and so does what lies behind the last row of A and B."""
     from avelang_b200 import gemm
-    for m, n, k in ((3, 50, 33), (40, 500, 33), (200, 3000, 250)):
+    for m, n, k in ((3, 50, 33), (40, 500, 33), (200, 3000, 250), (2600, 2050, 33)):
         aq, a, bq, b, sa, sb, _ = make(m, n, k, k, "fp32", None)
         outs = []
         for fill in (0, 77):
@@ -119,7 +120,7 @@ def test_what_lies_behind_a_row_is_not_read_into_it(built_lib):
 def test_scales(built_lib):
     """Scales of zero, NaN, infinity and of very different size; a NaN stays in its row or column."""
     from avelang_b200 import gemm
-    for m in (4, 40, 400):
+    for m in (4, 40, 400, 20000):
         aq, a, bq, b, sa, sb, _ = make(m, 300, 64, m, "fp32", None)
         plain = gemm.gemm_int8_transposed_b(device_rows(aq, 64), device_rows(bq, 64), sa.cuda(), sb.cuda(), out_dtype=torch.float32).cpu()
         sa[1], sa[2], sb[5], sb[7] = 0.0, float("nan"), float("nan"), 0.0
@@ -172,7 +173,7 @@ def test_captured_and_on_other_streams(built_lib):
     """Products of every size captured into two graphs, replayed in turn on new operands, beside eager calls on a stream of their own."""
     from avelang_b200 import gdn, gemm, norm
     gen = torch.Generator().manual_seed(2)
-    sizes = [(1, 512, 300), (64, 2048, 512), (700, 3000, 128)]
+    sizes = [(1, 512, 300), (64, 2048, 512), (700, 3000, 128), (2600, 2050, 200)]
     sets = [[torch.randn(m, k, generator=gen).bfloat16().cuda(), torch.randn(m, k, generator=gen).bfloat16().cuda(), *gemm.quantize_rows_int8(torch.randn(n, k, generator=gen).cuda())] for m, n, k in sizes]
 
     def step(x, res, wq, ws):
