@@ -49,13 +49,13 @@ __device__ __forceinline__ float finish(int32_t sum, float a_scale, float b_scal
 // ------------------------------------------------------------------------------------------------ many tiles
 // A pair of CTAs works on a tile of 256 rows x bn columns (whole chunks of 128 bytes of the result, at most 256): each loads its 128 rows of A and bn / 2 rows of B, the leader issues
 // MMAs of 256 x bn x 32 for both, and each finishes the 128 rows whose sums lie in its tensor memory, in one of two accumulators, while the next tile's products run.
-//   warp 0      TMA producer: a ring of 6 stages of 32 KB; the bytes of both CTAs are counted at the leader's barrier
+//   warp 0      TMA producer: a ring of 5 stages of 32 KB; the bytes of both CTAs are counted at the leader's barrier
 //   warp 1      of the leader: MMAs; a stage is free in both CTAs when its products are done
-//   warps 2..5  sums -> fp32 -> result: 32 rows x 128 bytes a warp through shared memory and out as one TMA store, or element by element where the rows of C
-//               do not lie on 16 bytes
-constexpr int PAIR_STAGES = 6, PAIR_STAGE = 2 * BM * BK, PAIR_THREADS = 192, PAIR_ROWS = 2 * BM;
-constexpr int GROUP_M = 8;  // row tiles that are swept together, so that their rows of A stay in L2
-constexpr int PAIR_OUT = PAIR_STAGES * PAIR_STAGE, PAIR_COLS = PAIR_OUT + 4 * 4096, PAIR_SMEM = PAIR_COLS + 4 * 2048 + 1024;
+//   warps 2..9  sums -> fp32 -> result, two warps a quarter of the rows, every other chunk of 128 bytes each: 32 rows of it through shared memory and out as one
+//               TMA store, or element by element where the rows of C do not lie on 16 bytes
+constexpr int PAIR_STAGES = 5, PAIR_STAGE = 2 * BM * BK, PAIR_THREADS = 320, PAIR_ROWS = 2 * BM;
+constexpr int GROUP_M = 16;  // row tiles that are swept together, so that their rows of A stay in L2
+constexpr int PAIR_OUT = PAIR_STAGES * PAIR_STAGE, PAIR_COLS = PAIR_OUT + 8 * 4096, PAIR_SMEM = PAIR_COLS + 8 * 1024 + 1024;
 
 template <class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
@@ -69,17 +69,16 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_rank();
   const int mt = (int)((M + PAIR_ROWS - 1) / PAIR_ROWS), nt = (int)((N + bn - 1) / bn), kb_count = (int)((K + BK - 1) / BK);
-  const int64_t tiles = (int64_t)mt * nt, first = blockIdx.x / 2, step = gridDim.x / 2;
-  auto tile_m = [&](int64_t tile, int& m, int& n) {
-    const int64_t group = tile / ((int64_t)GROUP_M * nt);
-    const int r = (int)(tile - group * GROUP_M * nt), rows = min(GROUP_M, mt - (int)group * GROUP_M);
-    m = (int)group * GROUP_M + r % rows;
-    n = r / rows;
+  const uint32_t tiles = (uint32_t)mt * (uint32_t)nt, first = blockIdx.x / 2, step = gridDim.x / 2;
+  auto tile_at = [&](uint32_t tile, int& m, int& n) {
+    const uint32_t per = (uint32_t)(GROUP_M * nt), group = tile / per, r = tile - group * per, rows = min((uint32_t)GROUP_M, (uint32_t)mt - group * GROUP_M);
+    n = (int)(r / rows);
+    m = (int)(group * GROUP_M + r - (uint32_t)n * rows);
   };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < PAIR_STAGES; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], 8); }
+    for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], 16); }
     tc::mbar_init(&drained, 1);
     abort_flag = 0;
     tc::fence_barrier_init();
@@ -99,9 +98,9 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     int s = 0; uint32_t ph = 0;
     int64_t turns = 0;
     bool ok = true;
-    for (int64_t tile = first; tile < tiles && ok; tile += step) {
+    for (uint32_t tile = first; tile < tiles && ok; tile += step) {
       int m, n;
-      tile_m(tile, m, n);
+      tile_at(tile, m, n);
       for (int kb = 0; kb < kb_count; ++kb) {
         if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
         if (tc::elect_one()) {
@@ -128,7 +127,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       const uint32_t idesc = idesc_i8(PAIR_ROWS, bn);
       int s = 0, local = 0; uint32_t ph = 0;
       bool ok = true;
-      for (int64_t tile = first; tile < tiles; tile += step, ++local) {
+      for (uint32_t tile = first; tile < tiles; tile += step, ++local) {
         const int buf = local & 1;
         if (!tc::mbar_wait_cluster(&acc_empty[buf], ((uint32_t)(local >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
         tc::tc_fence_after_sync();
@@ -159,48 +158,66 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   } else {
     const int quarter = warp & 3;  // tensor memory lanes this warp may touch
     constexpr int V = rows::kVec<T>, CW = 128 / (int)sizeof(T);  // columns a chunk
-    uint8_t* out = smem + PAIR_OUT + quarter * 4096;
-    float* cols = reinterpret_cast<float*>(smem + PAIR_COLS) + quarter * 512;  // [256] scales, [256] bias
+    const int half = (warp - 2) >> 2;  // which chunks
+    uint8_t* out = smem + PAIR_OUT + (warp - 2) * 4096;
+    float* cols = reinterpret_cast<float*>(smem + PAIR_COLS) + (warp - 2) * 256;  // scales and bias of this warp's columns, CW of a chunk behind those of the one before
+    // The scales of a tile are fetched while the one before is finished (fetched and waited for in line they took 1600 to 1900 cycles a tile).
+    float next_scale[4], next_bias[4], next_a = 0.f;
+    int next_m = 0, next_n = 0;
+    auto prefetch = [&](uint32_t tile) {
+      if (tile >= tiles) return;
+      tile_at(tile, next_m, next_n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = lane + 32 * j;
+        const int64_t c = (int64_t)next_n * bn + (i / CW * 2 + half) * CW + i % CW;
+        next_scale[j] = c < N ? e.b_scale[c] : 0.f;
+        next_bias[j] = c < N ? bias_at<T>(e, c) : 0.f;
+      }
+      const int64_t row = (int64_t)next_m * PAIR_ROWS + rank * BM + quarter * 32 + lane;
+      next_a = row < M ? e.a_scale[row] : 0.f;
+    };
+    prefetch(first);
     int local = 0;
-    for (int64_t tile = first; tile < tiles; tile += step, ++local) {
-      int m, n;
-      tile_m(tile, m, n);
-      const int buf = local & 1;
+    for (uint32_t tile = first; tile < tiles; tile += step, ++local) {
+      const int m = next_m, n = next_n, buf = local & 1;
       const int64_t row0 = (int64_t)m * PAIR_ROWS + rank * BM + quarter * 32, col0 = (int64_t)n * bn;
       const int n_left = (int)min((int64_t)bn, N - col0);
       __syncwarp();
-      for (int c = lane; c < n_left; c += 32) {
-        cols[c] = e.b_scale[col0 + c];
-        cols[256 + c] = bias_at<T>(e, col0 + c);
-      }
-      const float a_scale = row0 + lane < M ? e.a_scale[row0 + lane] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { cols[lane + 32 * j] = next_scale[j]; cols[128 + lane + 32 * j] = next_bias[j]; }
+      const float a_scale = next_a;
       __syncwarp();
+      prefetch(tile + step);
       if (!tc::mbar_wait_unrolled(&acc_full[buf], (uint32_t)(local >> 1) & 1u, &abort_flag)) break;
       tc::tc_fence_after_sync();
+      auto release = [&] {  // this warp's part of the accumulator is out of tensor memory
+        tc::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_cluster(tc::mapa(tc::smem_u32(&acc_empty[buf]), 0));
+      };
+      if (half * CW >= n_left) release();  // (a narrow last tile)
 #pragma unroll 1
-      for (int c = 0; c < n_left; c += CW) {
+      for (int c = half * CW, at = 0; c < n_left; c += 2 * CW, at += CW) {
+        uint32_t r[CW];
+#pragma unroll
+        for (int part = 0; part < CW; part += 32)
+          tc::tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + c + part), *reinterpret_cast<uint32_t(*)[32]>(r + part));
+        tc::tmem_ld_wait();
+        if (c + 2 * CW >= n_left) release();
         uint4 packed[8];  // a row's 128 bytes
 #pragma unroll
-        for (int part = 0; part < CW; part += 32) {
-          uint32_t r[32];
-          tc::tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + c + part), r);
-          tc::tmem_ld_wait();
+        for (int v = 0; v < CW; v += V) {
+          float2 f[V / 2];
 #pragma unroll
-          for (int v = 0; v < 32; v += V) {
-            float2 f[V / 2];
-#pragma unroll
-            for (int i = 0; i < V; i += 4) {
-              const float4 sc = *reinterpret_cast<const float4*>(cols + c + part + v + i), bi = *reinterpret_cast<const float4*>(cols + 256 + c + part + v + i);
-              f[i / 2] = make_float2(finish((int32_t)r[v + i], a_scale, sc.x, bi.x), finish((int32_t)r[v + i + 1], a_scale, sc.y, bi.y));
-              f[i / 2 + 1] = make_float2(finish((int32_t)r[v + i + 2], a_scale, sc.z, bi.z), finish((int32_t)r[v + i + 3], a_scale, sc.w, bi.w));
-            }
-            packed[(part + v) / V] = rows::narrow<T>(f);
+          for (int i = 0; i < V; i += 4) {
+            const float4 sc = *reinterpret_cast<const float4*>(cols + at + v + i), bi = *reinterpret_cast<const float4*>(cols + 128 + at + v + i);
+            const float2 x = __fmul2_rn(make_float2((float)(int32_t)r[v + i], (float)(int32_t)r[v + i + 1]), rows::splat(a_scale));
+            const float2 y = __fmul2_rn(make_float2((float)(int32_t)r[v + i + 2], (float)(int32_t)r[v + i + 3]), rows::splat(a_scale));
+            f[i / 2] = __ffma2_rn(x, make_float2(sc.x, sc.y), make_float2(bi.x, bi.y));
+            f[i / 2 + 1] = __ffma2_rn(y, make_float2(sc.z, sc.w), make_float2(bi.z, bi.w));
           }
-        }
-        if (c + CW >= n_left) {  // the accumulator is out of tensor memory
-          tc::tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive_cluster(tc::mapa(tc::smem_u32(&acc_empty[buf]), 0));
+          packed[v / V] = rows::narrow<T>(f);
         }
         if (lane == 0) tc::bulk_wait_read<0>();  // the chunk before has left
         __syncwarp();
@@ -213,15 +230,35 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             tc::tma_store_2d(&tmC, out, (int)col0 + c, (int)row0);
             tc::bulk_commit();
           }
-        } else {
+        } else {  // rows wherever they lie: a word a lane, 16-bit types as the aligned pairs of a row and what is left at its ends
           __syncwarp();
           const int live = (int)max((int64_t)0, min((int64_t)32, M - row0)), width = min(CW, n_left - c);
           T* dst = reinterpret_cast<T*>(e.c) + row0 * e.ldc + col0 + c;
-#pragma unroll 4
-          for (int i = 0; i < live; ++i)
+          const bool odd0 = ((reinterpret_cast<uintptr_t>(dst) >> 1) & 1) != 0, flip = (e.ldc & 1) != 0;
+          const uint32_t place = (uint32_t)(((lane >> 2) << 4) + (lane & 3) * 4);
+#pragma unroll 1
+          for (int i0 = 0; i0 < live; i0 += 8, dst += 8 * e.ldc) {
+            uint32_t w[8];  // (loads and stores of eight rows apart: one behind the other they wait for each other)
 #pragma unroll
-            for (int k = lane; k < CW; k += 32)
-              if (k < width) dst[i * e.ldc + k] = *reinterpret_cast<const T*>(out + i * 128 + (((k / V) ^ (i & 7)) << 4) + (k % V) * (int)sizeof(T));
+            for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const uint32_t*>(out + (i0 + j) * 128 + (place ^ (uint32_t)(j << 4)));
+            T* to = dst;
+#pragma unroll
+            for (int j = 0; j < 8; ++j, to += e.ldc) {
+              if constexpr (sizeof(T) == 4) {
+                if (lane < width && i0 + j < live) *reinterpret_cast<uint32_t*>(to + lane) = w[j];
+              } else {
+                const uint32_t behind = __shfl_down_sync(0xffffffffu, w[j], 1);
+                const bool odd = odd0 != (flip && (j & 1) != 0);
+                const int k = 2 * lane + (odd ? 1 : 0);
+                const uint32_t v = __byte_perm(w[j], behind, odd ? 0x5432 : 0x3210);
+                if (i0 + j < live) {
+                  if (k + 1 < width) *reinterpret_cast<uint32_t*>(to + k) = v;
+                  const bool begin = odd && lane == 0;
+                  if (begin || k + 1 == width) *reinterpret_cast<uint16_t*>(to + (begin ? 0 : k)) = (uint16_t)(begin ? w[j] : v);
+                }
+              }
+            }
+          }
           __syncwarp();
         }
       }
@@ -464,7 +501,7 @@ int pair_width(int64_t M, int64_t N, int pairs, int chunk) {
   int best = BN;
   int64_t best_cost = INT64_MAX;
   for (int bn = BN; bn >= 128; bn -= chunk) {
-    const int64_t nt = (N + bn - 1) / bn, cost = (mt * nt + pairs - 1) / pairs * bn;
+    const int64_t nt = (N + bn - 1) / bn, cost = (mt * nt + pairs - 1) / pairs * (bn + 128);
     if (cost < best_cost) { best_cost = cost; best = bn; }
   }
   return best;
@@ -488,6 +525,7 @@ int launch_pairs(const AveGemmInt8Args& a, const Epilogue& e, int pairs, cudaStr
   rc = allow_smem<kernel>(PAIR_SMEM);
   if (rc != AVE_GDN_OK) return rc;
   const int64_t tiles = ((a.M + PAIR_ROWS - 1) / PAIR_ROWS) * ((a.N + bn - 1) / bn);
+  if (tiles > INT32_MAX) return AVE_GDN_UNSUPPORTED;
   AVE_CUDA_TRY(launch_after(kernel, (unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, PAIR_SMEM, stream, tmA, tmB, tmC, e, a.M, a.N, a.K, a.status, bn));
   return AVE_GDN_OK;
 }

@@ -291,9 +291,10 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
                : "memory");
 }
-// an arrival at a barrier of another CTA (an address of the cluster's window), and a bounded wait that sees what was done in front of such arrivals
+// An arrival at a barrier of another CTA (an address of the cluster's window) that says that this thread's tcgen05 operations are done: it publishes nothing that
+// was written to memory.  (With release.cluster it waited for the thread's loads on their way as well, several hundred cycles.)  And a bounded wait for such arrivals.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
   for (uint32_t it = 0; it < kWaitLimit; ++it) {
