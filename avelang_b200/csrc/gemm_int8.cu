@@ -1,10 +1,12 @@
 // C[M,N] = (A[M,K] * B[N,K]^T) a_scale[m] b_scale[n] + bias[n]: int8 operands, exact int32 sums in tensor memory (kind::i8), one rounding to bf16, fp16
 // or fp32 behind fp32 scaling.  K is at most 131071, so that |sum| <= 128 * 128 * K stays below 2^31.
 //
-// Two forms.  Many tiles: persistent pairs of CTAs on tiles of 256 x bn (gemm_int8_pair_kernel).  Few tiles: one tile a cluster of `split` CTAs, each of
-// which takes a contiguous share of K; the partial sums meet over distributed shared memory (gemm_int8_cluster_kernel).  Sums are whole numbers and all forms
+// Three forms.  Persistent pairs of CTAs on tiles of 256 x bn (gemm_int8_pair_kernel).  Few rows: one tile of up to 128 rows a cluster of `split` CTAs, each of
+// which takes a contiguous share of K; the partial sums meet over distributed shared memory (gemm_int8_cluster_kernel).  One to four rows: B streamed through the
+// ordinary units (gemm_int8_stream_kernel).  Sums are whole numbers and all forms
 // finish them in the same way: a result depends neither on the form nor on the split.
 #include <mutex>
+#include <type_traits>
 
 #include "rows.cuh"
 #include "tc.cuh"
@@ -46,21 +48,21 @@ __device__ __forceinline__ float bias_at(const Epilogue& e, int64_t n) { return 
 // (sum * a_scale) * b_scale + bias: a sum of 24 bits and more is rounded to fp32 first, 2^-24 of its value
 __device__ __forceinline__ float finish(int32_t sum, float a_scale, float b_scale, float bias) { return fmaf(__fmul_rn((float)sum, a_scale), b_scale, bias); }
 
-// ------------------------------------------------------------------------------------------------ many tiles
+// ------------------------------------------------------------------------------------------------ pairs of CTAs
 // A pair of CTAs works on a tile of 256 rows x bn columns (whole chunks of 128 bytes of the result, at most 256): each loads its 128 rows of A and bn / 2 rows of B, the leader issues
 // MMAs of 256 x bn x 32 for both, and each finishes the 128 rows whose sums lie in its tensor memory, in one of two accumulators, while the next tile's products run.
-//   warp 0      TMA producer: a ring of 5 stages of 32 KB; the bytes of both CTAs are counted at the leader's barrier
+//   warp 0      TMA producer: a ring of stages of 128 bytes of K, 5 of 32 KB with 256 columns, 9 with 64; the bytes of both CTAs are counted at the leader's barrier
 //   warp 1      of the leader: MMAs; a stage is free in both CTAs when its products are done
 //   warps 2..9  sums -> fp32 -> result, two warps a quarter of the rows, every other chunk of 128 bytes each: 32 rows of it through shared memory and out as one
 //               TMA store, or element by element where the rows of C do not lie on 16 bytes
-constexpr int PAIR_STAGES = 5, PAIR_STAGE = 2 * BM * BK, PAIR_THREADS = 320, PAIR_ROWS = 2 * BM;
+constexpr int PAIR_STAGES = 9, PAIR_RING = 184 * 1024, PAIR_THREADS = 320, PAIR_ROWS = 2 * BM;  // ring: depth limit and bytes of a CTA
 constexpr int GROUP_M = 16;  // row tiles that are swept together, so that their rows of A stay in L2
-constexpr int PAIR_OUT = PAIR_STAGES * PAIR_STAGE, PAIR_COLS = PAIR_OUT + 8 * 4096, PAIR_SMEM = PAIR_COLS + 8 * 1024 + 1024;
+constexpr int PAIR_OUT = PAIR_RING, PAIR_COLS = PAIR_OUT + 8 * 4096, PAIR_SMEM = PAIR_COLS + 8 * 1024 + 1024;
 
-template <class T>
+template <class T, int KS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC, const Epilogue e,
-                      int64_t M, int64_t N, int64_t K, uint32_t* status, int bn) {
+                      int64_t M, int64_t N, int64_t K, uint32_t* status, int bn, int stages) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = tc::align1024(smem_raw);
   __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], drained;
@@ -68,7 +70,8 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   __shared__ volatile uint32_t abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_rank();
-  const int mt = (int)((M + PAIR_ROWS - 1) / PAIR_ROWS), nt = (int)((N + bn - 1) / bn), kb_count = (int)((K + BK - 1) / BK);
+  const int mt = (int)((M + PAIR_ROWS - 1) / PAIR_ROWS), nt = (int)((N + bn - 1) / bn), kb_count = (int)((K + KS * BK - 1) / (KS * BK));  // in stages of KS blocks
+  const uint32_t b_bytes = (uint32_t)(bn / 2 * BK), stage_bytes = KS * (BM * BK + b_bytes);
   const uint32_t tiles = (uint32_t)mt * (uint32_t)nt, first = blockIdx.x / 2, step = gridDim.x / 2;
   auto tile_at = [&](uint32_t tile, int& m, int& n) {
     const uint32_t per = (uint32_t)(GROUP_M * nt), group = tile / per, r = tile - group * per, rows = min((uint32_t)GROUP_M, (uint32_t)mt - group * GROUP_M);
@@ -77,7 +80,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < PAIR_STAGES; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
+    for (int s = 0; s < stages; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
     for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], 16); }
     tc::mbar_init(&drained, 1);
     abort_flag = 0;
@@ -94,7 +97,6 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   pdl_wait();
 
   if (warp == 0) {
-    const uint32_t stage_bytes = (uint32_t)((BM + bn / 2) * BK);
     int s = 0; uint32_t ph = 0;
     int64_t turns = 0;
     bool ok = true;
@@ -104,27 +106,31 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       for (int kb = 0; kb < kb_count; ++kb) {
         if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
         if (tc::elect_one()) {
-          uint8_t* st = smem + s * PAIR_STAGE;
+          uint8_t* st = smem + s * (int)stage_bytes;
           const uint32_t bar = tc::mapa(tc::smem_u32(&full[s]), 0);
           if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * stage_bytes);
-          tc::tma_load_2d_pair(st, &tmA, bar, kb * BK, m * PAIR_ROWS + (int)rank * BM);
-          tc::tma_load_2d_pair(st + BM * BK, &tmB, bar, kb * BK, n * bn + (int)rank * (bn / 2));
+#pragma unroll
+          for (int j = 0; j < KS; ++j) {
+            tc::tma_load_2d_pair(st + j * BM * BK, &tmA, bar, (kb * KS + j) * BK, m * PAIR_ROWS + (int)rank * BM);
+            tc::tma_load_2d_pair(st + KS * BM * BK + j * (int)b_bytes, &tmB, bar, (kb * KS + j) * BK, n * bn + (int)rank * (bn / 2));
+          }
         }
         __syncwarp();
         ++turns;
-        if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+        if (++s == stages) { s = 0; ph ^= 1u; }
       }
     }
     if (ok)  // the leader's last arrivals at this CTA's barriers
-      for (int i = 0; i < PAIR_STAGES && i < turns; ++i) {
+      for (int i = 0; i < stages && i < turns; ++i) {
         if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) break;
-        if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+        if (++s == stages) { s = 0; ph ^= 1u; }
       }
     else if (rank == 0)  // copies may be on their way: those of both CTAs are counted here
-      for (int64_t i = turns > PAIR_STAGES ? turns - PAIR_STAGES : 0; i < turns; ++i) tc::drain(&full[i % PAIR_STAGES], (uint32_t)(i / PAIR_STAGES) & 1u);
+      for (int64_t i = turns > stages ? turns - stages : 0; i < turns; ++i) tc::drain(&full[i % stages], (uint32_t)(i / stages) & 1u);
   } else if (warp == 1) {
     if (rank == 0) {
-      const uint32_t idesc = idesc_i8(PAIR_ROWS, bn);
+      const uint32_t idesc = idesc_i8(PAIR_ROWS, bn), stage0 = (tc::smem_u32(smem) >> 4) | (uint32_t)tc::desc_lo(0, 16);
+      constexpr uint32_t hi = tc::desc_hi(1024, true);
       int s = 0, local = 0; uint32_t ph = 0;
       bool ok = true;
       for (uint32_t tile = first; tile < tiles; tile += step, ++local) {
@@ -136,14 +142,17 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           if (!tc::mbar_wait_unrolled(&full[s], ph, &abort_flag)) { ok = false; break; }
           tc::tc_fence_after_sync();
           if (tc::elect_one()) {
-            const uint32_t a_addr = tc::smem_u32(smem + s * PAIR_STAGE);
-            const uint64_t da = tc::smem_desc_sw128(a_addr, 16, 1024), db = tc::smem_desc_sw128(a_addr + BM * BK, 16, 1024);
+            const uint32_t a_lo = stage0 + (uint32_t)s * (stage_bytes >> 4);  // low words of the descriptors; the high ones are constant
 #pragma unroll
-            for (int k = 0; k < BK / 32; ++k) mma_i8_pair(d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (kb | k) != 0 ? 1u : 0u);
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+              for (int k = 0; k < BK / 32; ++k)
+                mma_i8_pair(d, tc::smem_desc(a_lo + (uint32_t)(j * BM * BK / 16 + 2 * k), hi), tc::smem_desc(a_lo + (uint32_t)(KS * BM * BK / 16 + 2 * k) + (uint32_t)j * (b_bytes >> 4), hi), idesc,
+                            (kb | j | k) != 0 ? 1u : 0u);
             tc::mma_commit_pair(&empty[s]);
           }
           __syncwarp();
-          if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+          if (++s == stages) { s = 0; ph ^= 1u; }
         }
         if (!ok) break;
         if (tc::elect_one()) tc::mma_commit_pair(&acc_full[buf]);
@@ -277,8 +286,8 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   }
 }
 
-// ------------------------------------------------------------------------------------------------ few tiles
-struct Plan { int bn, split, stages, ks, a_rows; };  // tile width, CTAs a tile, ring depth, blocks of 128 a stage, rows of A
+// ------------------------------------------------------------------------------------------------ few rows
+struct Plan { int bn, split, stages, ks, a_rows; int64_t cost; };  // tile width, CTAs a tile, ring depth, blocks of 128 a stage, rows of A, bytes (see make_plan)
 
 template <class T>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -292,8 +301,8 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bn = plan.bn, split = plan.split, stages = plan.stages;
   const int a_bytes = plan.a_rows * BK, b_bytes = bn * BK, stage_bytes = plan.ks * (a_bytes + b_bytes);
-  const int nt = (int)((N + bn - 1) / bn), kb_count = (int)((K + plan.ks * BK - 1) / (plan.ks * BK));  // in stages of ks blocks
-  const int rank = (int)(blockIdx.x % split), tile = (int)(blockIdx.x / split), tm = tile / nt, tn = tile % nt;
+  const int kb_count = (int)((K + plan.ks * BK - 1) / (plan.ks * BK));  // in stages of ks blocks
+  const int rank = (int)(blockIdx.x % split), tn = (int)(blockIdx.x / split);
   const int per = (kb_count + split - 1) / split, kb0 = rank * per, kb1 = min(kb_count, kb0 + per);
 
   pdl_trigger();
@@ -324,7 +333,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         uint8_t* st = smem + s * stage_bytes;
         tc::mbar_expect_tx(&full[s], (uint32_t)stage_bytes);
         for (int j = 0; j < plan.ks; ++j) tc::tma_load_2d(st + plan.ks * a_bytes + j * b_bytes, &tmB, &full[s], (kb * plan.ks + j) * BK, tn * bn);
-        for (int j = 0; j < plan.ks; ++j) tc::tma_load_2d(st + j * a_bytes, &tmA, &full[s], (kb * plan.ks + j) * BK, tm * BM);
+        for (int j = 0; j < plan.ks; ++j) tc::tma_load_2d(st + j * a_bytes, &tmA, &full[s], (kb * plan.ks + j) * BK, 0);
       }
       __syncwarp();
       if (++s == stages) { s = 0; ph ^= 1u; }
@@ -365,7 +374,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
   tc::tc_fence_after_sync();
   __syncwarp();
   tc::cluster_sync();  // ... in every CTA of the cluster: the rings may be overwritten
-  const int rows = (int)min((int64_t)BM, M - (int64_t)tm * BM), slice = (rows + split - 1) / split, pitch = bn + 4;
+  const int rows = (int)M, slice = (rows + split - 1) / split, pitch = bn + 4;
   if (ok && warp >= 2) {
     const int row = (warp & 3) * 32 + lane;
     const bool live = row < rows;
@@ -396,7 +405,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
         x[4] += b.x; x[5] += b.y; x[6] += b.z; x[7] += b.w;
       }
-      const int64_t col = (int64_t)tn * bn + c, at = (int64_t)tm * BM + rank * slice + r;
+      const int64_t col = (int64_t)tn * bn + c, at = rank * slice + r;
       const float a_scale = e.a_scale[at];
       T* dst = reinterpret_cast<T*>(e.c) + at * e.ldc + col;
       if (e.vector != 0 && col + 8 <= N) {
@@ -428,19 +437,16 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
   }
 }
 
-// Tile width, K split and ring depth: among the cluster sizes that still give every tile its SMs, the one with the fewest bytes through the busiest SM
-// (its operand tiles, plus what the exchange costs); tiles of full width, unsplit, where there are more of them than SMs.
-// `clusters[s]`: clusters of s CTAs that run at once.
-Plan make_plan(int64_t M, int64_t N, int64_t K, int sms, const int* clusters) {
-  const int64_t mt = (M + BM - 1) / BM, kb = (K + BK - 1) / BK;
-  const int64_t a_rows = M < BM ? (M + 7) / 8 * 8 : BM;
-  auto depth = [&](int64_t stage) { return (int)(RING / stage < STAGES ? RING / stage : STAGES); };
+// Tile width, K split and ring depth for at most 128 rows: among the cluster sizes that still give every tile its SMs, the one with the fewest bytes through
+// the busiest SM (its operand tiles, plus what the exchange costs).  `clusters[s]`: clusters of s CTAs that run at once.  No plan (bn == 0): more tiles than SMs.
+Plan make_plan(int64_t M, int64_t N, int64_t K, const int* clusters) {
+  const int64_t kb = (K + BK - 1) / BK, a_rows = (M + 7) / 8 * 8;
   Plan best{};
-  int64_t best_cost = INT64_MAX;
+  best.cost = INT64_MAX;
   for (int split = 1; split <= 8; ++split) {
-    const int64_t tiles_n = clusters[split] / mt;
-    if (tiles_n == 0) continue;
-    const int64_t bn = ((N + tiles_n - 1) / tiles_n + 15) / 16 * 16, block = (a_rows + bn) * BK;
+    const int64_t tiles = clusters[split];
+    if (tiles == 0) continue;
+    const int64_t bn = ((N + tiles - 1) / tiles + 15) / 16 * 16, block = (a_rows + bn) * BK;
     if (bn > BN) continue;
     // blocks a stage: up to 48 KB a stage, at least three stages, no padding of K beyond one block a CTA
     int ks = 1;
@@ -450,14 +456,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int sms, const int* clusters) {
     const int64_t stage = ks * block, exchange = split == 1 ? 0 : 65536 + a_rows * bn * 4;
     const int64_t least = ks > 2 ? ks * 8192 : 16384;
     const int64_t cost = per * (stage > least ? stage : least) + exchange;
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = {(int)bn, split, depth(stage), ks, (int)a_rows};
-    }
-  }
-  if (best.bn == 0) {  // more tiles than SMs
-    const int64_t nt = (N + BN - 1) / BN, bn = ((N + nt - 1) / nt + 15) / 16 * 16;
-    best = {(int)bn, 1, depth((a_rows + bn) * BK), 1, (int)a_rows};
+    if (cost < best.cost) best = {(int)bn, split, (int)(RING / stage < STAGES ? RING / stage : STAGES), ks, (int)a_rows, cost};
   }
   return best;
 }
@@ -495,20 +494,122 @@ int operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int
   return make_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, const_cast<void*>(base), 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Width of the pairs' column tiles, whole chunks of the results' 128 bytes: the one with the least time, in columns, of the busiest pair
-int pair_width(int64_t M, int64_t N, int pairs, int chunk) {
-  const int64_t mt = (M + PAIR_ROWS - 1) / PAIR_ROWS;
-  int best = BN;
-  int64_t best_cost = INT64_MAX;
-  for (int bn = BN; bn >= 128; bn -= chunk) {
-    const int64_t nt = (N + bn - 1) / bn, cost = (mt * nt + pairs - 1) / pairs * (bn + 128);
-    if (cost < best_cost) { best_cost = cost; best = bn; }
+// ------------------------------------------------------------------------------------------------ one to four rows
+// The time is that of streaming B and, from two rows on, of the products: four a lane and instruction (dp4a, of which an SM takes about 11 lanes a cycle).  A warp takes
+// R rows of B, 16 loads of 512 bytes on their way, and MT rows of A from L1; with WK == 4 the warps of a CTA share the same rows of B, each a part of K.  The lanes' sums
+// meet in one reduction each.  (The bytes of a piece behind K are cleared in A; reading them is in bounds, rows are whole pieces apart.)
+template <class T, int MT, int R, int WK>
+__global__ void __launch_bounds__(128) gemm_int8_stream_kernel(const int8_t* A, const int8_t* B, const Epilogue e, int M, int64_t N, int K, int64_t lda, int64_t ldb) {
+  constexpr int PU = 16 / R;  // pieces of a row at a time
+  __shared__ int32_t part[WK][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, turn = WK == 1 ? 0 : warp;
+  const int64_t n0 = (WK == 1 ? (int64_t)blockIdx.x * 4 + warp : (int64_t)blockIdx.x) * R;
+  pdl_trigger();
+  pdl_wait();
+  if (n0 >= N) return;  // (the whole CTA, or with WK == 1 a warp, which meets no other)
+  int32_t sum[MT][R] = {};
+  const int8_t* b = B + n0 * ldb;
+  for (int k0 = turn * PU * 512; k0 < K; k0 += WK * PU * 512) {
+    uint4 w[R][PU];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int p = 0; p < PU; ++p) {
+        const int k = k0 + p * 512 + lane * 16;
+        w[r][p] = make_uint4(0, 0, 0, 0);
+        if (k < K && n0 + r < N)
+          asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[r][p].x), "=r"(w[r][p].y), "=r"(w[r][p].z), "=r"(w[r][p].w) : "l"(b + r * ldb + k));
+      }
+#pragma unroll
+    for (int p = 0; p < PU; ++p) {
+      const int k = k0 + p * 512 + lane * 16;
+      if (k >= K) break;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m >= M) break;
+        uint4 x = *reinterpret_cast<const uint4*>(A + m * lda + k);
+        if (k + 16 > K) {
+          uint32_t* words = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int there = K - k - 4 * i;  // bytes of this word in front of K
+            words[i] = there >= 4 ? words[i] : there <= 0 ? 0u : words[i] & ((1u << (8 * there)) - 1u);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          sum[m][r] = __dp4a((int)w[r][p].x, (int)x.x, sum[m][r]);
+          sum[m][r] = __dp4a((int)w[r][p].y, (int)x.y, sum[m][r]);
+          sum[m][r] = __dp4a((int)w[r][p].z, (int)x.z, sum[m][r]);
+          sum[m][r] = __dp4a((int)w[r][p].w, (int)x.w, sum[m][r]);
+        }
+      }
+    }
+  }
+  int32_t mine = 0;  // lane m R + r finishes row m, column r
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int32_t total = __reduce_add_sync(0xffffffffu, sum[m][r]);
+      if (lane == m * R + r) mine = total;
+    }
+  if constexpr (WK > 1) {
+    part[warp][lane] = mine;
+    __syncthreads();
+    if (warp != 0) return;
+    mine = 0;
+#pragma unroll
+    for (int i = 0; i < WK; ++i) mine += part[i][lane];
+  }
+  const int m = lane / R;
+  const int64_t n = n0 + lane % R;
+  if (m < M && m < MT && n < N)
+    reinterpret_cast<T*>(e.c)[m * e.ldc + n] = Elem<T>::down(finish(mine, e.a_scale[m], e.b_scale[n], bias_at<T>(e, n)));
+}
+
+template <class T, int MT, int WK>
+int run_stream(const AveGemmInt8Args& a, const Epilogue& e, cudaStream_t stream) {
+  constexpr int R = 4, columns = (WK == 1 ? 4 : 1) * R;  // (one or two rows of B a warp are slower, 12352 x 2048 5.8 and 10.1 us)
+  AVE_CUDA_TRY(launch_after(gemm_int8_stream_kernel<T, MT, R, WK>, (unsigned)((a.N + columns - 1) / columns), 128, 0, stream, reinterpret_cast<const int8_t*>(a.a),
+                            reinterpret_cast<const int8_t*>(a.b), e, (int)a.M, a.N, (int)a.K, a.lda, a.ldb));
+  return AVE_GDN_OK;
+}
+// Up to two rows, up to four where there is little of B, whatever its shape.  (us, this form and clusters: 1 x 12352 x 2048 5.1 and 7.4, 2 rows 7.0 and 7.5, 4 rows 10.7 and 7.5;
+// 2 x 4096 x 4096 6.3 and 6.1, 2 x 400 x 8192 3.6 and 5.1; 4 x 1544 x 2048 5.3 and 4.9, 4 x 12352 x 512 4.7 and 5.0, 4 x 1000 x 512 2.5 and 4.2.)
+bool streams(const AveGemmInt8Args& a) {
+  const int64_t whole = (a.K + 15) / 16 * 16;
+  if ((a.M == 1 && a.lda < whole) || (a.N == 1 && a.ldb < whole)) return false;  // (a single row that ends inside a piece)
+  return a.M <= 2 || (a.M <= 4 && a.K <= 1024 && a.N * a.K <= 1 << 23);
+}
+// K shared by a CTA's warps where there are few warps or long rows (us, shared and not: 1 x 400 x 8192 2.7 and 6.3, 1 x 2048 x 4096 3.0 and 4.0, 1 x 8192 x 8192 7.9 and 9.5,
+// 1 x 4096 x 4096 4.8 and 4.4, 1 x 12352 x 2048 8.5 and 5.1)
+template <class T>
+int launch_stream(const AveGemmInt8Args& a, const Epilogue& e, cudaStream_t stream) {
+  if (a.M > 2) return run_stream<T, 4, 1>(a, e, stream);
+  if (a.K > 4096 || (a.K > 2048 && a.N < 4 * 592)) return a.M == 1 ? run_stream<T, 1, 4>(a, e, stream) : run_stream<T, 2, 4>(a, e, stream);
+  return a.M == 1 ? run_stream<T, 1, 1>(a, e, stream) : run_stream<T, 2, 1>(a, e, stream);
+}
+
+// Width of the pairs' column tiles and what a product with it takes, in ns.  A block of 128 of K takes 112, 138, 194 and 265 ns with 64, 128, 192 and 256 columns where every
+// pair has one tile at most (the narrow ones wait for their operands, 20 to 28 KB a CTA and block), and 208, 277, 347 and 417 where all are busy for longer (L2 and the power cap;
+// 8192 x 2048 x 4096 with 256 columns 55 us, 61 with 192), a tile's results at least 9 ns a column, and launch, first operands and last results 4 us and 6 ns a column.
+// `across`: rows of operands that do not lie on 128 bytes, whose blocks reach across two lines each (256 rows x 1544 x 2048 6.1 us, with 1999 of 2000 bytes 8.2).
+struct Width { int bn; int64_t ns; };
+Width pair_width(int64_t M, int64_t N, int64_t K, bool across, int pairs) {
+  constexpr int alone_ns[4] = {112, 138, 194, 265}, busy_ns[4] = {208, 277, 347, 417};
+  const int64_t mt = (M + PAIR_ROWS - 1) / PAIR_ROWS, kb = (K + BK - 1) / BK;
+  Width best{0, INT64_MAX};
+  for (int bn = BN; bn >= 64; bn -= 64) {
+    const int64_t turns = (mt * ((N + bn - 1) / bn) + pairs - 1) / pairs, block = (turns > 1 ? busy_ns : alone_ns)[bn / 64 - 1];
+    const int64_t products = kb * block * (across ? 4 : 3) / 3, results = 300 + 9 * bn;
+    const int64_t ns = 4000 + 6 * bn + turns * (products > results ? products : results);
+    if (ns < best.ns) best = {bn, ns};
   }
   return best;
 }
 template <class T>
-int launch_pairs(const AveGemmInt8Args& a, const Epilogue& e, int pairs, cudaStream_t stream) {
-  const int bn = pair_width(a.M, a.N, pairs, 128 / (int)sizeof(T));
+int launch_pairs(const AveGemmInt8Args& a, const Epilogue& e, int bn, int pairs, cudaStream_t stream) {
   CUtensorMap tmA, tmB, tmC{};
   int rc = operand_map(&tmA, a.a, a.M, a.K, a.lda, BM);
   if (rc != AVE_GDN_OK) return rc;
@@ -521,13 +622,19 @@ int launch_pairs(const AveGemmInt8Args& a, const Epilogue& e, int pairs, cudaStr
     rc = make_tmap(&tmC, dt, (int)size, a.c, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != AVE_GDN_OK) return rc;
   }
-  constexpr auto* kernel = &gemm_int8_pair_kernel<T>;
-  rc = allow_smem<kernel>(PAIR_SMEM);
-  if (rc != AVE_GDN_OK) return rc;
   const int64_t tiles = ((a.M + PAIR_ROWS - 1) / PAIR_ROWS) * ((a.N + bn - 1) / bn);
   if (tiles > INT32_MAX) return AVE_GDN_UNSUPPORTED;
-  AVE_CUDA_TRY(launch_after(kernel, (unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, PAIR_SMEM, stream, tmA, tmB, tmC, e, a.M, a.N, a.K, a.status, bn));
-  return AVE_GDN_OK;
+  auto launch = [&](auto blocks) {
+    constexpr int KS = decltype(blocks)::value;
+    constexpr auto* kernel = &gemm_int8_pair_kernel<T, KS>;
+    const int rc = allow_smem<kernel>(PAIR_SMEM);
+    if (rc != AVE_GDN_OK) return rc;
+    const int fit = PAIR_RING / (KS * (BM + bn / 2) * BK), stages = fit < PAIR_STAGES ? fit : PAIR_STAGES;
+    AVE_CUDA_TRY(launch_after(kernel, (unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, PAIR_SMEM, stream, tmA, tmB, tmC, e, a.M, a.N, a.K, a.status, bn, stages));
+    return (int)AVE_GDN_OK;
+  };
+  if (bn <= 128) return launch(std::integral_constant<int, 2>());
+  return launch(std::integral_constant<int, 1>());
 }
 
 template <class T>
@@ -537,12 +644,17 @@ int launch_t(const AveGemmInt8Args& a, cudaStream_t stream) {
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const int size = (int)sizeof(T);
   const Epilogue e{a.a_scale, a.b_scale, a.bias, a.c, a.ldc, a.bias_dtype == AVE_DTYPE_FP32, aligned16(a.c) && rows::on16(a.ldc, size)};
+  if (streams(a)) return launch_stream<T>(a, e, stream);
   const int* clusters = cluster_counts(dev, sms);
-  if (clusters == nullptr) return AVE_GDN_UNSUPPORTED;
+  if (clusters == nullptr || clusters[2] == 0) return AVE_GDN_UNSUPPORTED;
+  // The pairs from 129 rows on, and from 64 where they take less by the two estimates: a cluster's 4.2 us and what comes through its busiest SM at 60 bytes a ns.
+  // (us, clusters and pairs: N = 12352, K = 2048, 32 rows 8.2 and 9.5, 64 rows 9.7 and 8.4, 128 rows 13.7 and 8.6; N = 2048, K = 4096, 7.9 and 7.9, 7.7 and 7.9,
+  // 10.3 and 7.9; N = 1544, K = 2048, 5.6 and 6.1, 5.6 and 6.1, 6.3 and 6.1.)
   const int pairs = clusters[2];
-  const int64_t mt = (a.M + PAIR_ROWS - 1) / PAIR_ROWS, nt = (a.N + BN - 1) / BN;
-  if (a.M > BM && mt * nt >= pairs) return launch_pairs<T>(a, e, pairs, stream);
-  const Plan plan = make_plan(a.M, a.N, a.K, sms, clusters);
+  const Width width = pair_width(a.M, a.N, a.K, a.lda % 128 != 0 || a.ldb % 128 != 0, pairs);
+  Plan plan{};
+  if (a.M <= BM) plan = make_plan(a.M, a.N, a.K, clusters);
+  if (plan.bn == 0 || (a.M >= 64 && width.ns <= 4200 + plan.cost / 60)) return launch_pairs<T>(a, e, width.bn, pairs, stream);
   CUtensorMap tmA, tmB;
   int rc = operand_map(&tmA, a.a, a.M, a.K, a.lda, plan.a_rows);
   if (rc != AVE_GDN_OK) return rc;
@@ -553,8 +665,7 @@ int launch_t(const AveGemmInt8Args& a, cudaStream_t stream) {
   if (rc != AVE_GDN_OK) return rc;
   uint32_t cols = 32;
   while ((int)cols < plan.bn) cols *= 2;
-  const int64_t ctas = ((a.M + BM - 1) / BM) * ((a.N + plan.bn - 1) / plan.bn) * plan.split;
-  if (ctas > INT32_MAX) return AVE_GDN_UNSUPPORTED;
+  const int64_t ctas = (a.N + plan.bn - 1) / plan.bn * plan.split;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
