@@ -1356,9 +1356,11 @@ void check_like(const Tensor& t, const char* name, const Tensor& x) {
 // 8-bit rows in the shape of x, a whole number of 16 bytes apart, and a place for their scales
 std::pair<Tensor, Tensor> empty_int8(const Tensor& x) {
   const int64_t n = x.size(-1);
+  const Tensor scale = empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+  if (n % 16 == 0) return {empty(x.sizes(), at::kChar, x), scale};
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = (n + 15) / 16 * 16;
-  return {empty(shape, at::kChar, x).narrow(-1, 0, n), empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x)};
+  return {empty(shape, at::kChar, x).narrow(-1, 0, n), scale};
 }
 
 // rms_norm(x, weight, eps, residual, zero_centered, return_stats, out, sum_out) -> out, or a tuple of out[, sum][, rstd]

@@ -58,11 +58,23 @@ __global__ void __launch_bounds__(THREADS, 1) rms_backward_kernel(const AveRmsNo
   for (int s = 0; s < S - 1; ++s) fetch(first + s * step, s);
   const float inv_n = 1.f / (float)n, offset = (a.flags & AVE_RMS_FLAG_ZERO_CENTERED) ? 1.f : 0.f;
   const bool wide = a.w_dtype == AVE_DTYPE_FP32;
-  float2 dw[P][H];
+  constexpr bool kKept = P * V <= 32 && TPR < 1024;  // a thread's weights stay in registers
+  float2 dw[P][H], kept[kKept ? P : 1][H];
 #pragma unroll
-  for (int p = 0; p < P; ++p)
+  for (int p = 0; p < P; ++p) {
 #pragma unroll
     for (int i = 0; i < H; ++i) dw[p][i] = splat(0.f);
+    if constexpr (kKept)
+      if ((p * TPR + sub) * V < n) params<T>(kept[p], a.weight, wide, aligned, (p * TPR + sub) * V, offset);
+  }
+  auto weights = [&](float2 (&w)[H], int p, int c) {
+    if constexpr (kKept) {
+#pragma unroll
+      for (int i = 0; i < H; ++i) w[i] = kept[p][i];
+    } else {
+      params<T>(w, a.weight, wide, aligned, c, offset);
+    }
+  };
   int stage = 0;
   for (int64_t turn = 0; turn < turns; ++turn) {
     const int64_t r = first + turn * step;
@@ -81,7 +93,7 @@ __global__ void __launch_bounds__(THREADS, 1) rms_backward_kernel(const AveRmsNo
         float2 h[H], g[H], w[H];
         widen<T>(h, row[p * THREADS]);
         widen<T>(g, row[(P + p) * THREADS]);
-        params<T>(w, a.weight, wide, aligned, c, offset);
+        weights(w, p, c);
 #pragma unroll
         for (int i = 0; i < H; ++i) s2 = __ffma2_rn(__fmul2_rn(g[i], w[i]), __fmul2_rn(h[i], splat(rstd)), s2);
       }
@@ -97,7 +109,7 @@ __global__ void __launch_bounds__(THREADS, 1) rms_backward_kernel(const AveRmsNo
       float2 h[H], g[H], w[H], d[H];
       widen<T>(h, row[p * THREADS]);
       widen<T>(g, row[(P + p) * THREADS]);
-      params<T>(w, a.weight, wide, aligned, c, offset);
+      weights(w, p, c);
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         h[i] = __fmul2_rn(h[i], splat(rstd));
@@ -136,13 +148,72 @@ __global__ void __launch_bounds__(THREADS, 1) rms_backward_kernel(const AveRmsNo
   if constexpr (GROUPS > 1) add_groups<THREADS, GROUPS>(reinterpret_cast<const float*>(ring), out, n, TPR * P * V);
 }
 
-// Rows that do not lie on 16 bytes, or longer than the ring's: element by element, read again for the second pass
+// Rows that do not lie on 16 bytes: element by element, neighbouring threads on neighbouring columns, a row in registers
 template <class T, int THREADS, int TPR, int P>
-__global__ void __launch_bounds__(THREADS) rms_backward_elements_kernel(const AveRmsNormBwdArgs a, float* partial) {
+__global__ void __launch_bounds__(THREADS, 1) rms_backward_elements_kernel(const AveRmsNormBwdArgs a, float* partial) {
   constexpr int GROUPS = THREADS / TPR;
   __shared__ float sums[2][2 * THREADS / 32];
   extern __shared__ float cols[];  // [GROUPS][TPR * P], with several groups
   const int sub = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int bar = TPR > 32 && GROUPS > 1 ? 1 + group : 0;
+  const T *dy = reinterpret_cast<const T*>(a.d_y), *x = reinterpret_cast<const T*>(a.x), *d_sum = reinterpret_cast<const T*>(a.d_sum);
+  const bool wide = a.w_dtype == AVE_DTYPE_FP32, add = d_sum != nullptr;
+  const float inv_n = 1.f / (float)a.n, offset = (a.flags & AVE_RMS_FLAG_ZERO_CENTERED) ? 1.f : 0.f;
+  const int n = (int)a.n;
+  pdl_wait();
+  float w[P], dw[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    w[p] = p * TPR + sub >= n ? 0.f : a.weight == nullptr ? 1.f : param<T>(a.weight, wide, p * TPR + sub) + offset;
+    dw[p] = 0.f;
+  }
+  int turn = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < a.rows; r0 += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+    const int64_t r = r0 + group;
+    const bool live = r < a.rows;
+    const float rstd = live ? a.rstd[r] : 0.f;
+    T h_in[P], g_in[P], d_in[P];
+    const T zero = Elem<T>::down(0.f);
+    auto fetch = [&](T (&v)[P], const T* row, bool wanted) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) v[p] = wanted && live && p * TPR + sub < n ? row[p * TPR + sub] : zero;
+    };
+    fetch(h_in, x + r * a.x_stride, true);
+    fetch(g_in, dy + r * a.dy_stride, true);
+    fetch(d_in, d_sum + r * a.ds_stride, add);
+    float sum = 0.f, none = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const float h = Elem<T>::up(h_in[p]) * rstd, g = Elem<T>::up(g_in[p]);
+      dw[p] = fmaf(g, h, dw[p]);
+      sum = fmaf(g * w[p], h, sum);
+    }
+    group_reduce<TPR, false>(sum, none, sums[turn], bar);
+    if (!live) continue;
+    const float c1 = sum * inv_n;
+    T* to = reinterpret_cast<T*>(a.d_x) + r * a.dx_stride + sub;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (p * TPR + sub >= n) break;
+      const float h = Elem<T>::up(h_in[p]) * rstd;
+      to[p * TPR] = Elem<T>::down(fmaf(fmaf(h, -c1, Elem<T>::up(g_in[p]) * w[p]), rstd, Elem<T>::up(d_in[p])));  // (without d_sum plus zero)
+    }
+  }
+  if (partial == nullptr) return;
+  pdl_trigger();
+  float* out = partial + (int64_t)blockIdx.x * n;
+  float* sink = GROUPS == 1 ? out : cols + group * TPR * P;
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if (p * TPR + sub < n) sink[p * TPR + sub] = dw[p];
+  if constexpr (GROUPS > 1) add_groups<THREADS, GROUPS>(cols, out, n, TPR * P);
+}
+
+// Rows longer than those: a row a CTA, read again for the second pass
+template <class T, int TPR, int P>
+__global__ void __launch_bounds__(TPR, 1) rms_backward_long_kernel(const AveRmsNormBwdArgs a, float* partial) {
+  __shared__ float sums[2][2 * TPR / 32];
+  const int sub = threadIdx.x;
   const T *dy = reinterpret_cast<const T*>(a.d_y), *x = reinterpret_cast<const T*>(a.x), *d_sum = reinterpret_cast<const T*>(a.d_sum);
   const bool wide = a.w_dtype == AVE_DTYPE_FP32;
   const float inv_n = 1.f / (float)a.n, offset = (a.flags & AVE_RMS_FLAG_ZERO_CENTERED) ? 1.f : 0.f;
@@ -153,23 +224,18 @@ __global__ void __launch_bounds__(THREADS) rms_backward_elements_kernel(const Av
 #pragma unroll
   for (int p = 0; p < P; ++p) dw[p] = 0.f;
   int turn = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < a.rows; r0 += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
-    const int64_t r = r0 + group;
-    const bool live = r < a.rows;
-    const float rstd = live ? a.rstd[r] : 0.f;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, turn ^= 1) {
+    const float rstd = a.rstd[r];
     float sum = 0.f, none = 0.f;
-    if (live) {
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        const int c = p * TPR + sub;
-        if (c >= n) break;
-        const float g = Elem<T>::up(dy[r * a.dy_stride + c]), xh = Elem<T>::up(x[r * a.x_stride + c]) * rstd;
-        dw[p] = fmaf(g, xh, dw[p]);
-        sum = fmaf(g * weight(c), xh, sum);
-      }
+    for (int p = 0; p < P; ++p) {
+      const int c = p * TPR + sub;
+      if (c >= n) break;
+      const float g = Elem<T>::up(dy[r * a.dy_stride + c]), xh = Elem<T>::up(x[r * a.x_stride + c]) * rstd;
+      dw[p] = fmaf(g, xh, dw[p]);
+      sum = fmaf(g * weight(c), xh, sum);
     }
     group_reduce<TPR, false>(sum, none, sums[turn]);
-    if (!live) continue;
     const float c1 = sum * inv_n;
 #pragma unroll 4
     for (int c = sub; c < n; c += TPR) {
@@ -181,44 +247,44 @@ __global__ void __launch_bounds__(THREADS) rms_backward_elements_kernel(const Av
   if (partial == nullptr) return;
   pdl_trigger();
   float* out = partial + (int64_t)blockIdx.x * n;
-  float* to = GROUPS == 1 ? out : cols + group * TPR * P;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const int c = p * TPR + sub;
-    if (c < n) to[c] = dw[p];
+    if (c < n) out[c] = dw[p];
   }
-  if constexpr (GROUPS > 1) add_groups<THREADS, GROUPS>(cols, out, n, TPR * P);
 }
 
-// Adds the CTAs' sums: 32 columns a CTA, eight warps take every eighth row of sums
+// Adds the CTAs' sums: 32 columns a CTA, each warp takes every 32nd row of sums
 template <class T>
-__global__ void __launch_bounds__(256) rms_columns_kernel(const float* partial, void* d_weight, int w_dtype, int n, int parts) {
-  __shared__ float part[8][33];
+__global__ void __launch_bounds__(1024) rms_columns_kernel(const float* partial, void* d_weight, int w_dtype, int n, int parts) {
+  __shared__ float part[32][33];
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = blockIdx.x * 32 + lane;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  float s = 0.f;
   if (c < n) {
-    int i = warp;
-    for (; i + 24 < parts; i += 32)
+    float v[4];  // four rows on their way
+    for (int i = warp; i < parts; i += 128) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[k] += partial[(int64_t)(i + 8 * k) * n + c];
-    for (; i < parts; i += 8) s[0] += partial[(int64_t)i * n + c];
+      for (int k = 0; k < 4; ++k) v[k] = i + 32 * k < parts ? partial[(int64_t)(i + 32 * k) * n + c] : 0.f;
+      s += (v[0] + v[1]) + (v[2] + v[3]);
+    }
   }
-  part[warp][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+  part[warp][lane] = s;
   __syncthreads();
   if (warp != 0 || c >= n) return;
-  float t = 0.f;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int k = 0; k < 8; ++k) t += part[k][lane];
-  if (w_dtype == AVE_DTYPE_FP32) reinterpret_cast<float*>(d_weight)[c] = t;
-  else reinterpret_cast<T*>(d_weight)[c] = Elem<T>::down(t);
+  for (int k = 0; k < 32; ++k) t[k & 3] += part[k][lane];
+  const float sum = (t[0] + t[1]) + (t[2] + t[3]);
+  if (w_dtype == AVE_DTYPE_FP32) reinterpret_cast<float*>(d_weight)[c] = sum;
+  else reinterpret_cast<T*>(d_weight)[c] = Elem<T>::down(sum);
 }
 
 template <class T>
 int add_columns(const AveRmsNormBwdArgs& a, int parts, cudaStream_t stream) {
   if (a.d_weight == nullptr) return AVE_GDN_OK;
-  AVE_CUDA_TRY(launch_after(rms_columns_kernel<T>, (unsigned)((a.n + 31) / 32), 256, 0, stream, (const float*)a.workspace, a.d_weight, a.w_dtype, (int)a.n, parts));
+  AVE_CUDA_TRY(launch_after(rms_columns_kernel<T>, (unsigned)((a.n + 31) / 32), 1024, 0, stream, (const float*)a.workspace, a.d_weight, a.w_dtype, (int)a.n, parts));
   return AVE_GDN_OK;
 }
 template <class T, int THREADS, int TPR, int P, int S>
@@ -243,10 +309,19 @@ int run_elements(const AveRmsNormBwdArgs& a, cudaStream_t stream) {
   constexpr int GROUPS = THREADS / TPR;
   constexpr size_t smem = GROUPS > 1 ? (size_t)THREADS * P * 4 : 0;
   static_assert(smem <= 40 * 1024, "column sums in the default shared memory");
-  const int64_t ctas = (a.rows + GROUPS - 1) / GROUPS;
-  const int grid = (int)(ctas < MAX_PARTS ? ctas : MAX_PARTS);
+  constexpr auto* kernel = &rms_backward_elements_kernel<T, THREADS, TPR, P>;
+  static const int per = ctas_an_sm(kernel, THREADS, smem);
+  const int64_t ctas = (a.rows + GROUPS - 1) / GROUPS, room = (int64_t)sm_count() * per, most = room < MAX_PARTS ? room : MAX_PARTS;
+  const int grid = (int)(ctas < most ? ctas : most);
   float* partial = a.d_weight != nullptr ? reinterpret_cast<float*>(a.workspace) : nullptr;
-  AVE_CUDA_TRY(launch_after(rms_backward_elements_kernel<T, THREADS, TPR, P>, (unsigned)grid, THREADS, smem, stream, a, partial));
+  AVE_CUDA_TRY(launch_after(kernel, (unsigned)grid, THREADS, smem, stream, a, partial));
+  return add_columns<T>(a, grid, stream);
+}
+template <class T>
+int run_long(const AveRmsNormBwdArgs& a, cudaStream_t stream) {
+  const int grid = (int)(a.rows < 2 * sm_count() && a.rows < MAX_PARTS ? a.rows : 2 * sm_count() < MAX_PARTS ? 2 * sm_count() : MAX_PARTS);
+  float* partial = a.d_weight != nullptr ? reinterpret_cast<float*>(a.workspace) : nullptr;
+  AVE_CUDA_TRY(launch_after(rms_backward_long_kernel<T, 1024, 28>, (unsigned)grid, 1024, 0, stream, a, partial));
   return add_columns<T>(a, grid, stream);
 }
 
@@ -256,12 +331,17 @@ int backward_t(const AveRmsNormBwdArgs& a, cudaStream_t stream) {
   const bool wide = a.n % V == 0 && aligned16(a.x) && on16(a.x_stride, size) && aligned16(a.d_y) && on16(a.dy_stride, size) && aligned16(a.d_x) &&
                     on16(a.dx_stride, size) && aligned16(a.d_sum) && on16(a.ds_stride, size);
   const int64_t pieces = a.n / V;
-  if (!wide || pieces > 4096) {
-    if (a.n <= 64) return run_elements<T, 256, 8, 8>(a, stream);
-    if (a.n <= 512) return run_elements<T, 256, 32, 16>(a, stream);
-    if (a.n <= 4096) return run_elements<T, 256, 256, 16>(a, stream);
-    return run_elements<T, 1024, 1024, 28>(a, stream);
+  if (!wide && a.n <= 8192) {
+    if (a.n <= 8) return run_elements<T, 256, 8, 1>(a, stream);
+    if (a.n <= 64) return run_elements<T, 256, 32, 2>(a, stream);
+    if (a.n <= 256) return run_elements<T, 512, 32, 8>(a, stream);
+    if (a.n <= 512) return run_elements<T, 512, 64, 8>(a, stream);
+    if (a.n <= 1024) return run_elements<T, 512, 128, 8>(a, stream);
+    if (a.n <= 2048) return run_elements<T, 512, 256, 8>(a, stream);
+    if (a.n <= 4096) return run_elements<T, 512, 512, 8>(a, stream);
+    return run_elements<T, 1024, 1024, 8>(a, stream);
   }
+  if (!wide || pieces > 4096) return run_long<T>(a, stream);
   if (pieces <= 8) return run_ring<T, 256, 8, 1, 3>(a, stream);
   if (pieces <= 32) return run_ring<T, 512, 32, 1, 3>(a, stream);
   if (a.rows <= 2 * 148) {
