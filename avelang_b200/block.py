@@ -7,6 +7,9 @@ gated RMSNorm (fused into the delta-rule epilogue) -> all-gather of the per-head
 Partitioning: rank r of G owns key heads [r*Hk/G, (r+1)*Hk/G) and the value heads that read them.  Every
 (sequence, value head) recurrence is independent, so nothing crosses GPUs before the final all-gather; the
 in-projection weight is sliced by output column so that each rank produces exactly its own heads.
+
+With ``int8=True`` the projections take 8-bit integers: the weights a scale for each output channel, made once when the block is built, the
+activations one for each token, made by the norm in front (``GdnBlockTP.layer``) or by a pass of their own.
 """
 from __future__ import annotations
 
@@ -55,6 +58,11 @@ def projection_rows(shard: HeadShard, dk: int, dv: int) -> torch.Tensor:
     return torch.cat(parts)
 
 
+def quantizable(w: torch.Tensor) -> torch.Tensor:
+    """Weights in a dtype that ``gemm.quantize_rows_int8`` takes: as they came where it does, else fp32."""
+    return w if w.dtype in (torch.bfloat16, torch.float16, torch.float32) else w.float()
+
+
 def pad_rows(n: int, multiple: int = 8) -> int:
     return (n + multiple - 1) // multiple * multiple
 
@@ -62,19 +70,23 @@ def pad_rows(n: int, multiple: int = 8) -> int:
 class GdnBlockShard:
     """One rank's slice of the block.  ``w_in`` is the full fused projection weight ``[2*Hk*dk + 2*Hv*dv + 2*Hv, hidden]``;
     ``conv_w`` the full depthwise filter ``[2*Hk*dk + Hv*dv, 4]``; ``A_log``, ``dt_bias``, ``norm_weight`` per value head /
-    per feature.  Only this rank's rows are kept on the device."""
+    per feature.  Only this rank's rows are kept on the device, as bf16 or, with ``int8``, as 8-bit rows and their scales (``w``, ``w_scale``)."""
 
-    def __init__(self, w_in, conv_w, A_log, dt_bias, norm_weight, *, Hk, Hv, dk, dv, rank=0, world=1, device="cuda"):
+    def __init__(self, w_in, conv_w, A_log, dt_bias, norm_weight, *, Hk, Hv, dk, dv, rank=0, world=1, device="cuda", int8=False):
         self.shard = HeadShard(rank, world, Hk, Hv)
         self.Hk, self.Hv, self.dk, self.dv = Hk, Hv, dk, dv
         self.hk_local, self.hv_local = Hk // world, Hv // world
         rows = projection_rows(self.shard, dk, dv)
         self.n_rows = rows.numel()
-        w = w_in[rows].to(torch.bfloat16)
+        self.int8, self.w_scale = bool(int8), None
+        w = quantizable(w_in[rows]) if int8 else w_in[rows].to(torch.bfloat16)
         pad = pad_rows(self.n_rows) - self.n_rows
         if pad:
             w = torch.cat([w, torch.zeros(pad, w.shape[1], dtype=w.dtype)], 0)
         self.w = w.to(device).contiguous()
+        if int8:  # from the weights as they came: one rounding
+            from . import gemm
+            self.w, self.w_scale = gemm.quantize_rows_int8(self.w)
         nq, nk, nv = self.hk_local * dk, self.hk_local * dk, self.hv_local * dv
         self.splits = (nq, nk, nv, nv, self.hv_local, self.hv_local)
         conv_rows = rows[: nq + nk + nv].clone()
@@ -85,14 +97,26 @@ class GdnBlockShard:
         self.dt_bias = dt_bias[vh.start:vh.stop].float().to(device).contiguous()
         self.norm_weight = None if norm_weight is None else norm_weight.float().to(device).contiguous()
 
+    def project_in(self, x) -> torch.Tensor:
+        """This rank's columns of the in-projection, bf16 ``[B * T, columns]``.  x: bf16 ``[B, T, hidden]``, with ``int8`` also the pair of 8-bit rows and
+        scales that ``norm.rms_norm_int8`` gives."""
+        from . import gemm
+        pair = isinstance(x, tuple)
+        if pair and not self.int8:
+            raise ValueError("8-bit rows need a block built with int8=True.")
+        if not self.int8:
+            return gemm.gemm_pipeline_transposed_b(x.reshape(-1, x.shape[-1]), self.w)
+        q, scale = x if pair else gemm.quantize_rows_int8(x)
+        return gemm.gemm_int8_transposed_b(q.reshape(-1, q.shape[-1]), self.w, scale, self.w_scale)
+
     def forward_local(self, x: torch.Tensor, cu_seqlens=None, out=None, out_peers=None, keep: dict | None = None) -> torch.Tensor:
-        """x: bf16 [B, T, hidden] (replicated on every rank).  Returns this rank's normalised head outputs
+        """x: bf16 [B, T, hidden] (replicated on every rank), or what ``project_in`` takes.  Returns this rank's normalised head outputs
         [B, T, Hv/G, dv] (written into ``out`` / scattered to ``out_peers`` when given).  ``keep``: a dict that receives
         the delta-rule stage's own inputs (q, k, v after the convolution, g, beta, z), so that a test can hold that
         stage alone against the checker."""
-        from . import gdn, gemm
-        B, T, hidden = x.shape
-        y2 = gemm.gemm_pipeline_transposed_b(x.reshape(B * T, hidden), self.w)
+        from . import gdn
+        B, T = (x[0] if isinstance(x, tuple) else x).shape[:2]
+        y2 = self.project_in(x)
         y = y2.reshape(B, T, -1)
         nq, nk, nv, nz, nb, na = self.splits
         qkv_in = y[:, :, : nq + nk + nv]
@@ -118,8 +142,8 @@ class GdnBlockShard:
         if not fused_gather or self.shard.world == 1:
             return gather_heads(self.forward_local(x, cu_seqlens), self.shard.world, group)
         import torch.distributed as dist
-        B, T, _ = x.shape
-        full, peers = self._symmetric_output(B, T, x.device, group)
+        B, T = (x[0] if isinstance(x, tuple) else x).shape[:2]
+        full, peers = self._symmetric_output(B, T, self.w.device, group)
         hl = self.hv_local
         mine = full[:, :, self.shard.rank * hl:(self.shard.rank + 1) * hl]
         self._stream_barrier(group)   # every rank is done reading the previous contents of the buffers
@@ -166,17 +190,35 @@ class GdnBlockTP(GdnBlockShard):
     output by its column slice of ``w_out [hidden, Hv*dv]`` (row-parallel linear) and the partial results are summed
     with one all-reduce, so no all-gather of head outputs is needed."""
 
-    def __init__(self, w_in, conv_w, A_log, dt_bias, norm_weight, w_out, *, Hk, Hv, dk, dv, rank=0, world=1, device="cuda"):
+    def __init__(self, w_in, conv_w, A_log, dt_bias, norm_weight, w_out, *, Hk, Hv, dk, dv, rank=0, world=1, device="cuda", int8=False):
         super().__init__(w_in, conv_w, A_log, dt_bias, norm_weight, Hk=Hk, Hv=Hv, dk=dk, dv=dv, rank=rank, world=world,
-                         device=device)
+                         device=device, int8=int8)
         cols = output_projection_columns(self.shard, dv)
-        self.w_out = w_out[:, cols].to(torch.bfloat16).to(device).contiguous()  # [hidden, hl*dv]
+        self.w_out_scale = None
+        if int8:
+            from . import gemm
+            self.w_out, self.w_out_scale = gemm.quantize_rows_int8(quantizable(w_out[:, cols]).to(device))
+        else:
+            self.w_out = w_out[:, cols].to(torch.bfloat16).to(device).contiguous()  # [hidden, hl*dv]
 
     def forward(self, x: torch.Tensor, cu_seqlens=None, group=None, fused_reduce=False) -> torch.Tensor:
-        """Returns the block output after the output projection, ``[B, T, hidden]`` bf16, identical on every rank."""
-        B, T, _ = x.shape
+        """Returns the block output after the output projection, ``[B, T, hidden]`` bf16, identical on every rank.  x: as in ``forward_local``."""
+        B, T = (x[0] if isinstance(x, tuple) else x).shape[:2]
         o = self.forward_local(x, cu_seqlens)                                   # [B, T, hl, dv]
         return self.project(o.reshape(B * T, -1), group, fused_reduce).reshape(B, T, -1)
+
+    def layer(self, x: torch.Tensor, residual, weight, eps=1e-6, *, zero_centered=False, cu_seqlens=None, group=None, fused_reduce=False):
+        """The block behind its norm in a residual stream: ``h = x + residual`` (x itself where ``residual`` is None), then the RMS norm of h with
+        ``weight`` and the block.  Returns ``(output, h)``, both ``[B, T, hidden]`` bf16; they are the next layer's x and residual.  With ``int8`` the norm
+        leaves 8-bit rows, which the in-projection takes as they are."""
+        from . import norm
+        if self.int8:
+            got = norm.rms_norm_int8(x, weight, eps, residual=residual, zero_centered=zero_centered)
+            y, h = got[:2], x if residual is None else got[2]
+        else:
+            got = norm.rms_norm(x, weight, eps, residual=residual, zero_centered=zero_centered)
+            y, h = (got, x) if residual is None else got
+        return self.forward(y, cu_seqlens, group, fused_reduce), h
 
     def project(self, o2d: torch.Tensor, group=None, fused_reduce=False) -> torch.Tensor:
         """Output projection of this rank's normalised head outputs ``[M, hl*dv]`` and the sum over ranks, ``[M, hidden]``.
@@ -184,10 +226,16 @@ class GdnBlockTP(GdnBlockShard):
         each row of the partial product into the staging buffer of the rank that owns the row (symmetric memory, plain
         peer stores over NVLink, under the next tile's main loop); after a barrier every owner sums its rows in fp32 and
         stores them into every rank's result; a last barrier.  The fused result lives in a cached symmetric buffer that
-        the next fused call overwrites."""
+        the next fused call overwrites.  It takes bf16 operands, so a block of more than one rank built with ``int8`` refuses it."""
         from . import gemm
+        if self.int8 and fused_reduce and self.shard.world > 1:
+            raise ValueError("fused_reduce takes bf16 operands: not with int8=True.")
         if not fused_reduce or self.shard.world == 1:
-            part = gemm.gemm_pipeline_transposed_b(o2d, self.w_out)              # this rank's partial sum
+            if self.int8:
+                q, scale = gemm.quantize_rows_int8(o2d)
+                part = gemm.gemm_int8_transposed_b(q, self.w_out, scale, self.w_out_scale)
+            else:
+                part = gemm.gemm_pipeline_transposed_b(o2d, self.w_out)          # this rank's partial sum
             if self.shard.world > 1:
                 import torch.distributed as dist
                 dist.all_reduce(part, group=group)
