@@ -67,7 +67,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   uint8_t* smem = tc::align1024(smem_raw);
   __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile uint32_t abort_flag;
+  __shared__ volatile uint32_t abort_flag, issued[2];  // stages whose copies the leader's and the other CTA's producer have asked for (kept by the leader)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_rank();
   const int mt = (int)((M + PAIR_ROWS - 1) / PAIR_ROWS), nt = (int)((N + bn - 1) / bn), kb_count = (int)((K + KS * BK - 1) / (KS * BK));  // in stages of KS blocks
@@ -84,6 +84,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], 16); }
     tc::mbar_init(&drained, 1);
     abort_flag = 0;
+    issued[0] = issued[1] = 0;
     tc::fence_barrier_init();
     tc::prefetch_tmap(&tmA);
     tc::prefetch_tmap(&tmB);
@@ -98,7 +99,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 
   if (warp == 0) {
     int s = 0; uint32_t ph = 0;
-    int64_t turns = 0;
+    uint32_t turns = 0;
     bool ok = true;
     for (uint32_t tile = first; tile < tiles && ok; tile += step) {
       int m, n;
@@ -121,12 +122,11 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       }
     }
     if (ok)  // the leader's last arrivals at this CTA's barriers
-      for (int i = 0; i < stages && i < turns; ++i) {
+      for (uint32_t i = 0; i < (uint32_t)stages && i < turns; ++i) {
         if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) break;
         if (++s == stages) { s = 0; ph ^= 1u; }
       }
-    else if (rank == 0)  // copies may be on their way: those of both CTAs are counted here
-      for (int64_t i = turns > stages ? turns - stages : 0; i < turns; ++i) tc::drain(&full[i % stages], (uint32_t)(i / stages) & 1u);
+    if (lane == 0) tc::st_cluster_u32(tc::mapa(tc::smem_u32(const_cast<uint32_t*>(&issued[rank])), 0), turns);
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t idesc = idesc_i8(PAIR_ROWS, bn), stage0 = (tc::smem_u32(smem) >> 4) | (uint32_t)tc::desc_lo(0, 16);
@@ -157,11 +157,6 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (!ok) break;
         if (tc::elect_one()) tc::mma_commit_pair(&acc_full[buf]);
         __syncwarp();
-      }
-      if (!ok) {
-        if (tc::elect_one()) tc::mma_commit_pair(&drained);
-        __syncwarp();
-        tc::drain(&drained, 0u);
       }
     }
   } else {
@@ -278,8 +273,25 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   __syncwarp();
   tc::tc_fence_before_sync();
   __syncthreads();
-  if (threadIdx.x == 0 && abort_flag != 0u && status != nullptr) atomicOr(status, AVE_GDN_DEV_WAIT_EXPIRED);
+  if (threadIdx.x == 0 && abort_flag != 0u) {
+    if (status != nullptr) atomicOr(status, AVE_GDN_DEV_WAIT_EXPIRED);
+    tc::st_cluster_u32(tc::mapa(tc::smem_u32(const_cast<uint32_t*>(&abort_flag)), rank ^ 1u), 1u);
+  }
   tc::cluster_sync();  // neither CTA ends, or gives tensor memory back, while the other may reach it
+  if (abort_flag != 0u) {  // in both or in neither: copies and products may be on their way, and all are counted at the leader's barriers
+    if (rank == 0 && threadIdx.x == 0) {
+      const uint32_t own = issued[0], other = issued[1], all = own > other ? own : other, begin = all > (uint32_t)stages ? all - (uint32_t)stages : 0u;
+      for (uint32_t i = own; i < other; ++i) tc::mbar_expect_tx(&full[i % stages], stage_bytes);       // the other CTA's alone
+      for (uint32_t i = other; i < own; ++i) tc::mbar_complete_tx(&full[i % stages], stage_bytes);    // this one's alone
+      for (uint32_t i = begin; i < all; ++i) tc::drain(&full[i % stages], i / stages & 1u);
+    }
+    if (rank == 0 && warp == 1) {
+      if (tc::elect_one()) tc::mma_commit_pair(&drained);
+      __syncwarp();
+      tc::drain(&drained, 0u);
+    }
+    tc::cluster_sync();
+  }
   if (warp == 1) {
     tc::tc_fence_after_sync();
     tc::tmem_dealloc_pair(tmem_base, 512);
@@ -362,17 +374,14 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
       __syncwarp();
       if (++s == stages) { s = 0; ph ^= 1u; }
     }
-    if (ok) {
-      if (tc::elect_one()) tc::mma_commit(&acc_full);
-    } else {
-      tc::drain_mmas(&drained);
-    }
+    if (ok && tc::elect_one()) tc::mma_commit(&acc_full);
   }
   __syncwarp();  // the other lanes of the issuing warps must not poll beside them
   // the accumulator is complete, so every operand tile has landed and been read
   const bool ok = tc::mbar_wait_unrolled(&acc_full, 0, &abort_flag);
   tc::tc_fence_after_sync();
   __syncwarp();
+  if (!ok && warp == 1) tc::drain_mmas(&drained);
   tc::cluster_sync();  // ... in every CTA of the cluster: the rings may be overwritten
   const int rows = (int)M, slice = (rows + split - 1) / split, pitch = bn + 4;
   if (ok && warp >= 2) {
