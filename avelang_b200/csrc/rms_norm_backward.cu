@@ -4,7 +4,8 @@
 //
 // Bound by HBM: dy, h and d_h (the gradient that comes back beside the norm, where h is used further) are read once, dx is written once.  Rows come
 // through a ring in shared memory as in the forward pass; a thread keeps its columns for every row it meets, so that the sums of the weight's
-// gradient are registers.  A CTA's sums go to scratch and a second kernel adds them in a fixed order.
+// gradient are registers.  A CTA's sums go to scratch and a second kernel adds them in a fixed order, 2.5 us behind the first.  bf16 with d_h: 131072 x 2048 308 us, 8192 x 2048 28
+// us (21 at the copy rate), 8192 x 2047, element by element, 50; 1001 x 1409 fp32 7.1.
 #include "rows.cuh"
 
 namespace ave {

@@ -5,9 +5,9 @@ The reference ships its kernel libraries as modules of the ``avelang_kernels`` p
 test/examples/gemm/amdgpu/test_amdgpu_gemm.py:7).  The same spelling reaches the B200 path:
 
     from avelang_kernels import gdn    # chunk_gated_delta_rule, fused_recurrent_gated_delta_rule, gated_rmsnorm, ...
-    from avelang_kernels import gemm   # gemm_pipeline_transposed_b (counterpart of amdgpu_gemm.gemm_pipeline_transposed_b)
+    from avelang_kernels import gemm   # gemm_pipeline_transposed_b (counterpart of amdgpu_gemm.gemm_pipeline_transposed_b), gemm_int8_transposed_b, ...
     from avelang_kernels import linear_attention  # chunk_linear_attention, fused_recurrent_linear_attention, ...
-    from avelang_kernels import norm   # layer_norm, layer_norm_backward
+    from avelang_kernels import norm   # layer_norm, rms_norm, rms_norm_int8, ...
 
 They are the modules of ``avelang_b200`` themselves (one implementation under two import paths); importing them registers the ``torch.ops.avelang_gdn``
 operators through which every entry point reaches the C library."""
