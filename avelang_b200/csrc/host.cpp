@@ -13,8 +13,10 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/InferenceMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -167,7 +169,13 @@ PyObject* wrap_pair(const Tensor& a, const Tensor& b) {
 const void* ptr(const Tensor* t) { return t != nullptr && t->numel() > 0 ? t->data_ptr() : nullptr; }
 template <class T>
 T* ptr_as(const Tensor* t) { return reinterpret_cast<T*>(const_cast<void*>(ptr(t))); }
+// Fresh memory beside `like`.  Where nothing watches (no dispatch mode, an ordinary tensor on the current device) it comes from torch's allocator without a round through the
+// dispatcher, which costs a call with three results more than its kernel's launch.
 Tensor empty(at::IntArrayRef shape, at::ScalarType dt, const Tensor& like) {
+  if (__builtin_expect(like.is_cuda() && !like.key_set().has(c10::DispatchKey::Python) && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+                           like.get_device() == c10::cuda::current_device() && !at::globalContext().deterministicAlgorithms(),
+                       1))
+    return Tensor(at::detail::empty_generic(shape, c10::cuda::CUDACachingAllocator::get(), c10::DispatchKeySet(c10::DispatchKey::CUDA), dt, std::nullopt));
   return at::empty(shape, like.options().dtype(dt).requires_grad(false));
 }
 // fp32, contiguous; the tensor itself when it is both already
