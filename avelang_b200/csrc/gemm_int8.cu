@@ -68,7 +68,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile uint32_t abort_flag, issued[2];  // stages whose copies the leader's and the other CTA's producer have asked for (kept by the leader)
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // (uniform to the compiler, and with it tiles, rows and addresses)
   const uint32_t rank = tc::cluster_rank();
   const int mt = (int)((M + PAIR_ROWS - 1) / PAIR_ROWS), nt = (int)((N + bn - 1) / bn), kb_count = (int)((K + KS * BK - 1) / (KS * BK));  // in stages of KS blocks
   const uint32_t b_bytes = (uint32_t)(bn / 2 * BK), stage_bytes = KS * (BM * BK + b_bytes);
@@ -240,28 +240,33 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           T* dst = reinterpret_cast<T*>(e.c) + row0 * e.ldc + col0 + c;
           const bool odd0 = ((reinterpret_cast<uintptr_t>(dst) >> 1) & 1) != 0, flip = (e.ldc & 1) != 0;
           const uint32_t place = (uint32_t)(((lane >> 2) << 4) + (lane & 3) * 4);
-#pragma unroll 1
-          for (int i0 = 0; i0 < live; i0 += 8, dst += 8 * e.ldc) {
+          auto eight = [&](int i0, auto all) {  // rows i0 .. i0 + 7; `all`: each exists
             uint32_t w[8];  // (loads and stores of eight rows apart: one behind the other they wait for each other)
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const uint32_t*>(out + (i0 + j) * 128 + (place ^ (uint32_t)(j << 4)));
             T* to = dst;
 #pragma unroll
             for (int j = 0; j < 8; ++j, to += e.ldc) {
+              const bool there = decltype(all)::value || i0 + j < live;
               if constexpr (sizeof(T) == 4) {
-                if (lane < width && i0 + j < live) *reinterpret_cast<uint32_t*>(to + lane) = w[j];
+                if (lane < width && there) *reinterpret_cast<uint32_t*>(to + lane) = w[j];
               } else {
                 const uint32_t behind = __shfl_down_sync(0xffffffffu, w[j], 1);
                 const bool odd = odd0 != (flip && (j & 1) != 0);
                 const int k = 2 * lane + (odd ? 1 : 0);
                 const uint32_t v = __byte_perm(w[j], behind, odd ? 0x5432 : 0x3210);
-                if (i0 + j < live) {
+                if (there) {
                   if (k + 1 < width) *reinterpret_cast<uint32_t*>(to + k) = v;
                   const bool begin = odd && lane == 0;
                   if (begin || k + 1 == width) *reinterpret_cast<uint16_t*>(to + (begin ? 0 : k)) = (uint16_t)(begin ? w[j] : v);
                 }
               }
             }
+          };
+#pragma unroll 1
+          for (int i0 = 0; i0 < live; i0 += 8, dst += 8 * e.ldc) {
+            if (i0 + 8 <= live) eight(i0, std::true_type());
+            else eight(i0, std::false_type());
           }
           __syncwarp();
         }
