@@ -1390,6 +1390,8 @@ PyObject* rms_norm(PyObject* const* p) {
     h2 = result_rows(h, "sum_out");
   }
   if (sum_out != nullptr) REQ(same_or_apart(x2, h2) && same_or_apart(r2, h2), "sum_out must be x or residual themselves or share no element with them");
+  if (w != nullptr)  // (read for every row)
+    REQ((out == nullptr || !ranges_meet(*out, *w)) && (sum_out == nullptr || !ranges_meet(*sum_out, *w)), "out and sum_out must share no memory with weight");
   const bool zero_centered = truth(p[4]);
   if constexpr (kInt8) {
     const auto [q, scale] = empty_int8(x);

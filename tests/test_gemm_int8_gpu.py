@@ -41,7 +41,7 @@ def make(m, n, k, seed, dt, bias):
 
 SIZES = [(1, 1, 1), (1, 16, 16), (1, 12352, 2048), (2, 130, 33), (3, 1544, 2048), (4, 100, 8192), (5, 7, 100), (8, 2048, 4096), (9, 257, 640), (16, 4096, 512), (17, 12352, 256), (33, 48, 1000),
          (64, 2048, 4096), (100, 1544, 127), (128, 256, 128), (129, 255, 129), (200, 12352, 384), (256, 512, 2048), (300, 1000, 1999), (1000, 1544, 200), (1003, 4104, 96), (2500, 300, 72), (4096, 2048, 256), (2900, 2571, 100),
-         (5000, 1032, 513), (257, 20000, 64), (130, 19003, 1000), (10000, 1540, 33)]
+         (5000, 1032, 513), (257, 20000, 64), (130, 19003, 1000), (10000, 1540, 33), (2, 40000, 64), (20, 40001, 80), (128, 38000, 48)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -232,3 +232,34 @@ def test_a_layer_s_step(built_lib, tokens):
     yd = torch.tanh((hd / torch.sqrt(hd.square().mean(-1, keepdim=True) + 1e-6) * w.double()) @ w_in.double().t()) @ w_out.double().t()
     want = hd + yd
     assert float((total.cpu().double() - want).norm() / want.norm()) < 0.02
+
+
+@pytest.mark.parametrize("n", [12352, 12351])
+def test_offsets_beyond_32_bits(built_lib, n):
+    """A result of more than 2^31 elements: its first and last rows, and those around the element 2^31."""
+    from avelang_b200 import gemm
+    m, k = 180000, 32
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    a, b = (torch.randint(-128, 128, (r, k), generator=gen, dtype=torch.int8, device="cuda") for r in (m, n))
+    sa, sb = torch.rand(m, generator=gen, device="cuda"), torch.rand(n, generator=gen, device="cuda")
+    got = gemm.gemm_int8_transposed_b(a, b, sa, sb)
+    for at in (0, (1 << 31) // n - 1, m - 3):
+        rows = slice(at, at + 3)
+        check(got[rows], a[rows].cpu(), b.cpu(), sa[rows].cpu(), sb.cpu(), None)
+
+
+def test_rows_of_operands_beyond_32_bits(built_lib):
+    """Rows of B more than 2^31 bytes apart from the first, in every form."""
+    from avelang_b200 import gemm
+    n, k, pitch = 40, 200, 1 << 26
+    pool = torch.empty(n * pitch, dtype=torch.int8, device="cuda")
+    b = pool.as_strided((n, k), (pitch, 1))
+    b.copy_(torch.randint(-128, 128, (n, k), dtype=torch.int8, device="cuda"))
+    sb = torch.rand(n, device="cuda") + 0.5
+    for m in (1, 2, 30, 100, 300):
+        a = torch.randint(-128, 128, (m, 208), dtype=torch.int8, device="cuda")[:, :k]
+        sa = torch.rand(m, device="cuda") + 0.5
+        got = gemm.gemm_int8_transposed_b(a, b, sa, sb, out_dtype=torch.float32)
+        check(got, a.cpu(), b.cpu(), sa.cpu(), sb.cpu(), None)
+    del b, pool
+    torch.cuda.empty_cache()

@@ -98,6 +98,8 @@ def test_norm_refusals(built_lib):
             ("out must be x or residual themselves", lambda: N.rms_norm(bf(4, 64), w, residual=wide[:4], out=wide[1:5])),
             ("out and sum_out must share no element", lambda: N.rms_norm(x, w, residual=bf(4, 64), out=x, sum_out=x)),
             ("out and sum_out must share no element", lambda: N.rms_norm(x, w, residual=x, out=wide[:4], sum_out=wide[3:7])),
+            ("must share no memory with weight", lambda: N.rms_norm(x, wide[3], out=wide[:4])),
+            ("must share no memory with weight", lambda: N.rms_norm(x, wide[3], residual=bf(4, 64), sum_out=wide[:4])),
             ("d_y must be a torch.bfloat16 tensor", lambda: N.rms_norm_backward(f32(4, 64), x, f32(4), w)),
             ("d_sum must be a torch.bfloat16 tensor", lambda: N.rms_norm_backward(x, x, f32(4), w, d_sum=bf(64))),
             ("rstd must be a contiguous fp32 tensor of 4", lambda: N.rms_norm_backward(x, x, f32(5), w)),

@@ -305,3 +305,30 @@ def test_captured_steps_and_streams(built_lib):
         torch.cuda.synchronize()
         for want, out, other in zip(wants, outs, sides):
             assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, out, other))
+
+
+@pytest.mark.parametrize("n", [2048, 2047])
+def test_offsets_beyond_32_bits(built_lib, n):
+    """More than 2^31 elements: the first and the last rows, and those around the element 2^31, in the norm, its 8-bit form, its gradients and the way back from 8 bits."""
+    from avelang_b200 import gemm, norm
+    rows = 1050000
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(rows, n, generator=gen, device="cuda", dtype=torch.bfloat16)
+    w = torch.rand(n, generator=gen, device="cuda") + 0.5
+    parts = [slice(at, at + 3) for at in (0, (1 << 31) // n - 1, rows - 3)]
+    y, h, rstd = norm.rms_norm(x, w, residual=x, return_stats=True)
+    for p in parts:
+        check_norm(y[p], h[p], rstd[p], x[p].cpu(), x[p].cpu(), w.cpu(), False, 1e-6)
+    q, scale = norm.rms_norm_int8(x, w)
+    back = gemm.dequantize_rows_int8(q, scale)
+    for p in parts:
+        check_int8(q[p], scale[p], reference(x[p].cpu(), None, w.cpu(), False, 1e-6)[2])
+        assert torch.equal(back[p], (q[p].float() * scale[p][:, None]).bfloat16())
+    del q, back
+    dx, _ = norm.rms_norm_backward(y, h, rstd, w, d_sum=x)
+    for p in parts:
+        ref, loss, _, _ = gradients(y[p].cpu(), h[p].cpu(), rstd[p].cpu(), w.cpu(), x[p].cpu(), False)
+        e = half(x.dtype)
+        assert ((dx[p].cpu().double() - ref).abs() <= e * ref.abs() + (1 + e) * loss + tiny(x.dtype)).all()
+    del x, y, h, dx
+    torch.cuda.empty_cache()
