@@ -62,7 +62,7 @@ constexpr int PAIR_OUT = PAIR_RING, PAIR_COLS = PAIR_OUT + 8 * 4096, PAIR_SMEM =
 template <class T, int KS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC, const Epilogue e,
-                      int64_t M, int64_t N, int64_t K, uint32_t* status, int bn, int stages) {
+                      int64_t M, int64_t N, int64_t K, uint32_t* status, int bn, int stages, uint32_t whole) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = tc::align1024(smem_raw);
   __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], drained;
@@ -72,12 +72,18 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const uint32_t rank = tc::cluster_rank();
   const int mt = (int)((M + PAIR_ROWS - 1) / PAIR_ROWS), nt = (int)((N + bn - 1) / bn), kb_count = (int)((K + KS * BK - 1) / (KS * BK));  // in stages of KS blocks
   const uint32_t b_bytes = (uint32_t)(bn / 2 * BK), stage_bytes = KS * (BM * BK + b_bytes);
-  const uint32_t tiles = (uint32_t)mt * (uint32_t)nt, first = blockIdx.x / 2, step = gridDim.x / 2;
-  auto tile_at = [&](uint32_t tile, int& m, int& n) {
-    const uint32_t per = (uint32_t)(GROUP_M * nt), group = tile / per, r = tile - group * per, rows = min((uint32_t)GROUP_M, (uint32_t)mt - group * GROUP_M);
-    n = (int)(r / rows);
-    m = (int)(group * GROUP_M + r - (uint32_t)n * rows);
+  // Units of work: the first `whole` tiles, then the halves (of the columns) of those that are left.  B comes in boxes of half of a CTA's rows where there are halves.
+  const uint32_t all_tiles = (uint32_t)mt * (uint32_t)nt, tiles = whole + 2 * (all_tiles - whole), first = blockIdx.x / 2, step = gridDim.x / 2;
+  const bool halves = whole < all_tiles;
+  auto width_at = [&](uint32_t unit) { return unit < whole ? bn : bn / 2; };
+  auto tile_at = [&](uint32_t unit, int& m, int64_t& col, int& width) {
+    const uint32_t tile = unit < whole ? unit : whole + (unit - whole) / 2, per = (uint32_t)(GROUP_M * nt), group = tile / per, r = tile - group * per,
+                   rows = min((uint32_t)GROUP_M, (uint32_t)mt - group * GROUP_M), n = r / rows;
+    m = (int)(group * GROUP_M + r - n * rows);
+    width = width_at(unit);
+    col = (int64_t)n * bn + (unit >= whole && ((unit - whole) & 1) != 0 ? width : 0);
   };
+  auto landing = [&](int width) { return KS * (uint32_t)((BM + width / 2) * BK); };  // bytes of a stage of one CTA
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
@@ -102,18 +108,22 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     uint32_t turns = 0;
     bool ok = true;
     for (uint32_t tile = first; tile < tiles && ok; tile += step) {
-      int m, n;
-      tile_at(tile, m, n);
+      int m, width;
+      int64_t col;
+      tile_at(tile, m, col, width);
+      const int row_b = (int)col + (int)rank * (width / 2);
+      const bool second = halves && width == bn;
       for (int kb = 0; kb < kb_count; ++kb) {
         if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
         if (tc::elect_one()) {
           uint8_t* st = smem + s * (int)stage_bytes;
           const uint32_t bar = tc::mapa(tc::smem_u32(&full[s]), 0);
-          if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * stage_bytes);
+          if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * landing(width));
 #pragma unroll
           for (int j = 0; j < KS; ++j) {
             tc::tma_load_2d_pair(st + j * BM * BK, &tmA, bar, (kb * KS + j) * BK, m * PAIR_ROWS + (int)rank * BM);
-            tc::tma_load_2d_pair(st + KS * BM * BK + j * (int)b_bytes, &tmB, bar, (kb * KS + j) * BK, n * bn + (int)rank * (bn / 2));
+            tc::tma_load_2d_pair(st + KS * BM * BK + j * (int)b_bytes, &tmB, bar, (kb * KS + j) * BK, row_b);
+            if (second) tc::tma_load_2d_pair(st + KS * BM * BK + j * (int)b_bytes + bn / 4 * BK, &tmB, bar, (kb * KS + j) * BK, row_b + bn / 4);
           }
         }
         __syncwarp();
@@ -129,12 +139,13 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     if (lane == 0) tc::st_cluster_u32(tc::mapa(tc::smem_u32(const_cast<uint32_t*>(&issued[rank])), 0), turns);
   } else if (warp == 1) {
     if (rank == 0) {
-      const uint32_t idesc = idesc_i8(PAIR_ROWS, bn), stage0 = (tc::smem_u32(smem) >> 4) | (uint32_t)tc::desc_lo(0, 16);
+      const uint32_t stage0 = (tc::smem_u32(smem) >> 4) | (uint32_t)tc::desc_lo(0, 16);
       constexpr uint32_t hi = tc::desc_hi(1024, true);
       int s = 0, local = 0; uint32_t ph = 0;
       bool ok = true;
       for (uint32_t tile = first; tile < tiles; tile += step, ++local) {
         const int buf = local & 1;
+        const uint32_t idesc = idesc_i8(PAIR_ROWS, width_at(tile));
         if (!tc::mbar_wait_cluster(&acc_empty[buf], ((uint32_t)(local >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
         tc::tc_fence_after_sync();
         const uint32_t d = tmem_base + (uint32_t)buf * BN;
@@ -167,14 +178,15 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     float* cols = reinterpret_cast<float*>(smem + PAIR_COLS) + (warp - 2) * 256;  // scales and bias of this warp's columns, CW of a chunk behind those of the one before
     // The scales of a tile are fetched while the one before is finished (fetched and waited for in line they took 1600 to 1900 cycles a tile).
     float next_scale[4], next_bias[4], next_a = 0.f;
-    int next_m = 0, next_n = 0;
+    int next_m = 0, next_width = 0;
+    int64_t next_col = 0;
     auto prefetch = [&](uint32_t tile) {
       if (tile >= tiles) return;
-      tile_at(tile, next_m, next_n);
+      tile_at(tile, next_m, next_col, next_width);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = lane + 32 * j;
-        const int64_t c = (int64_t)next_n * bn + (i / CW * 2 + half) * CW + i % CW;
+        const int64_t c = next_col + (i / CW * 2 + half) * CW + i % CW;
         next_scale[j] = c < N ? e.b_scale[c] : 0.f;
         next_bias[j] = c < N ? bias_at<T>(e, c) : 0.f;
       }
@@ -184,9 +196,9 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     prefetch(first);
     int local = 0;
     for (uint32_t tile = first; tile < tiles; tile += step, ++local) {
-      const int m = next_m, n = next_n, buf = local & 1;
-      const int64_t row0 = (int64_t)m * PAIR_ROWS + rank * BM + quarter * 32, col0 = (int64_t)n * bn;
-      const int n_left = (int)min((int64_t)bn, N - col0);
+      const int m = next_m, width_now = next_width, buf = local & 1;
+      const int64_t row0 = (int64_t)m * PAIR_ROWS + rank * BM + quarter * 32, col0 = next_col;
+      const int n_left = (int)min((int64_t)width_now, N - col0);  // (of a second half possibly none)
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 4; ++j) { cols[lane + 32 * j] = next_scale[j]; cols[128 + lane + 32 * j] = next_bias[j]; }
@@ -286,8 +298,9 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   if (abort_flag != 0u) {  // in both or in neither: copies and products may be on their way, and all are counted at the leader's barriers
     if (rank == 0 && threadIdx.x == 0) {
       const uint32_t own = issued[0], other = issued[1], all = own > other ? own : other, begin = all > (uint32_t)stages ? all - (uint32_t)stages : 0u;
-      for (uint32_t i = own; i < other; ++i) tc::mbar_expect_tx(&full[i % stages], stage_bytes);       // the other CTA's alone
-      for (uint32_t i = other; i < own; ++i) tc::mbar_complete_tx(&full[i % stages], stage_bytes);    // this one's alone
+      auto bytes = [&](uint32_t i) { return landing(width_at(first + i / (uint32_t)kb_count * step)); };
+      for (uint32_t i = own; i < other; ++i) tc::mbar_expect_tx(&full[i % stages], bytes(i));       // the other CTA's alone
+      for (uint32_t i = other; i < own; ++i) tc::mbar_complete_tx(&full[i % stages], bytes(i));    // this one's alone
       for (uint32_t i = begin; i < all; ++i) tc::drain(&full[i % stages], i / stages & 1u);
     }
     if (rank == 0 && warp == 1) {
@@ -617,25 +630,30 @@ int launch_stream(const AveGemmInt8Args& a, const Epilogue& e, cudaStream_t stre
 // pair has one tile at most (the narrow ones wait for their operands, 20 to 28 KB a CTA and block), and 208, 277, 347 and 417 where all are busy for longer (L2 and the power cap;
 // 8192 x 2048 x 4096 with 256 columns 55 us, 61 with 192), a tile's results at least 9 ns a column, and launch, first operands and last results 4 us and 6 ns a column.
 // `across`: rows of operands that do not lie on 128 bytes, whose blocks reach across two lines each (256 rows x 1544 x 2048 6.1 us, with 1999 of 2000 bytes 8.2).
-struct Width { int bn; int64_t ns; };
+struct Width { int bn; int64_t ns; bool halves; };  // halves: the last turn's tiles are taken as two each
 Width pair_width(int64_t M, int64_t N, int64_t K, bool across, int pairs) {
   constexpr int alone_ns[4] = {112, 138, 194, 265}, busy_ns[4] = {208, 277, 347, 417};
   const int64_t mt = (M + PAIR_ROWS - 1) / PAIR_ROWS, kb = (K + BK - 1) / BK;
-  Width best{0, INT64_MAX};
+  Width best{0, INT64_MAX, false};
   for (int bn = BN; bn >= 64; bn -= 64) {
     const int64_t turns = (mt * ((N + bn - 1) / bn) + pairs - 1) / pairs, block = (turns > 1 ? busy_ns : alone_ns)[bn / 64 - 1];
     const int64_t products = kb * block * (across ? 4 : 3) / 3, results = 300 + 9 * bn;
-    const int64_t ns = 4000 + 6 * bn + turns * (products > results ? products : results);
-    if (ns < best.ns) best = {bn, ns};
+    const int64_t turn = products > results ? products : results, left = mt * ((N + bn - 1) / bn) % pairs;
+    // a last turn of at most half of the pairs in halves: their products take two thirds of the time (8192 x 2048 x 4096, 3.5 turns, 55 us, 50
+    // so; 2048 x 12352 x 2048 43 and 41)
+    const bool halves = bn == BN && turns > 1 && left > 0 && 2 * left <= pairs;
+    const int64_t ns = 4000 + 6 * bn + turns * turn - (halves ? turn / 3 : 0);
+    if (ns < best.ns) best = {bn, ns, halves};
   }
   return best;
 }
 template <class T>
-int launch_pairs(const AveGemmInt8Args& a, const Epilogue& e, int bn, int pairs, cudaStream_t stream) {
+int launch_pairs(const AveGemmInt8Args& a, const Epilogue& e, const Width& width, int pairs, cudaStream_t stream) {
+  const int bn = width.bn;
   CUtensorMap tmA, tmB, tmC{};
   int rc = operand_map(&tmA, a.a, a.M, a.K, a.lda, BM);
   if (rc != AVE_GDN_OK) return rc;
-  rc = operand_map(&tmB, a.b, a.N, a.K, a.ldb, bn / 2);
+  rc = operand_map(&tmB, a.b, a.N, a.K, a.ldb, width.halves ? bn / 4 : bn / 2);
   if (rc != AVE_GDN_OK) return rc;
   if (e.vector != 0) {
     const uint64_t size = sizeof(T), dims[2] = {(uint64_t)a.N, (uint64_t)a.M}, strides[2] = {size, (uint64_t)a.ldc * size};
@@ -646,13 +664,14 @@ int launch_pairs(const AveGemmInt8Args& a, const Epilogue& e, int bn, int pairs,
   }
   const int64_t tiles = ((a.M + PAIR_ROWS - 1) / PAIR_ROWS) * ((a.N + bn - 1) / bn);
   if (tiles > INT32_MAX) return AVE_GDN_UNSUPPORTED;
+  const uint32_t whole = (uint32_t)(width.halves ? tiles / pairs * pairs : tiles);
   auto launch = [&](auto blocks) {
     constexpr int KS = decltype(blocks)::value;
     constexpr auto* kernel = &gemm_int8_pair_kernel<T, KS>;
     const int rc = allow_smem<kernel>(PAIR_SMEM);
     if (rc != AVE_GDN_OK) return rc;
     const int fit = PAIR_RING / (KS * (BM + bn / 2) * BK), stages = fit < PAIR_STAGES ? fit : PAIR_STAGES;
-    AVE_CUDA_TRY(launch_after(kernel, (unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, PAIR_SMEM, stream, tmA, tmB, tmC, e, a.M, a.N, a.K, a.status, bn, stages));
+    AVE_CUDA_TRY(launch_after(kernel, (unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, PAIR_SMEM, stream, tmA, tmB, tmC, e, a.M, a.N, a.K, a.status, bn, stages, whole));
     return (int)AVE_GDN_OK;
   };
   if (bn <= 128) return launch(std::integral_constant<int, 2>());
@@ -676,7 +695,7 @@ int launch_t(const AveGemmInt8Args& a, cudaStream_t stream) {
   const Width width = pair_width(a.M, a.N, a.K, a.lda % 128 != 0 || a.ldb % 128 != 0, pairs);
   Plan plan{};
   if (a.M <= BM) plan = make_plan(a.M, a.N, a.K, clusters);
-  if (plan.bn == 0 || (a.M >= 64 && width.ns <= 4200 + plan.cost / 60)) return launch_pairs<T>(a, e, width.bn, pairs, stream);
+  if (plan.bn == 0 || (a.M >= 64 && width.ns <= 4200 + plan.cost / 60)) return launch_pairs<T>(a, e, width, pairs, stream);
   CUtensorMap tmA, tmB;
   int rc = operand_map(&tmA, a.a, a.M, a.K, a.lda, plan.a_rows);
   if (rc != AVE_GDN_OK) return rc;

@@ -41,7 +41,7 @@ def make(m, n, k, seed, dt, bias):
 
 SIZES = [(1, 1, 1), (1, 16, 16), (1, 12352, 2048), (2, 130, 33), (3, 1544, 2048), (4, 100, 8192), (5, 7, 100), (8, 2048, 4096), (9, 257, 640), (16, 4096, 512), (17, 12352, 256), (33, 48, 1000),
          (64, 2048, 4096), (100, 1544, 127), (128, 256, 128), (129, 255, 129), (200, 12352, 384), (256, 512, 2048), (300, 1000, 1999), (1000, 1544, 200), (1003, 4104, 96), (2500, 300, 72), (4096, 2048, 256), (2900, 2571, 100),
-         (5000, 1032, 513), (257, 20000, 64), (130, 19003, 1000), (10000, 1540, 33), (2, 40000, 64), (20, 40001, 80), (128, 38000, 48)]
+         (5000, 1032, 513), (257, 20000, 64), (130, 19003, 1000), (10000, 1540, 33), (2, 40000, 64), (20, 40001, 80), (128, 38000, 48), (2560, 2304, 700), (2100, 2500, 130), (5120, 1050, 96), (4864, 1153, 40), (1300, 4100, 65)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
