@@ -114,7 +114,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       const int row_b = (int)col + (int)rank * (width / 2);
       const bool second = halves && width == bn;
       for (int kb = 0; kb < kb_count; ++kb) {
-        if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+        if (!tc::mbar_wait_together(&empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
         if (tc::elect_one()) {
           uint8_t* st = smem + s * (int)stage_bytes;
           const uint32_t bar = tc::mapa(tc::smem_u32(&full[s]), 0);
@@ -133,7 +133,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     }
     if (ok)  // the leader's last arrivals at this CTA's barriers
       for (uint32_t i = 0; i < (uint32_t)stages && i < turns; ++i) {
-        if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) break;
+        if (!tc::mbar_wait_together(&empty[s], ph ^ 1u, &abort_flag)) break;
         if (++s == stages) { s = 0; ph ^= 1u; }
       }
     if (lane == 0) tc::st_cluster_u32(tc::mapa(tc::smem_u32(const_cast<uint32_t*>(&issued[rank])), 0), turns);
@@ -146,11 +146,11 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       for (uint32_t tile = first; tile < tiles; tile += step, ++local) {
         const int buf = local & 1;
         const uint32_t idesc = idesc_i8(PAIR_ROWS, width_at(tile));
-        if (!tc::mbar_wait_cluster(&acc_empty[buf], ((uint32_t)(local >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
+        if (!tc::mbar_wait_together<true>(&acc_empty[buf], ((uint32_t)(local >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
         tc::tc_fence_after_sync();
         const uint32_t d = tmem_base + (uint32_t)buf * BN;
         for (int kb = 0; kb < kb_count; ++kb) {
-          if (!tc::mbar_wait_unrolled(&full[s], ph, &abort_flag)) { ok = false; break; }
+          if (!tc::mbar_wait_together(&full[s], ph, &abort_flag)) { ok = false; break; }
           tc::tc_fence_after_sync();
           if (tc::elect_one()) {
             const uint32_t a_lo = stage0 + (uint32_t)s * (stage_bytes >> 4);  // low words of the descriptors; the high ones are constant
@@ -205,7 +205,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       const float a_scale = next_a;
       __syncwarp();
       prefetch(tile + step);
-      if (!tc::mbar_wait_unrolled(&acc_full[buf], (uint32_t)(local >> 1) & 1u, &abort_flag)) break;
+      if (!tc::mbar_wait_together(&acc_full[buf], (uint32_t)(local >> 1) & 1u, &abort_flag)) break;
       tc::tc_fence_after_sync();
       auto release = [&] {  // this warp's part of the accumulator is out of tensor memory
         tc::tc_fence_before_sync();
@@ -366,7 +366,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     int s = 0; uint32_t ph = 0;
     int kb = kb0;
     for (; kb < kb1; ++kb) {
-      if (!tc::mbar_wait_unrolled(&empty[s], ph ^ 1u, &abort_flag)) break;
+      if (kb - kb0 >= stages && !tc::mbar_wait_together(&empty[s], ph ^ 1u, &abort_flag)) break;
       if (tc::elect_one()) {
         uint8_t* st = smem + s * stage_bytes;
         tc::mbar_expect_tx(&full[s], (uint32_t)stage_bytes);
@@ -383,7 +383,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     int s = 0; uint32_t ph = 0;
     bool ok = true;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!tc::mbar_wait_unrolled(&full[s], ph, &abort_flag)) { ok = false; break; }
+      if (!tc::mbar_wait_together(&full[s], ph, &abort_flag)) { ok = false; break; }
       tc::tc_fence_after_sync();
       if (tc::elect_one()) {
         // with fewer than 128 rows in the A tile the MMA reads whatever lies behind it: those lanes are never read back
@@ -404,13 +404,14 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
   }
   __syncwarp();  // the other lanes of the issuing warps must not poll beside them
   // the accumulator is complete, so every operand tile has landed and been read
-  const bool ok = tc::mbar_wait_unrolled(&acc_full, 0, &abort_flag);
+  (void)tc::mbar_wait_unrolled(&acc_full, 0, &abort_flag);
   tc::tc_fence_after_sync();
   __syncwarp();
-  if (!ok && warp == 1) tc::drain_mmas(&drained);
   tc::cluster_sync();  // ... in every CTA of the cluster: the rings may be overwritten
+  const bool ok = abort_flag == 0u;  // (all waits are over: the same for the whole CTA)
+  if (!ok && warp == 1) tc::drain_mmas(&drained);
   const int rows = (int)M, slice = (rows + split - 1) / split, pitch = bn + 4;
-  if (ok && warp >= 2) {
+  if (warp >= 2) {
     const int row = (warp & 3) * 32 + lane;
     const bool live = row < rows;
     const int owner = live ? row / slice : 0;
