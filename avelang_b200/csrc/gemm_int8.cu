@@ -131,8 +131,8 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (++s == stages) { s = 0; ph ^= 1u; }
       }
     }
-    if (ok)  // the leader's last arrivals at this CTA's barriers
-      for (uint32_t i = 0; i < (uint32_t)stages && i < turns; ++i) {
+    if (ok)  // the leader's last arrivals at this CTA's barriers (a stage that was never filled counts as free)
+      for (int i = 0; i < stages; ++i) {
         if (!tc::mbar_wait_together(&empty[s], ph ^ 1u, &abort_flag)) break;
         if (++s == stages) { s = 0; ph ^= 1u; }
       }

@@ -158,6 +158,12 @@ def test_clusters(tmp_path, dtype, blocks, ctas):
     assert done.returncode == 0, done.stdout + done.stderr
 
 
+def test_pairs_with_fewer_blocks_than_stages(tmp_path):
+    """Arrivals of finished products that are as late as the whole tile: neither CTA ends in front of them."""
+    done = run(tmp_path, SOURCE, True, "__nv_bfloat16", 2, [(256, 66, 100, 64, 9, 99, 80, 8), (200, 130, 300, 128, 4, 99, 130, 0)], 12, late=150, far=3000000)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
 @pytest.mark.parametrize("dtype,blocks", list(PAIRS))
 def test_pairs_behind_an_expired_wait(tmp_path, dtype, blocks):
     """Operands, products and arrivals that come late, waits that some lanes of a warp have given up and others have not: every CTA comes to its end."""
