@@ -67,7 +67,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   uint8_t* smem = tc::align1024(smem_raw);
   __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile uint32_t abort_flag, issued[2];  // stages whose copies the leader's and the other CTA's producer have asked for (kept by the leader)
+  __shared__ volatile uint32_t abort_flag, issued[2], ended[2];  // stages whose copies the leader's and the other CTA's producer have asked for (kept by the leader); stages and tiles whose products the leader has issued
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // (uniform to the compiler, and with it tiles, rows and addresses)
   const uint32_t rank = tc::cluster_rank();
   const int mt = (int)((M + PAIR_ROWS - 1) / PAIR_ROWS), nt = (int)((N + bn - 1) / bn), kb_count = (int)((K + KS * BK - 1) / (KS * BK));  // in stages of KS blocks
@@ -90,7 +90,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     for (int b = 0; b < 2; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], 16); }
     tc::mbar_init(&drained, 1);
     abort_flag = 0;
-    issued[0] = issued[1] = 0;
+    issued[0] = issued[1] = ended[0] = ended[1] = 0;
     tc::fence_barrier_init();
     tc::prefetch_tmap(&tmA);
     tc::prefetch_tmap(&tmB);
@@ -141,7 +141,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     if (rank == 0) {
       const uint32_t stage0 = (tc::smem_u32(smem) >> 4) | (uint32_t)tc::desc_lo(0, 16);
       constexpr uint32_t hi = tc::desc_hi(1024, true);
-      int s = 0, local = 0; uint32_t ph = 0;
+      int s = 0, local = 0; uint32_t ph = 0, blocks = 0;
       bool ok = true;
       for (uint32_t tile = first; tile < tiles; tile += step, ++local) {
         const int buf = local & 1;
@@ -163,12 +163,14 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             tc::mma_commit_pair(&empty[s]);
           }
           __syncwarp();
+          ++blocks;
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
         if (!ok) break;
         if (tc::elect_one()) tc::mma_commit_pair(&acc_full[buf]);
         __syncwarp();
       }
+      if (lane < 4) tc::st_cluster_u32(tc::mapa(tc::smem_u32(const_cast<uint32_t*>(&ended[lane & 1])), (uint32_t)lane >> 1), (lane & 1) == 0 ? blocks : (uint32_t)local);
     }
   } else {
     const int quarter = warp & 3;  // tensor memory lanes this warp may touch
@@ -301,7 +303,12 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     tc::st_cluster_u32(tc::mapa(tc::smem_u32(const_cast<uint32_t*>(&abort_flag)), rank ^ 1u), 1u);
   }
   tc::cluster_sync();  // neither CTA ends, or gives tensor memory back, while the other may reach it
-  if (abort_flag != 0u) {  // in both or in neither: copies and products may be on their way, and all are counted at the leader's barriers
+  if (abort_flag != 0u) {  // in both or in neither: copies and products may be on their way, all counted at the leader's barriers, and arrivals of finished products at either's
+    if (threadIdx.x == 0) {
+      const uint32_t blocks = ended[0], accs = ended[1];
+      for (uint32_t i = blocks > (uint32_t)stages ? blocks - (uint32_t)stages : 0u; i < blocks; ++i) tc::drain(&empty[i % stages], i / stages & 1u);
+      for (uint32_t i = accs > 2u ? accs - 2u : 0u; i < accs; ++i) tc::drain(&acc_full[i & 1u], i >> 1 & 1u);
+    }
     if (rank == 0 && threadIdx.x == 0) {
       const uint32_t own = issued[0], other = issued[1], all = own > other ? own : other, begin = all > (uint32_t)stages ? all - (uint32_t)stages : 0u;
       auto bytes = [&](uint32_t i) { return landing(width_at(first + i / (uint32_t)kb_count * step)); };
@@ -309,8 +316,8 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       for (uint32_t i = other; i < own; ++i) tc::mbar_complete_tx(&full[i % stages], bytes(i));    // this one's alone
       for (uint32_t i = begin; i < all; ++i) tc::drain(&full[i % stages], i / stages & 1u);
     }
-    if (rank == 0 && warp == 1) {
-      if (tc::elect_one()) tc::mma_commit_pair(&drained);
+    if (warp == 1) {
+      if (rank == 0 && tc::elect_one()) tc::mma_commit_pair(&drained);
       __syncwarp();
       tc::drain(&drained, 0u);
     }

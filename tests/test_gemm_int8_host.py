@@ -166,8 +166,9 @@ def test_pairs_with_fewer_blocks_than_stages(tmp_path):
 
 @pytest.mark.parametrize("dtype,blocks", list(PAIRS))
 def test_pairs_behind_an_expired_wait(tmp_path, dtype, blocks):
-    """Operands, products and arrivals that come late, waits that some lanes of a warp have given up and others have not: every CTA comes to its end."""
-    done = run(tmp_path, SOURCE, True, dtype, blocks, PAIRS[dtype, blocks], 16, late=4, far=4000000, limit=100, level=0)
+    """Operands, products and arrivals that come late, waits that some lanes of a warp have given up and others have not: every CTA comes to its end, with
+    nothing on its way into it."""
+    done = run(tmp_path, SOURCE, True, dtype, blocks, PAIRS[dtype, blocks], 16, late=4, far=4000000, limit=100, level=1)
     assert done.returncode == 0, done.stdout + done.stderr
 
 
