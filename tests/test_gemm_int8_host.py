@@ -174,5 +174,5 @@ def test_pairs_behind_an_expired_wait(tmp_path, dtype, blocks):
 
 @pytest.mark.parametrize("dtype,blocks,ctas", list(CLUSTERS))
 def test_clusters_behind_an_expired_wait(tmp_path, dtype, blocks, ctas):
-    done = run(tmp_path, SOURCE, False, dtype, blocks, CLUSTERS[dtype, blocks, ctas], 16, late=4, far=4000000, limit=400, level=0, ctas=ctas)
+    done = run(tmp_path, SOURCE, False, dtype, blocks, CLUSTERS[dtype, blocks, ctas], 16, late=4, far=4000000, limit=400, level=1, ctas=ctas)
     assert done.returncode == 0, done.stdout + done.stderr
