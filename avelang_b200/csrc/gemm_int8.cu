@@ -197,7 +197,8 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     };
     prefetch(first);
     int local = 0;
-    for (uint32_t tile = first; tile < tiles; tile += step, ++local) {
+    uint32_t tile = first;
+    for (; tile < tiles; tile += step, ++local) {
       const int m = next_m, width_now = next_width, buf = local & 1;
       const int64_t row0 = (int64_t)m * PAIR_ROWS + rank * BM + quarter * 32, col0 = next_col;
       const int n_left = (int)min((int64_t)width_now, N - col0);  // (of a second half possibly none)
@@ -293,6 +294,15 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       }
     }
     if (lane == 0) tc::bulk_wait_all();
+    for (; tile < tiles; tile += step) {  // a wait has given up: what this warp leaves unwritten is NaN
+      int m, width;
+      int64_t col;
+      tile_at(tile, m, col, width);
+      const int64_t row = (int64_t)m * PAIR_ROWS + rank * BM + quarter * 32 + lane, n_left = min((int64_t)width, N - col);
+      if (row < M)
+        for (int c = 0; c < n_left; ++c)
+          if ((c / CW & 1) == half) reinterpret_cast<T*>(e.c)[row * e.ldc + col + c] = Elem<T>::down(__uint_as_float(0x7fffffffu));
+    }
   }
 
   __syncwarp();
@@ -340,7 +350,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
   uint8_t* smem = tc::align1024(smem_raw);
   __shared__ uint64_t full[STAGES], empty[STAGES], acc_full, drained;
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile uint32_t abort_flag;
+  __shared__ volatile uint32_t abort_flag, failed;  // of this CTA; of any of the cluster
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bn = plan.bn, split = plan.split, stages = plan.stages;
   const int a_bytes = plan.a_rows * BK, b_bytes = bn * BK, stage_bytes = plan.ks * (a_bytes + b_bytes);
@@ -353,7 +363,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     for (int s = 0; s < stages; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
     tc::mbar_init(&acc_full, 1);
     tc::mbar_init(&drained, 1);
-    abort_flag = 0;
+    abort_flag = failed = 0;
     tc::fence_barrier_init();
     tc::prefetch_tmap(&tmA);
     tc::prefetch_tmap(&tmB);
@@ -421,7 +431,10 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
       __syncwarp();
     };
     if (warp == 1) last(empty);
-    else if (!ok) last(full);
+    else if (!ok) {
+      last(full);
+      if (lane < split) tc::st_cluster_u32(tc::mapa(tc::smem_u32(const_cast<uint32_t*>(&failed)), (uint32_t)lane), 1u);
+    }
     if (!ok && warp == 1) {
       if (turns == kb1 - kb0) tc::drain(&acc_full, 0u);
       tc::drain_mmas(&drained);
@@ -450,6 +463,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
   {
     const int32_t* part = reinterpret_cast<const int32_t*>(smem);
     const int mine = min(slice, rows - rank * slice), vec = bn / 8;
+    const bool whole = failed == 0u;
     for (int i = threadIdx.x; i < mine * vec; i += THREADS) {
       const int r = i / vec, c = (i - r * vec) * 8;
       int32_t x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -459,7 +473,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         x[4] += b.x; x[5] += b.y; x[6] += b.z; x[7] += b.w;
       }
       const int64_t col = (int64_t)tn * bn + c, at = rank * slice + r;
-      const float a_scale = e.a_scale[at];
+      const float a_scale = whole ? e.a_scale[at] : __uint_as_float(0x7fffffffu);  // (sums that miss a share: NaN)
       T* dst = reinterpret_cast<T*>(e.c) + at * e.ldc + col;
       if (e.vector != 0 && col + 8 <= N) {
         float2 f[4];

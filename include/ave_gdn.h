@@ -506,7 +506,8 @@ int ave_quantize_rows_int8(const AveQuantRowsArgs* args, void* stream);
 int ave_dequantize_rows_int8(const AveQuantRowsArgs* args, void* stream);
 
 /* C[m][n] = sum_k A[m][k] B[n][k] * a_scale[m] * b_scale[n] + bias[n]: int8 A and B, exact sums (1 <= K <= 131071), (sum * a_scale) * b_scale + bias in
- * fp32 and one rounding.  Rows of A and B lie on 16 bytes; K need not be a multiple of anything.  An expired wait sets AVE_GDN_DEV_WAIT_EXPIRED. */
+ * fp32 and one rounding.  Rows of A and B lie on 16 bytes; K need not be a multiple of anything.  An expired wait sets AVE_GDN_DEV_WAIT_EXPIRED,
+ * and results that it keeps from being complete are NaN. */
 typedef struct AveGemmInt8Args {
   uint32_t struct_size;
   uint32_t flags;           /* 0 */

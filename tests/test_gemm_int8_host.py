@@ -167,12 +167,12 @@ def test_pairs_with_fewer_blocks_than_stages(tmp_path):
 @pytest.mark.parametrize("dtype,blocks", list(PAIRS))
 def test_pairs_behind_an_expired_wait(tmp_path, dtype, blocks):
     """Operands, products and arrivals that come late, waits that some lanes of a warp have given up and others have not: every CTA comes to its end, with
-    nothing on its way into it."""
-    done = run(tmp_path, SOURCE, True, dtype, blocks, PAIRS[dtype, blocks], 16, late=4, far=4000000, limit=100, level=1)
+    nothing on its way into it, and results are right or NaN."""
+    done = run(tmp_path, SOURCE, True, dtype, blocks, PAIRS[dtype, blocks], 16, late=4, far=4000000, limit=100)
     assert done.returncode == 0, done.stdout + done.stderr
 
 
 @pytest.mark.parametrize("dtype,blocks,ctas", list(CLUSTERS))
 def test_clusters_behind_an_expired_wait(tmp_path, dtype, blocks, ctas):
-    done = run(tmp_path, SOURCE, False, dtype, blocks, CLUSTERS[dtype, blocks, ctas], 16, late=4, far=4000000, limit=400, level=1, ctas=ctas)
+    done = run(tmp_path, SOURCE, False, dtype, blocks, CLUSTERS[dtype, blocks, ctas], 16, late=4, far=4000000, limit=400, ctas=ctas)
     assert done.returncode == 0, done.stdout + done.stderr
