@@ -360,7 +360,9 @@ int backward_t(const AveRmsNormBwdArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-size_t rms_norm_backward_workspace_bytes(const AveRmsNormBwdArgs& a) { return a.d_weight != nullptr ? (size_t)MAX_PARTS * (size_t)a.n * 4 : 0; }
+size_t rms_norm_backward_workspace_bytes(const AveRmsNormBwdArgs& a) {  // (no CTA without a row)
+  return a.d_weight != nullptr ? (size_t)(a.rows < MAX_PARTS ? a.rows : MAX_PARTS) * (size_t)a.n * 4 : 0;
+}
 
 int launch_rms_norm_backward(const AveRmsNormBwdArgs& a, cudaStream_t stream) {
   switch (a.x_dtype) {
