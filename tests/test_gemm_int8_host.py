@@ -168,11 +168,42 @@ def test_pairs_with_fewer_blocks_than_stages(tmp_path):
 def test_pairs_behind_an_expired_wait(tmp_path, dtype, blocks):
     """Operands, products and arrivals that come late, waits that some lanes of a warp have given up and others have not: every CTA comes to its end, with
     nothing on its way into it, and results are right or NaN."""
-    done = run(tmp_path, SOURCE, True, dtype, blocks, PAIRS[dtype, blocks], 16, late=4, far=4000000, limit=100)
+    done = run(tmp_path, SOURCE, True, dtype, blocks, PAIRS[dtype, blocks], 8, late=4, far=4000000, limit=100)
     assert done.returncode == 0, done.stdout + done.stderr
 
 
 @pytest.mark.parametrize("dtype,blocks,ctas", list(CLUSTERS))
 def test_clusters_behind_an_expired_wait(tmp_path, dtype, blocks, ctas):
-    done = run(tmp_path, SOURCE, False, dtype, blocks, CLUSTERS[dtype, blocks, ctas], 16, late=4, far=4000000, limit=400, ctas=ctas)
+    done = run(tmp_path, SOURCE, False, dtype, blocks, CLUSTERS[dtype, blocks, ctas], 8, late=4, far=4000000, limit=400, ctas=ctas)
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+def without(was, now, count=1):
+    assert SOURCE.count(was) == count, was
+    return SOURCE.replace(was, now)
+
+
+ENDS = dict(seeds=16, late=4, far=4000000)
+HALVES = [(256, 700, 385, 256, 5, 0, 704, 0)]
+ONE = [(256, 256, 640, 256, 5, 9, 256, 0)]
+
+
+def test_half_tiles_behind_an_expired_wait(tmp_path):
+    """Copies that one CTA of a pair has asked for alone are made up for by the bytes of their own tile."""
+    done = run(tmp_path, SOURCE, True, "__half", 1, HALVES, 16, late=4, far=4000000, limit=60)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
+@pytest.mark.parametrize("pair,key,cases,was,now,fault,more", [
+    (True, ("__half", 1), None, "if (begin || k + 1 == width)", "if (begin)", "results", dict(seeds=1)),
+    (True, ("__half", 1), ONE, "tc::mbar_wait_together(&acc_full[buf]", "tc::mbar_wait_unrolled(&acc_full[buf]", "do not end", dict(seeds=16, late=20, far=400000, limit=600)),
+    (True, ("__half", 1), HALVES, "tc::mbar_complete_tx(&full[i % stages], bytes(i))", "tc::mbar_complete_tx(&full[i % stages], landing(bn))", "do not end", dict(ENDS, limit=60)),
+    (True, ("__half", 1), HALVES, "tc::mbar_expect_tx(&full[i % stages], bytes(i))", "tc::mbar_expect_tx(&full[i % stages], landing(bn))", "do not end", dict(ENDS, limit=60)),
+    (True, ("__half", 1), None, "tc::drain(&empty[i % stages], i / stages & 1u);\n", ";\n", "on their way", dict(ENDS, limit=100)),
+    (True, ("float", 1), None, "for (; tile < tiles; tile += step) {  //", "for (; false;) {  //", "behind an expired wait", dict(ENDS, limit=100)),
+    (False, ("float", 2, 3), None, "last(full);", ";", "on their way", dict(ENDS, limit=400)),
+    (False, ("float", 2, 3), None, "whole ? e.a_scale[at] : __uint_as_float(0x7fffffffu)", "e.a_scale[at]", "behind an expired wait", dict(ENDS, limit=400))])
+def test_the_walks_see_what_is_missing(tmp_path, pair, key, cases, was, now, fault, more):
+    """A store, a wait, a count or a mark that is left out of the source."""
+    done = run(tmp_path, without(was, now), pair, key[0], key[1], cases or (PAIRS if pair else CLUSTERS)[key], ctas=2 if pair else key[2], **more)
+    assert done.returncode == 1 and fault in done.stdout, done.stdout + done.stderr
