@@ -1,7 +1,7 @@
 // RMS norm with the residual's addition, its form with 8-bit results, and rows in 8 bits and back.
 //
 //   h = round(x + residual),   y = h r w,   r = 1 / sqrt(mean(h^2) + eps)
-//   scale = max|y| / 127,   q = round(y / scale) = round(h w 127 / max|h w|)      (the row's r cancels)
+//   scale = max|y| / 127,   q = round(y / scale) = round(h w (127 / max|h w|))    (the row's r cancels; the factor is rounded to fp32)
 //
 // All of it is bound by HBM: x and residual are read once, h and y are written once.  Rows of whole 16-byte pieces come through a ring in shared
 // memory, filled by copies that each thread makes for itself (no barrier, nothing to wait for but its own copies), so that what is on its way does

@@ -35,8 +35,9 @@ def gemm_int8_transposed_b(A, B, a_scale, b_scale, bias=None, out=None, *, out_d
 
 def quantize_rows_int8(x):
     """``(q, scale)``: the rows of ``x`` (bf16, fp16 or fp32, last dimension up to 28672) in 8 bits.  ``scale`` (fp32, in the leading shape of ``x``) is
-    the row's largest ``|x|`` / 127, ``q`` (int8, rows a multiple of 16 bytes apart) is ``x / scale`` to nearest, ties to even.  A row that holds a NaN
-    or an infinity has a NaN as its scale and zeros in ``q``; one whose scale would be below the smallest normal number has zeros in both."""
+    the row's largest ``|x|`` / 127, ``q`` (int8, rows a multiple of 16 bytes apart) is ``x`` times 127 / largest, that factor rounded to fp32, to
+    nearest, ties to even (``x / scale`` but for the factor's rounding).  A row that holds a NaN or an infinity has a NaN as its scale and zeros in
+    ``q``; one whose scale would be below the smallest normal number has zeros in both."""
     return gdn._native.quantize_rows(x)
 
 

@@ -63,9 +63,10 @@ def rms_norm(x, weight=None, eps=1e-6, *, residual=None, zero_centered=False, re
 def rms_norm_int8(x, weight=None, eps=1e-6, *, residual=None, zero_centered=False, sum_out=None):
     """``rms_norm`` with each row of the result in 8 bits: ``(q, scale)``, or ``(q, scale, h)`` with ``residual``, as
     ``gemm.gemm_int8_transposed_b`` takes them.  ``scale`` (fp32, in the leading shape of ``x``) is the row's largest ``|y|`` / 127, ``q`` (int8,
-    rows a multiple of 16 bytes apart) is ``y / scale`` to nearest, ties to even; ``y`` itself is not rounded in between.  A row that holds a NaN
-    or an infinity has a NaN as its scale and zeros in ``q``; one whose scale would be below the smallest normal number, or whose largest ``|h *
-    weight|`` is below 3.8e-37, has zeros in both."""
+    rows a multiple of 16 bytes apart) is ``h * weight`` (in fp32) times 127 / its largest in the row, that factor rounded to fp32, to nearest,
+    ties to even: ``y / scale`` but for the factor's rounding; ``y`` itself is not rounded in between.  A row that holds a NaN or an infinity has
+    a NaN as its scale and zeros in ``q``; one whose scale would be below the smallest normal number, or whose largest ``|h * weight|`` is below
+    3.8e-37, has zeros in both."""
     return _native.rms_norm_int8(x, weight, eps, residual, zero_centered, sum_out)
 
 

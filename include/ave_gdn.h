@@ -451,7 +451,8 @@ size_t ave_layer_norm_backward_workspace_bytes(const AveLayerNormBwdArgs* args);
 
 /* RMS norm over rows of n elements, 1 <= n <= 28672: h = round(x + residual) (x itself without a residual), y = h * rstd * weight,
  * rstd = 1 / sqrt(mean(h^2) + eps); with AVE_RMS_FLAG_ZERO_CENTERED the weight is 1 + weight.  With AVE_RMS_FLAG_INT8 y is held as
- * q * scale: scale = max|y| / 127 of the row, q = y / scale to nearest, ties to even.  A row that holds a NaN or an infinity then has a NaN as
+ * q * scale: scale = max|y| / 127 of the row, q = h * weight (in fp32) times 127 / its largest in the row, that factor rounded to
+ * fp32, to nearest, ties to even: y / scale but for the factor's rounding.  A row that holds a NaN or an infinity then has a NaN as
  * its scale, one whose scale would be below the smallest normal number (or whose largest |h * weight| is below 3.8e-37) zero, both with q = 0. */
 #define AVE_RMS_FLAG_ZERO_CENTERED 1u
 #define AVE_RMS_FLAG_INT8 2u
