@@ -564,7 +564,8 @@ int operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int
 // ------------------------------------------------------------------------------------------------ one to four rows
 // The time is that of streaming B and, from two rows on, of the products: four a lane and instruction (dp4a, of which an SM takes about 11 lanes a cycle).  A warp takes
 // R rows of B, 16 loads of 512 bytes on their way, and MT rows of A from L1; with WK == 4 the warps of a CTA share the same rows of B, each a part of K.  The lanes' sums
-// meet in one reduction each.  (The bytes of a piece behind K are cleared in A; reading them is in bounds, rows are whole pieces apart.)
+// meet in one reduction each.  (The bytes of a piece behind K are cleared in A. They are read with the bytes in front of them in one aligned piece, behind the last row of an operand as well, and
+// may be anything.)
 template <class T, int MT, int R, int WK>
 __global__ void __launch_bounds__(128) gemm_int8_stream_kernel(const int8_t* A, const int8_t* B, const Epilogue e, int M, int64_t N, int K, int64_t lda, int64_t ldb) {
   constexpr int PU = 16 / R;  // pieces of a row at a time

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, 1) rms_elements_kernel(
   }
 }
 
-// Values of 8-bit rows: a thread writes 16 bytes of a row at a time, or, where the results do not lie on 16 bytes, one column and its neighbours the next ones (8192 x 2047
+// Values of 8-bit rows: a thread reads an aligned piece of a row (what lies in it behind the row's end, the last row's too, may be anything) and writes 16 bytes at a time, or, where the results do not lie on 16 bytes, one column and its neighbours the next ones (8192 x 2047
 // 101 us with 16 columns a thread written one by one, 12 so)
 template <class T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const AveQuantRowsArgs a, int pieces) {

@@ -26,10 +26,10 @@ def gemm_pipeline_transposed_b(A: torch.Tensor, B: torch.Tensor, out: torch.Tens
 # ---------------------------------------------------------------- 8 bits
 def gemm_int8_transposed_b(A, B, a_scale, b_scale, bias=None, out=None, *, out_dtype=None):
     """``C[m, n] = (sum_k A[m, k] B[n, k]) * a_scale[m] * b_scale[n] + bias[n]``: int8 ``A [M, K]`` and ``B [N, K]`` with rows a multiple of 16 bytes
-    apart (K itself may be odd, 131071 at most), fp32 scales of M and of N elements.  The sums are exact; they are scaled, in this order, and
-    the bias (in the dtype of the result or fp32) is added in fp32, behind one rounding of sums of more than 24 bits.  The result is bf16, or
-    ``out_dtype``, or of the dtype of ``out`` (bf16, fp16 or fp32), which shares no memory with the operands.  A row or column whose scale is NaN
-    is NaN, and so are results that a bounded wait on the device has given up on; ``gdn.read_status()`` says so."""
+    apart (K itself may be odd, 131071 at most; what lies behind it in a row's last 16 bytes, the last row's too, is read but not used), fp32 scales
+    of M and of N elements.  The sums are exact; they are scaled, in this order, and the bias (in the dtype of the result or fp32) is added in fp32,
+    behind one rounding of sums of more than 24 bits.  The result is bf16, or ``out_dtype``, or of the dtype of ``out`` (bf16, fp16 or fp32), which
+    shares no memory with the operands.  A row or column whose scale is NaN is NaN, and so are results that a bounded wait on the device has given up on; ``gdn.read_status()`` says so."""
     return gdn._native.gemm_int8(A, B, a_scale, b_scale, bias, out, out_dtype)
 
 

@@ -498,7 +498,7 @@ typedef struct AveQuantRowsArgs {
   uint32_t struct_size;
   uint32_t flags;   /* 0 */
   void* x;          /* [rows, n] of x_dtype; read when quantising, written when dequantising */
-  void* q;          /* int8 [rows, n], rows on 16 bytes, each with room for a whole number of 16 */
+  void* q;          /* int8 [rows, n], rows on 16 bytes, each, the last one too, with room for a whole number of 16 */
   float* scale;     /* fp32 [rows] */
   int64_t rows, n, x_stride, q_stride;
   int32_t x_dtype, reserved0;
@@ -507,8 +507,9 @@ int ave_quantize_rows_int8(const AveQuantRowsArgs* args, void* stream);
 int ave_dequantize_rows_int8(const AveQuantRowsArgs* args, void* stream);
 
 /* C[m][n] = sum_k A[m][k] B[n][k] * a_scale[m] * b_scale[n] + bias[n]: int8 A and B, exact sums (1 <= K <= 131071), (sum * a_scale) * b_scale + bias in
- * fp32 and one rounding.  Rows of A and B lie on 16 bytes; K need not be a multiple of anything.  An expired wait sets AVE_GDN_DEV_WAIT_EXPIRED,
- * and results that it keeps from being complete are NaN. */
+ * fp32 and one rounding.  Rows of A and B lie on 16 bytes, each, the last one too, with room for a whole number of 16; K need not be a
+ * multiple of anything, and what lies behind it in a row's last 16 bytes is read but not used.  An expired wait sets
+ * AVE_GDN_DEV_WAIT_EXPIRED, and results that it keeps from being complete are NaN. */
 typedef struct AveGemmInt8Args {
   uint32_t struct_size;
   uint32_t flags;           /* 0 */
