@@ -2,9 +2,9 @@
 // or fp32 behind fp32 scaling.  K is at most 131071, so that |sum| <= 128 * 128 * K stays below 2^31.
 //
 // Three forms.  Persistent pairs of CTAs on tiles of 256 x bn (gemm_int8_pair_kernel).  Few rows: one tile of up to 128 rows a cluster of `split` CTAs, each of
-// which takes a contiguous share of K; the partial sums meet over distributed shared memory (gemm_int8_cluster_kernel).  One to four rows: B streamed through the
-// ordinary units (gemm_int8_stream_kernel).  Sums are whole numbers and all forms
-// finish them in the same way: a result depends neither on the form nor on the split.
+// which takes a contiguous share of K; the partial sums meet over distributed shared memory (gemm_int8_cluster_kernel).  One or two rows, up to four where B
+// is small: B streamed through the ordinary units (gemm_int8_stream_kernel).  Sums are whole numbers and all forms finish them in the same way: a result depends neither on the
+// form nor on the split.
 #include <mutex>
 #include <type_traits>
 
@@ -55,6 +55,8 @@ __device__ __forceinline__ float finish(int32_t sum, float a_scale, float b_scal
 //   warp 1      of the leader: MMAs; a stage is free in both CTAs when its products are done
 //   warps 2..9  sums -> fp32 -> result, two warps a quarter of the rows, every other chunk of 128 bytes each: 32 rows of it through shared memory and out as one
 //               TMA store, or element by element where the rows of C do not lie on 16 bytes
+// Behind a wait that has expired every role leaves, the finishing warps write NaN where they have no sums, both CTAs meet, the leader makes up for copies that only one of them has asked
+// for, both wait (with a limit) for copies, products and arrivals that are on their way, and they meet again before tensor memory is given back.
 constexpr int PAIR_STAGES = 9, PAIR_RING = 184 * 1024, PAIR_THREADS = 320, PAIR_ROWS = 2 * BM;  // ring: depth limit and bytes of a CTA
 constexpr int GROUP_M = 16;  // row tiles that are swept together, so that their rows of A stay in L2
 constexpr int PAIR_OUT = PAIR_RING, PAIR_COLS = PAIR_OUT + 8 * 4096, PAIR_SMEM = PAIR_COLS + 8 * 1024 + 1024;

@@ -6,7 +6,7 @@
 // All of it is bound by HBM: x and residual are read once, h and y are written once.  Rows of whole 16-byte pieces come through a ring in shared
 // memory, filled by copies that each thread makes for itself (no barrier, nothing to wait for but its own copies), so that what is on its way does
 // not depend on registers; the sum of squares, and the largest |h w|, are formed in one pass over the row's pieces, and a second pass over shared
-// memory writes the results.  131072 x 2048 bf16: with a residual 350 us (6.1 TB/s of 6.5), to 8 bits 320 (5.9), 8-bit rows alone 139 (5.8) and back 132 (6.1); one row 1.7 to 1.9 us.
+// memory writes the results.  131072 x 2048 bf16: with a residual 355 to 361 us (6.0 TB/s of 6.5), to 8 bits 320 (5.9), 8-bit rows alone 139 (5.8) and back 132 (6.1); one row 1.7 to 1.9 us.
 // Other rows go element by element (8192 x 2047 bf16 with a residual 35 us, 22 with 2048 columns).
 #include "rows.cuh"
 

@@ -1,6 +1,6 @@
 // Blackwell (sm_100a) building blocks in inline PTX: mbarrier with bounded waits, TMA (tiled and bulk)
 // copies, tensor-memory allocation, tcgen05 MMA / commit / ld / st, and the shared-memory and instruction
-// descriptors the MMA reads.  No cluster multicast is used anywhere.
+// descriptors the MMA reads.  No load is multicast; a pair's commit arrives at the same barrier in both CTAs of its cluster.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
