@@ -117,7 +117,7 @@ class GdnBlockShard:
         from . import gdn
         B, T = (x[0] if isinstance(x, tuple) else x).shape[:2]
         y2 = self.project_in(x)
-        y = y2.reshape(B, T, -1)
+        y = y2.reshape(B, T, y2.shape[1])
         nq, nk, nv, nz, nb, na = self.splits
         qkv_in = y[:, :, : nq + nk + nv]
         z = y[:, :, nq + nk + nv: nq + nk + nv + nz].reshape(B, T, self.hv_local, self.dv)
@@ -205,7 +205,7 @@ class GdnBlockTP(GdnBlockShard):
         """Returns the block output after the output projection, ``[B, T, hidden]`` bf16, identical on every rank.  x: as in ``forward_local``."""
         B, T = (x[0] if isinstance(x, tuple) else x).shape[:2]
         o = self.forward_local(x, cu_seqlens)                                   # [B, T, hl, dv]
-        return self.project(o.reshape(B * T, -1), group, fused_reduce).reshape(B, T, -1)
+        return self.project(o.reshape(B * T, self.hv_local * self.dv), group, fused_reduce).reshape(B, T, self.w_out.shape[0])
 
     def layer(self, x: torch.Tensor, residual, weight, eps=1e-6, *, zero_centered=False, cu_seqlens=None, group=None, fused_reduce=False):
         """The block behind its norm in a residual stream: ``h = x + residual`` (x itself where ``residual`` is None), then the RMS norm of h with
